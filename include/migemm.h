@@ -663,6 +663,159 @@ mg_status mg_skip_rms_norm_f32_split_dev(mg_ctx *ctx, const float *x_dev,
                                          double epsilon, float *y_dev, float *sum_dev,
                                          int64_t block_size, void *split_dev);
 
+/* ----------------------------------------------------------- rotary positions */
+
+/* Rotary tables and what is turned by them.  Device pointers; the struct itself is
+ * read during the call. */
+typedef struct mg_rope {
+  const float *cos_table;      /* [max_pos, half_rot], as GroupQueryAttention's caches */
+  const float *sin_table;
+  int64_t max_pos;
+  int64_t half_rot;            /* pairs turned; elements past 2 half_rot pass through */
+  int32_t interleaved;         /* pairs (2i, 2i + 1); else (i, i + half_rot) */
+  const int32_t *positions;    /* int32, one a row, or NULL (the default of the op) */
+} mg_rope;
+
+/* How rotary frequencies are scaled for contexts longer than the trained one. */
+typedef enum mg_rope_scaling_kind {
+  MG_ROPE_NONE = 0,
+  MG_ROPE_LINEAR = 1, /* every frequency / factor */
+  MG_ROPE_NTK = 2,    /* base * factor^(R / (R - 2)), R = 2 half_rot */
+  MG_ROPE_YARN = 3,   /* / factor below, kept above, a ramp over the pairs that turn low
+                         to high times in original_length positions; values times
+                         value_factor */
+  MG_ROPE_BANDS = 4   /* / factor below low turns in original_length positions, kept above
+                         high, linear in the turns between */
+} mg_rope_scaling_kind;
+typedef struct mg_rope_scaling {
+  int32_t kind;
+  double factor;          /* >= 1 */
+  double original_length; /* YARN, BANDS */
+  double low, high;       /* turns: YARN's beta_slow and beta_fast, BANDS' factors */
+  double value_factor;    /* on cos and sin, all kinds */
+} mg_rope_scaling;
+
+/* cos_dev / sin_dev [count, half_rot] for positions first .. first + count - 1:
+ * value_factor * cos(p f_i) with f_i = base^(-i / half_rot) scaled as above (NULL:
+ * MG_ROPE_NONE, value_factor 1).  Angles are formed in 64 bits, so far positions are as
+ * exact as near ones.  These are the cos_cache / sin_cache inputs of
+ * GroupQueryAttention.  half_rot <= 128, positions < 2^31. */
+mg_status mg_rotary_tables_f32_dev(mg_ctx *ctx, int64_t first, int64_t count, int64_t half_rot,
+                                   double base, const mg_rope_scaling *scaling, float *cos_dev,
+                                   float *sin_dev);
+
+/* RotaryEmbedding as its own node: the rotation that GroupQueryAttention applies inside
+ * (lib/src/onnx_ops.dart:2653-2722), in 64 bits, rounded once.  x and y hold batch x seq x
+ * heads vectors of head_size; strides are elements of {batch, seq, head}, NULL =
+ * [batch, seq, heads, head_size] contiguous; the elements of a vector are adjacent.
+ * rope->positions is [batch, seq], NULL = 0 .. seq - 1 in every batch.  A row whose
+ * position lies outside the tables gets NaN in its turned elements.  y may be x (with the
+ * same strides); it must not overlap it otherwise. */
+mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t batch, int64_t seq,
+                                      int64_t heads, int64_t head_size, const int64_t *x_strides,
+                                      const mg_rope *rope, float *y_dev,
+                                      const int64_t *y_strides);
+
+/* ------------------------------------------------------- quantised KV cache */
+
+/* A paged KV cache held in 8 or 4 bits, written in place (GroupQueryAttention's fp32
+ * present = past + new is copied whole each step, lib/src/onnx_ops.dart:1829-2012).
+ * Each (token, KV head) vector x of head_size elements has its own scale:
+ *   INT8  s = amax / 127, q = x / s rounded half to even, value q s
+ *   E4M3  s = amax / 448, q = x / s rounded half to even to e4m3 (fn), value q s
+ *   INT4  m = (max + min) / 2, h = (max - min) / 30, n = ((x - m) / h + 15) / 2 rounded half
+ *         to even, value m + (2 n - 15) h
+ * with s, m, h rounded to fp32 and the quotients not rounded before q or n.  A vector that
+ * holds Infinity or NaN reads back as NaN throughout. */
+typedef enum mg_kv_format { MG_KV_INT8 = 0, MG_KV_E4M3 = 1, MG_KV_INT4 = 2 } mg_kv_format;
+typedef struct mg_kv_cache mg_kv_cache;
+
+/* pages of page_size tokens (16, 32, 64, 128 or 256) for kv_heads heads of head_size
+ * (1 .. 256).  Memory: per (token, head) 2 head_size codes, head_size padded to a multiple
+ * of 64, and 8 bytes of scales (INT4: 16).  The cache belongs to the context's device;
+ * contexts of that device may share it, ordered by the caller. */
+mg_status mg_kv_cache_create(mg_ctx *ctx, int32_t format, int64_t pages, int64_t page_size,
+                             int64_t kv_heads, int64_t head_size, mg_kv_cache **out);
+/* Waits for the device, then frees.  NULL: MG_INVALID_ARGUMENT. */
+mg_status mg_kv_cache_release(mg_kv_cache *cache);
+mg_status mg_kv_cache_info(const mg_kv_cache *cache, int64_t *pages, int64_t *page_size,
+                           int64_t *kv_heads, int64_t *head_size, int64_t *device_bytes);
+
+/* A batch of sequences over a cache.  Rows of q, k, v and y are packed: sequence b owns
+ * rows row_start[b] .. row_start[b + 1] - 1, and row i of it is position past[b] + i of the
+ * sequence, held at place (past[b] + i) % page_size of page page_table[b][(past[b] + i) /
+ * page_size].  The three arrays are device memory, read by the kernels (so a captured graph
+ * replays with what they hold then); the numbers bound them for the launch:
+ *   0 <= row_start[b] <= row_start[b + 1] <= rows, at most max_new rows a sequence, and
+ *   past[b] + its rows <= max_len.
+ * A sequence that breaks a bound is refused: nothing of it is read or written.  A page
+ * number outside the cache or the table is refused likewise: not written, and read as NaN.
+ * Both are remembered until mg_kv_cache_refused asks.  Rows that belong to no sequence are
+ * left as they were.  Sequences may share pages that they only read. */
+typedef struct mg_seq_batch {
+  int64_t batch;
+  int64_t rows;
+  int64_t max_new;
+  int64_t max_len;
+  const int32_t *row_start;   /* [batch + 1] */
+  const int32_t *past;        /* [batch] */
+  const int32_t *page_table;  /* [batch, table_stride] */
+  int64_t table_stride;
+} mg_seq_batch;
+
+/* Whether a call on this cache refused a sequence or a page since the last question
+ * (waits for the context's stream). */
+mg_status mg_kv_cache_refused(mg_ctx *ctx, mg_kv_cache *cache, int32_t *refused);
+
+/* Host-only: where the rows of a batch go, by the kernels' own rules, from host arrays in
+ * seqs: slots[r] = page * page_size + place, -1 for a row that is refused or belongs to no
+ * sequence; *refused (may be NULL) as above.  No device is touched. */
+mg_status mg_kv_cache_slots(const mg_seq_batch *seqs, int64_t pages, int64_t page_size,
+                            int64_t *slots, int32_t *refused);
+
+/* Writes the rows' keys and values: k_dev / v_dev row r, head h at r * stride + h *
+ * head_size (stride 0 = kv_heads * head_size).  With rope (may be NULL) keys are rotated
+ * first, at rope->positions[r] or, NULL, at their position in the sequence; a position
+ * outside the tables makes the key NaN. */
+mg_status mg_kv_cache_append_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                     const float *k_dev, int64_t k_stride, const float *v_dev,
+                                     int64_t v_stride, const mg_rope *rope);
+/* Reads the same rows back as fp32 values. */
+mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                   float *k_dev, int64_t k_stride, float *v_dev,
+                                   int64_t v_stride);
+
+/* Grouped-query attention of the rows over the cache (GroupQueryAttention without the copy,
+ * lib/src/onnx_ops.dart:1829-2012): y row r, head h = softmax(scale * q . K^T) . V over the
+ * cached positions that the row sees, KV head h / (num_heads / kv_heads).  The rows' own
+ * keys and values have been appended before.  Row i of sequence b sees positions
+ * 0 .. past[b] + i; with tree_dev (may be NULL) it sees 0 .. past[b] - 1 and position
+ * past[b] + j where bit j % 64 of its word tree_dev[r * tree_words + j / 64] is set: the
+ * ancestors of a drafted token and itself.  Rows that see nothing get zeros.  q is rotated by
+ * rope (may be NULL) as keys are by append.  scale defaults to 1 / sqrt(head_size).  Products
+ * are formed from fp16 digit pairs of q and of the weights against the exact codes, sums in
+ * fp32.  Strides: 0 = num_heads * head_size.  The call takes workspace for partial results
+ * when a sequence's keys are split. */
+mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                        const float *q_dev, int64_t q_stride, int32_t num_heads,
+                                        const mg_rope *rope, const uint64_t *tree_dev,
+                                        int32_t tree_words, int32_t has_scale, float scale,
+                                        float *y_dev, int64_t y_stride);
+
+/* -------------------------------------------------------- log probabilities */
+
+/* Of each row of logits [rows, vocab] (row r at r * row_stride, 0 = vocab): the log
+ * probability of tokens_dev[r] (NULL: none asked, logprob_dev unused; a token outside the
+ * vocabulary gives NaN), the entropy of the row (entropy_dev may be NULL), and the top
+ * largest logits' tokens with their log probabilities, largest first, equal ones by token
+ * (top 0 .. 64, at most vocab; top_ids_dev / top_logprobs_dev [rows, top]).  A logit of -inf
+ * has no weight; a row that holds NaN or +inf, or only -inf, gives NaN, its alternatives
+ * ranked with NaN above all. */
+mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_t rows,
+                                    int64_t vocab, int64_t row_stride, const int32_t *tokens_dev,
+                                    float *logprob_dev, float *entropy_dev, int32_t top,
+                                    int32_t *top_ids_dev, float *top_logprobs_dev);
+
 /* ----------------------------------------------------------------- weights */
 
 mg_status mg_weight_release(mg_weight *w);

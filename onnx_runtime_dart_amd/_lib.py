@@ -110,6 +110,18 @@ SIGNATURES = {
     "mg_weight_f32_create": [_P, _P, _I64, _I64, _I32, _PP],
     "mg_gemm_f32_w": [_P, _P, _I64, _I64, _P, _F, _F, _P, _P, _I32, _P],
     "mg_gemm_f32_w_dev": [_P, _P, _I64, _I64, _P, _F, _F, _P, _P, _I32, _P],
+    "mg_rotary_tables_f32_dev": [_P, _I64, _I64, _I64, C.c_double, _P, _P, _P],
+    "mg_rotary_embedding_f32_dev": [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P],
+    "mg_kv_cache_create": [_P, _I32, _I64, _I64, _I64, _I64, _PP],
+    "mg_kv_cache_release": [_P],
+    "mg_kv_cache_info": [_P, _P, _P, _P, _P, _P],
+    "mg_kv_cache_refused": [_P, _P, _P],
+    "mg_kv_cache_slots": [_P, _I64, _I64, _P, _P],
+    "mg_kv_cache_append_f32_dev": [_P, _P, _P, _P, _I64, _P, _I64, _P],
+    "mg_kv_cache_read_f32_dev": [_P, _P, _P, _P, _I64, _P, _I64],
+    "mg_kv_cache_attention_f32_dev": [_P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _F, _P,
+                                      _I64],
+    "mg_token_logprobs_f32_dev": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P],
     "mg_weight_release": [_P],
     "mg_weight_info": [_P, C.POINTER(_I64), C.POINTER(_I64), C.POINTER(_I64)],
 }

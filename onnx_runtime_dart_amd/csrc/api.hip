@@ -9,10 +9,14 @@
 #include <cstdarg>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
+#include "kv_common.h"
+#include "logprobs_common.h"
 #include "mg_internal.h"
+#include "rope_common.h"
 
 // Defined in int8.hip.
 mg_status mg_int8_run_batched(mg_ctx *ctx, const void *a_dev, int32_t a_signed,
@@ -2634,6 +2638,393 @@ mg_status mg_skip_rms_norm_f32_split_dev(mg_ctx *ctx, const float *x_dev, const 
   MG_TRY(mg_check_control(ctx, 0));
   return mg_elem_rms_norm_split(ctx, x_dev, skip_dev, gamma_dev, bias_dev, epsilon, rows, d,
                                 y_dev, skip_dev ? sum_dev : nullptr, kpad, split_dev);
+}
+
+}  // extern "C"
+
+// --------------------------------------------------------------------------
+// Rotary positions, the quantised KV cache with its attention, log probabilities.
+
+namespace {
+
+mg_status bad_arg(const char *what, const char *why) {
+  return mg_fail(MG_INVALID_ARGUMENT, std::string(what) + ": " + why);
+}
+
+// Tables as an op uses them on vectors of head_size elements.
+mg_status check_rope(const char *what, const mg_rope &r, int64_t head_size) {
+  if (r.half_rot < 1 || 2 * r.half_rot > head_size || r.half_rot > MG_ROPE_MAX_HALF)
+    return bad_arg(what, "half_rot must be 1 .. head_size / 2, at most 128");
+  if (r.max_pos < 1 || r.max_pos > 0x7fffffff || !r.cos_table || !r.sin_table)
+    return bad_arg(what, "cos and sin tables must be [max_pos, half_rot]");
+  return MG_OK;
+}
+
+// Most rows, positions and tokens of a batch (32-bit indices in the kernels).
+constexpr int64_t MG_KV_MOST = 0x7fffff00;
+
+mg_status check_seqs(const char *what, const mg_seq_batch *s) {
+  if (!s) return bad_arg(what, "null batch");
+  if (s->batch < 0 || s->batch > 65535 || s->rows < 0 || s->rows > MG_KV_MOST || s->max_new < 0 ||
+      s->max_new > s->rows || s->max_len < s->max_new || s->max_len > MG_KV_MOST ||
+      s->table_stride < 0)
+    return bad_arg(what, "batch must be 0 .. 65535, 0 <= max_new <= rows, max_new <= max_len, "
+                         "rows and max_len below 2^31 - 256");
+  if (s->batch > 0 && s->max_new > 0 &&
+      (!s->row_start || !s->past || (s->table_stride && !s->page_table)))
+    return bad_arg(what, "null row_start, past or page_table");
+  return MG_OK;
+}
+
+mg_status check_cache(const char *what, const mg_ctx *ctx, const mg_kv_cache *c,
+                      const mg_seq_batch *s) {
+  if (!ctx || !c) return bad_arg(what, "null argument");
+  if (c->device != ctx->device) return bad_arg(what, "cache of another device");
+  return check_seqs(what, s);
+}
+
+// A row stride, 0 = the row's own length.
+mg_status check_stride(const char *what, int64_t *stride, int64_t len) {
+  if (*stride == 0) *stride = len;
+  if (*stride < len || *stride > (int64_t)1 << 40)
+    return bad_arg(what, "row stride shorter than a row");
+  return MG_OK;
+}
+
+// The frequencies of scaled tables (half values).
+mg_status rope_frequencies(const char *what, int64_t half, double base, const mg_rope_scaling &s,
+                           double *f) {
+  const double two_pi = 6.283185307179586477;
+  const bool bands = s.kind == MG_ROPE_YARN || s.kind == MG_ROPE_BANDS;
+  if (!(base > 1.0) || !std::isfinite(base)) return bad_arg(what, "base must be finite, above 1");
+  if (s.kind < MG_ROPE_NONE || s.kind > MG_ROPE_BANDS) return bad_arg(what, "unknown scaling");
+  if (!std::isfinite(s.value_factor) || s.value_factor <= 0.0)
+    return bad_arg(what, "value_factor must be positive");
+  if (s.kind != MG_ROPE_NONE && !(s.factor >= 1.0 && std::isfinite(s.factor)))
+    return bad_arg(what, "factor must be finite, 1 at least");
+  if (bands && !(s.original_length >= 1.0 && s.low > 0.0 && s.high > s.low &&
+                 std::isfinite(s.original_length) && std::isfinite(s.high)))
+    return bad_arg(what, "original_length must be 1 at least and 0 < low < high");
+  if (s.kind == MG_ROPE_NTK && half < 2) return bad_arg(what, "NTK scaling needs half_rot 2 at least");
+  if (s.kind == MG_ROPE_NTK) base *= std::pow(s.factor, (double)half / (double)(half - 1));
+  double lo = 0.0, hi = 0.0;
+  if (s.kind == MG_ROPE_YARN) {
+    // The pairs that turn high and low times in the original length.
+    auto pair_of = [&](double turns) {
+      return (double)half * std::log(s.original_length / (turns * two_pi)) / std::log(base);
+    };
+    lo = std::max(std::floor(pair_of(s.high)), 0.0);
+    hi = std::min(std::ceil(pair_of(s.low)), (double)(2 * half - 1));
+  }
+  for (int64_t i = 0; i < half; i++) {
+    f[i] = std::pow(base, -(double)i / (double)half);
+    if (s.kind == MG_ROPE_LINEAR) f[i] /= s.factor;
+    if (bands) {
+      // Share of the unscaled frequency.
+      const double x = s.kind == MG_ROPE_YARN
+                           ? 1.0 - ((double)i - lo) / std::max(hi - lo, 0.001)
+                           : (s.original_length * f[i] / two_pi - s.low) / (s.high - s.low);
+      const double keep = std::min(std::max(x, 0.0), 1.0);
+      f[i] = f[i] / s.factor * (1.0 - keep) + f[i] * keep;
+    }
+  }
+  return MG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+mg_status mg_rotary_tables_f32_dev(mg_ctx *ctx, int64_t first, int64_t count, int64_t half_rot,
+                                   double base, const mg_rope_scaling *scaling, float *cos_dev,
+                                   float *sin_dev) {
+  const char *what = "RotaryTables";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx) return bad_arg(what, "null context");
+  if (first < 0 || count < 0 || first > 0x7fffffff || count > 0x7fffffff - first)
+    return bad_arg(what, "positions must be 0 .. 2^31 - 1");
+  if (half_rot < 1 || half_rot > MG_ROPE_MAX_HALF) return bad_arg(what, "half_rot must be 1 .. 128");
+  const mg_rope_scaling s = scaling ? *scaling : mg_rope_scaling{MG_ROPE_NONE, 1, 0, 0, 0, 1};
+  double f[MG_ROPE_MAX_HALF];
+  MG_TRY(rope_frequencies(what, half_rot, base, s, f));
+  if (count == 0) return MG_OK;
+  if (!cos_dev || !sin_dev) return bad_arg(what, "null buffer");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_rope_tables_run(ctx, first, count, half_rot, f, s.value_factor, cos_dev, sin_dev);
+}
+
+mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t batch, int64_t seq,
+                                      int64_t heads, int64_t head_size, const int64_t *x_strides,
+                                      const mg_rope *rope, float *y_dev,
+                                      const int64_t *y_strides) {
+  const char *what = "RotaryEmbedding";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx || !rope) return bad_arg(what, "null argument");
+  constexpr int64_t most = (int64_t)1 << 38;  // elements: a grid below 2^31 workgroups
+  if (batch < 0 || seq < 0 || heads < 0 || head_size < 1 || batch > most || seq > 0x7fffffff ||
+      heads > most || head_size > 65536 || (batch && seq > most / batch) ||
+      (batch * seq && heads * head_size > most / (batch * seq)))
+    return bad_arg(what, "dimensions out of range");
+  MG_TRY(check_rope(what, *rope, head_size));
+  if (batch * seq * heads == 0) return MG_OK;
+  if (!x_dev || !y_dev) return bad_arg(what, "null buffer");
+  mg_rotate_problem p{x_dev, y_dev, batch, seq, heads, head_size, {}, {}, *rope};
+  for (int i = 0; i < 3; i++) {
+    const int64_t own = i == 0 ? seq * heads * head_size : i == 1 ? heads * head_size : head_size;
+    p.xs[i] = x_strides ? x_strides[i] : own;
+    p.ys[i] = y_strides ? y_strides[i] : own;
+    if (p.xs[i] < 0 || p.ys[i] < 0 || p.xs[i] > most || p.ys[i] > most)
+      return bad_arg(what, "strides out of range");
+    const int64_t n = i == 0 ? batch : i == 1 ? seq : heads;
+    if (n > 1 && p.ys[i] < head_size) return bad_arg(what, "output vectors overlap");
+    if (x_dev == y_dev && n > 1 && p.xs[i] != p.ys[i])
+      return bad_arg(what, "in place needs equal strides");
+  }
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_rotate_run(ctx, p);
+}
+
+mg_status mg_kv_cache_create(mg_ctx *ctx, int32_t format, int64_t pages, int64_t page_size,
+                             int64_t kv_heads, int64_t head_size, mg_kv_cache **out) {
+  const char *what = "KvCache";
+  g_last_error.clear();
+  if (!ctx || !out) return bad_arg(what, "null argument");
+  *out = nullptr;
+  if (format < MG_KV_INT8 || format > MG_KV_INT4) return bad_arg(what, "unknown format");
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return bad_arg(what, "page_size must be 16, 32, 64, 128 or 256");
+  if (head_size < 1 || head_size > 256)
+    return mg_fail(MG_UNSUPPORTED, "KvCache: head_size must be 1 .. 256");
+  if (pages < 1 || kv_heads < 1 || kv_heads > 4096 || pages > MG_KV_MOST ||
+      pages * page_size > ((int64_t)1 << 40) / kv_heads)
+    return bad_arg(what, "pages and kv_heads must be positive, 2^40 vectors at most");
+  mg_kv_cache c;
+  c.device = ctx->device;
+  c.fmt = format;
+  while ((1 << c.plog) < page_size) c.plog++;
+  c.kv_heads = (int)kv_heads;
+  c.d = (int)head_size;
+  c.dp = (int)((head_size + 63) / 64 * 64);
+  c.pages = pages;
+  const int64_t tokens = pages * kv_heads * page_size;
+  const size_t codes = mg_align((size_t)(tokens * c.dp * kv_bits(format) / 8));
+  const size_t scales = mg_align((size_t)(tokens * kv_scales(format) * 4));
+  const size_t total = 2 * codes + scales + 256;
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, (int64_t)total));
+  mg_kv_cache *p = new (std::nothrow) mg_kv_cache(c);
+  if (!p) return mg_fail(MG_OUT_OF_MEMORY, "KvCache: out of host memory");
+  void *base = nullptr;
+  const hipError_t e = hipMalloc(&base, total);
+  if (e != hipSuccess) {
+    delete p;
+    (void)hipGetLastError();
+    return mg_fail(e == hipErrorOutOfMemory ? MG_OUT_OF_MEMORY : MG_DEVICE_ERROR,
+                   std::string("KvCache: hipMalloc: ") + hipGetErrorString(e));
+  }
+  p->k = static_cast<uint8_t *>(base);
+  p->v = p->k + codes;
+  p->sc = reinterpret_cast<float *>(p->v + codes);
+  p->refused = reinterpret_cast<int32_t *>(p->v + codes + scales);
+  p->bytes = (int64_t)total;
+  // (Waited for: the cache may be used on another context's stream next.)
+  mg_status st = mg_kv_clear(ctx, p);
+  if (st == MG_OK && hipStreamSynchronize(ctx->stream) != hipSuccess)
+    st = mg_fail(MG_DEVICE_ERROR, "KvCache: clearing failed");
+  if (st != MG_OK) {
+    (void)hipFree(base);
+    delete p;
+    return st;
+  }
+  *out = p;
+  return MG_OK;
+}
+
+mg_status mg_kv_cache_release(mg_kv_cache *cache) {
+  g_last_error.clear();
+  if (!cache) return bad_arg("KvCache", "null cache");
+  int was = 0;
+  const bool known = hipGetDevice(&was) == hipSuccess;
+  MG_HIP(hipSetDevice(cache->device));
+  const hipError_t e = hipFree(cache->k);  // (waits for the device)
+  delete cache;
+  if (known) (void)hipSetDevice(was);
+  if (e != hipSuccess)
+    return mg_fail(MG_DEVICE_ERROR, std::string("KvCache: hipFree: ") + hipGetErrorString(e));
+  return MG_OK;
+}
+
+mg_status mg_kv_cache_info(const mg_kv_cache *cache, int64_t *pages, int64_t *page_size,
+                           int64_t *kv_heads, int64_t *head_size, int64_t *device_bytes) {
+  g_last_error.clear();
+  if (!cache) return bad_arg("KvCache", "null cache");
+  if (pages) *pages = cache->pages;
+  if (page_size) *page_size = (int64_t)1 << cache->plog;
+  if (kv_heads) *kv_heads = cache->kv_heads;
+  if (head_size) *head_size = cache->d;
+  if (device_bytes) *device_bytes = cache->bytes;
+  return MG_OK;
+}
+
+mg_status mg_kv_cache_refused(mg_ctx *ctx, mg_kv_cache *cache, int32_t *refused) {
+  g_last_error.clear();
+  if (!ctx || !cache || !refused) return bad_arg("KvCache", "null argument");
+  if (cache->device != ctx->device) return bad_arg("KvCache", "cache of another device");
+  MG_TRY(mg_use_device(ctx));
+  int32_t word = 0;
+  const int32_t zero = 0;
+  MG_HIP(hipMemcpyAsync(&word, cache->refused, 4, hipMemcpyDeviceToHost, ctx->stream));
+  MG_HIP(hipStreamSynchronize(ctx->stream));
+  if (word) {
+    MG_HIP(hipMemcpyAsync(cache->refused, &zero, 4, hipMemcpyHostToDevice, ctx->stream));
+    MG_HIP(hipStreamSynchronize(ctx->stream));
+  }
+  *refused = word != 0;
+  return MG_OK;
+}
+
+mg_status mg_kv_cache_slots(const mg_seq_batch *seqs, int64_t pages, int64_t page_size,
+                            int64_t *slots, int32_t *refused) {
+  const char *what = "KvCache";
+  g_last_error.clear();
+  MG_TRY(check_seqs(what, seqs));
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) || pages < 1)
+    return bad_arg(what, "page_size must be 16, 32, 64, 128 or 256");
+  if (seqs->rows && !slots) return bad_arg(what, "null buffer");
+  int plog = 0;
+  while ((1 << plog) < page_size) plog++;
+  int32_t any = 0;
+  for (int64_t r = 0; r < seqs->rows; r++) slots[r] = -1;
+  for (int64_t b = 0; b < seqs->batch && seqs->max_new > 0; b++) {
+    const kv_seq q = kv_sequence(*seqs, b);
+    any |= q.bad;
+    for (int64_t i = 0; i < q.n; i++) {
+      const int64_t page = kv_page(*seqs, b, q.past + i, plog, pages);
+      any |= page < 0;
+      if (page >= 0) slots[q.start + i] = page * page_size + ((q.past + i) & (page_size - 1));
+    }
+  }
+  if (refused) *refused = any;
+  return MG_OK;
+}
+
+mg_status mg_kv_cache_append_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                     const float *k_dev, int64_t k_stride, const float *v_dev,
+                                     int64_t v_stride, const mg_rope *rope) {
+  const char *what = "KvCacheAppend";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  MG_TRY(check_cache(what, ctx, cache, seqs));
+  MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
+  MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
+  if (rope) MG_TRY(check_rope(what, *rope, cache->d));
+  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_kv_append_run(ctx, *cache, *seqs, k_dev, k_stride, v_dev, v_stride, rope);
+}
+
+mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                   float *k_dev, int64_t k_stride, float *v_dev,
+                                   int64_t v_stride) {
+  const char *what = "KvCacheRead";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  MG_TRY(check_cache(what, ctx, cache, seqs));
+  MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
+  MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
+  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_kv_read_run(ctx, *cache, *seqs, k_dev, k_stride, v_dev, v_stride);
+}
+
+mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                        const float *q_dev, int64_t q_stride, int32_t num_heads,
+                                        const mg_rope *rope, const uint64_t *tree_dev,
+                                        int32_t tree_words, int32_t has_scale, float scale,
+                                        float *y_dev, int64_t y_stride) {
+  const char *what = "KvCacheAttention";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  MG_TRY(check_cache(what, ctx, cache, seqs));
+  if (num_heads < 1 || num_heads % cache->kv_heads)
+    return bad_arg(what, "num_heads must be a multiple of kv_heads");
+  MG_TRY(check_stride(what, &q_stride, (int64_t)num_heads * cache->d));
+  MG_TRY(check_stride(what, &y_stride, (int64_t)num_heads * cache->d));
+  if (rope) MG_TRY(check_rope(what, *rope, cache->d));
+  if (tree_dev && (tree_words < 1 || (int64_t)tree_words * 64 < seqs->max_new))
+    return bad_arg(what, "tree_words must hold a bit for each of max_new rows");
+  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (!q_dev || !y_dev) return bad_arg(what, "null buffer");
+  mg_kv_attn a{};
+  a.c = *cache;
+  a.s = *seqs;
+  a.q = q_dev;
+  a.y = y_dev;
+  a.q_stride = q_stride;
+  a.y_stride = y_stride;
+  a.heads = num_heads;
+  a.group = num_heads / cache->kv_heads;
+  if (rope) a.rope = *rope;
+  a.tree = tree_dev;
+  a.tree_words = tree_dev ? tree_words : 0;
+  a.scale2 = (float)((has_scale ? (double)scale : 1.0 / std::sqrt((double)cache->d)) *
+                     1.44269504088896340736);
+  if (seqs->max_new * (int64_t)a.group > MG_KV_MOST)
+    return mg_fail(MG_UNSUPPORTED, "KvCacheAttention: too many rows");
+  size_t need = mg_kv_attn_plan(ctx, &a, true);
+  MG_TRY(mg_use_device(ctx));
+  // Without the workspace (byte budget, stream capture) the keys are not split.
+  if (need && !mg_ws_optional(ctx, need)) need = mg_kv_attn_plan(ctx, &a, false);
+  if ((int64_t)a.s.batch * a.nsplit * a.nblk * a.c.kv_heads > 0x7fffffff)
+    return mg_fail(MG_UNSUPPORTED, "KvCacheAttention: too many rows");
+  MG_TRY(mg_check_control(ctx, (int64_t)need));
+  a.part = need ? static_cast<float *>(ctx->ws) : nullptr;
+  return mg_kv_attn_run(ctx, a);
+}
+
+mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_t rows,
+                                    int64_t vocab, int64_t row_stride, const int32_t *tokens_dev,
+                                    float *logprob_dev, float *entropy_dev, int32_t top,
+                                    int32_t *top_ids_dev, float *top_logprobs_dev) {
+  const char *what = "TokenLogProbs";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx) return bad_arg(what, "null context");
+  if (rows < 0 || rows > 0x7fffff || vocab < 1 || vocab > 0x7fffff00)
+    return bad_arg(what, "rows must be 0 .. 2^23 - 1 and vocab 1 .. 2^31 - 256");
+  if (top < 0 || top > MG_LOGPROBS_MAX_TOP || top > vocab)
+    return bad_arg(what, "top must be 0 .. 64, at most vocab");
+  MG_TRY(check_stride(what, &row_stride, vocab));
+  if (rows == 0) return MG_OK;
+  if (!logits_dev || (tokens_dev && !logprob_dev) || (top && (!top_ids_dev || !top_logprobs_dev)))
+    return bad_arg(what, "null buffer");
+  mg_logprobs p{};
+  p.x = logits_dev;
+  p.tokens = tokens_dev;
+  p.logprob = tokens_dev ? logprob_dev : nullptr;
+  p.entropy = entropy_dev;
+  p.ids = top_ids_dev;
+  p.lps = top_logprobs_dev;
+  p.rows = rows;
+  p.stride = row_stride;
+  p.vocab = (int)vocab;
+  p.top = top;
+  if (!p.logprob && !p.entropy && !top) return MG_OK;
+  size_t need = mg_logprobs_plan(ctx, &p, true);
+  MG_TRY(mg_use_device(ctx));
+  // Without the workspace (byte budget, stream capture) a row stays with one workgroup.
+  if (need && !mg_ws_optional(ctx, need)) need = mg_logprobs_plan(ctx, &p, false);
+  MG_TRY(mg_check_control(ctx, (int64_t)need));
+  p.part = need ? static_cast<mg_logprobs_part *>(ctx->ws) : nullptr;
+  return mg_logprobs_run(ctx, p);
 }
 
 }  // extern "C"

@@ -25,6 +25,7 @@ graph's prepacked-weight cache (lib/src/onnx_graph.dart:102-105).
 from __future__ import annotations
 
 import ctypes as C
+import math
 import threading
 
 import numpy as np
@@ -584,6 +585,250 @@ def skip_rms_norm_f32_dev(x_ptr: int, skip_ptr: int, shape, gamma_ptr: int, gamm
                                        C.c_void_p(sum_ptr) if sum_ptr else None))
 
 
+# ------------------------------------- rotary positions, quantised KV cache
+
+
+class RopeScaling(C.Structure):
+    """mg_rope_scaling: how rotary frequencies are scaled for long contexts.
+
+    kind "none", "linear", "ntk", "yarn" or "bands"; low and high (turns in
+    original_length positions) default to 1 and 32 for "yarn", 1 and 4 for "bands";
+    value_factor (on cos and sin) to 0.1 ln(factor) + 1 for "yarn", else 1."""
+    _fields_ = [("kind", C.c_int32), ("factor", C.c_double), ("original_length", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("value_factor", C.c_double)]
+    KINDS = ("none", "linear", "ntk", "yarn", "bands")
+
+    def __init__(self, kind: str = "none", *, factor: float = 1.0, original_length: float = 0.0,
+                 low: float = 1.0, high: float | None = None, value_factor: float | None = None):
+        if kind not in self.KINDS:
+            raise ArgumentError(f"RotaryTables: unknown scaling {kind}")
+        if high is None:
+            high = 32.0 if kind == "yarn" else 4.0
+        if value_factor is None:
+            value_factor = 0.1 * math.log(factor) + 1.0 if kind == "yarn" and factor > 0 else 1.0
+        super().__init__(self.KINDS.index(kind), factor, original_length, low, high, value_factor)
+
+
+class Rope(C.Structure):
+    """mg_rope: rotary tables [max_pos, half_rot] in HBM, how pairs are formed and,
+    optionally, the positions (int32) of the rows."""
+    _fields_ = [("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("max_pos", C.c_int64),
+                ("half_rot", C.c_int64), ("interleaved", C.c_int32), ("positions", C.c_void_p)]
+
+    def __init__(self, cos_ptr: int, sin_ptr: int, *, max_pos: int, half_rot: int,
+                 interleaved: bool = False, positions_ptr: int = 0):
+        super().__init__(cos_ptr, sin_ptr, max_pos, half_rot, int(bool(interleaved)),
+                         positions_ptr or None)
+
+
+class SeqBatch(C.Structure):
+    """mg_seq_batch: a batch of sequences over a KV cache.  The arrays (int32) are device
+    memory; rows, max_new and max_len bound what they hold."""
+    _fields_ = [("batch", C.c_int64), ("rows", C.c_int64), ("max_new", C.c_int64),
+                ("max_len", C.c_int64), ("row_start", C.c_void_p), ("past", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64)]
+
+    def __init__(self, *, batch: int, rows: int, max_new: int, max_len: int, row_start_ptr: int,
+                 past_ptr: int, page_table_ptr: int, table_stride: int):
+        super().__init__(batch, rows, max_new, max_len, row_start_ptr or None, past_ptr or None,
+                         page_table_ptr or None, table_stride)
+
+
+def _ref(x):
+    return None if x is None else C.byref(x)
+
+
+def rotary_tables_dev(cos_ptr: int, sin_ptr: int, first: int, count: int, half_rot: int, *,
+                      base: float = 10000.0, scaling: RopeScaling | None = None,
+                      ctx: Context | None = None):
+    """cos / sin tables [count, half_rot] of positions first .. first + count - 1 in HBM."""
+    ctx = ctx or default_context()
+    check(lib.mg_rotary_tables_f32_dev(ctx.handle, first, count, half_rot, base, _ref(scaling),
+                                       cos_ptr, sin_ptr))
+
+
+def rotary_embedding_dev(x_ptr: int, batch: int, seq: int, heads: int, head_size: int, rope: Rope,
+                         y_ptr: int, *, x_strides=None, y_strides=None,
+                         ctx: Context | None = None):
+    """RotaryEmbedding on device buffers; strides are elements of (batch, seq, head), None =
+    [batch, seq, heads, head_size]."""
+    ctx = ctx or default_context()
+    xs = None if x_strides is None else (C.c_int64 * 3)(*x_strides)
+    ys = None if y_strides is None else (C.c_int64 * 3)(*y_strides)
+    check(lib.mg_rotary_embedding_f32_dev(ctx.handle, x_ptr, batch, seq, heads, head_size, xs,
+                                          C.byref(rope), y_ptr, ys))
+
+
+class KvCache:
+    """A paged KV cache in 8 or 4 bits in HBM (mg_kv_cache), written in place."""
+
+    FORMATS = {"int8": 0, "e4m3": 1, "int4": 2}
+    handle = None
+
+    def __init__(self, pages: int, *, kv_heads: int, head_size: int, page_size: int = 64,
+                 fmt: str = "int8", ctx: Context | None = None):
+        if fmt not in self.FORMATS:
+            raise ArgumentError(f"KvCache: unknown format {fmt}")
+        self.ctx = ctx or default_context()
+        self.pages, self.page_size = int(pages), int(page_size)
+        self.kv_heads, self.head_size, self.fmt = int(kv_heads), int(head_size), fmt
+        h = C.c_void_p()
+        check(lib.mg_kv_cache_create(self.ctx.handle, self.FORMATS[fmt], self.pages,
+                                     self.page_size, self.kv_heads, self.head_size, C.byref(h)))
+        self.handle = h
+
+    def release(self):
+        if self.handle:
+            lib.mg_kv_cache_release(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+    @property
+    def device_bytes(self) -> int:
+        n = C.c_int64(0)
+        check(lib.mg_kv_cache_info(self.handle, None, None, None, None, C.byref(n)))
+        return n.value
+
+    def refused(self) -> bool:
+        """Whether a call refused a sequence or a page since the last question."""
+        n = C.c_int32(0)
+        check(lib.mg_kv_cache_refused(self.ctx.handle, self.handle, C.byref(n)))
+        return bool(n.value)
+
+    def append_dev(self, seqs: SeqBatch, k_ptr: int, v_ptr: int, *, rope: Rope | None = None,
+                   k_stride: int = 0, v_stride: int = 0):
+        """Writes the rows' keys (rotated by rope) and values."""
+        check(lib.mg_kv_cache_append_f32_dev(self.ctx.handle, self.handle, C.byref(seqs), k_ptr,
+                                             k_stride, v_ptr, v_stride, _ref(rope)))
+
+    def read_dev(self, seqs: SeqBatch, k_ptr: int, v_ptr: int, *, k_stride: int = 0,
+                 v_stride: int = 0):
+        """Reads the rows back as fp32 values."""
+        check(lib.mg_kv_cache_read_f32_dev(self.ctx.handle, self.handle, C.byref(seqs), k_ptr,
+                                           k_stride, v_ptr, v_stride))
+
+    def attend_dev(self, seqs: SeqBatch, q_ptr: int, y_ptr: int, num_heads: int, *,
+                   rope: Rope | None = None, tree_ptr: int = 0, tree_words: int = 0, scale=None,
+                   q_stride: int = 0, y_stride: int = 0):
+        """Attention of the rows over their sequences' cached keys and values: causal, or
+        with tree words (uint64 [rows, tree_words]) by drafted ancestors."""
+        check(lib.mg_kv_cache_attention_f32_dev(
+            self.ctx.handle, self.handle, C.byref(seqs), q_ptr, q_stride, num_heads, _ref(rope),
+            tree_ptr or None, tree_words, int(scale is not None),
+            0.0 if scale is None else scale, y_ptr, y_stride))
+
+    # Host arrays: row_start [batch + 1], past [batch], page_table [batch, n] as in SeqBatch;
+    # rope = (cos, sin, interleaved) or (cos, sin, interleaved, positions [rows]).
+
+    def _host(self, row_start, past, page_table, rows, arrays, out_shapes, rope, call):
+        row_start, past = (np.ascontiguousarray(x, np.int32).ravel() for x in (row_start, past))
+        page_table = np.ascontiguousarray(page_table, np.int32)
+        if past.size != max(row_start.size - 1, 0) or page_table.ndim != 2 or \
+                page_table.shape[0] != past.size or row_start.size < 1:
+            raise ArgumentError("KvCache: row_start must be [batch + 1], past [batch], page_table "
+                                "[batch, pages]")
+        n = np.diff(row_start.astype(np.int64))
+        if past.size and (row_start[0] < 0 or (n < 0).any() or row_start[-1] > rows or
+                          (past < 0).any()):
+            raise ArgumentError("KvCache: row_start must rise from 0 to the rows, past be >= 0")
+        bufs = [DeviceBuffer.from_array(x, self.ctx) for x in [row_start, past, page_table, *arrays]]
+        outs = [DeviceBuffer.from_array(np.zeros(sh, np.float32), self.ctx) for sh in out_shapes]
+        try:
+            r = None
+            if rope is not None:
+                cos, sin = (np.ascontiguousarray(x, np.float32) for x in rope[:2])
+                if cos.ndim != 2 or cos.shape != sin.shape:
+                    raise ArgumentError("KvCache: cos and sin must be [max_pos, half_rot]")
+                pos = rope[3] if len(rope) > 3 else None
+                bufs += [DeviceBuffer.from_array(cos, self.ctx), DeviceBuffer.from_array(sin, self.ctx)]
+                at = len(bufs) - 2
+                if pos is not None:
+                    pos = np.ascontiguousarray(pos, np.int32).ravel()
+                    if pos.size != rows:
+                        raise ArgumentError("KvCache: one position a row")
+                    bufs.append(DeviceBuffer.from_array(pos, self.ctx))
+                r = Rope(bufs[at].ptr, bufs[at + 1].ptr, max_pos=cos.shape[0], half_rot=cos.shape[1],
+                         interleaved=rope[2], positions_ptr=0 if pos is None else bufs[-1].ptr)
+            seqs = SeqBatch(batch=past.size, rows=rows, max_new=int(n.max(initial=0)),
+                            max_len=int((n + past).max(initial=0)), row_start_ptr=bufs[0].ptr,
+                            past_ptr=bufs[1].ptr, page_table_ptr=bufs[2].ptr,
+                            table_stride=page_table.shape[1])
+            call(seqs, r, [b.ptr for b in bufs[3:3 + len(arrays)]], [o.ptr for o in outs])
+            got = [o.to_array(sh, np.float32) for o, sh in zip(outs, out_shapes)]
+            self.ctx.synchronize()
+            return got
+        finally:
+            for b in bufs + outs:
+                b.free()
+
+    def append(self, k, v, *, row_start, past, page_table, rope=None):
+        """Writes host rows k, v [rows, kv_heads, head_size]."""
+        k, v = (np.ascontiguousarray(x, np.float32) for x in (k, v))
+        if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (self.kv_heads, self.head_size):
+            raise ArgumentError("KvCache: k and v must be [rows, kv_heads, head_size]")
+        self._host(row_start, past, page_table, k.shape[0], [k, v], [], rope,
+                   lambda seqs, r, ins, outs: self.append_dev(seqs, ins[0], ins[1], rope=r))
+
+    def read(self, rows: int, *, row_start, past, page_table):
+        """k, v [rows, kv_heads, head_size] of the rows' positions (zeros where no row is)."""
+        shape = (rows, self.kv_heads, self.head_size)
+        return self._host(row_start, past, page_table, rows, [], [shape, shape], None,
+                          lambda seqs, r, ins, outs: self.read_dev(seqs, *outs))
+
+    def attend(self, q, *, row_start, past, page_table, rope=None, tree=None, scale=None):
+        """y [rows, num_heads, head_size] of host queries; tree uint64 [rows, words] or None."""
+        q = np.ascontiguousarray(q, np.float32)
+        if q.ndim != 3 or q.shape[2] != self.head_size:
+            raise ArgumentError("KvCache: q must be [rows, num_heads, head_size]")
+        ins = [q]
+        if tree is not None:
+            tree = np.ascontiguousarray(tree, np.uint64)
+            if tree.ndim != 2 or tree.shape[0] != q.shape[0]:
+                raise ArgumentError("KvCache: tree must be uint64 [rows, words]")
+            ins.append(tree)
+        return self._host(row_start, past, page_table, q.shape[0], ins, [q.shape], rope,
+                          lambda seqs, r, p, outs: self.attend_dev(
+                              seqs, p[0], outs[0], q.shape[1], rope=r, scale=scale,
+                              tree_ptr=p[1] if tree is not None else 0,
+                              tree_words=tree.shape[1] if tree is not None else 0))[0]
+
+
+def kv_cache_slots(row_start, past, page_table, *, rows: int, max_new: int, max_len: int,
+                   pages: int, page_size: int):
+    """(slots [rows], refused): where the rows of a batch go, by the kernels' own rules
+    (host-only)."""
+    row_start, past, page_table = (np.ascontiguousarray(x, np.int32)
+                                   for x in (row_start, past, page_table))
+    if page_table.ndim != 2 or page_table.shape[0] != past.size or row_start.size != past.size + 1:
+        raise ArgumentError("KvCache: row_start must be [batch + 1], past [batch], page_table "
+                            "[batch, pages]")
+    seqs = SeqBatch(batch=past.size, rows=rows, max_new=max_new, max_len=max_len,
+                    row_start_ptr=row_start.ctypes.data, past_ptr=past.ctypes.data,
+                    page_table_ptr=page_table.ctypes.data, table_stride=page_table.shape[1])
+    slots = np.empty(max(rows, 0), np.int64)
+    refused = C.c_int32(0)
+    check(lib.mg_kv_cache_slots(C.byref(seqs), pages, page_size, _ptr(slots), C.byref(refused)))
+    return slots, bool(refused.value)
+
+
+def token_logprobs_dev(logits_ptr: int, rows: int, vocab: int, *, tokens_ptr: int = 0,
+                       logprob_ptr: int = 0, entropy_ptr: int = 0, top: int = 0,
+                       top_ids_ptr: int = 0, top_logprobs_ptr: int = 0, row_stride: int = 0,
+                       ctx: Context | None = None):
+    """Log probabilities of given tokens, entropy and the top largest of each row of logits
+    in HBM (0 for an output that is not wanted)."""
+    ctx = ctx or default_context()
+    check(lib.mg_token_logprobs_f32_dev(ctx.handle, logits_ptr, rows, vocab, row_stride,
+                                        tokens_ptr or None, logprob_ptr or None,
+                                        entropy_ptr or None, top, top_ids_ptr or None,
+                                        top_logprobs_ptr or None))
+
+
 # ---------------------------------------------------------------------- ops
 
 
@@ -958,6 +1203,83 @@ def group_query_attention_dev(q_ptr: int, k_ptr: int, v_ptr: int, batch: int, se
         vp(bias_ptr), bias_heads, int(scale is not None),
         float(scale if scale is not None else 0.0), 0.0, -1, vp(y_ptr), vp(present_key_ptr),
         vp(present_value_ptr)))
+
+
+def rotary_tables(count: int, half_rot: int, *, first: int = 0, base: float = 10000.0,
+                  scaling: RopeScaling | None = None, ctx: Context | None = None):
+    """(cos, sin) [count, half_rot] of positions first .. first + count - 1."""
+    shape = (count, half_rot)
+    return _run_dev([], [shape, shape], lambda pc, ps: rotary_tables_dev(
+        pc, ps, first, count, half_rot, base=base, scaling=scaling, ctx=ctx), ctx)
+
+
+def op_rotary_embedding(x, cos_cache, sin_cache, position_ids=None, *, interleaved: bool = False,
+                        num_heads: int = 0, ctx: Context | None = None) -> np.ndarray:
+    """RotaryEmbedding (the rotation of lib/src/onnx_ops.dart:2653-2722 as its own node): x
+    [batch, seq, hidden] with num_heads heads, or [batch, heads, seq, head_size];
+    caches [max_pos, half_rot]; position_ids [batch, seq], or None for 0 .. seq - 1."""
+    x, cos, sin = (np.ascontiguousarray(a, np.float32) for a in (x, cos_cache, sin_cache))
+    if cos.ndim != 2 or cos.shape != sin.shape:
+        raise ArgumentError("RotaryEmbedding: cos and sin caches must be [max_pos, half_rot]")
+    if x.ndim == 4:
+        batch, heads, seq, d = x.shape
+        strides = (heads * seq * d, d, seq * d)
+    elif x.ndim == 3 and num_heads > 0 and x.shape[2] % num_heads == 0:
+        (batch, seq), heads, d = x.shape[:2], num_heads, x.shape[2] // num_heads
+        strides = None
+    else:
+        raise ArgumentError("RotaryEmbedding: x must be [batch, seq, hidden] of num_heads heads or "
+                            "[batch, heads, seq, head_size]")
+    ctx = ctx or default_context()
+    pos = None
+    if position_ids is not None:
+        pos = np.ascontiguousarray(position_ids, np.int32)
+        if pos.shape != (batch, seq):
+            raise ArgumentError("RotaryEmbedding: position_ids must be [batch, seq]")
+    pb = None if pos is None else DeviceBuffer.from_array(pos, ctx)
+
+    def call(px, pc, ps, py):
+        rotary_embedding_dev(px, batch, seq, heads, d,
+                             Rope(pc, ps, max_pos=cos.shape[0], half_rot=cos.shape[1],
+                                  interleaved=interleaved, positions_ptr=pb.ptr if pb else 0),
+                             py, x_strides=strides, y_strides=strides, ctx=ctx)
+
+    try:
+        return _run_dev([x, cos, sin], [x.shape], call, ctx)[0]
+    finally:
+        if pb:
+            pb.free()
+
+
+def op_token_logprobs(logits, tokens=None, *, top: int = 0, ctx: Context | None = None):
+    """(logprobs [...] or None, entropy [...], top token ids [..., top], their log
+    probabilities [..., top]) of logits [..., vocab] and tokens [...]."""
+    x = np.ascontiguousarray(logits, np.float32)
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ArgumentError("TokenLogProbs: logits must be [..., vocab]")
+    lead, vocab = x.shape[:-1], x.shape[-1]
+    rows = x.size // vocab
+    ins = [x]
+    if tokens is not None:
+        tokens = np.asarray(tokens)
+        if tokens.dtype.kind not in "iu" or tokens.shape != lead:
+            raise ArgumentError("TokenLogProbs: one integer token a row of logits")
+        # (Any token outside the vocabulary is -1: int32 could wrap into it.)
+        ins.append(np.where((tokens < 0) | (tokens >= vocab), -1, tokens).astype(np.int32))
+    ctx = ctx or default_context()
+    bufs = [DeviceBuffer.from_array(a, ctx) for a in ins]
+    n = max(rows, 1)
+    outs = [DeviceBuffer(4 * k, ctx) for k in (n, n, n * max(top, 1), n * max(top, 1))]
+    try:
+        token_logprobs_dev(bufs[0].ptr, rows, vocab, tokens_ptr=bufs[1].ptr if tokens is not None else 0,
+                           logprob_ptr=outs[0].ptr, entropy_ptr=outs[1].ptr, top=top,
+                           top_ids_ptr=outs[2].ptr, top_logprobs_ptr=outs[3].ptr, ctx=ctx)
+        return (outs[0].to_array(lead, np.float32) if tokens is not None else None,
+                outs[1].to_array(lead, np.float32), outs[2].to_array(lead + (top,), np.int32),
+                outs[3].to_array(lead + (top,), np.float32))
+    finally:
+        for b in bufs + outs:
+            b.free()
 
 
 # ------------------------------------------------------------ convolution
