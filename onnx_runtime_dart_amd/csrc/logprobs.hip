@@ -4,14 +4,24 @@
 // With m the row's running maximum, S = sum e^(x - m) and A = sum e^(x - m) (x - m):
 //   log p_t = x_t - m - log S,   H = log S - A / S,
 // both parts of H being >= 0, so nothing cancels.  When m grows to m', S and A become
-// e^(m - m') S and e^(m - m') (A + (m - m') S).
+// e^(m - m') S and e^(m - m') (A + (m - m') S).  Each lane keeps its own m, S and A over 16
+// logits at a time (fp32 sums of at most a few thousand terms, each at most 1); lanes and
+// waves join in 64 bits.  A NaN or +inf logit makes S NaN, a row of -inf leaves S 0:
+// neither has a distribution.
 //
 // The alternatives: each wave keeps its 64 largest entries sorted across its lanes, as
 // (key, token) with key the logit's bits in an order that unsigned integers have (NaN
-// above all).  An entry enters when it beats the top-th one; after the first few hundred
-// elements of a row that is rare (about top ln(n / top) times in n).
+// above all).  An entry enters when it beats the top-th one, found by one comparison per 16
+// logits and lane; the top-th largest of the lanes' own maxima over the first 16 bounds the
+// row's top-th from below, so that few entries enter only to leave again.  The sorted
+// lists of waves and of a row's runs join by taking the largest head, top times.
+//
+// The pass over the logits bounds it, 16-byte loads of which every lane has four in flight:
+// 1000 rows of 128256 in 107 us (4.8 TB/s, this card's copy rate; one logit a lane at a time
+// and every entry offered to the list: 358 us).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "mg_internal.h"
@@ -35,70 +45,135 @@ struct Sums {
   float m;
   double s, a;
 };
-// The sums of two parts of a row.
-__device__ inline Sums join(const Sums &x, const Sums &y) {
-  if (!(x.m > -INFINITY) && x.m == x.m && x.s == 0) return y;
-  if (!(y.m > -INFINITY) && y.m == y.m && y.s == 0) return x;
-  Sums r;
-  r.m = fmaxf(x.m, y.m);
-  const double dx = (double)x.m - r.m, dy = (double)y.m - r.m;
-  const double ex = exp(dx), ey = exp(dy);
-  r.s = x.s * ex + y.s * ey;
-  r.a = ex * (x.a + (x.s > 0 ? dx * x.s : 0)) + ey * (y.a + (y.s > 0 ? dy * y.s : 0));
+constexpr float kLowest = -3.402823466e38f;  // the running maximum before any logit
+
+// e^d; d below -200 (that of -inf included) counts as -200: 0 in fp32.
+__device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// Sums of x brought to the maximum m >= x.m.
+__device__ inline Sums moved(const Sums &x, float m) {
+  const float d = fmaxf(x.m - m, -200.f), e = x.m == m ? 1.f : exp_of(d);
+  return Sums{m, x.s * e, (x.a + (double)d * x.s) * e};
+}
+
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+__device__ inline double wave_sum(double x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ inline Sums wave_join(const Sums &x) {
+  Sums r = moved(x, wave_max(x.m));
+  r.s = wave_sum(r.s);
+  r.a = wave_sum(r.a);
   return r;
 }
 
-// Puts (k, id) into the sorted list of the wave (key, then lower token first).
-__device__ inline void insert(uint32_t &lk, int &li, uint32_t k, int id, int lane) {
-  const bool ahead = lk > k || (lk == k && li < id);
-  const int at = __popcll(__ballot(ahead));
-  const uint32_t pk = __shfl_up(lk, 1);
-  const int pi = __shfl_up(li, 1);
-  if (lane == at) {
-    lk = k;
-    li = id;
-  } else if (lane > at) {
-    lk = pk;
-    li = pi;
-  }
+// The value of lane l - 1 (lane 0: any).
+template <class T>
+__device__ inline T lane_before(T x) {
+  const int u = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(u, u, 0x138, 0xf, 0xf, false));
+}
+template <class T>
+__device__ inline T lane_value(T x, int l) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
 }
 
-// Offers each lane's (k, id) to the list; only lanes with ok.
-__device__ inline void offer(uint32_t &lk, int &li, uint32_t k, int id, bool ok, int top, int lane) {
-  uint32_t tk = __shfl(lk, top - 1);
-  int ti = __shfl(li, top - 1);
-  uint64_t want = __ballot(ok && (k > tk || (k == tk && id < ti)));
+// A wave's sorted entries, one a lane, and the top-th of them.
+struct List {
+  uint32_t key, tk;
+  int id, ti;
+};
+__device__ inline bool beats(uint32_t k, int i, uint32_t ok, int oi) {
+  return k > ok || (k == ok && i < oi);
+}
+// Puts in each lane's entry (of lanes with ok) that beats the top-th.
+__device__ inline void offer(List &l, uint32_t key, int id, bool ok, int top, int lane) {
+  uint64_t want = __ballot(ok && beats(key, id, l.tk, l.ti));
   while (want) {
-    const int l = __ffsll((unsigned long long)want) - 1;
+    const int w = __builtin_ctzll(want);
+    const uint32_t k = lane_value(key, w);
+    const int i = lane_value(id, w);
+    const int at = __popcll(__ballot(beats(l.key, l.id, k, i)));
+    const uint32_t pk = lane_before(l.key);
+    const int pi = lane_before(l.id);
+    if (lane >= at) {
+      l.key = lane == at ? k : pk;
+      l.id = lane == at ? i : pi;
+    }
+    l.tk = lane_value(l.key, top - 1);
+    l.ti = lane_value(l.id, top - 1);
     want &= want - 1;
-    insert(lk, li, __shfl(k, l), __shfl(id, l), lane);
+    want &= __ballot(beats(key, id, l.tk, l.ti));
   }
 }
-
-__device__ inline Sums wave_join(Sums x) {
+// The n-th largest (from 0) of the lanes' keys.
+__device__ inline uint32_t nth_largest(uint32_t x, int n, int lane) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    Sums y;
-    y.m = __shfl_xor(x.m, o);
-    y.s = __shfl_xor(x.s, o);
-    y.a = __shfl_xor(x.a, o);
-    x = join(x, y);
+  for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j; j >>= 1) {
+      const uint32_t y = __shfl_xor(x, j);
+      const bool larger = ((lane & j) == 0) == ((lane & k) == 0);  // descending
+      x = larger ? max(x, y) : min(x, y);
+    }
+  return lane_value(x, n);
+}
+
+// Joins up to 64 sorted lists of `top` entries, lane l's at key[l * pitch], id[l * pitch]
+// (n of them): lane j gets the j-th entry of all.
+__device__ inline void join_lists(const uint32_t *key, const int *id, int pitch, int n, int top,
+                                  int lane, uint32_t &ok, int &oi) {
+  int at = 0;
+  uint32_t k = 0;
+  int i = 0x7fffffff;
+  if (lane < n) {
+    k = key[lane * pitch];
+    i = id[lane * pitch];
   }
-  return x;
+  for (int j = 0; j < top; j++) {
+    uint32_t bk = k;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) bk = max(bk, __shfl_xor(bk, o));
+    // The lowest token of those with the largest key.
+    uint64_t who = __ballot(k == bk);
+    int l = __builtin_ctzll(who);
+    int bi = lane_value(i, l);
+    for (who &= who - 1; who; who &= who - 1) {
+      const int o = __builtin_ctzll(who), t = lane_value(i, o);
+      if (t < bi) {
+        bi = t;
+        l = o;
+      }
+    }
+    if (lane == j) {
+      ok = bk;
+      oi = bi;
+    }
+    if (lane == l) {
+      at++;
+      k = at < top ? key[lane * pitch + at] : 0;
+      i = at < top ? id[lane * pitch + at] : 0x7fffffff;
+    }
+  }
 }
 
 // The row's results, by one wave that holds its sums and list.
-__device__ inline void finish(const mg_logprobs &p, int64_t row, Sums t, bool nan, uint32_t lk,
-                              int li, int lane) {
-  const float *x = p.x + row * p.stride;
-  // NaN and +inf anywhere, and nothing but -inf, leave no distribution.
-  const bool none = nan || !(t.m > -INFINITY) || t.m == INFINITY;
-  const double lz = none ? __builtin_nan("") : log(t.s);
+__device__ inline void finish(const mg_logprobs &p, int64_t row, const Sums &t, uint32_t lk, int li,
+                              int lane) {
+  const double lz = t.s > 0 ? log(t.s) : __builtin_nan("");
   if (lane == 0) {
     if (p.logprob) {
       const int tok = p.tokens[row];
-      p.logprob[row] = tok < 0 || tok >= p.vocab ? __builtin_nanf("")
-                                                 : (float)((double)x[tok] - (double)t.m - lz);
+      p.logprob[row] =
+          tok < 0 || tok >= p.vocab
+              ? __builtin_nanf("")
+              : (float)((double)p.x[row * p.stride + tok] - (double)t.m - lz);
     }
     if (p.entropy) p.entropy[row] = (float)(lz - t.a / t.s);
   }
@@ -108,62 +183,120 @@ __device__ inline void finish(const mg_logprobs &p, int64_t row, Sums t, bool na
   }
 }
 
-// One workgroup a row (nsplit 1) or one of nsplit runs of a row.
-__global__ __launch_bounds__(256) void k_logprobs(mg_logprobs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x / p.nsplit;
-  const int split = blockIdx.x % p.nsplit;
-  const int v0 = split * p.run, v1 = min(p.vocab, v0 + p.run);
+constexpr int kQuads = 4;              // quads of logits a lane takes at a time
+constexpr int kChunk = 64 * 4 * kQuads;  // logits a wave takes at a time
+
+// One workgroup a row (nsplit 1) or one of nsplit runs of a row; its waves take chunks of
+// the run in turn.
+template <bool TOP>
+__global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t row = blockIdx.x / (unsigned)p.nsplit;
+  const int split = blockIdx.x % (unsigned)p.nsplit;
   const float *x = p.x + row * p.stride;
-  float m = -INFINITY, s = 0.f, a = 0.f;
-  bool nan = false;
-  uint32_t lk = 0;
-  int li = 0x7fffffff;
-  for (int v = v0 + wave * 64; v < v1; v += 256) {
-    const int id = v + lane;
-    const bool ok = id < v1;
-    const float z = ok ? x[id] : -INFINITY;
-    nan |= z != z;
-    if (z > m) {
-      const float d = m - z, e = m > -INFINITY ? exp2f(d * kLog2e) : 0.f;
-      a = m > -INFINITY ? e * (a + d * s) : 0.f;
-      s *= e;
-      m = z;
+  // Quads start at 16-byte addresses: logit v is element v + off of the quads.
+  const int off = (int)(reinterpret_cast<uintptr_t>(x) >> 2 & 3);
+  const float *base = x - off;
+  // (64 bits: a vocabulary may come near 2^31.)
+  const int64_t end = (int64_t)p.vocab + off;
+  const int64_t e0 = (int64_t)split * p.run, e1 = min(end, e0 + p.run);
+  float m = kLowest, s = 0.f, a = 0.f;
+  List l{0, 0, 0x7fffffff, 0x7fffffff};
+  bool first = true;
+  for (int64_t c0 = e0 + wave * kChunk; c0 < e1; c0 += 4 * kChunk) {
+    float z[kQuads][4];
+    const int64_t mine = c0 + lane * 4;
+    if (c0 >= off && c0 + kChunk <= e1) {
+#pragma unroll
+      for (int q = 0; q < kQuads; q++) {
+        const float4 v = *reinterpret_cast<const float4 *>(base + mine + q * 256);
+        z[q][0] = v.x, z[q][1] = v.y, z[q][2] = v.z, z[q][3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kQuads; q++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int64_t e = mine + q * 256 + j;
+          z[q][j] = e >= off && e < e1 ? base[e] : -__builtin_inff();
+        }
     }
-    if (z > -INFINITY) {
-      const float d = z - m, e = exp2f(d * kLog2e);
-      s += e;
-      a += e * d;
+    float big = z[0][0];
+#pragma unroll
+    for (int q = 0; q < kQuads; q++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) big = fmaxf(big, z[q][j]);
+    const float now = fmaxf(m, big);
+    const float d = fmaxf(m - now, -200.f), by = exp_of(d);
+    a = (a + d * s) * by;
+    s *= by;
+    m = now;
+#pragma unroll
+    for (int q = 0; q < kQuads; q++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float t = z[q][j] - m, e = exp_of(t);
+        s += e;
+        a = fmaf(e, fmaxf(t, -200.f), a);
+      }
+    if (TOP) {
+      // (NaN: never the maximum, always a candidate.)
+      uint32_t bk = key_of(big);
+      bool odd = false;
+#pragma unroll
+      for (int q = 0; q < kQuads; q++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) odd |= z[q][j] != z[q][j];
+      if (odd) bk = 0xffffffffu;
+      uint32_t least = l.tk;
+      if (first) {
+        least = max(least, nth_largest(bk, p.top - 1, lane));
+        first = false;
+      }
+      if (__any(bk >= least)) {
+#pragma unroll
+        for (int q = 0; q < kQuads; q++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int64_t e = mine + q * 256 + j;
+            const uint32_t k = key_of(z[q][j]);
+            offer(l, k, (int)(e - off), e >= off && e < e1 && k >= least, p.top, lane);
+          }
+      }
     }
-    if (p.top > 0) offer(lk, li, key_of(z), id, ok, p.top, lane);
   }
-  nan = __any(nan);
   Sums t = wave_join(Sums{m, (double)s, (double)a});
   __shared__ Sums st[4];
-  __shared__ int sn[4];
-  __shared__ uint32_t sk[4][64];
-  __shared__ int si[4][64];
-  if (lane == 0) {
-    st[wave] = t;
-    sn[wave] = nan;
+  __shared__ uint32_t sk[4 * 64];
+  __shared__ int si[4 * 64];
+  if (lane == 0) st[wave] = t;
+  if (TOP) {
+    sk[threadIdx.x] = l.key;
+    si[threadIdx.x] = l.id;
   }
-  sk[wave][lane] = lk;
-  si[wave][lane] = li;
   __syncthreads();
   if (wave) return;
-  for (int w = 1; w < 4; w++) {
-    t = join(t, st[w]);
-    nan |= sn[w] != 0;
-    if (p.top > 0) offer(lk, li, sk[w][lane], si[w][lane], lane < p.top && si[w][lane] != 0x7fffffff, p.top, lane);
+  float all = st[0].m;
+#pragma unroll
+  for (int w = 1; w < 4; w++) all = fmaxf(all, st[w].m);
+  t = Sums{all, 0, 0};
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const Sums y = moved(st[w], all);
+    t.s += y.s;
+    t.a += y.a;
   }
+  uint32_t lk = 0;
+  int li = 0x7fffffff;
+  if (TOP) join_lists(sk, si, 64, 4, p.top, lane, lk, li);
   if (p.nsplit == 1) {
-    finish(p, row, t, nan, lk, li, lane);
+    finish(p, row, t, lk, li, lane);
     return;
   }
   mg_logprobs_part &o = p.part[blockIdx.x];
   if (lane == 0) {
     o.m = t.m;
-    o.nan = nan;
     o.s = t.s;
     o.a = t.a;
   }
@@ -173,44 +306,49 @@ __global__ __launch_bounds__(256) void k_logprobs(mg_logprobs p) {
   }
 }
 
-__global__ __launch_bounds__(64) void k_logprobs_join(mg_logprobs p) {
+// Joins the at most 64 runs of a row.
+__global__ __launch_bounds__(64) void k_logprobs_join(const mg_logprobs p) {
+  constexpr int T = MG_LOGPROBS_MAX_TOP, PITCH = T + 1;
+  __shared__ uint32_t sk[64 * PITCH];
+  __shared__ int si[64 * PITCH];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
   const mg_logprobs_part *o = p.part + row * p.nsplit;
-  Sums t{-INFINITY, 0, 0};
-  bool nan = false;
+  for (int e = lane; e < p.nsplit * p.top; e += 64) {
+    const int r = e / p.top, j = e - r * p.top;
+    sk[r * PITCH + j] = o[r].key[j];
+    si[r * PITCH + j] = o[r].id[j];
+  }
+  Sums t{kLowest, 0, 0};
+  if (lane < p.nsplit) t = Sums{o[lane].m, o[lane].s, o[lane].a};
+  t = wave_join(t);
+  __syncthreads();
   uint32_t lk = 0;
   int li = 0x7fffffff;
-  for (int i = lane; i < p.nsplit; i += 64) {
-    t = join(t, Sums{o[i].m, o[i].s, o[i].a});
-    nan |= o[i].nan != 0;
-  }
-  t = wave_join(t);
-  nan = __any(nan);
-  if (p.top > 0)
-    for (int i = 0; i < p.nsplit; i++) {
-      const bool ok = lane < p.top;
-      const uint32_t k = ok ? o[i].key[lane] : 0;
-      const int id = ok ? o[i].id[lane] : 0x7fffffff;
-      offer(lk, li, k, id, ok && id != 0x7fffffff, p.top, lane);
-    }
-  finish(p, row, t, nan, lk, li, lane);
+  if (p.top) join_lists(sk, si, PITCH, p.nsplit, p.top, lane, lk, li);
+  finish(p, row, t, lk, li, lane);
 }
 
 }  // namespace
 
 size_t mg_logprobs_plan(const mg_ctx *ctx, mg_logprobs *p, bool split) {
+  // Runs for about one workgroup a compute unit, of one chunk a wave at least and at most 64 a
+  // row (one lane each where they join).
   int64_t n = 1;
-  if (split && p->rows < 2 * ctx->num_cus)
-    n = std::min<int64_t>((2 * ctx->num_cus + p->rows - 1) / p->rows, (p->vocab + 2047) / 2048);
-  n = std::max<int64_t>(1, n);
-  p->run = (int)(((p->vocab + n - 1) / n + 255) / 256 * 256);
-  p->nsplit = (p->vocab + p->run - 1) / p->run;
+  if (split && p->rows < ctx->num_cus)
+    n = std::min<int64_t>({ctx->num_cus / p->rows, (p->vocab + 4 * kChunk - 1) / (4 * kChunk), 64});
+  p->run = (int)std::min<int64_t>(((p->vocab + 3 + n - 1) / n + kChunk - 1) / kChunk * kChunk,
+                                  0x7ffffc00);
+  p->nsplit = (int)(((int64_t)p->vocab + 3 + p->run - 1) / p->run);
   return p->nsplit > 1 ? (size_t)p->rows * p->nsplit * sizeof(mg_logprobs_part) : 0;
 }
 
 mg_status mg_logprobs_run(mg_ctx *ctx, const mg_logprobs &p) {
-  k_logprobs<<<dim3((unsigned)(p.rows * p.nsplit)), dim3(256), 0, ctx->stream>>>(p);
+  const dim3 grid((unsigned)(p.rows * p.nsplit));
+  if (p.top)
+    k_logprobs<true><<<grid, dim3(256), 0, ctx->stream>>>(p);
+  else
+    k_logprobs<false><<<grid, dim3(256), 0, ctx->stream>>>(p);
   MG_TRY(mg_launch_check("log probabilities"));
   if (p.nsplit == 1) return MG_OK;
   k_logprobs_join<<<dim3((unsigned)p.rows), dim3(64), 0, ctx->stream>>>(p);

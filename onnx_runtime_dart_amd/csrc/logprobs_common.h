@@ -9,7 +9,6 @@ constexpr int MG_LOGPROBS_MAX_TOP = 64;
 struct mg_logprobs_part {
   double s, a;
   float m;
-  int32_t nan;
   uint32_t key[MG_LOGPROBS_MAX_TOP];
   int32_t id[MG_LOGPROBS_MAX_TOP];
 };
