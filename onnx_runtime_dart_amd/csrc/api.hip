@@ -2983,11 +2983,11 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   MG_TRY(mg_use_device(ctx));
   // Without the workspace (byte budget, stream capture) the keys are not split.
   if (need && !mg_ws_optional(ctx, need)) need = mg_kv_attn_plan(ctx, &a, false);
-  if ((int64_t)a.s.batch * a.nsplit * a.nblk * a.c.kv_heads > 0x7fffffff)
+  if ((int64_t)a.s.batch * a.nsplit * a.nblk * a.c.kv_heads > 0x7fffffff ||
+      (a.nsplit > 1 && a.s.batch * a.c.kv_heads * a.s.max_new * a.group > 0x7fffffff))
     return mg_fail(MG_UNSUPPORTED, "KvCacheAttention: too many rows");
   MG_TRY(mg_check_control(ctx, (int64_t)need));
-  a.part = need ? static_cast<float *>(ctx->ws) : nullptr;
-  return mg_kv_attn_run(ctx, a);
+  return mg_kv_attn_run(ctx, a, ctx->ws);
 }
 
 mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_t rows,
@@ -2998,8 +2998,8 @@ mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_
   ProfScope prof_(ctx, what);
   g_last_error.clear();
   if (!ctx) return bad_arg(what, "null context");
-  if (rows < 0 || rows > 0x7fffff || vocab < 1 || vocab > 0x7fffff00)
-    return bad_arg(what, "rows must be 0 .. 2^23 - 1 and vocab 1 .. 2^31 - 256");
+  if (rows < 0 || rows > 0x7fffff || vocab < 1 || vocab > 0x7ffff800)
+    return bad_arg(what, "rows must be 0 .. 2^23 - 1 and vocab 1 .. 2^31 - 2048");
   if (top < 0 || top > MG_LOGPROBS_MAX_TOP || top > vocab)
     return bad_arg(what, "top must be 0 .. 64, at most vocab");
   MG_TRY(check_stride(what, &row_stride, vocab));

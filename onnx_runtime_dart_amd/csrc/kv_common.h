@@ -71,11 +71,16 @@ struct mg_kv_attn {
   const uint64_t *tree;
   int tree_words;
   float scale2;  // scale * log2(e)
-  // The plan: rows (query, head of the group) a workgroup takes, whether its waves split
-  // keys (else rows), key splits of kc keys, row blocks a sequence, partials.
-  int mode, rows_wg, nblk, nsplit, kc;
+  bool vec;  // q, y and the tables take 16-byte accesses
+  // The plan: rows (query, head of the group) a workgroup takes, whether its waves split the
+  // keys of 16 rows (else rows), key splits of kc keys, row blocks a sequence.
+  bool keys;
+  int rows_wg, nblk, nsplit, kc;
+  // Partial results of (row, split): outputs, then (maximum, sum).
+  int64_t parts;
   float *part;
+  float2 *part_ml;
 };
 // Fills the plan (split: keys may be split) and returns the workspace of its partials.
 size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split);
-mg_status mg_kv_attn_run(mg_ctx *ctx, const mg_kv_attn &a);
+mg_status mg_kv_attn_run(mg_ctx *ctx, mg_kv_attn a, void *ws);

@@ -20,7 +20,9 @@
 // that), so most tiles rescale nothing and exchange nothing between lanes.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv_common.h"
 #include "rope_common.h"
@@ -29,6 +31,7 @@ namespace {
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
@@ -121,7 +124,7 @@ __device__ inline void load_run(uint32_t (&w)[KW], const uint8_t *p) {
   }
 }
 
-// Max over the four lanes that hold one row.
+// Max and sum over the four lanes that hold one row.
 __device__ inline float row_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -130,31 +133,163 @@ __device__ inline float row_sum(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
-// 2^-e with |x| in [2^(e-1), 2^e), 2^102 at most; 1 for 0, Infinity and NaN.
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+// 2^-e with |x| in [2^(e-1), 2^e), 2^102 at most; 1 for 0.
 __device__ inline float pow2_under(float x) {
   const int e = (int)(__float_as_uint(x) >> 23 & 255u);
-  if (e == 255 || x == 0.f) return 1.f;
-  return ldexpf(1.f, 126 - max(e, 24));
+  return x == 0.f ? 1.f : ldexpf(1.f, 126 - max(e, 24));
 }
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Floats of a row's partial result: DP outputs, the maximum, the sum, padded.
-__host__ __device__ constexpr int part_row(int dp) { return dp + 4; }
-
-struct Tile {
-  int64_t page[2];  // of each 16 keys, 0 where there is none
-  bool none[2];
+template <int FMT, int NB>
+struct Shape {
+  static constexpr int DP = 16 * NB, KS = DP / 32;
+  static constexpr int KW = FMT == MG_KV_INT4 ? DP / 32 : DP / 16;  // dwords of a lane's run, 16 keys
+  static constexpr int RB = DP * (FMT == MG_KV_INT4 ? 4 : 8) / 8;   // bytes of a vector
 };
 
+// A tile of 32 keys: where its two runs of 16 lie, and the lane's codes and scales.  The
+// parts are loaded apart, each as soon as the last tile's are used.
+template <int FMT, int NB>
+struct Tile {
+  using S = Shape<FMT, NB>;
+  int64_t at[2];  // (page, head) times page size plus place
+  int64_t ph[2];  // (page, head)
+  bool none[2];   // no such page: its keys read as NaN
+  uint32_t k[2][S::KW], v[2][S::KW];
+  float4 ks[2], vs[2], kz[2], vz[2];
+
+  __device__ inline void locate(const mg_kv_attn &a, int b, int h, int total, int t0) {
+    const int psize = 1 << a.c.plog;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int64_t p = t0 + 16 * u < total ? kv_page(a.s, b, t0 + 16 * u, a.c.plog, a.c.pages) : 0;
+      none[u] = p < 0;
+      ph[u] = (p < 0 ? 0 : p) * a.c.kv_heads + h;
+      at[u] = (ph[u] << a.c.plog) + ((t0 + 16 * u) & (psize - 1));
+    }
+  }
+  __device__ inline void load_k(const mg_kv_attn &a, int g, int c) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      load_run<S::KW>(k[u], a.c.k + at[u] * S::RB + (c * S::RB + g * (S::RB / 4)));
+  }
+  __device__ inline void load_v(const mg_kv_attn &a, int g, int c) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      load_run<S::KW>(v[u], a.c.v + at[u] * S::RB + (4 * g * S::RB + c * (4 * S::KW)));
+  }
+  __device__ inline void load_scales(const mg_kv_attn &a, int g) {
+    const int psize = 1 << a.c.plog;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      // (page, head)'s scales: kv_scales runs of psize.
+      const float *sc = a.c.sc + (ph[u] * (kv_scales(FMT) - 1) << a.c.plog) + at[u] + 4 * g;
+      ks[u] = *reinterpret_cast<const float4 *>(sc);
+      vs[u] = *reinterpret_cast<const float4 *>(sc + psize);
+      if (FMT == MG_KV_INT4) {
+        kz[u] = *reinterpret_cast<const float4 *>(sc + 2 * psize);
+        vz[u] = *reinterpret_cast<const float4 *>(sc + 3 * psize);
+      }
+      if (none[u]) {
+        const float nan = __builtin_nanf("");
+        ks[u] = make_float4(nan, nan, nan, nan);
+      }
+    }
+  }
+};
+
+__device__ inline void spread(float (&x)[8], const float4 (&v)[2], float f) {
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    x[4 * u] = v[u].x * f;
+    x[4 * u + 1] = v[u].y * f;
+    x[4 * u + 2] = v[u].z * f;
+    x[4 * u + 3] = v[u].w * f;
+  }
+}
+
+// The workgroup's queries, turned and scaled, in shared memory: `n` rows from row r0 of
+// sequence sq; rows past the last are zero.
+template <int DP>
+__device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int h, int r0, int rows,
+                                     int n, float *lds) {
+  constexpr int QP = DP + 4;
+  const int half = (int)a.rope.half_rot;
+  if (a.vec) {
+    // Units of eight elements: four pairs of halves, or eight adjacent ones.
+    constexpr int UNITS = DP / 8;
+    const int turned = a.rope.interleaved ? half / 4 : 0;  // units of pairs side by side
+    const int halves = a.rope.interleaved ? 0 : half / 4;
+    for (int i = threadIdx.x; i < n * UNITS; i += 256) {
+      const int r = i / UNITS, u = i - r * UNITS, row = r0 + r;
+      const int d0 = u < halves ? 4 * u : halves ? 2 * half + 8 * (u - halves) : 8 * u;
+      const int d1 = u < halves ? d0 + half : d0 + 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), z = x;
+      if (row < rows && d0 < a.c.d) {
+        const int qi = row / a.group, j = row - qi * a.group;
+        const int64_t at = sq.start + qi;
+        const float *q = a.q + at * a.q_stride + (int64_t)(h * a.group + j) * a.c.d;
+        x = *reinterpret_cast<const float4 *>(q + d0);
+        if (d1 < a.c.d) z = *reinterpret_cast<const float4 *>(q + d1);
+        if (u < halves + turned) {
+          const int64_t pos = a.rope.positions ? a.rope.positions[at] : sq.past + qi;
+          const bool in = (uint64_t)pos < (uint64_t)a.rope.max_pos;
+          const int64_t t = (in ? pos : 0) * half + 4 * u;
+          const float4 cs = *reinterpret_cast<const float4 *>(a.rope.cos_table + t);
+          const float4 sn = *reinterpret_cast<const float4 *>(a.rope.sin_table + t);
+          auto pair = [&](float &p, float &w, float co, float si) {
+            const double c = in ? (double)co : __builtin_nan(""), s = si, pd = p, wd = w;
+            p = (float)(pd * c - wd * s);
+            w = (float)(wd * c + pd * s);
+          };
+          if (halves) {
+            pair(x.x, z.x, cs.x, sn.x);
+            pair(x.y, z.y, cs.y, sn.y);
+            pair(x.z, z.z, cs.z, sn.z);
+            pair(x.w, z.w, cs.w, sn.w);
+          } else {
+            pair(x.x, x.y, cs.x, sn.x);
+            pair(x.z, x.w, cs.y, sn.y);
+            pair(z.x, z.y, cs.z, sn.z);
+            pair(z.z, z.w, cs.w, sn.w);
+          }
+        }
+      }
+      const float f = a.scale2;
+      *reinterpret_cast<float4 *>(lds + r * QP + d0) = make_float4(f * x.x, f * x.y, f * x.z, f * x.w);
+      *reinterpret_cast<float4 *>(lds + r * QP + d1) = make_float4(f * z.x, f * z.y, f * z.z, f * z.w);
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < n * DP; i += 256) {
+    const int r = i / DP, d = i - r * DP, row = r0 + r;
+    float x = 0.f;
+    if (row < rows && d < a.c.d) {
+      const int qi = row / a.group, j = row - qi * a.group;
+      const int64_t at = sq.start + qi;
+      const int64_t pos = half && a.rope.positions ? a.rope.positions[at] : sq.past + qi;
+      x = a.scale2 *
+          rope_at(a.q + at * a.q_stride + (int64_t)(h * a.group + j) * a.c.d, d, pos, a.rope);
+    }
+    lds[r * QP + d] = x;
+  }
+}
+
+// KEYS: the four waves take tiles in turn for the same 16 rows; else rows of their own.
 template <int FMT, int NB, int QB, bool KEYS>
 __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
-  constexpr int DP = 16 * NB, KS = DP / 32;
-  constexpr int KW = FMT == MG_KV_INT4 ? DP / 32 : DP / 16;  // dwords of a lane's run, 16 keys
-  constexpr int RB = DP * (FMT == MG_KV_INT4 ? 4 : 8) / 8;   // bytes of a vector
-  constexpr int ROWS = 16 * QB * (KEYS ? 1 : 4);             // rows of the workgroup
+  using S = Shape<FMT, NB>;
+  constexpr int DP = S::DP, KS = S::KS, KW = S::KW;
+  constexpr int ROWS = 16 * QB * (KEYS ? 1 : 4);  // rows of the workgroup
   constexpr int QP = DP + 4;
-  // 64 rows' queries; later the four waves' results of the same 16 rows.
-  static_assert(!KEYS || QB == 1, "the waves' results fill the queries' place");
-  __shared__ __attribute__((aligned(16))) float lds[64 * QP];
+  static_assert(!KEYS || QB == 1, "the waves' results take the place of 64 rows");
+  // The rows' queries; later (KEYS) the four waves' results.
+  __shared__ __attribute__((aligned(16))) float lds[(KEYS ? 64 : ROWS) * QP];
   __shared__ float stat[4][2][16 * QB];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -175,64 +310,69 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
   if (r0 >= rows) return;
   // Keys of this workgroup: those its last row sees, of its split.
   const int total = sq.past + sq.n;
-  const int last = min(r0 + ROWS, rows) - 1;
-  const int kend = a.tree ? total : sq.past + last / a.group + 1;
+  const int kend = a.tree ? total : sq.past + (min(r0 + ROWS, rows) - 1) / a.group + 1;
   const int kbeg = split * a.kc;
   if (kbeg >= kend && split > 0) return;
-  half8v qh[QB][KS], ql[QB][KS];
-  float f[QB], qs[QB];
-  int see[QB];               // keys below it are seen (tree: past)
-  int64_t word[QB];          // the row's words of the tree
-  const int wr0 = KEYS ? 0 : wave * 16 * QB;
-#pragma unroll
-  for (int qb = 0; qb < QB; qb++) {
-    // Queries: turned and scaled in shared memory, 16 rows of each wave at a time.
-    constexpr int STAGED = KEYS ? 16 : 64;
-    __syncthreads();
-    for (int i = threadIdx.x; i < STAGED * DP; i += 256) {
-      const int r = i / DP, d = i - r * DP;
-      const int row = r0 + (r >> 4) * 16 * QB + qb * 16 + (r & 15);
-      float x = 0.f;
-      if (row < rows && d < a.c.d) {
-        const int qi = row / a.group, j = row - qi * a.group;
-        const int64_t at = sq.start + qi;
-        const int64_t pos = a.rope.half_rot && a.rope.positions ? a.rope.positions[at] : sq.past + qi;
-        x = a.scale2 *
-            rope_at(a.q + at * a.q_stride + (int64_t)(h * a.group + j) * a.c.d, d, pos, a.rope);
-      }
-      lds[r * QP + d] = x;
-    }
-    __syncthreads();
-    const float *x = lds + ((KEYS ? 0 : wave * 16) + c) * QP + g * (DP / 4);
-    float mx = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP / 4; d++) mx = fmaxf(mx, fabsf(x[d]));
-    mx = row_max(mx);
-    const float dn = 1024.f * pow2_under(mx);
-    f[qb] = 1.f / dn;
-    float sum = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float v = x[8 * s + k_slot<FMT>(j)] * dn;
-        const _Float16 hi = (_Float16)v;
-        qh[qb][s][j] = hi;
-        ql[qb][s][j] = (_Float16)(v - (float)hi);
-        sum += v;
-      }
-    qs[qb] = FMT == MG_KV_INT4 ? row_sum(sum) : 0.f;
-    const int row = min(r0 + wr0 + qb * 16 + c, rows - 1), qi = row / a.group;
-    see[qb] = a.tree ? sq.past : sq.past + qi + 1;
-    word[qb] = (int64_t)(sq.start + qi) * a.tree_words;
-  }
-  // Keys below `plain` are seen by every row of the wave.
-  const int plain = a.tree ? sq.past : sq.past + min(r0 + wr0, rows - 1) / a.group + 1;
-  // Keys that some row of the wave sees, of this split.
+  const int wr0 = KEYS ? 0 : wave * 16 * QB;  // the wave's first row
+  // Keys that some row of the wave sees, of this split, and those that all of them see.
   const int wend = r0 + wr0 >= rows ? 0
                    : a.tree         ? total
                                     : sq.past + (min(r0 + wr0 + 16 * QB, rows) - 1) / a.group + 1;
   const int kfin = min(wend, kend - kbeg > a.kc ? kbeg + a.kc : kend);
+  const int plain = a.tree ? sq.past : sq.past + min(r0 + wr0, rows - 1) / a.group + 1;
+  constexpr int STEP = KEYS ? 128 : 32;
+  int t0 = kbeg + (KEYS ? 32 * wave : 0);
+  // The first tile's loads run while the queries are made.
+  Tile<FMT, NB> t;
+  bool refused = false;
+  if (t0 < kfin) {
+    t.locate(a, b, h, total, t0);
+    t.load_k(a, g, c);
+    t.load_scales(a, g);
+    t.load_v(a, g, c);
+    refused = t.none[0] || t.none[1];
+  }
+
+  stage_queries<DP>(a, sq, h, r0, rows, ROWS, lds);
+  __syncthreads();
+  half8v qh[QB][KS], ql[QB][KS];
+  float qs[QB];
+  int see[QB];       // keys below it are seen (tree: past)
+  int64_t word[QB];  // the row's words of the tree
+  float f;
+  {
+    // One power of two for the wave's rows: the largest element under 2^15, so that a
+    // digit pair is exact to 2^-22 of any element down to 2^-17 of it, and to 2^-39 of it below.
+    float mx = 0.f;
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+      for (int d = 0; d < DP / 4; d++) {
+        const float v = fabsf(lds[(wr0 + qb * 16 + c) * QP + g * (DP / 4) + d]);
+        mx = v < __builtin_inff() ? fmaxf(mx, v) : mx;
+      }
+    const float dn = 32768.f * pow2_under(wave_max(mx));
+    f = 1.f / dn;
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+      const float *x = lds + (wr0 + qb * 16 + c) * QP + g * (DP / 4);
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float v = x[8 * s + k_slot<FMT>(j)] * dn;
+          const _Float16 hi = (_Float16)v;
+          qh[qb][s][j] = hi;
+          ql[qb][s][j] = (_Float16)(v - (float)hi);
+          sum += v;
+        }
+      qs[qb] = FMT == MG_KV_INT4 ? row_sum(sum) : 0.f;
+      const int row = min(r0 + wr0 + qb * 16 + c, rows - 1), qi = row / a.group;
+      see[qb] = a.tree ? sq.past : sq.past + qi + 1;
+      word[qb] = (int64_t)(sq.start + qi) * a.tree_words;
+    }
+  }
 
   float4v o[QB][NB];
   float m[QB], l[QB], z[QB];
@@ -245,74 +385,12 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
   }
   float vn = ldexpf(1.f, 100);
 
-  const int psize = 1 << a.c.plog;
-  auto pages = [&](int t0, Tile &t) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int64_t p = t0 + 16 * u < total ? kv_page(a.s, b, t0 + 16 * u, a.c.plog, a.c.pages) : 0;
-      t.none[u] = p < 0;
-      t.page[u] = p < 0 ? 0 : p;
-    }
-  };
-  bool refused = false;
-  const int step = KEYS ? 128 : 32;
-  for (int t0 = kbeg + (KEYS ? 32 * wave : 0); t0 < kfin; t0 += step) {
-    Tile t;
-    pages(t0, t);
-    uint32_t kw[2][KW], vw[2][KW];
-    float4 ks[2], vs[2], kz[2], vz[2];
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int64_t ph = t.page[u] * a.c.kv_heads + h;
-      const int slot = (t0 + 16 * u) & (psize - 1);
-      load_run<KW>(kw[u], a.c.k + (ph * psize + slot + c) * RB + g * (RB / 4));
-      load_run<KW>(vw[u], a.c.v + (ph * psize + slot + 4 * g) * RB + c * (4 * KW));
-      const float *sc = a.c.sc + ph * kv_scales(FMT) * psize + slot + 4 * g;
-      ks[u] = *reinterpret_cast<const float4 *>(sc);
-      vs[u] = *reinterpret_cast<const float4 *>(sc + psize);
-      if (FMT == MG_KV_INT4) {
-        kz[u] = *reinterpret_cast<const float4 *>(sc + 2 * psize);
-        vz[u] = *reinterpret_cast<const float4 *>(sc + 3 * psize);
-      }
-      if (t.none[u]) {
-        const float nan = __builtin_nanf("");
-        ks[u] = make_float4(nan, nan, nan, nan);
-        refused = true;
-      }
-    }
-    float ksa[8], vsa[8], kza[8], vza[8];
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      ksa[4 * u] = ks[u].x, ksa[4 * u + 1] = ks[u].y, ksa[4 * u + 2] = ks[u].z, ksa[4 * u + 3] = ks[u].w;
-      vsa[4 * u] = vs[u].x, vsa[4 * u + 1] = vs[u].y, vsa[4 * u + 2] = vs[u].z, vsa[4 * u + 3] = vs[u].w;
-      if (FMT == MG_KV_INT4) {
-        kza[4 * u] = kz[u].x, kza[4 * u + 1] = kz[u].y, kza[4 * u + 2] = kz[u].z, kza[4 * u + 3] = kz[u].w;
-        vza[4 * u] = vz[u].x, vza[4 * u + 1] = vz[u].y, vza[4 * u + 2] = vz[u].z, vza[4 * u + 3] = vz[u].w;
-      }
-    }
-    const bool masked = t0 + 32 > plain;  // some row may not see some key
+  // One tile; MASKED: some row may not see some key.
+  auto tile = [&](auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    const int tn = t0 + STEP;
+    const bool more = tn < kfin;
     auto key = [&](int j) { return t0 + 16 * (j >> 2) + 4 * g + (j & 3); };
-    // V scales relative to the largest seen.
-    {
-      float big = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        if (masked && key(j) >= kfin) vsa[j] = 0.f;
-        big = fmaxf(big, vsa[j]);
-      }
-      if (__any(big * vn > 16.f)) {
-        big = row_max(big);
-        for (int x = 1; x < 16; x <<= 1) big = fmaxf(big, __shfl_xor(big, x));
-        const float now = 8.f * pow2_under(big), by = now / vn;
-        vn = now;
-#pragma unroll
-        for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-          for (int i = 0; i < NB; i++) o[qb][i] *= by;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) vsa[j] *= vn;
-    }
     float4v acc[QB][2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -320,7 +398,7 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
       for (int qb = 0; qb < QB; qb++) acc[qb][u] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < KS; s++) {
-        const half8v ka = k_operand<FMT, KW>(kw[u], s);
+        const half8v ka = k_operand<FMT, KW>(t.k[u], s);
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
           acc[qb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[qb][s], acc[qb][u], 0, 0, 0);
@@ -328,12 +406,41 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
         }
       }
     }
+    if (more) {
+      t.locate(a, b, h, total, tn);
+      t.load_k(a, g, c);
+    }
+    float ksf[8], vsn[8], kzf[8], vz[8];
+    spread(ksf, t.ks, f);
+    spread(vsn, t.vs, 1.f);
+    if (FMT == MG_KV_INT4) {
+      spread(kzf, t.kz, f);
+      spread(vz, t.vz, 1.f);
+    }
+    // V scales relative to the largest seen.
+    {
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if (MASKED && key(j) >= kfin) vsn[j] = 0.f;
+        big = fmaxf(big, vsn[j]);
+      }
+      if (__builtin_expect(__any(big * vn > 16.f), 0)) {
+        const float now = 8.f * pow2_under(wave_max(big)), by = now / vn;
+        vn = now;
+#pragma unroll
+        for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+          for (int i = 0; i < NB; i++) o[qb][i] *= by;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) vsn[j] *= vn;
+    }
     half8v ph[QB], pl[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; qb++) {
-      float s[8], w[8];
       uint32_t seen = 0xff;
-      if (masked) {
+      if (MASKED) {
         seen = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -344,50 +451,75 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
           if (ok && k < kfin) seen |= 1u << j;
         }
       }
+      // Scores less `from`, -inf where not seen.
+      float d[8];
+      auto scores = [&](float from) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float x = acc[qb][j >> 2][j & 3] * f[qb];
-        s[j] = x * ksa[j];
-        if (FMT == MG_KV_INT4) s[j] = fmaf(qs[qb] * f[qb], kza[j], s[j]);
-        if (masked && !(seen >> j & 1)) s[j] = -__builtin_inff();
-      }
-      float top = s[0];
-#pragma unroll
-      for (int j = 1; j < 8; j++) top = fmaxf(top, s[j]);
-      if (__any(top > m[qb] + kSlack)) {
-        const float now = fmaxf(m[qb], row_max(top));
-        const float by = exp2f(m[qb] - now);
+        for (int j = 0; j < 8; j++) {
+          const float base = FMT == MG_KV_INT4 ? fmaf(qs[qb], kzf[j], -from) : -from;
+          d[j] = fmaf(acc[qb][j >> 2][j & 3], ksf[j], base);
+          if (MASKED) d[j] = seen >> j & 1 ? d[j] : -__builtin_inff();
+        }
+      };
+      auto top = [&]() {
+        return fmaxf(fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])),
+                     fmaxf(fmaxf(d[4], d[5]), fmaxf(d[6], d[7])));
+      };
+      scores(m[qb]);
+      if (__builtin_expect(__any(top() > kSlack), 0)) {
+        scores(0.f);
+        const float now = fmaxf(m[qb], row_max(top()));
+        const float by = exp2_of(m[qb] - now);
         m[qb] = now;
         l[qb] *= by;
         z[qb] *= by;
 #pragma unroll
         for (int i = 0; i < NB; i++) o[qb][i] *= by;
+        scores(now);
       }
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float p = exp2f(s[j] - m[qb]);
-        l[qb] += p;
-        w[j] = p * vsa[j];
-        if (FMT == MG_KV_INT4) {
-          const float pz = p * vza[j];
-          z[qb] += masked && !(seen >> j & 1) ? 0.f : pz;
+      for (int j = 0; j < 8; j += 2) {
+        const float p0 = exp2_of(d[j]), p1 = exp2_of(d[j + 1]);
+        l[qb] += p0;
+        l[qb] += p1;
+        float w0 = p0 * vsn[j], w1 = p1 * vsn[j + 1];
+        // (MASKED: 0 times a NaN that the row does not see.)
+        if (MASKED) {
+          w0 = seen >> j & 1 ? w0 : 0.f;
+          w1 = seen >> (j + 1) & 1 ? w1 : 0.f;
         }
-        if (masked && !(seen >> j & 1)) w[j] = 0.f;
-        const _Float16 hi = (_Float16)w[j];
-        ph[qb][j] = hi;
-        pl[qb][j] = (_Float16)(w[j] - (float)hi);
+        if (FMT == MG_KV_INT4) {
+          const float z0 = p0 * vz[j], z1 = p1 * vz[j + 1];
+          z[qb] += !MASKED || seen >> j & 1 ? z0 : 0.f;
+          z[qb] += !MASKED || seen >> (j + 1) & 1 ? z1 : 0.f;
+        }
+        const half2v hi = __builtin_convertvector(float2v{w0, w1}, half2v);
+        const half2v lo =
+            __builtin_convertvector(float2v{w0 - (float)hi[0], w1 - (float)hi[1]}, half2v);
+        ph[qb][j] = hi[0];
+        ph[qb][j + 1] = hi[1];
+        pl[qb][j] = lo[0];
+        pl[qb][j + 1] = lo[1];
       }
+    }
+    if (more) {
+      t.load_scales(a, g);
+      refused |= t.none[0] || t.none[1];
     }
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-      const half8v va = v_operand<FMT, KW>(vw[0], vw[1], i);
+      const half8v va = v_operand<FMT, KW>(t.v[0], t.v[1], i);
 #pragma unroll
       for (int qb = 0; qb < QB; qb++) {
         o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qb], o[qb][i], 0, 0, 0);
         o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qb], o[qb][i], 0, 0, 0);
       }
     }
-  }
+    if (more) t.load_v(a, g, c);
+    t0 = tn;
+  };
+  while (t0 < kfin && t0 + 32 <= plain) tile(std::false_type{});
+  while (t0 < kfin) tile(std::true_type{});
   if (refused && lane == 0) atomicOr(a.c.refused, 1);
   const float iv = 1.f / vn;
 #pragma unroll
@@ -395,122 +527,157 @@ __global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
     l[qb] = row_sum(l[qb]);
     z[qb] = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
   }
-  // Where a row's outputs and statistics go: y, or its partial of this split.
+  // A run of n outputs of row r0 + r from dim d, to y or to the split's partial results.
   const int64_t prow = ((int64_t)b * a.c.kv_heads + h) * a.s.max_new * a.group;
-  auto put = [&](int r, int d, float v, float mm, float ll) {
+  auto put4 = [&](int r, int d, float4 v, float ll) {
     const int row = r0 + r;
     if (row >= rows) return;
     if (a.nsplit > 1) {
-      float *p = a.part + ((prow + row) * a.nsplit + split) * part_row(DP);
-      p[d] = v;
-      if (d == 0) {
-        p[DP] = mm;
-        p[DP + 1] = ll;
-      }
-    } else if (d < a.c.d) {
-      const int qi = row / a.group, j = row - qi * a.group;
-      a.y[(sq.start + qi) * a.y_stride + (int64_t)(h * a.group + j) * a.c.d + d] =
-          ll == 0.f ? 0.f : v / ll;
+      *reinterpret_cast<float4 *>(a.part + ((prow + row) * a.nsplit + split) * DP + d) = v;
+      return;
     }
+    const int qi = row / a.group, j = row - qi * a.group;
+    float *y = a.y + (sq.start + qi) * a.y_stride + (int64_t)(h * a.group + j) * a.c.d + d;
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    if (a.vec) {
+      if (d < a.c.d) *reinterpret_cast<float4 *>(y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    } else {
+      if (d < a.c.d) y[0] = v.x * inv;
+      if (d + 1 < a.c.d) y[1] = v.y * inv;
+      if (d + 2 < a.c.d) y[2] = v.z * inv;
+      if (d + 3 < a.c.d) y[3] = v.w * inv;
+    }
+  };
+  auto put_stat = [&](int r, float mm, float ll) {
+    if (r0 + r < rows && a.nsplit > 1)
+      a.part_ml[(prow + r0 + r) * a.nsplit + split] = make_float2(mm, ll);
   };
   if (KEYS) {
     // The four waves' results of the same rows, joined.
     if (g == 0) {
-#pragma unroll
-      for (int qb = 0; qb < QB; qb++) {
-        stat[wave][0][qb * 16 + c] = m[qb];
-        stat[wave][1][qb * 16 + c] = l[qb];
-      }
+      stat[wave][0][c] = m[0];
+      stat[wave][1][c] = l[0];
     }
     __syncthreads();
+    const float all = fmaxf(fmaxf(stat[0][0][c], stat[1][0][c]), fmaxf(stat[2][0][c], stat[3][0][c]));
+    const float by = exp2_of(m[0] - all);
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      const int r = qb * 16 + c;
-      const float all = fmaxf(fmaxf(stat[0][0][r], stat[1][0][r]), fmaxf(stat[2][0][r], stat[3][0][r]));
-      const float by = exp2f(m[qb] - all);
+    for (int e = 0; e < 4; e++)
 #pragma unroll
-      for (int i = 0; i < NB; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          lds[(wave * 16 + r) * QP + NB * (4 * g + e) + i] = (o[qb][i][e] * iv + z[qb]) * by;
-    }
+      for (int i = 0; i < NB; i += 4)
+        *reinterpret_cast<float4 *>(lds + (wave * 16 + c) * QP + NB * (4 * g + e) + i) =
+            make_float4((o[0][i][e] * iv + z[0]) * by, (o[0][i + 1][e] * iv + z[0]) * by,
+                        (o[0][i + 2][e] * iv + z[0]) * by, (o[0][i + 3][e] * iv + z[0]) * by);
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * DP; i += 256) {
-      const int r = i / DP, d = i - r * DP;
-      float all = stat[0][0][r], ll = 0.f, v = 0.f;
+    for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
+      const int r = i / (DP / 4), d = 4 * (i - r * (DP / 4));
+      float mm = stat[0][0][r], ll = 0.f;
 #pragma unroll
-      for (int w = 1; w < 4; w++) all = fmaxf(all, stat[w][0][r]);
+      for (int w = 1; w < 4; w++) mm = fmaxf(mm, stat[w][0][r]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        ll += stat[w][1][r] * exp2f(stat[w][0][r] - all);
-        v += lds[(w * 16 + r) * QP + d];
+        ll += stat[w][1][r] * exp2_of(stat[w][0][r] - mm);
+        const float4 x = *reinterpret_cast<const float4 *>(lds + (w * 16 + r) * QP + d);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
       }
-      put(r, d, v, all, ll);
+      put4(r, d, v, ll);
+      if (d == 0) put_stat(r, mm, ll);
     }
   } else {
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++)
+    for (int qb = 0; qb < QB; qb++) {
+      const int r = wr0 + qb * 16 + c;
 #pragma unroll
-      for (int i = 0; i < NB; i++)
+      for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          put(wr0 + qb * 16 + c, NB * (4 * g + e) + i, o[qb][i][e] * iv + z[qb], m[qb], l[qb]);
+        for (int i = 0; i < NB; i += 4)
+          put4(r, NB * (4 * g + e) + i,
+               make_float4(o[qb][i][e] * iv + z[qb], o[qb][i + 1][e] * iv + z[qb],
+                           o[qb][i + 2][e] * iv + z[qb], o[qb][i + 3][e] * iv + z[qb]),
+               l[qb]);
+      if (g == 0) put_stat(r, m[qb], l[qb]);
+    }
   }
 }
 
-// Joins a row's splits: one wave a row.
+// Joins a row's splits, a workgroup a row: LP lanes take four dims each, 256 / LP groups of
+// them take splits in turn.
+template <int LP>
 __global__ __launch_bounds__(256) void k_kv_join(const mg_kv_attn a) {
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t per = a.s.max_new * a.group;  // rows of a (sequence, KV head)
-  const int64_t at = (int64_t)blockIdx.x * 4 + wave;
-  const int64_t bh = at / per;
-  const int row = (int)(at - bh * per);
-  const int b = (int)(bh / a.c.kv_heads), h = (int)(bh - (int64_t)b * a.c.kv_heads);
-  if (b >= a.s.batch) return;
+  constexpr int G = 256 / LP;
+  __shared__ float4 sum[256];
+  __shared__ float sl[G];
+  const int per = (int)a.s.max_new * a.group;  // rows of a (sequence, KV head)
+  const int64_t at = blockIdx.x;
+  const int bh = (int)(at / per), row = (int)(at - (int64_t)bh * per);
+  const int b = bh / a.c.kv_heads, h = bh - b * a.c.kv_heads;
   const kv_seq sq = kv_sequence(a.s, b);
   if (sq.bad || row >= sq.n * a.group) return;
   const int last = min((row / a.rows_wg + 1) * a.rows_wg, sq.n * a.group) - 1;
   const int kend = a.tree ? sq.past + sq.n : sq.past + last / a.group + 1;
   const int n = max(1, min(a.nsplit, (kend + a.kc - 1) / a.kc));
-  const int dp = a.c.dp, pr = part_row(dp);
-  const float *p = a.part + at * a.nsplit * pr;
+  const int dp = a.c.dp, grp = threadIdx.x / LP, d = 4 * (threadIdx.x % LP);
+  const float2 *ml = a.part_ml + at * a.nsplit;
+  const float *p = a.part + at * a.nsplit * dp + d;
+  // (Each wave finds the maximum for itself.)
   float all = kNoMax;
-  for (int i = lane; i < n; i += 64) all = fmaxf(all, p[(int64_t)i * pr + dp]);
-#pragma unroll
-  for (int x = 32; x; x >>= 1) all = fmaxf(all, __shfl_xor(all, x));
-  float v[4] = {}, l = 0.f;
-  for (int i = 0; i < n; i++) {
-    const float *q = p + (int64_t)i * pr;
-    const float by = exp2f(q[dp] - all);
-    l += q[dp + 1] * by;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (lane + 64 * e < dp) v[e] += q[lane + 64 * e] * by;
+  for (int i = threadIdx.x & 63; i < n; i += 64) all = fmaxf(all, ml[i].x);
+  all = wave_max(all);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  if (d < dp) {
+#pragma unroll 4
+    for (int i = grp; i < n; i += G) {
+      const float2 s = ml[i];
+      const float4 x = *reinterpret_cast<const float4 *>(p + (int64_t)i * dp);
+      const float by = exp2_of(s.x - all);
+      l += s.y * by;
+      v.x += x.x * by;
+      v.y += x.y * by;
+      v.z += x.z * by;
+      v.w += x.w * by;
+    }
   }
+  sum[threadIdx.x] = v;
+  if (threadIdx.x % LP == 0) sl[grp] = l;
+  __syncthreads();
+  if (threadIdx.x >= LP || d >= a.c.d) return;
+  for (int i = 1; i < G; i++) {
+    const float4 x = sum[i * LP + threadIdx.x];
+    v.x += x.x;
+    v.y += x.y;
+    v.z += x.z;
+    v.w += x.w;
+    l = i == 1 ? sl[0] + sl[1] : l + sl[i];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int qi = row / a.group, j = row - qi * a.group;
-  float *y = a.y + (sq.start + qi) * a.y_stride + (int64_t)(h * a.group + j) * a.c.d;
-#pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (lane + 64 * e < a.c.d) y[lane + 64 * e] = l == 0.f ? 0.f : v[e] / l;
+  float *y = a.y + (sq.start + qi) * a.y_stride + (int64_t)(h * a.group + j) * a.c.d + d;
+  y[0] = v.x * inv;
+  if (d + 1 < a.c.d) y[1] = v.y * inv;
+  if (d + 2 < a.c.d) y[2] = v.z * inv;
+  if (d + 3 < a.c.d) y[3] = v.w * inv;
 }
 
 template <int FMT, int NB>
-mg_status launch(mg_ctx *ctx, const mg_kv_attn &a) {
+void launch(mg_ctx *ctx, const mg_kv_attn &a) {
   const dim3 grid((unsigned)(a.s.batch * a.nsplit * a.nblk * a.c.kv_heads));
-  constexpr int QB = NB > 8 ? 1 : 2;
   hipStream_t st = ctx->stream;
-  if (a.mode == 0)
+  if (a.keys) {
     k_kv_attn<FMT, NB, 1, true><<<grid, dim3(256), 0, st>>>(a);
-  else if (a.mode == 1)
+  } else if (a.rows_wg == 64) {
     k_kv_attn<FMT, NB, 1, false><<<grid, dim3(256), 0, st>>>(a);
-  else
-    k_kv_attn<FMT, NB, QB, false><<<grid, dim3(256), 0, st>>>(a);
-  return mg_launch_check("KV cache attention");
+  } else if constexpr (NB <= 8) {
+    k_kv_attn<FMT, NB, 2, false><<<grid, dim3(256), 0, st>>>(a);
+  }
 }
 
 template <int FMT>
-mg_status launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
+void launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
   switch (a.c.dp / 64) {
     case 1: return launch<FMT, 4>(ctx, a);
     case 2: return launch<FMT, 8>(ctx, a);
@@ -522,30 +689,49 @@ mg_status launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
 }  // namespace
 
 size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
-  const int64_t rows = a->s.max_new * a->group;
-  const int qb = a->c.dp > 128 ? 1 : 2;
-  a->mode = rows <= 16 ? 0 : rows <= 64 || qb == 1 ? 1 : 2;
-  a->rows_wg = a->mode == 0 ? 16 : a->mode == 1 ? 64 : 64 * qb;
+  const int64_t rows = a->s.max_new * a->group, heads = a->s.batch * a->c.kv_heads;
+  const int64_t most = std::max<int64_t>(1, (a->s.max_len + 127) / 128);  // splits of 128 keys
+  a->keys = rows <= 16;
+  // Rows a workgroup: more rows share a key's conversion, fewer fill the card.
+  a->rows_wg = 16;
+  if (!a->keys) {
+    a->rows_wg = a->c.dp <= 128 ? 128 : 64;
+    while (a->rows_wg > 64 && (rows <= a->rows_wg / 2 ||
+                               heads * ((rows + a->rows_wg - 1) / a->rows_wg) * most < 2 * ctx->num_cus))
+      a->rows_wg /= 2;
+  }
   a->nblk = (int)((rows + a->rows_wg - 1) / a->rows_wg);
-  // Key splits: enough workgroups for two a compute unit, 128 keys a split at least.
-  const int64_t base = a->s.batch * a->nblk * a->c.kv_heads;
-  const int64_t want = split ? std::max<int64_t>(1, 4 * ctx->num_cus / base) : 1;
+  // Key splits: enough workgroups for the card, 128 keys a split at least.
+  const int64_t base = heads * a->nblk;
+  const int64_t want =
+      split && base < 2 * ctx->num_cus ? std::max<int64_t>(1, 4 * ctx->num_cus / base) : 1;
   int64_t kc = (a->s.max_len + want - 1) / want;
   kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
   a->nsplit = (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
   a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
-  if (a->nsplit == 1) return 0;
-  return (size_t)(a->s.batch * a->c.kv_heads * rows * a->nsplit) * part_row(a->c.dp) * 4;
+  a->parts = heads * rows * a->nsplit;
+  return a->nsplit == 1 ? 0 : (size_t)a->parts * (a->c.dp * 4 + sizeof(float2));
 }
 
-mg_status mg_kv_attn_run(mg_ctx *ctx, const mg_kv_attn &a) {
+mg_status mg_kv_attn_run(mg_ctx *ctx, mg_kv_attn a, void *ws) {
+  a.part = static_cast<float *>(ws);
+  a.part_ml = reinterpret_cast<float2 *>(a.part + a.parts * a.c.dp);
+  const auto odd = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  a.vec = a.c.d % 4 == 0 && a.q_stride % 4 == 0 && a.y_stride % 4 == 0 && !odd(a.q) && !odd(a.y) &&
+          a.rope.half_rot % 4 == 0 && !odd(a.rope.cos_table) && !odd(a.rope.sin_table);
   switch (a.c.fmt) {
-    case MG_KV_INT8: MG_TRY(launch_dims<MG_KV_INT8>(ctx, a)); break;
-    case MG_KV_E4M3: MG_TRY(launch_dims<MG_KV_E4M3>(ctx, a)); break;
-    default: MG_TRY(launch_dims<MG_KV_INT4>(ctx, a)); break;
+    case MG_KV_INT8: launch_dims<MG_KV_INT8>(ctx, a); break;
+    case MG_KV_E4M3: launch_dims<MG_KV_E4M3>(ctx, a); break;
+    default: launch_dims<MG_KV_INT4>(ctx, a); break;
   }
+  MG_TRY(mg_launch_check("KV cache attention"));
   if (a.nsplit == 1) return MG_OK;
-  const int64_t rows = a.s.batch * a.c.kv_heads * a.s.max_new * a.group;
-  k_kv_join<<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, ctx->stream>>>(a);
+  const dim3 rows((unsigned)(a.s.batch * a.c.kv_heads * a.s.max_new * a.group));
+  if (a.c.dp == 64)
+    k_kv_join<16><<<rows, dim3(256), 0, ctx->stream>>>(a);
+  else if (a.c.dp == 128)
+    k_kv_join<32><<<rows, dim3(256), 0, ctx->stream>>>(a);
+  else
+    k_kv_join<64><<<rows, dim3(256), 0, ctx->stream>>>(a);
   return mg_launch_check("KV cache attention, join");
 }
