@@ -282,7 +282,7 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
 
 // KEYS: the four waves take tiles in turn for the same 16 rows; else rows of their own.
 template <int FMT, int NB, int QB, bool KEYS>
-__global__ __launch_bounds__(256) void k_kv_attn(const mg_kv_attn a) {
+__global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, KW = S::KW;
   constexpr int ROWS = 16 * QB * (KEYS ? 1 : 4);  // rows of the workgroup
