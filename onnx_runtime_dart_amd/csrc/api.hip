@@ -2998,8 +2998,8 @@ mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_
   ProfScope prof_(ctx, what);
   g_last_error.clear();
   if (!ctx) return bad_arg(what, "null context");
-  if (rows < 0 || rows > 0x7fffff || vocab < 1 || vocab > 0x7ffff800)
-    return bad_arg(what, "rows must be 0 .. 2^23 - 1 and vocab 1 .. 2^31 - 2048");
+  if (rows < 0 || rows > 0x7fffff || vocab < 1 || vocab > 0x7fffd000)
+    return bad_arg(what, "rows must be 0 .. 2^23 - 1 and vocab 1 .. 2^31 - 12288");
   if (top < 0 || top > MG_LOGPROBS_MAX_TOP || top > vocab)
     return bad_arg(what, "top must be 0 .. 64, at most vocab");
   MG_TRY(check_stride(what, &row_stride, vocab));

@@ -56,21 +56,37 @@ __device__ inline Sums moved(const Sums &x, float m) {
   return Sums{m, x.s * e, (x.a + (double)d * x.s) * e};
 }
 
-__device__ inline float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+// x of another lane by a register move (0 where there is none; rows: those that take part).
+template <int CTRL, int ROWS = 0xf>
+__device__ inline uint32_t moved_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true);
 }
-__device__ inline double wave_sum(double x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// Over the wave: within rows of 16 lanes, then across them (0x142, 0x143: a row's last lane to
+// the next row's, the second row's to the last two); lane 63 has it all.
+__device__ inline uint32_t wave_max(uint32_t x) {
+  x = max(x, moved_lane<0x111>(x));
+  x = max(x, moved_lane<0x112>(x));
+  x = max(x, moved_lane<0x114>(x));
+  x = max(x, moved_lane<0x118>(x));
+  x = max(x, moved_lane<0x142>(x));
+  x = max(x, moved_lane<0x143>(x));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
-__device__ inline Sums wave_join(const Sums &x) {
-  Sums r = moved(x, wave_max(x.m));
-  r.s = wave_sum(r.s);
-  r.a = wave_sum(r.a);
-  return r;
+__device__ inline float wave_sum(float x) {
+  auto with = [&](uint32_t y) { x += __uint_as_float(y); };
+  with(moved_lane<0x111>(__float_as_uint(x)));
+  with(moved_lane<0x112>(__float_as_uint(x)));
+  with(moved_lane<0x114>(__float_as_uint(x)));
+  with(moved_lane<0x118>(__float_as_uint(x)));
+  with(moved_lane<0x142, 0xa>(__float_as_uint(x)));
+  with(moved_lane<0x143, 0xc>(__float_as_uint(x)));
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+// A wave's sums from its lanes' (of at most 64 fp32 terms each way).
+__device__ inline Sums wave_join(float m, float s, float a) {
+  const float all = of_key(wave_max(key_of(m)));
+  const float d = fmaxf(m - all, -200.f), e = m == all ? 1.f : exp_of(d);
+  return Sums{all, (double)wave_sum(s * e), (double)wave_sum((a + d * s) * e)};
 }
 
 // The value of lane l - 1 (lane 0: any).
@@ -112,34 +128,36 @@ __device__ inline void offer(List &l, uint32_t key, int id, bool ok, int top, in
     want &= __ballot(beats(key, id, l.tk, l.ti));
   }
 }
-// The n-th largest (from 0) of the lanes' keys.
-__device__ inline uint32_t nth_largest(uint32_t x, int n, int lane) {
+// A bound from below of the n-th largest (from 1) of the lanes' keys, exact to its upper half: the
+// largest number with zeros in its lower half that n of them reach.
+__device__ inline uint32_t nth_largest(uint32_t x, int n) {
+  uint32_t least = 0;
 #pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j; j >>= 1) {
-      const uint32_t y = __shfl_xor(x, j);
-      const bool larger = ((lane & j) == 0) == ((lane & k) == 0);  // descending
-      x = larger ? max(x, y) : min(x, y);
-    }
-  return lane_value(x, n);
+  for (int b = 31; b >= 16; b--) {
+    const uint32_t t = least | 1u << b;
+    if (__popcll(__ballot(x >= t)) >= n) least = t;
+  }
+  return least;
 }
 
 // Joins up to 64 sorted lists of `top` entries, lane l's at key[l * pitch], id[l * pitch]
-// (n of them): lane j gets the j-th entry of all.
+// (n of them): lane j gets the j-th entry of all.  Each lane holds its list's next two.
 __device__ inline void join_lists(const uint32_t *key, const int *id, int pitch, int n, int top,
                                   int lane, uint32_t &ok, int &oi) {
-  int at = 0;
-  uint32_t k = 0;
-  int i = 0x7fffffff;
-  if (lane < n) {
+  int at = 1;
+  uint32_t k = 0, k1 = 0;
+  int i = 0x7fffffff, i1 = 0x7fffffff;
+  const bool mine = lane < n;
+  if (mine) {
     k = key[lane * pitch];
     i = id[lane * pitch];
+    if (top > 1) {
+      k1 = key[lane * pitch + 1];
+      i1 = id[lane * pitch + 1];
+    }
   }
   for (int j = 0; j < top; j++) {
-    uint32_t bk = k;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) bk = max(bk, __shfl_xor(bk, o));
+    const uint32_t bk = wave_max(k);
     // The lowest token of those with the largest key.
     uint64_t who = __ballot(k == bk);
     int l = __builtin_ctzll(who);
@@ -156,25 +174,28 @@ __device__ inline void join_lists(const uint32_t *key, const int *id, int pitch,
       oi = bi;
     }
     if (lane == l) {
+      k = k1;
+      i = i1;
       at++;
-      k = at < top ? key[lane * pitch + at] : 0;
-      i = at < top ? id[lane * pitch + at] : 0x7fffffff;
+      const bool more = mine && at < top;
+      k1 = more ? key[lane * pitch + at] : 0;
+      i1 = more ? id[lane * pitch + at] : 0x7fffffff;
     }
   }
 }
 
+// The logit of the row's given token (NaN: none), asked for early by the wave that finishes.
+__device__ inline float given(const mg_logprobs &p, int64_t row) {
+  if (!p.logprob) return 0.f;
+  const int tok = p.tokens[row];
+  return tok < 0 || tok >= p.vocab ? __builtin_nanf("") : p.x[row * p.stride + tok];
+}
 // The row's results, by one wave that holds its sums and list.
 __device__ inline void finish(const mg_logprobs &p, int64_t row, const Sums &t, uint32_t lk, int li,
-                              int lane) {
+                              float xt, int lane) {
   const double lz = t.s > 0 ? log(t.s) : __builtin_nan("");
   if (lane == 0) {
-    if (p.logprob) {
-      const int tok = p.tokens[row];
-      p.logprob[row] =
-          tok < 0 || tok >= p.vocab
-              ? __builtin_nanf("")
-              : (float)((double)p.x[row * p.stride + tok] - (double)t.m - lz);
-    }
+    if (p.logprob) p.logprob[row] = (float)((double)xt - (double)t.m - lz);
     if (p.entropy) p.entropy[row] = (float)(lz - t.a / t.s);
   }
   if (lane < p.top) {
@@ -201,6 +222,7 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   // (64 bits: a vocabulary may come near 2^31.)
   const int64_t end = (int64_t)p.vocab + off;
   const int64_t e0 = (int64_t)split * p.run, e1 = min(end, e0 + p.run);
+  const float xt = wave == 0 && p.nsplit == 1 ? given(p, row) : 0.f;
   float m = kLowest, s = 0.f, a = 0.f;
   List l{0, 0, 0x7fffffff, 0x7fffffff};
   bool first = true;
@@ -251,7 +273,7 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
       if (odd) bk = 0xffffffffu;
       uint32_t least = l.tk;
       if (first) {
-        least = max(least, nth_largest(bk, p.top - 1, lane));
+        least = max(least, nth_largest(bk, p.top));
         first = false;
       }
       if (__any(bk >= least)) {
@@ -266,7 +288,7 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
       }
     }
   }
-  Sums t = wave_join(Sums{m, (double)s, (double)a});
+  Sums t = wave_join(m, s, a);
   __shared__ Sums st[4];
   __shared__ uint32_t sk[4 * 64];
   __shared__ int si[4 * 64];
@@ -291,7 +313,7 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   int li = 0x7fffffff;
   if (TOP) join_lists(sk, si, 64, 4, p.top, lane, lk, li);
   if (p.nsplit == 1) {
-    finish(p, row, t, lk, li, lane);
+    finish(p, row, t, lk, li, xt, lane);
     return;
   }
   mg_logprobs_part &o = p.part[blockIdx.x];
@@ -306,27 +328,42 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   }
 }
 
-// Joins the at most 64 runs of a row.
-__global__ __launch_bounds__(64) void k_logprobs_join(const mg_logprobs p) {
+// Joins the at most 64 runs of a row: four waves fetch the lists, one joins them.
+__global__ __launch_bounds__(256) void k_logprobs_join(const mg_logprobs p) {
   constexpr int T = MG_LOGPROBS_MAX_TOP, PITCH = T + 1;
   __shared__ uint32_t sk[64 * PITCH];
   __shared__ int si[64 * PITCH];
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const bool last = threadIdx.x < 64;
   const int64_t row = blockIdx.x;
   const mg_logprobs_part *o = p.part + row * p.nsplit;
-  for (int e = lane; e < p.nsplit * p.top; e += 64) {
-    const int r = e / p.top, j = e - r * p.top;
-    sk[r * PITCH + j] = o[r].key[j];
-    si[r * PITCH + j] = o[r].id[j];
-  }
+  float xt = 0.f;
   Sums t{kLowest, 0, 0};
-  if (lane < p.nsplit) t = Sums{o[lane].m, o[lane].s, o[lane].a};
-  t = wave_join(t);
+  if (last) {
+    xt = given(p, row);
+    if (lane < p.nsplit) t = Sums{o[lane].m, o[lane].s, o[lane].a};
+  }
+#pragma unroll 4
+  for (int e = threadIdx.x; e < p.nsplit * T; e += 256) {
+    const int r = e / T, j = e % T;
+    if (j < p.top) {
+      sk[r * PITCH + j] = o[r].key[j];
+      si[r * PITCH + j] = o[r].id[j];
+    }
+  }
   __syncthreads();
+  if (!last) return;
+  // (64 bits: the runs' sums may differ by far in size and number.)
+  t = moved(t, of_key(wave_max(key_of(t.m))));
+#pragma unroll
+  for (int w = 32; w; w >>= 1) {
+    t.s += __shfl_xor(t.s, w);
+    t.a += __shfl_xor(t.a, w);
+  }
   uint32_t lk = 0;
   int li = 0x7fffffff;
   if (p.top) join_lists(sk, si, PITCH, p.nsplit, p.top, lane, lk, li);
-  finish(p, row, t, lk, li, lane);
+  finish(p, row, t, lk, li, xt, lane);
 }
 
 }  // namespace
@@ -336,9 +373,10 @@ size_t mg_logprobs_plan(const mg_ctx *ctx, mg_logprobs *p, bool split) {
   // row (one lane each where they join).
   int64_t n = 1;
   if (split && p->rows < ctx->num_cus)
-    n = std::min<int64_t>({ctx->num_cus / p->rows, (p->vocab + 4 * kChunk - 1) / (4 * kChunk), 64});
-  p->run = (int)std::min<int64_t>(((p->vocab + 3 + n - 1) / n + kChunk - 1) / kChunk * kChunk,
-                                  0x7ffffc00);
+    n = std::min<int64_t>({2 * ctx->num_cus / p->rows, (p->vocab + 4 * kChunk - 1) / (4 * kChunk), 64});
+  // (Whole chunks of every wave.)
+  p->run = (int)std::min<int64_t>(((p->vocab + 3 + n - 1) / n + 4 * kChunk - 1) / (4 * kChunk) *
+                                      (4 * kChunk), 0x7fffe000);
   p->nsplit = (int)(((int64_t)p->vocab + 3 + p->run - 1) / p->run);
   return p->nsplit > 1 ? (size_t)p->rows * p->nsplit * sizeof(mg_logprobs_part) : 0;
 }
@@ -351,6 +389,6 @@ mg_status mg_logprobs_run(mg_ctx *ctx, const mg_logprobs &p) {
     k_logprobs<false><<<grid, dim3(256), 0, ctx->stream>>>(p);
   MG_TRY(mg_launch_check("log probabilities"));
   if (p.nsplit == 1) return MG_OK;
-  k_logprobs_join<<<dim3((unsigned)p.rows), dim3(64), 0, ctx->stream>>>(p);
+  k_logprobs_join<<<dim3((unsigned)p.rows), dim3(256), 0, ctx->stream>>>(p);
   return mg_launch_check("log probabilities, join");
 }
