@@ -153,23 +153,28 @@ struct Shape {
 };
 
 // A tile of 32 keys: where its two runs of 16 lie, and the lane's codes and scales.  The
-// parts are loaded apart, each as soon as the last tile's are used.
+// parts are loaded apart.
 template <int FMT, int NB>
 struct Tile {
   using S = Shape<FMT, NB>;
-  int64_t at[2];  // (page, head) times page size plus place
-  int64_t ph[2];  // (page, head)
-  bool none[2];   // no such page: its keys read as NaN
+  int64_t page[2];  // of the tile to be loaded, -1: none
+  int64_t at[2];    // (page, head) times page size plus place
+  int64_t ph[2];    // (page, head)
+  bool none[2];     // no such page: its keys read as NaN
   uint32_t k[2][S::KW], v[2][S::KW];
   float4 ks[2], vs[2], kz[2], vz[2];
 
-  __device__ inline void locate(const mg_kv_attn &a, int b, int h, int total, int t0) {
+  __device__ inline void look_up(const mg_kv_attn &a, int b, int total, int t0) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      page[u] = t0 + 16 * u < total ? kv_page(a.s, b, t0 + 16 * u, a.c.plog, a.c.pages) : 0;
+  }
+  __device__ inline void locate(const mg_kv_attn &a, int h, int t0) {
     const int psize = 1 << a.c.plog;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const int64_t p = t0 + 16 * u < total ? kv_page(a.s, b, t0 + 16 * u, a.c.plog, a.c.pages) : 0;
-      none[u] = p < 0;
-      ph[u] = (p < 0 ? 0 : p) * a.c.kv_heads + h;
+      none[u] = page[u] < 0;
+      ph[u] = (page[u] < 0 ? 0 : page[u]) * a.c.kv_heads + h;
       at[u] = (ph[u] << a.c.plog) + ((t0 + 16 * u) & (psize - 1));
     }
   }
@@ -280,16 +285,15 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
   }
 }
 
-// KEYS: the four waves take tiles in turn for the same 16 rows; else rows of their own.
+// KEYS: the four waves take tiles in turn for the same rows; else rows of their own.
 template <int FMT, int NB, int QB, bool KEYS>
 __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, KW = S::KW;
   constexpr int ROWS = 16 * QB * (KEYS ? 1 : 4);  // rows of the workgroup
   constexpr int QP = DP + 4;
-  static_assert(!KEYS || QB == 1, "the waves' results take the place of 64 rows");
   // The rows' queries; later (KEYS) the four waves' results.
-  __shared__ __attribute__((aligned(16))) float lds[(KEYS ? 64 : ROWS) * QP];
+  __shared__ __attribute__((aligned(16))) float lds[64 * QB * QP];
   __shared__ float stat[4][2][16 * QB];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -321,16 +325,21 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
   const int kfin = min(wend, kend - kbeg > a.kc ? kbeg + a.kc : kend);
   const int plain = a.tree ? sq.past : sq.past + min(r0 + wr0, rows - 1) / a.group + 1;
   constexpr int STEP = KEYS ? 128 : 32;
+  // With registers to spare the next tile's loads start before this one's products, else each
+  // part's as soon as this one's is used.
+  constexpr bool AHEAD = QB == 1 && NB <= 8;
   int t0 = kbeg + (KEYS ? 32 * wave : 0);
   // The first tile's loads run while the queries are made.
-  Tile<FMT, NB> t;
+  Tile<FMT, NB> t, next;
   bool refused = false;
   if (t0 < kfin) {
-    t.locate(a, b, h, total, t0);
+    t.look_up(a, b, total, t0);
+    t.locate(a, h, t0);
     t.load_k(a, g, c);
     t.load_scales(a, g);
     t.load_v(a, g, c);
     refused = t.none[0] || t.none[1];
+    next.look_up(a, b, total, t0 + STEP);
   }
 
   stage_queries<DP>(a, sq, h, r0, rows, ROWS, lds);
@@ -390,6 +399,14 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
     constexpr bool MASKED = decltype(masked_tag)::value;
     const int tn = t0 + STEP;
     const bool more = tn < kfin;
+    if (AHEAD && more) {
+      next.locate(a, h, tn);
+      next.load_k(a, g, c);
+      next.load_scales(a, g);
+      next.load_v(a, g, c);
+      refused |= next.none[0] || next.none[1];
+      next.look_up(a, b, total, tn + STEP);
+    }
     auto key = [&](int j) { return t0 + 16 * (j >> 2) + 4 * g + (j & 3); };
     float4v acc[QB][2];
 #pragma unroll
@@ -406,9 +423,10 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
         }
       }
     }
-    if (more) {
-      t.locate(a, b, h, total, tn);
-      t.load_k(a, g, c);
+    if (!AHEAD && more) {
+      next.locate(a, h, tn);
+      next.load_k(a, g, c);
+      next.look_up(a, b, total, tn + STEP);
     }
     float ksf[8], vsn[8], kzf[8], vz[8];
     spread(ksf, t.ks, f);
@@ -502,9 +520,9 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
         pl[qb][j + 1] = lo[1];
       }
     }
-    if (more) {
-      t.load_scales(a, g);
-      refused |= t.none[0] || t.none[1];
+    if (!AHEAD && more) {
+      next.load_scales(a, g);
+      refused |= next.none[0] || next.none[1];
     }
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -515,7 +533,8 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
         o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qb], o[qb][i], 0, 0, 0);
       }
     }
-    if (more) t.load_v(a, g, c);
+    if (!AHEAD && more) next.load_v(a, g, c);
+    t = next;
     t0 = tn;
   };
   while (t0 < kfin && t0 + 32 <= plain) tile(std::false_type{});
@@ -555,21 +574,29 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
   if (KEYS) {
     // The four waves' results of the same rows, joined.
     if (g == 0) {
-      stat[wave][0][c] = m[0];
-      stat[wave][1][c] = l[0];
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++) {
+        stat[wave][0][qb * 16 + c] = m[qb];
+        stat[wave][1][qb * 16 + c] = l[qb];
+      }
     }
     __syncthreads();
-    const float all = fmaxf(fmaxf(stat[0][0][c], stat[1][0][c]), fmaxf(stat[2][0][c], stat[3][0][c]));
-    const float by = exp2_of(m[0] - all);
 #pragma unroll
-    for (int e = 0; e < 4; e++)
+    for (int qb = 0; qb < QB; qb++) {
+      const int r = qb * 16 + c;
+      const float all =
+          fmaxf(fmaxf(stat[0][0][r], stat[1][0][r]), fmaxf(stat[2][0][r], stat[3][0][r]));
+      const float by = exp2_of(m[qb] - all);
 #pragma unroll
-      for (int i = 0; i < NB; i += 4)
-        *reinterpret_cast<float4 *>(lds + (wave * 16 + c) * QP + NB * (4 * g + e) + i) =
-            make_float4((o[0][i][e] * iv + z[0]) * by, (o[0][i + 1][e] * iv + z[0]) * by,
-                        (o[0][i + 2][e] * iv + z[0]) * by, (o[0][i + 3][e] * iv + z[0]) * by);
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int i = 0; i < NB; i += 4)
+          *reinterpret_cast<float4 *>(lds + (wave * ROWS + r) * QP + NB * (4 * g + e) + i) =
+              make_float4((o[qb][i][e] * iv + z[qb]) * by, (o[qb][i + 1][e] * iv + z[qb]) * by,
+                          (o[qb][i + 2][e] * iv + z[qb]) * by, (o[qb][i + 3][e] * iv + z[qb]) * by);
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
+    for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
       const int r = i / (DP / 4), d = 4 * (i - r * (DP / 4));
       float mm = stat[0][0][r], ll = 0.f;
 #pragma unroll
@@ -578,7 +605,7 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
 #pragma unroll
       for (int w = 0; w < 4; w++) {
         ll += stat[w][1][r] * exp2_of(stat[w][0][r] - mm);
-        const float4 x = *reinterpret_cast<const float4 *>(lds + (w * 16 + r) * QP + d);
+        const float4 x = *reinterpret_cast<const float4 *>(lds + (w * ROWS + r) * QP + d);
         v.x += x.x;
         v.y += x.y;
         v.z += x.z;
@@ -690,24 +717,22 @@ void launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
 
 size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
   const int64_t rows = a->s.max_new * a->group, heads = a->s.batch * a->c.kv_heads;
-  const int64_t most = std::max<int64_t>(1, (a->s.max_len + 127) / 128);  // splits of 128 keys
-  a->keys = rows <= 16;
-  // Rows a workgroup: more rows share a key's conversion, fewer fill the card.
-  a->rows_wg = 16;
-  if (!a->keys) {
-    a->rows_wg = a->c.dp <= 128 ? 128 : 64;
-    while (a->rows_wg > 64 && (rows <= a->rows_wg / 2 ||
-                               heads * ((rows + a->rows_wg - 1) / a->rows_wg) * most < 2 * ctx->num_cus))
-      a->rows_wg /= 2;
-  }
+  // Workgroups that run at once, two a compute unit: more start late, and a start (lengths,
+  // pages, queries) costs what some ten tiles do.
+  const int64_t room = 2 * ctx->num_cus;
+  a->rows_wg = a->c.dp <= 128 ? 128 : 64;
+  if (rows <= a->rows_wg / 2) a->rows_wg = 64;
+  a->keys = rows <= 16 || (rows <= 256 && heads * ((rows + 15) / 16) <= room / 2);
+  if (a->keys) a->rows_wg = 16;
   a->nblk = (int)((rows + a->rows_wg - 1) / a->rows_wg);
-  // Key splits: enough workgroups for the card, 128 keys a split at least.
+  // Key splits to fill the room, 128 keys each at least; none for sequences of up to 512, which
+  // cost less than the join.
   const int64_t base = heads * a->nblk;
-  const int64_t want =
-      split && base < 2 * ctx->num_cus ? std::max<int64_t>(1, 4 * ctx->num_cus / base) : 1;
+  const int64_t want = split && a->s.max_len > 512 ? std::max<int64_t>(1, room / base) : 1;
   int64_t kc = (a->s.max_len + want - 1) / want;
   kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
   a->nsplit = (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
+  if (want == 1) a->nsplit = 1;
   a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
   a->parts = heads * rows * a->nsplit;
   return a->nsplit == 1 ? 0 : (size_t)a->parts * (a->c.dp * 4 + sizeof(float2));
