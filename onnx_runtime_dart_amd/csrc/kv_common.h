@@ -28,6 +28,13 @@ struct mg_kv_cache {
 __host__ __device__ inline int kv_bits(int fmt) { return fmt == MG_KV_INT4 ? 4 : 8; }
 __host__ __device__ inline int kv_scales(int fmt) { return fmt == MG_KV_INT4 ? 4 : 2; }
 
+// What all lanes read alike and no kernel that reads it so writes: a scalar load, which other
+// loads in flight need not be waited for with.
+template <class T>
+__device__ inline T kv_scalar(const T *p) {
+  return *(const __attribute__((address_space(4))) T *)p;
+}
+
 // Sequence b's rows [start, start + n) at positions past ..; n = 0 with bad set when a
 // number breaks the batch's bounds.
 struct kv_seq {

@@ -58,6 +58,11 @@ __device__ inline half2v nib2(uint32_t w, int i) {
   const half2v off = {(_Float16)1039.f, (_Float16)1039.f};
   return __builtin_bit_cast(half2v, (x & 0x001e001eu) | 0x64006400u) - off;
 }
+__device__ inline half2v nib2_any(uint32_t w, int i) {
+  const uint32_t x = (uint32_t)(((uint64_t)w << 1) >> (4 * i));
+  const half2v off = {(_Float16)1039.f, (_Float16)1039.f};
+  return __builtin_bit_cast(half2v, (x & 0x001e001eu) | 0x64006400u) - off;
+}
 __device__ inline half8v join4(half2v a, half2v b, half2v c, half2v d) {
   half8v r;
   r[0] = a[0];
@@ -143,6 +148,13 @@ __device__ inline float pow2_under(float x) {
   const int e = (int)(__float_as_uint(x) >> 23 & 255u);
   return x == 0.f ? 1.f : ldexpf(1.f, 126 - max(e, 24));
 }
+// The second digit of x after the first.  (One mixed fma, exact before its rounding; a -1 that
+// the compiler knows is turned into a conversion and a difference.)
+__device__ inline _Float16 rest_of(float x, _Float16 hi) {
+  float minus = -1.f;
+  asm("" : "+s"(minus));
+  return (_Float16)fmaf((float)hi, minus, x);
+}
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <int FMT, int NB>
@@ -152,55 +164,67 @@ struct Shape {
   static constexpr int RB = DP * (FMT == MG_KV_INT4 ? 4 : 8) / 8;   // bytes of a vector
 };
 
-// A tile of 32 keys: where its two runs of 16 lie, and the lane's codes and scales.  The
-// parts are loaded apart.
+// Where the two runs of 16 keys of a tile lie: the same for a whole wave, so in scalar registers
+// (the lanes add 32-bit offsets).
+struct Place {
+  int page[2];    // table entries of the tile looked up last, not yet checked; -1: none
+  int64_t at[2];  // of the located one: (page, head) times page size plus place
+  int64_t sc[2];  // and its scales, in floats
+  bool none[2];   // no such page: its keys read as NaN
+
+  // (The entries are first used a tile later, in locate.)
+  __device__ inline void look_up(const mg_kv_attn &a, int b, int total, int t0) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int t = t0 + 16 * u;
+      const int64_t entry = t >> a.c.plog;
+      page[u] = -1;
+      if (t >= total) page[u] = 0;
+      else if (entry < a.s.table_stride) page[u] = kv_scalar(a.s.page_table + b * a.s.table_stride + entry);
+    }
+  }
+  template <int FMT>
+  __device__ inline void locate(const mg_kv_attn &a, int h, int t0) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      none[u] = page[u] < 0 || page[u] >= a.c.pages;
+      const int64_t ph = (int64_t)(none[u] ? 0 : page[u]) * a.c.kv_heads + h;
+      const int slot = (t0 + 16 * u) & ((1 << a.c.plog) - 1);
+      at[u] = (ph << a.c.plog) + slot;
+      sc[u] = (ph * kv_scales(FMT) << a.c.plog) + slot;
+    }
+  }
+};
+
+// A tile of 32 keys in a wave's registers: codes and scales.  The parts are loaded apart.
 template <int FMT, int NB>
 struct Tile {
   using S = Shape<FMT, NB>;
-  int64_t page[2];  // of the tile to be loaded, -1: none
-  int64_t at[2];    // (page, head) times page size plus place
-  int64_t ph[2];    // (page, head)
-  bool none[2];     // no such page: its keys read as NaN
   uint32_t k[2][S::KW], v[2][S::KW];
   float4 ks[2], vs[2], kz[2], vz[2];
 
-  __device__ inline void look_up(const mg_kv_attn &a, int b, int total, int t0) {
+  __device__ inline void load_k(const mg_kv_attn &a, const Place &p, int g, int c) {
 #pragma unroll
     for (int u = 0; u < 2; u++)
-      page[u] = t0 + 16 * u < total ? kv_page(a.s, b, t0 + 16 * u, a.c.plog, a.c.pages) : 0;
+      load_run<S::KW>(k[u], a.c.k + p.at[u] * S::RB + (uint32_t)(c * S::RB + g * (S::RB / 4)));
   }
-  __device__ inline void locate(const mg_kv_attn &a, int h, int t0) {
-    const int psize = 1 << a.c.plog;
+  __device__ inline void load_v(const mg_kv_attn &a, const Place &p, int g, int c) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      load_run<S::KW>(v[u], a.c.v + p.at[u] * S::RB + (uint32_t)(4 * g * S::RB + c * (4 * S::KW)));
+  }
+  __device__ inline void load_scales(const mg_kv_attn &a, const Place &p, int g) {
+    const uint32_t psize = 1u << a.c.plog;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      none[u] = page[u] < 0;
-      ph[u] = (page[u] < 0 ? 0 : page[u]) * a.c.kv_heads + h;
-      at[u] = (ph[u] << a.c.plog) + ((t0 + 16 * u) & (psize - 1));
-    }
-  }
-  __device__ inline void load_k(const mg_kv_attn &a, int g, int c) {
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-      load_run<S::KW>(k[u], a.c.k + at[u] * S::RB + (c * S::RB + g * (S::RB / 4)));
-  }
-  __device__ inline void load_v(const mg_kv_attn &a, int g, int c) {
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-      load_run<S::KW>(v[u], a.c.v + at[u] * S::RB + (4 * g * S::RB + c * (4 * S::KW)));
-  }
-  __device__ inline void load_scales(const mg_kv_attn &a, int g) {
-    const int psize = 1 << a.c.plog;
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      // (page, head)'s scales: kv_scales runs of psize.
-      const float *sc = a.c.sc + (ph[u] * (kv_scales(FMT) - 1) << a.c.plog) + at[u] + 4 * g;
-      ks[u] = *reinterpret_cast<const float4 *>(sc);
-      vs[u] = *reinterpret_cast<const float4 *>(sc + psize);
+      const float *sc = a.c.sc + p.sc[u];
+      ks[u] = *reinterpret_cast<const float4 *>(sc + (uint32_t)(4 * g));
+      vs[u] = *reinterpret_cast<const float4 *>(sc + (psize + 4 * g));
       if (FMT == MG_KV_INT4) {
-        kz[u] = *reinterpret_cast<const float4 *>(sc + 2 * psize);
-        vz[u] = *reinterpret_cast<const float4 *>(sc + 3 * psize);
+        kz[u] = *reinterpret_cast<const float4 *>(sc + (2 * psize + 4 * g));
+        vz[u] = *reinterpret_cast<const float4 *>(sc + (3 * psize + 4 * g));
       }
-      if (none[u]) {
+      if (p.none[u]) {
         const float nan = __builtin_nanf("");
         ks[u] = make_float4(nan, nan, nan, nan);
       }
@@ -285,149 +309,277 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
   }
 }
 
-// KEYS: the four waves take tiles in turn for the same rows; else rows of their own.
-template <int FMT, int NB, int QB, bool KEYS>
-__global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_kv_attn a) {
-  using S = Shape<FMT, NB>;
-  constexpr int DP = S::DP, KS = S::KS, KW = S::KW;
-  constexpr int ROWS = 16 * QB * (KEYS ? 1 : 4);  // rows of the workgroup
-  constexpr int QP = DP + 4;
-  // The rows' queries; later (KEYS) the four waves' results.
-  __shared__ __attribute__((aligned(16))) float lds[64 * QB * QP];
-  __shared__ float stat[4][2][16 * QB];
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  // Workgroup -> (sequence, split, row block, KV head), heads innermost.
+// One tile's weights for QB blocks of 16 rows: the scores of the lane's eight keys, in units that
+// make its running maximum m current, and from them the digits of the weights times the V scales.
+// l and z are the lane's share of the sum and (INT4) of the sum of weights times middles.
+// masked: only the keys of `seen` count (a branch of the whole wave, or a constant).  `between`
+// is work of the caller's that runs along with the exponentials.
+template <int FMT, int NB, int QB, class Between>
+__device__ inline void weigh(Between between, bool masked, const float4v (&acc)[QB][2], const float (&ksf)[8],
+                             const float (&vsn)[8], const float (&kzf)[8], const float (&vz)[8],
+                             const float (&qs)[QB], const uint32_t (&seen)[QB], float (&m)[QB],
+                             float (&l)[QB], float (&z)[QB], float4v (&o)[QB][NB],
+                             half8v (&ph)[QB], half8v (&pl)[QB]) {
+  float d[QB][8];  // scores less m, of unseen keys too
+  auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < QB; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float base = FMT == MG_KV_INT4 ? fmaf(qs[q], kzf[j], -m[q]) : -m[q];
+        d[q][j] = fmaf(acc[q][j >> 2][j & 3], ksf[j], base);
+      }
+  };
+  auto top = [&](int q) __attribute__((always_inline)) {
+    return fmaxf(fmaxf(fmaxf(d[q][0], d[q][1]), fmaxf(d[q][2], d[q][3])),
+                 fmaxf(fmaxf(d[q][4], d[q][5]), fmaxf(d[q][6], d[q][7])));
+  };
+  scores();
+  float most = top(0);
+#pragma unroll
+  for (int q = 1; q < QB; q++) most = fmaxf(most, top(q));
+  // (An unseen key's score may bring a wave here, where only the seen ones count.)
+  if (__builtin_expect(__any(most > kSlack), 0)) {
+    float old[QB];
+#pragma unroll
+    for (int q = 0; q < QB; q++) {
+      old[q] = m[q];
+      m[q] = 0.f;
+    }
+    scores();
+#pragma unroll
+    for (int q = 0; q < QB; q++) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) d[q][j] = seen[q] >> j & 1 ? d[q][j] : -__builtin_inff();
+      m[q] = fmaxf(old[q], row_max(top(q)));
+      const float by = exp2_of(old[q] - m[q]);
+      l[q] *= by;
+      z[q] *= by;
+#pragma unroll
+      for (int i = 0; i < NB; i++) o[q][i] *= by;
+    }
+    scores();
+  }
+  between();
+  float e[QB][8], w[QB][8], zs[QB][8];
+#pragma unroll
+  for (int q = 0; q < QB; q++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      e[q][j] = exp2_of(d[q][j]);
+      w[q][j] = e[q][j] * vsn[j];
+      if (FMT == MG_KV_INT4) zs[q][j] = e[q][j] * vz[j];
+    }
+  if (masked) {
+    // An unseen key counts nothing, whatever its score and scales are.  (The empty statement
+    // keeps the selections in their branch; else every tile does them.)
+    asm volatile("");
+#pragma unroll
+    for (int q = 0; q < QB; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const bool on = seen[q] >> j & 1;
+        e[q][j] = on ? e[q][j] : 0.f;
+        w[q][j] = on ? w[q][j] : 0.f;
+        if (FMT == MG_KV_INT4) zs[q][j] = on ? zs[q][j] : 0.f;
+      }
+  }
+#pragma unroll
+  for (int q = 0; q < QB; q++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) l[q] += e[q][j];
+#pragma unroll
+  for (int q = 0; q < QB; q++)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      if (FMT == MG_KV_INT4) z[q] += zs[q][j] + zs[q][j + 1];
+      const half2v hi = __builtin_convertvector(float2v{w[q][j], w[q][j + 1]}, half2v);
+      ph[q][j] = hi[0];
+      ph[q][j + 1] = hi[1];
+      pl[q][j] = rest_of(w[q][j], hi[0]);
+      pl[q][j + 1] = rest_of(w[q][j + 1], hi[1]);
+    }
+}
+
+// Which of the lane's eight keys of the tile at t0 a row sees (bit j: key 16 (j / 4) + 4 g + j % 4),
+// of those below kfin.
+__device__ inline uint32_t seen_keys(const mg_kv_attn &a, const kv_seq &sq, int t0, int g, int see,
+                                     int64_t word, int kfin) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const int k = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+    bool ok = k < see;
+    if (a.tree && k >= sq.past && k < sq.past + sq.n)
+      ok = a.tree[word + ((k - sq.past) >> 6)] >> ((k - sq.past) & 63) & 1;
+    if (ok && k < kfin) seen |= 1u << j;
+  }
+  return seen;
+}
+
+// The digits of 16 rows' queries in matrix order from shared memory, times dn.
+template <int FMT, int KS>
+__device__ inline void query_digits(const float *x, float dn, half8v (&qh)[KS], half8v (&ql)[KS],
+                                    float &qs) {
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; s++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float v = x[8 * s + k_slot<FMT>(j)] * dn;
+      const _Float16 hi = (_Float16)v;
+      qh[s][j] = hi;
+      ql[s][j] = rest_of(v, hi);
+      sum += v;
+    }
+  qs = FMT == MG_KV_INT4 ? row_sum(sum) : 0.f;
+}
+// Largest finite size among n elements.
+__device__ inline float largest(const float *x, int n, float mx) {
+#pragma unroll
+  for (int d = 0; d < n; d++) {
+    const float v = fabsf(x[d]);
+    mx = v < __builtin_inff() ? fmaxf(mx, v) : mx;
+  }
+  return mx;
+}
+
+// Which sequence, split, row block and KV head a workgroup has (heads innermost), and its keys.
+struct Work {
+  kv_seq sq;
+  int b, h, split, r0, rows;  // rows: of the sequence
+  int kbeg, kend;             // keys that its last row sees, from its split's first on
+};
+// False: nothing to do.
+__device__ inline bool work_of(const mg_kv_attn &a, int ROWS, Work *w) {
   int id = (int)blockIdx.x;
-  const int h = id % a.c.kv_heads;
+  w->h = id % a.c.kv_heads;
   id /= a.c.kv_heads;
   const int blk = a.nblk - 1 - id % a.nblk;  // rows that see most keys first
   id /= a.nblk;
-  const int split = id % a.nsplit;
-  const int b = id / a.nsplit;
-  const kv_seq sq = kv_sequence(a.s, b);
-  if (sq.bad) {
-    if (blk == 0 && split == 0 && h == 0 && threadIdx.x == 0) atomicOr(a.c.refused, 1);
+  w->split = id % a.nsplit;
+  w->b = id / a.nsplit;
+  w->sq = kv_sequence(a.s, w->b);
+  if (w->sq.bad) {
+    if (blk == 0 && w->split == 0 && w->h == 0 && threadIdx.x == 0) atomicOr(a.c.refused, 1);
+    return false;
+  }
+  w->rows = w->sq.n * a.group;
+  w->r0 = blk * ROWS;
+  if (w->r0 >= w->rows) return false;
+  w->kend = a.tree ? w->sq.past + w->sq.n
+                   : w->sq.past + (min(w->r0 + ROWS, w->rows) - 1) / a.group + 1;
+  w->kbeg = w->split * a.kc;
+  return w->kbeg < w->kend || w->split == 0;
+}
+
+// Four outputs of row w.r0 + r from dim d, to y (divided by the sum ll) or to the split's
+// partial results.
+template <int DP>
+__device__ inline void put4(const mg_kv_attn &a, const Work &w, int r, int d, float4 v, float ll) {
+  const int row = w.r0 + r;
+  if (row >= w.rows) return;
+  if (a.nsplit > 1) {
+    const int64_t at = ((int64_t)w.b * a.c.kv_heads + w.h) * a.s.max_new * a.group + row;
+    *reinterpret_cast<float4 *>(a.part + (at * a.nsplit + w.split) * DP + d) = v;
     return;
   }
-  const int rows = sq.n * a.group, r0 = blk * ROWS;
-  if (r0 >= rows) return;
-  // Keys of this workgroup: those its last row sees, of its split.
+  const int qi = row / a.group, j = row - qi * a.group;
+  float *y = a.y + (w.sq.start + qi) * a.y_stride + (int64_t)(w.h * a.group + j) * a.c.d + d;
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  if (a.vec) {
+    if (d < a.c.d) *reinterpret_cast<float4 *>(y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  } else {
+    if (d < a.c.d) y[0] = v.x * inv;
+    if (d + 1 < a.c.d) y[1] = v.y * inv;
+    if (d + 2 < a.c.d) y[2] = v.z * inv;
+    if (d + 3 < a.c.d) y[3] = v.w * inv;
+  }
+}
+__device__ inline void put_stat(const mg_kv_attn &a, const Work &w, int r, float m, float l) {
+  if (a.nsplit == 1 || w.r0 + r >= w.rows) return;
+  const int64_t at = ((int64_t)w.b * a.c.kv_heads + w.h) * a.s.max_new * a.group + w.r0 + r;
+  a.part_ml[at * a.nsplit + w.split] = make_float2(m, l);
+}
+
+// Few rows: the four waves take tiles in turn for the same 16 rows and join their results.
+template <int FMT, int NB>
+__global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_attn a) {
+  using S = Shape<FMT, NB>;
+  constexpr int DP = S::DP, KS = S::KS, KW = S::KW, QP = DP + 4, STEP = 128;
+  // 16 rows' queries; later the four waves' results.
+  __shared__ __attribute__((aligned(16))) float lds[64 * QP];
+  __shared__ float stat[4][2][16];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  Work w;
+  if (!work_of(a, 16, &w)) return;
+  const kv_seq &sq = w.sq;
   const int total = sq.past + sq.n;
-  const int kend = a.tree ? total : sq.past + (min(r0 + ROWS, rows) - 1) / a.group + 1;
-  const int kbeg = split * a.kc;
-  if (kbeg >= kend && split > 0) return;
-  const int wr0 = KEYS ? 0 : wave * 16 * QB;  // the wave's first row
-  // Keys that some row of the wave sees, of this split, and those that all of them see.
-  const int wend = r0 + wr0 >= rows ? 0
-                   : a.tree         ? total
-                                    : sq.past + (min(r0 + wr0 + 16 * QB, rows) - 1) / a.group + 1;
-  const int kfin = min(wend, kend - kbeg > a.kc ? kbeg + a.kc : kend);
-  const int plain = a.tree ? sq.past : sq.past + min(r0 + wr0, rows - 1) / a.group + 1;
-  constexpr int STEP = KEYS ? 128 : 32;
-  // With registers to spare the next tile's loads start before this one's products, else each
-  // part's as soon as this one's is used.
-  constexpr bool AHEAD = QB == 1 && NB <= 8;
-  int t0 = kbeg + (KEYS ? 32 * wave : 0);
+  const int kfin = w.kend - w.kbeg > a.kc ? w.kbeg + a.kc : w.kend;
+  // Keys below it are seen by every row.
+  const int plain = a.tree ? sq.past : sq.past + w.r0 / a.group + 1;
+  int t0 = w.kbeg + 32 * wave;
   // The first tile's loads run while the queries are made.
   Tile<FMT, NB> t, next;
+  Place p;
   bool refused = false;
   if (t0 < kfin) {
-    t.look_up(a, b, total, t0);
-    t.locate(a, h, t0);
-    t.load_k(a, g, c);
-    t.load_scales(a, g);
-    t.load_v(a, g, c);
-    refused = t.none[0] || t.none[1];
-    next.look_up(a, b, total, t0 + STEP);
+    p.look_up(a, w.b, total, t0);
+    p.locate<FMT>(a, w.h, t0);
+    t.load_k(a, p, g, c);
+    t.load_scales(a, p, g);
+    t.load_v(a, p, g, c);
+    refused = p.none[0] || p.none[1];
+    p.look_up(a, w.b, total, t0 + STEP);
   }
-
-  stage_queries<DP>(a, sq, h, r0, rows, ROWS, lds);
+  stage_queries<DP>(a, sq, w.h, w.r0, w.rows, 16, lds);
   __syncthreads();
-  half8v qh[QB][KS], ql[QB][KS];
-  float qs[QB];
-  int see[QB];       // keys below it are seen (tree: past)
-  int64_t word[QB];  // the row's words of the tree
-  float f;
-  {
-    // One power of two for the wave's rows: the largest element under 2^15, so that a
-    // digit pair is exact to 2^-22 of any element down to 2^-17 of it, and to 2^-39 of it below.
-    float mx = 0.f;
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-      for (int d = 0; d < DP / 4; d++) {
-        const float v = fabsf(lds[(wr0 + qb * 16 + c) * QP + g * (DP / 4) + d]);
-        mx = v < __builtin_inff() ? fmaxf(mx, v) : mx;
-      }
-    const float dn = 32768.f * pow2_under(wave_max(mx));
-    f = 1.f / dn;
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      const float *x = lds + (wr0 + qb * 16 + c) * QP + g * (DP / 4);
-      float sum = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float v = x[8 * s + k_slot<FMT>(j)] * dn;
-          const _Float16 hi = (_Float16)v;
-          qh[qb][s][j] = hi;
-          ql[qb][s][j] = (_Float16)(v - (float)hi);
-          sum += v;
-        }
-      qs[qb] = FMT == MG_KV_INT4 ? row_sum(sum) : 0.f;
-      const int row = min(r0 + wr0 + qb * 16 + c, rows - 1), qi = row / a.group;
-      see[qb] = a.tree ? sq.past : sq.past + qi + 1;
-      word[qb] = (int64_t)(sq.start + qi) * a.tree_words;
-    }
-  }
+  // One power of two for the rows: the largest element under 2^15, so that a digit pair is
+  // exact to 2^-22 of any element down to 2^-17 of it, and to 2^-39 of it below.
+  const float *x = lds + c * QP + g * (DP / 4);
+  const float dn = 32768.f * pow2_under(wave_max(largest(x, DP / 4, 0.f))), f = 1.f / dn;
+  half8v qh[KS], ql[KS];
+  float qs[1];
+  query_digits<FMT, KS>(x, dn, qh, ql, qs[0]);
+  const int qi = min(w.r0 + c, w.rows - 1) / a.group;
+  const int see = a.tree ? sq.past : sq.past + qi + 1;
+  const int64_t word = (int64_t)(sq.start + qi) * a.tree_words;
 
-  float4v o[QB][NB];
-  float m[QB], l[QB], z[QB];
+  float4v o[1][NB];
 #pragma unroll
-  for (int qb = 0; qb < QB; qb++) {
-    m[qb] = kNoMax;
-    l[qb] = z[qb] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NB; i++) o[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
-  }
-  float vn = ldexpf(1.f, 100);
-
+  for (int i = 0; i < NB; i++) o[0][i] = float4v{0.f, 0.f, 0.f, 0.f};
+  float m[1] = {kNoMax}, l[1] = {0.f}, z[1] = {0.f}, vn = ldexpf(1.f, 100);
+  // With registers to spare the next tile's loads start before this one's products, else each
+  // part's as soon as this one's is used.
+  constexpr bool AHEAD = NB <= 8;
   // One tile; MASKED: some row may not see some key.
   auto tile = [&](auto masked_tag) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     const int tn = t0 + STEP;
     const bool more = tn < kfin;
-    if (AHEAD && more) {
-      next.locate(a, h, tn);
-      next.load_k(a, g, c);
-      next.load_scales(a, g);
-      next.load_v(a, g, c);
-      refused |= next.none[0] || next.none[1];
-      next.look_up(a, b, total, tn + STEP);
+    if (more) {
+      p.locate<FMT>(a, w.h, tn);
+      p.look_up(a, w.b, total, tn + STEP);
+      refused |= p.none[0] || p.none[1];
     }
-    auto key = [&](int j) { return t0 + 16 * (j >> 2) + 4 * g + (j & 3); };
-    float4v acc[QB][2];
+    if (AHEAD && more) {
+      next.load_k(a, p, g, c);
+      next.load_scales(a, p, g);
+      next.load_v(a, p, g, c);
+    }
+    float4v acc[1][2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-#pragma unroll
-      for (int qb = 0; qb < QB; qb++) acc[qb][u] = float4v{0.f, 0.f, 0.f, 0.f};
+      acc[0][u] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < KS; s++) {
         const half8v ka = k_operand<FMT, KW>(t.k[u], s);
-#pragma unroll
-        for (int qb = 0; qb < QB; qb++) {
-          acc[qb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[qb][s], acc[qb][u], 0, 0, 0);
-          acc[qb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[qb][s], acc[qb][u], 0, 0, 0);
-        }
+        acc[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[s], acc[0][u], 0, 0, 0);
+        acc[0][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[s], acc[0][u], 0, 0, 0);
       }
     }
-    if (!AHEAD && more) {
-      next.locate(a, h, tn);
-      next.load_k(a, g, c);
-      next.look_up(a, b, total, tn + STEP);
-    }
+    if (!AHEAD && more) next.load_k(a, p, g, c);
     float ksf[8], vsn[8], kzf[8], vz[8];
     spread(ksf, t.ks, f);
     spread(vsn, t.vs, 1.f);
@@ -440,194 +592,315 @@ __global__ __launch_bounds__(256, NB * QB <= 8 ? 2 : 1) void k_kv_attn(const mg_
       float big = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        if (MASKED && key(j) >= kfin) vsn[j] = 0.f;
+        if (MASKED && t0 + 16 * (j >> 2) + 4 * g + (j & 3) >= kfin) vsn[j] = 0.f;
         big = fmaxf(big, vsn[j]);
       }
       if (__builtin_expect(__any(big * vn > 16.f), 0)) {
         const float now = 8.f * pow2_under(wave_max(big)), by = now / vn;
         vn = now;
 #pragma unroll
-        for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-          for (int i = 0; i < NB; i++) o[qb][i] *= by;
+        for (int i = 0; i < NB; i++) o[0][i] *= by;
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) vsn[j] *= vn;
     }
-    half8v ph[QB], pl[QB];
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      uint32_t seen = 0xff;
-      if (MASKED) {
-        seen = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int k = key(j);
-          bool ok = k < see[qb];
-          if (a.tree && k >= sq.past && k < total)
-            ok = a.tree[word[qb] + ((k - sq.past) >> 6)] >> ((k - sq.past) & 63) & 1;
-          if (ok && k < kfin) seen |= 1u << j;
-        }
-      }
-      // Scores less `from`, -inf where not seen.
-      float d[8];
-      auto scores = [&](float from) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float base = FMT == MG_KV_INT4 ? fmaf(qs[qb], kzf[j], -from) : -from;
-          d[j] = fmaf(acc[qb][j >> 2][j & 3], ksf[j], base);
-          if (MASKED) d[j] = seen >> j & 1 ? d[j] : -__builtin_inff();
-        }
-      };
-      auto top = [&]() {
-        return fmaxf(fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])),
-                     fmaxf(fmaxf(d[4], d[5]), fmaxf(d[6], d[7])));
-      };
-      scores(m[qb]);
-      if (__builtin_expect(__any(top() > kSlack), 0)) {
-        scores(0.f);
-        const float now = fmaxf(m[qb], row_max(top()));
-        const float by = exp2_of(m[qb] - now);
-        m[qb] = now;
-        l[qb] *= by;
-        z[qb] *= by;
-#pragma unroll
-        for (int i = 0; i < NB; i++) o[qb][i] *= by;
-        scores(now);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float p0 = exp2_of(d[j]), p1 = exp2_of(d[j + 1]);
-        l[qb] += p0;
-        l[qb] += p1;
-        float w0 = p0 * vsn[j], w1 = p1 * vsn[j + 1];
-        // (MASKED: 0 times a NaN that the row does not see.)
-        if (MASKED) {
-          w0 = seen >> j & 1 ? w0 : 0.f;
-          w1 = seen >> (j + 1) & 1 ? w1 : 0.f;
-        }
-        if (FMT == MG_KV_INT4) {
-          const float z0 = p0 * vz[j], z1 = p1 * vz[j + 1];
-          z[qb] += !MASKED || seen >> j & 1 ? z0 : 0.f;
-          z[qb] += !MASKED || seen >> (j + 1) & 1 ? z1 : 0.f;
-        }
-        const half2v hi = __builtin_convertvector(float2v{w0, w1}, half2v);
-        const half2v lo =
-            __builtin_convertvector(float2v{w0 - (float)hi[0], w1 - (float)hi[1]}, half2v);
-        ph[qb][j] = hi[0];
-        ph[qb][j + 1] = hi[1];
-        pl[qb][j] = lo[0];
-        pl[qb][j + 1] = lo[1];
-      }
-    }
-    if (!AHEAD && more) {
-      next.load_scales(a, g);
-      refused |= next.none[0] || next.none[1];
-    }
+    half8v ph[1], pl[1];
+    const uint32_t seen[1] = {MASKED ? seen_keys(a, sq, t0, g, see, word, kfin) : 0xffu};
+    weigh<FMT, NB, 1>([] {}, MASKED, acc, ksf, vsn, kzf, vz, qs, seen, m, l, z, o, ph, pl);
+    if (!AHEAD && more) next.load_scales(a, p, g);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const half8v va = v_operand<FMT, KW>(t.v[0], t.v[1], i);
+      o[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[0], o[0][i], 0, 0, 0);
+      o[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[0], o[0][i], 0, 0, 0);
+    }
+    if (!AHEAD && more) next.load_v(a, p, g, c);
+    t = next;
+    t0 = tn;
+  };
+  while (t0 < kfin && t0 + 32 <= plain) tile(std::false_type{});
+  while (t0 < kfin) tile(std::true_type{});
+
+  if (refused && lane == 0) atomicOr(a.c.refused, 1);
+  const float iv = 1.f / vn;
+  l[0] = row_sum(l[0]);
+  z[0] = FMT == MG_KV_INT4 ? row_sum(z[0]) : 0.f;
+  if (g == 0) {
+    stat[wave][0][c] = m[0];
+    stat[wave][1][c] = l[0];
+  }
+  __syncthreads();
+  const float all = fmaxf(fmaxf(stat[0][0][c], stat[1][0][c]), fmaxf(stat[2][0][c], stat[3][0][c]));
+  const float by = exp2_of(m[0] - all);
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+#pragma unroll
+    for (int i = 0; i < NB; i += 4)
+      *reinterpret_cast<float4 *>(lds + (wave * 16 + c) * QP + NB * (4 * g + e) + i) =
+          make_float4((o[0][i][e] * iv + z[0]) * by, (o[0][i + 1][e] * iv + z[0]) * by,
+                      (o[0][i + 2][e] * iv + z[0]) * by, (o[0][i + 3][e] * iv + z[0]) * by);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
+    const int r = i / (DP / 4), d = 4 * (i - r * (DP / 4));
+    float mm = stat[0][0][r], ll = 0.f;
+#pragma unroll
+    for (int k = 1; k < 4; k++) mm = fmaxf(mm, stat[k][0][r]);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      ll += stat[k][1][r] * exp2_of(stat[k][0][r] - mm);
+      const float4 y = *reinterpret_cast<const float4 *>(lds + (k * 16 + r) * QP + d);
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
+    }
+    put4<DP>(a, w, r, d, v, ll);
+    if (d == 0) put_stat(a, w, r, mm, ll);
+  }
+}
+
+// A wave's quarter of a tile's codes on their way to shared memory: a run of steps of one half
+// tile's keys, a run of dim tiles of the values; and in one wave the tile's scales, a key a lane.
+template <int FMT, int NB>
+struct Quarter {
+  using S = Shape<FMT, NB>;
+  static constexpr int KF = S::KS / 2, VF = NB / 4;  // operands of K and of V that it makes
+  static constexpr int KD = FMT == MG_KV_INT4 ? KF : 2 * KF;
+  static constexpr int VD = FMT == MG_KV_INT4 ? (VF + 1) / 2 : VF;
+  uint32_t k[KD], v[2][VD];
+  float ks, vs, kz, vz;
+  bool none;  // of the lane's key
+
+  __device__ inline void load(const mg_kv_attn &a, const Place &p, int wave, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+    const uint8_t *kp = a.c.k + (wave & 2 ? p.at[1] : p.at[0]) * S::RB + (wave & 1) * 4 * KD;
+#pragma unroll
+    for (int i = 0; i < KD; i++)
+      k[i] = *reinterpret_cast<const uint32_t *>(kp + (uint32_t)(c * S::RB + g * (S::RB / 4) + 4 * i));
+    const int i0 = wave * VF;  // its first dim tile
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint8_t *vp = a.c.v + p.at[u] * S::RB;
+      const uint32_t o = 4 * g * S::RB + 4 * (FMT == MG_KV_INT4 ? (c * NB + i0) >> 1 : c * NB + i0);
+#pragma unroll
+      for (int i = 0; i < VD; i++) v[u][i] = *reinterpret_cast<const uint32_t *>(vp + (o + 4 * i));
+    }
+    if (wave == 3) {
+      const uint32_t psize = 1u << a.c.plog;
+      const bool u = lane >> 4 & 1;
+      const float *sc = a.c.sc + (u ? p.sc[1] : p.sc[0]) + c;
+      ks = sc[0];
+      vs = sc[psize];
+      if (FMT == MG_KV_INT4) {
+        kz = sc[2 * psize];
+        vz = sc[3 * psize];
+      }
+      none = u ? p.none[1] : p.none[0];
+    }
+  }
+  // The operands, [operand][lane]: K by half tile and step, V by dim tile.
+  __device__ inline void convert(uint4 *kt, uint4 *vt, int wave, int lane) const {
+#pragma unroll
+    for (int i = 0; i < KF; i++)
+      kt[(wave * KF + i) * 64 + lane] = __builtin_bit_cast(uint4, k_operand<FMT, KD>(k, i));
+#pragma unroll
+    for (int i = 0; i < VF; i++) {
+      half8v x;
+      if (FMT == MG_KV_INT4) {
+        // (Its first dim tile may be the second of a dword's pair.)
+        const int odd = VF % 2 ? wave & 1 : 0, n = 2 * ((odd + i) & 1), w = (odd + i) >> 1;
+        const uint32_t w0 = w ? v[0][VD - 1] : v[0][0], w1 = w ? v[1][VD - 1] : v[1][0];
+        x = join4(nib2_any(w0, n), nib2_any(w0, n + 1), nib2_any(w1, n), nib2_any(w1, n + 1));
+      } else {
+        half2v p, q, r, s;
+        four<FMT>(v[0][i % VD], p, q);
+        four<FMT>(v[1][i % VD], r, s);
+        x = join4(p, q, r, s);
+      }
+      vt[(wave * VF + i) * 64 + lane] = __builtin_bit_cast(uint4, x);
+    }
+  }
+};
+
+// Many rows: each of the four waves has 16 QB rows of its own.  They convert a quarter of each
+// tile each, into shared memory in matrix order (twice, so that one barrier a tile suffices): a
+// code is then converted once for 64 QB rows, not by every wave, and its 16-byte operands cost a
+// quarter of what the products take.
+template <int FMT, int NB, int QB>
+__global__ __launch_bounds__(256, 2) void k_kv_rows(const mg_kv_attn a) {
+  using S = Shape<FMT, NB>;
+  constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;
+  constexpr int KO = 2 * KS * 64, VO = NB * 64;  // operands of a tile
+  union Shared {
+    float q[ROWS * QP];  // the queries, before the tiles
+    struct {
+      uint4 k[2][KO], v[2][VO];
+    } t;
+  };
+  __shared__ __attribute__((aligned(16))) Shared sh;
+  __shared__ __attribute__((aligned(16))) float sc[2][4][32];  // scales of a tile's keys
+  __shared__ float unit[2], size[4];
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  Work w;
+  if (!work_of(a, ROWS, &w)) return;
+  const kv_seq &sq = w.sq;
+  const int total = sq.past + sq.n;
+  const int kfin = w.kend - w.kbeg > a.kc ? w.kbeg + a.kc : w.kend;  // of the workgroup
+  const int wr0 = wave * 16 * QB, first = w.r0 + wr0;  // the wave's first row
+  // Keys that some row of the wave sees, and those that all of them see.
+  const int wfin = first >= w.rows ? 0
+                   : a.tree        ? kfin
+                        : min(kfin, sq.past + (min(first + 16 * QB, w.rows) - 1) / a.group + 1);
+  const int plain = a.tree ? sq.past : sq.past + min(first, w.rows - 1) / a.group + 1;
+  Quarter<FMT, NB> raw;
+  Place p;
+  bool refused = false;
+  // The codes of the tile at t (looked up before), and the pages of the next.
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    p.locate<FMT>(a, w.h, t);
+    raw.load(a, p, wave, lane);
+    refused |= p.none[0] || p.none[1];
+    p.look_up(a, w.b, total, t + 32);
+  };
+  p.look_up(a, w.b, total, w.kbeg);
+  if (w.kbeg < kfin) fetch(w.kbeg);
+
+  stage_queries<DP>(a, sq, w.h, w.r0, w.rows, ROWS, sh.q);
+  __syncthreads();
+  float mx = 0.f;
+#pragma unroll
+  for (int qb = 0; qb < QB; qb++)
+    mx = largest(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), DP / 4, mx);
+  mx = wave_max(mx);
+  if (lane == 0) size[wave] = mx;
+  __syncthreads();
+  // One power of two for the workgroup's rows, as in k_kv_keys.
+  const float dn = 32768.f * pow2_under(fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3])));
+  const float f = 1.f / dn;
+  half8v qh[QB][KS], ql[QB][KS];
+  float qs[QB];
+  int qi[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; qb++) {
+    query_digits<FMT, KS>(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), dn, qh[qb], ql[qb], qs[qb]);
+    qi[qb] = min(first + qb * 16 + c, w.rows - 1) / a.group;
+  }
+  __syncthreads();  // the queries' place is the tiles' now
+
+  // Wave 3 keeps the unit of the V scales, 8 under the largest so far.
+  float vn = ldexpf(1.f, 100);
+  auto stage = [&](int at, int t0) __attribute__((always_inline)) {
+    raw.convert(sh.t.k[at], sh.t.v[at], wave, lane);
+    if (wave == 3) {
+      const bool in = t0 + (lane & 31) < total;
+      const float vs = in ? raw.vs : 0.f;
+      if (__builtin_expect(__any(vs * vn > 16.f), 0)) vn = 8.f * pow2_under(wave_max(vs));
+      if (lane < 32) {
+        sc[at][0][lane] = raw.none ? __builtin_nanf("") : raw.ks * f;
+        sc[at][1][lane] = vs * vn;
+        if (FMT == MG_KV_INT4) {
+          sc[at][2][lane] = raw.kz * f;
+          sc[at][3][lane] = raw.vz;
+        }
+      }
+      if (lane == 0) unit[at] = vn;
+    }
+  };
+
+  float4v o[QB][NB];
+  float m[QB], l[QB], z[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; qb++) {
+    m[qb] = kNoMax;
+    l[qb] = z[qb] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) o[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
+  }
+  float mine = ldexpf(1.f, 100);  // the unit of this wave's outputs
+  auto tile = [&](int at, int t0) __attribute__((always_inline)) {
+    const bool masked = t0 + 32 > plain;  // some row may not see some key
+    float4v acc[QB][2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++) acc[qb][u] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        const half8v ka = __builtin_bit_cast(half8v, sh.t.k[at][(u * KS + s) * 64 + lane]);
+#pragma unroll
+        for (int qb = 0; qb < QB; qb++) {
+          acc[qb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[qb][s], acc[qb][u], 0, 0, 0);
+          acc[qb][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[qb][s], acc[qb][u], 0, 0, 0);
+        }
+      }
+    }
+    float x[4][8];
+#pragma unroll
+    for (int k = 0; k < (FMT == MG_KV_INT4 ? 4 : 2); k++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const float4 v = *reinterpret_cast<const float4 *>(&sc[at][k][16 * u + 4 * g]);
+        x[k][4 * u] = v.x, x[k][4 * u + 1] = v.y, x[k][4 * u + 2] = v.z, x[k][4 * u + 3] = v.w;
+      }
+    const float now = unit[at];
+    if (__builtin_expect(__any(now != mine), 0)) {
+      const float by = now / mine;
+      mine = now;
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++)
+#pragma unroll
+        for (int i = 0; i < NB; i++) o[qb][i] *= by;
+    }
+    half8v ph[QB], pl[QB];
+    uint32_t seen[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) {
+      seen[qb] = 0xffu;
+      if (masked)
+        seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi[qb] + 1,
+                             (int64_t)(sq.start + qi[qb]) * a.tree_words, kfin);
+    }
+    weigh<FMT, NB, QB>([] {}, masked, acc, x[0], x[1], x[2], x[3], qs, seen, m, l, z, o, ph, pl);
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      const half8v va = __builtin_bit_cast(half8v, sh.t.v[at][i * 64 + lane]);
 #pragma unroll
       for (int qb = 0; qb < QB; qb++) {
         o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[qb], o[qb][i], 0, 0, 0);
         o[qb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[qb], o[qb][i], 0, 0, 0);
       }
     }
-    if (!AHEAD && more) next.load_v(a, g, c);
-    t = next;
-    t0 = tn;
   };
-  while (t0 < kfin && t0 + 32 <= plain) tile(std::false_type{});
-  while (t0 < kfin) tile(std::true_type{});
+
+  if (w.kbeg < kfin) stage(0, w.kbeg);
+  if (w.kbeg + 32 < kfin) fetch(w.kbeg + 32);
+  int at = 0;
+  for (int t0 = w.kbeg; t0 < kfin; t0 += 32) {
+    __syncthreads();  // tile t0 is there, and every wave is done with the one before
+    if (t0 + 32 < kfin) {
+      stage(at ^ 1, t0 + 32);
+      if (t0 + 64 < kfin) fetch(t0 + 64);
+    }
+    if (t0 < wfin) tile(at, t0);
+    at ^= 1;
+  }
+
   if (refused && lane == 0) atomicOr(a.c.refused, 1);
-  const float iv = 1.f / vn;
+  const float iv = 1.f / mine;
 #pragma unroll
   for (int qb = 0; qb < QB; qb++) {
-    l[qb] = row_sum(l[qb]);
-    z[qb] = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
-  }
-  // A run of n outputs of row r0 + r from dim d, to y or to the split's partial results.
-  const int64_t prow = ((int64_t)b * a.c.kv_heads + h) * a.s.max_new * a.group;
-  auto put4 = [&](int r, int d, float4 v, float ll) {
-    const int row = r0 + r;
-    if (row >= rows) return;
-    if (a.nsplit > 1) {
-      *reinterpret_cast<float4 *>(a.part + ((prow + row) * a.nsplit + split) * DP + d) = v;
-      return;
-    }
-    const int qi = row / a.group, j = row - qi * a.group;
-    float *y = a.y + (sq.start + qi) * a.y_stride + (int64_t)(h * a.group + j) * a.c.d + d;
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    if (a.vec) {
-      if (d < a.c.d) *reinterpret_cast<float4 *>(y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    } else {
-      if (d < a.c.d) y[0] = v.x * inv;
-      if (d + 1 < a.c.d) y[1] = v.y * inv;
-      if (d + 2 < a.c.d) y[2] = v.z * inv;
-      if (d + 3 < a.c.d) y[3] = v.w * inv;
-    }
-  };
-  auto put_stat = [&](int r, float mm, float ll) {
-    if (r0 + r < rows && a.nsplit > 1)
-      a.part_ml[(prow + r0 + r) * a.nsplit + split] = make_float2(mm, ll);
-  };
-  if (KEYS) {
-    // The four waves' results of the same rows, joined.
-    if (g == 0) {
+    const int r = wr0 + qb * 16 + c;
+    const float ll = row_sum(l[qb]), zz = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
 #pragma unroll
-      for (int qb = 0; qb < QB; qb++) {
-        stat[wave][0][qb * 16 + c] = m[qb];
-        stat[wave][1][qb * 16 + c] = l[qb];
-      }
-    }
-    __syncthreads();
+    for (int e = 0; e < 4; e++)
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      const int r = qb * 16 + c;
-      const float all =
-          fmaxf(fmaxf(stat[0][0][r], stat[1][0][r]), fmaxf(stat[2][0][r], stat[3][0][r]));
-      const float by = exp2_of(m[qb] - all);
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int i = 0; i < NB; i += 4)
-          *reinterpret_cast<float4 *>(lds + (wave * ROWS + r) * QP + NB * (4 * g + e) + i) =
-              make_float4((o[qb][i][e] * iv + z[qb]) * by, (o[qb][i + 1][e] * iv + z[qb]) * by,
-                          (o[qb][i + 2][e] * iv + z[qb]) * by, (o[qb][i + 3][e] * iv + z[qb]) * by);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
-      const int r = i / (DP / 4), d = 4 * (i - r * (DP / 4));
-      float mm = stat[0][0][r], ll = 0.f;
-#pragma unroll
-      for (int w = 1; w < 4; w++) mm = fmaxf(mm, stat[w][0][r]);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        ll += stat[w][1][r] * exp2_of(stat[w][0][r] - mm);
-        const float4 x = *reinterpret_cast<const float4 *>(lds + (w * ROWS + r) * QP + d);
-        v.x += x.x;
-        v.y += x.y;
-        v.z += x.z;
-        v.w += x.w;
-      }
-      put4(r, d, v, ll);
-      if (d == 0) put_stat(r, mm, ll);
-    }
-  } else {
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      const int r = wr0 + qb * 16 + c;
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int i = 0; i < NB; i += 4)
-          put4(r, NB * (4 * g + e) + i,
-               make_float4(o[qb][i][e] * iv + z[qb], o[qb][i + 1][e] * iv + z[qb],
-                           o[qb][i + 2][e] * iv + z[qb], o[qb][i + 3][e] * iv + z[qb]),
-               l[qb]);
-      if (g == 0) put_stat(r, m[qb], l[qb]);
-    }
+      for (int i = 0; i < NB; i += 4)
+        put4<DP>(a, w, r, NB * (4 * g + e) + i,
+                 make_float4(o[qb][i][e] * iv + zz, o[qb][i + 1][e] * iv + zz,
+                             o[qb][i + 2][e] * iv + zz, o[qb][i + 3][e] * iv + zz), ll);
+    if (g == 0) put_stat(a, w, r, m[qb], ll);
   }
 }
 
@@ -694,13 +967,12 @@ template <int FMT, int NB>
 void launch(mg_ctx *ctx, const mg_kv_attn &a) {
   const dim3 grid((unsigned)(a.s.batch * a.nsplit * a.nblk * a.c.kv_heads));
   hipStream_t st = ctx->stream;
-  if (a.keys) {
-    k_kv_attn<FMT, NB, 1, true><<<grid, dim3(256), 0, st>>>(a);
-  } else if (a.rows_wg == 64) {
-    k_kv_attn<FMT, NB, 1, false><<<grid, dim3(256), 0, st>>>(a);
-  } else if constexpr (NB <= 8) {
-    k_kv_attn<FMT, NB, 2, false><<<grid, dim3(256), 0, st>>>(a);
-  }
+  if (a.keys)
+    k_kv_keys<FMT, NB><<<grid, dim3(256), 0, st>>>(a);
+  else if (a.rows_wg == 64)
+    k_kv_rows<FMT, NB, 1><<<grid, dim3(256), 0, st>>>(a);
+  else if constexpr (NB <= 8)
+    k_kv_rows<FMT, NB, 2><<<grid, dim3(256), 0, st>>>(a);
 }
 
 template <int FMT>
