@@ -728,7 +728,7 @@ struct Quarter {
 // code is then converted once for 64 QB rows, not by every wave, and its 16-byte operands cost a
 // quarter of what the products take.
 template <int FMT, int NB, int QB>
-__global__ __launch_bounds__(256, 2) void k_kv_rows(const mg_kv_attn a) {
+__global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;
   constexpr int KO = 2 * KS * 64, VO = NB * 64;  // operands of a tile
@@ -989,23 +989,37 @@ void launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
 
 size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
   const int64_t rows = a->s.max_new * a->group, heads = a->s.batch * a->c.kv_heads;
-  // Workgroups that run at once, two a compute unit: more start late, and a start (lengths,
-  // pages, queries) costs what some ten tiles do.
-  const int64_t room = 2 * ctx->num_cus;
-  a->rows_wg = a->c.dp <= 128 ? 128 : 64;
-  if (rows <= a->rows_wg / 2) a->rows_wg = 64;
-  a->keys = rows <= 16 || (rows <= 256 && heads * ((rows + 15) / 16) <= room / 2);
-  if (a->keys) a->rows_wg = 16;
-  a->nblk = (int)((rows + a->rows_wg - 1) / a->rows_wg);
-  // Key splits to fill the room, 128 keys each at least; none for sequences of up to 512, which
-  // cost less than the join.
-  const int64_t base = heads * a->nblk;
-  const int64_t want = split && a->s.max_len > 512 ? std::max<int64_t>(1, room / base) : 1;
-  int64_t kc = (a->s.max_len + want - 1) / want;
-  kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
-  a->nsplit = (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
-  if (want == 1) a->nsplit = 1;
-  a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
+  // The plan with workgroups of rows_wg rows, `per_cu` of which run at once on a compute unit (more
+  // start late, and a start, lengths, pages and queries, costs what some ten tiles do).  Returns
+  // the keys that a place at work passes over.
+  const auto plan = [&](int rows_wg, int per_cu) {
+    const int64_t room = (int64_t)per_cu * ctx->num_cus;
+    a->rows_wg = rows_wg;
+    a->nblk = (int)((rows + rows_wg - 1) / rows_wg);
+    // Key splits to fill the room, 128 keys each at least; none for sequences of up to 512, which
+    // cost less than the join.
+    const int64_t base = heads * a->nblk;
+    const int64_t want = split && a->s.max_len > 512 ? std::max<int64_t>(1, room / base) : 1;
+    int64_t kc = (a->s.max_len + want - 1) / want;
+    kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
+    a->nsplit = want == 1 ? 1 : (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
+    a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
+    // All at once: as long as the longest.  Else the room shares the keys, and at the end half of
+    // one of the last, which have fewest, is not shared.
+    if (base * a->nsplit <= room) return std::min<int64_t>(a->kc, a->s.max_len);
+    const int64_t spread = a->tree ? 0 : a->s.max_new;
+    return base * (a->s.max_len - spread / 2) / room + (a->s.max_len - spread) / 2;
+  };
+  a->keys = rows <= 16 || (rows <= 256 && heads * ((rows + 15) / 16) <= ctx->num_cus);
+  if (a->keys) {
+    plan(16, 2);
+  } else if (a->c.dp > 128) {
+    plan(64, 2);
+  } else {
+    // 64 rows cost 7/8 of what 128 do, with three at once instead of two.
+    const int64_t few = plan(64, 3) * 7, many = plan(128, 2) * 8;
+    if (few < many) plan(64, 3);
+  }
   a->parts = heads * rows * a->nsplit;
   return a->nsplit == 1 ? 0 : (size_t)a->parts * (a->c.dp * 4 + sizeof(float2));
 }
