@@ -776,7 +776,8 @@ mg_status mg_kv_cache_slots(const mg_seq_batch *seqs, int64_t pages, int64_t pag
 /* Writes the rows' keys and values: k_dev / v_dev row r, head h at r * stride + h *
  * head_size (stride 0 = kv_heads * head_size).  With rope (may be NULL) keys are rotated
  * first, at rope->positions[r] or, NULL, at their position in the sequence; a position
- * outside the tables makes the key NaN. */
+ * outside the tables makes the key NaN.  More than 67108856 new rows a sequence:
+ * MG_UNSUPPORTED. */
 mg_status mg_kv_cache_append_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
                                      const float *k_dev, int64_t k_stride, const float *v_dev,
                                      int64_t v_stride, const mg_rope *rope);

@@ -2662,6 +2662,8 @@ mg_status check_rope(const char *what, const mg_rope &r, int64_t head_size) {
 
 // Most rows, positions and tokens of a batch (32-bit indices in the kernels).
 constexpr int64_t MG_KV_MOST = 0x7fffff00;
+// Most new rows of a sequence that one call writes or reads (four a workgroup).
+constexpr int64_t MG_KV_MOST_NEW = 4 * (MG_MOST_GROUPS - 1);
 
 mg_status check_seqs(const char *what, const mg_seq_batch *s) {
   if (!s) return bad_arg(what, "null batch");
@@ -2763,7 +2765,7 @@ mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t b
   ProfScope prof_(ctx, what);
   g_last_error.clear();
   if (!ctx || !rope) return bad_arg(what, "null argument");
-  constexpr int64_t most = (int64_t)1 << 38;  // elements: a grid below 2^31 workgroups
+  constexpr int64_t most = (int64_t)1 << 38;  // elements
   if (batch < 0 || seq < 0 || heads < 0 || head_size < 1 || batch > most || seq > 0x7fffffff ||
       heads > most || head_size > 65536 || (batch && seq > most / batch) ||
       (batch * seq && heads * head_size > most / (batch * seq)))
@@ -2922,6 +2924,7 @@ mg_status mg_kv_cache_append_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_s
   MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
   MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
   if (rope) MG_TRY(check_rope(what, *rope, cache->d));
+  if (seqs->max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheAppend: too many rows");
   if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
   if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
   MG_TRY(mg_use_device(ctx));
@@ -2938,6 +2941,7 @@ mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq
   MG_TRY(check_cache(what, ctx, cache, seqs));
   MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
   MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
+  if (seqs->max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheRead: too many rows");
   if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
   if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
   MG_TRY(mg_use_device(ctx));
@@ -2983,8 +2987,8 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   MG_TRY(mg_use_device(ctx));
   // Without the workspace (byte budget, stream capture) the keys are not split.
   if (need && !mg_ws_optional(ctx, need)) need = mg_kv_attn_plan(ctx, &a, false);
-  if ((int64_t)a.s.batch * a.nsplit * a.nblk * a.c.kv_heads > 0x7fffffff ||
-      (a.nsplit > 1 && a.s.batch * a.c.kv_heads * a.s.max_new * a.group > 0x7fffffff))
+  if ((int64_t)a.s.batch * a.nsplit * a.nblk * a.c.kv_heads > MG_MOST_GROUPS ||
+      (a.nsplit > 1 && a.s.batch * a.c.kv_heads * a.s.max_new * a.group > MG_MOST_GROUPS))
     return mg_fail(MG_UNSUPPORTED, "KvCacheAttention: too many rows");
   MG_TRY(mg_check_control(ctx, (int64_t)need));
   return mg_kv_attn_run(ctx, a, ctx->ws);

@@ -1006,9 +1006,9 @@ size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
     a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
     // All at once: as long as the longest.  Else the room shares the keys, and at the end half of
     // one of the last, which have fewest, is not shared.
-    if (base * a->nsplit <= room) return std::min<int64_t>(a->kc, a->s.max_len);
-    const int64_t spread = a->tree ? 0 : a->s.max_new;
-    return base * (a->s.max_len - spread / 2) / room + (a->s.max_len - spread) / 2;
+    if (base * a->nsplit <= room) return (double)std::min<int64_t>(a->kc, a->s.max_len);
+    const double len = (double)a->s.max_len, spread = a->tree ? 0 : (double)a->s.max_new;
+    return (double)base * (len - spread / 2) / (double)room + (len - spread) / 2;
   };
   a->keys = rows <= 16 || (rows <= 256 && heads * ((rows + 15) / 16) <= ctx->num_cus);
   if (a->keys) {
@@ -1017,7 +1017,7 @@ size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
     plan(64, 2);
   } else {
     // 64 rows cost 7/8 of what 128 do, with three at once instead of two.
-    const int64_t few = plan(64, 3) * 7, many = plan(128, 2) * 8;
+    const double few = plan(64, 3) * 7, many = plan(128, 2) * 8;
     if (few < many) plan(64, 3);
   }
   a->parts = heads * rows * a->nsplit;

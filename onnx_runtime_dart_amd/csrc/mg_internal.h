@@ -170,6 +170,8 @@ mg_status mg_use_device(mg_ctx *ctx);
 // staging slot are copied and waited for.
 mg_status mg_h2d_table(mg_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes);
 mg_status mg_launch_check(const char *what);
+// Most workgroups of 256 threads of a launch: its threads count in 32 bits.
+constexpr int64_t MG_MOST_GROUPS = 0xffffff;
 
 static inline size_t mg_align(size_t x, size_t a = 256) {
   return (x + a - 1) / a * a;

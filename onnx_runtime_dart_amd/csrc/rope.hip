@@ -139,9 +139,10 @@ __global__ __launch_bounds__(256) void k_rotate(const mg_rotate_problem p, IX to
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int W>
-void rotate(mg_ctx *ctx, const mg_rotate_problem &p) {
+mg_status rotate(mg_ctx *ctx, const mg_rotate_problem &p) {
   const int64_t units = (p.d - p.rope.half_rot) / W, groups = (p.heads + kHeads - 1) / kHeads;
   const int64_t n = p.batch * p.seq * groups * units;
+  if (n > 256 * MG_MOST_GROUPS) return mg_fail(MG_UNSUPPORTED, "RotaryEmbedding: too many elements");
   const dim3 grid((unsigned)((n + 255) / 256));
   // 32-bit indices where they suffice: their divisions cost a fraction of the 64-bit ones
   // (8191 rows of 32 heads: 166 us with 64-bit indices and an element a thread).
@@ -151,6 +152,7 @@ void rotate(mg_ctx *ctx, const mg_rotate_problem &p) {
   else
     k_rotate<W, uint64_t><<<grid, dim3(256), 0, ctx->stream>>>(p, (uint64_t)n, (uint64_t)units,
                                                                (uint64_t)groups);
+  return mg_launch_check("rotary embedding");
 }
 
 }  // namespace
@@ -162,7 +164,9 @@ mg_status mg_rope_tables_run(mg_ctx *ctx, int64_t first, int64_t count, int64_t 
     f.turns[i] = i < half ? freq[i] * 0.15915494309189533577 : 0.0;
   const int64_t n = count * half;
   const bool quad = half % 4 == 0 && aligned16(c) && aligned16(s);
-  const dim3 grid((unsigned)((n + (quad ? 1023 : 255)) / (quad ? 1024 : 256)));
+  const int64_t groups = (n + (quad ? 1023 : 255)) / (quad ? 1024 : 256);
+  if (groups > MG_MOST_GROUPS) return mg_fail(MG_UNSUPPORTED, "RotaryTables: too many entries");
+  const dim3 grid((unsigned)groups);
   hipStream_t st = ctx->stream;
   if (quad && n < 0x7ffffc00)
     k_rope_tables<4, uint32_t><<<grid, dim3(256), 0, st>>>(f, first, (uint32_t)n, (uint32_t)half,
@@ -183,9 +187,5 @@ mg_status mg_rotate_run(mg_ctx *ctx, const mg_rotate_problem &p) {
   bool quad = aligned16(p.x) && aligned16(p.y) && aligned16(p.rope.cos_table) &&
               aligned16(p.rope.sin_table) && p.d % 4 == 0 && p.rope.half_rot % 4 == 0;
   for (int i = 0; i < 3; i++) quad = quad && p.xs[i] % 4 == 0 && p.ys[i] % 4 == 0;
-  if (quad)
-    rotate<4>(ctx, p);
-  else
-    rotate<1>(ctx, p);
-  return mg_launch_check("rotary embedding");
+  return quad ? rotate<4>(ctx, p) : rotate<1>(ctx, p);
 }

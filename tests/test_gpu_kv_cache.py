@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import kv_reference as R
+from onnx_runtime_dart_amd.errors import UnsupportedError
 
 pytestmark = pytest.mark.gpu
 
@@ -480,6 +481,20 @@ def test_loose_bounds(ops):
     assert not cache.refused()
     for x in dev:
         x.free()
+    cache.release()
+
+
+def test_more_rows_than_a_launch_takes(ops):
+    # Refused from the bounds alone, whatever the arrays hold.
+    cache = ops.KvCache(1, kv_heads=4096, head_size=1, page_size=16)
+    x = ops.DeviceBuffer.from_array(np.zeros(100, np.int32))
+    s = ops.SeqBatch(batch=65535, rows=2**31 - 256, max_new=2**31 - 256, max_len=2**31 - 256,
+                     row_start_ptr=x.ptr, past_ptr=x.ptr, page_table_ptr=x.ptr, table_stride=1)
+    with pytest.raises(UnsupportedError):
+        cache.attend_dev(s, x.ptr, x.ptr, 4096)
+    with pytest.raises(UnsupportedError):
+        cache.attend_dev(s, x.ptr, x.ptr, 8192)
+    x.free()
     cache.release()
 
 

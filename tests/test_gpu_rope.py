@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from kv_reference import rotate
+from onnx_runtime_dart_amd.errors import UnsupportedError
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,14 @@ def test_infinities_stay_in_their_pair(ops):
     want[0, 0, [3, 7]] = True
     want[0, 1, [1, 5]] = True
     np.testing.assert_array_equal(bad, want)
+
+
+def test_more_than_a_launch_takes(ops):
+    # Refused from the sizes alone: the buffers hold a hundred elements.
+    x = ops.DeviceBuffer.from_array(np.zeros(100, np.float32))
+    rope = ops.Rope(x.ptr, x.ptr, max_pos=1, half_rot=1)
+    with pytest.raises(UnsupportedError):
+        ops.rotary_embedding_dev(x.ptr, 1, 2**31 - 1, 8, 3, rope, x.ptr)
+    with pytest.raises(UnsupportedError):
+        ops.rotary_tables_dev(x.ptr, x.ptr, 0, 2**31 - 1, 127)
+    x.free()

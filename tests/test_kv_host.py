@@ -84,6 +84,12 @@ def test_null_buffers_strides_and_heads():
     assert append(cache=other) == attend(cache=other) == 1
 
 
+def test_more_rows_than_a_launch_takes():
+    n = 67108857
+    s = seqs(rows=n, max_new=n, max_len=n)
+    assert append(s) == read(s) == 2
+
+
 def test_nothing_to_do_needs_no_device():
     none = seqs(batch=0, row_start_ptr=0, past_ptr=0, page_table_ptr=0)
     empty = seqs(rows=0, max_new=0, row_start_ptr=0, past_ptr=0, page_table_ptr=0)
