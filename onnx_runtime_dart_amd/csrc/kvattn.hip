@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "kv_common.h"
@@ -989,10 +990,10 @@ void launch_dims(mg_ctx *ctx, const mg_kv_attn &a) {
 
 size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
   const int64_t rows = a->s.max_new * a->group, heads = a->s.batch * a->c.kv_heads;
-  // The plan with workgroups of rows_wg rows, `per_cu` of which run at once on a compute unit (more
-  // start late, and a start, lengths, pages and queries, costs what some ten tiles do).  Returns
-  // the keys that a place at work passes over.
-  const auto plan = [&](int rows_wg, int per_cu) {
+  // Fills the plan with workgroups of rows_wg rows, `per_cu` of which run at once on a compute unit,
+  // and returns about how many microseconds it takes, with `start` for a workgroup's lengths, pages
+  // and queries and `tile` for 32 keys.
+  const auto plan = [&](int rows_wg, int per_cu, double start, double tile) {
     const int64_t room = (int64_t)per_cu * ctx->num_cus;
     a->rows_wg = rows_wg;
     a->nblk = (int)((rows + rows_wg - 1) / rows_wg);
@@ -1004,22 +1005,31 @@ size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
     kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
     a->nsplit = want == 1 ? 1 : (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
     a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
+    // The join writes and reads partial results, at some 4 MB a microsecond.
+    const double join = a->nsplit > 1 ? 4 + 2e-6 * (double)(heads * rows * a->nsplit * a->c.dp) : 0;
     // All at once: as long as the longest.  Else the room shares the keys, and at the end half of
     // one of the last, which have fewest, is not shared.
-    if (base * a->nsplit <= room) return (double)std::min<int64_t>(a->kc, a->s.max_len);
     const double len = (double)a->s.max_len, spread = a->tree ? 0 : (double)a->s.max_new;
-    return (double)base * (len - spread / 2) / (double)room + (len - spread) / 2;
+    const double n = (double)base / (double)room;
+    if (base * a->nsplit <= room) return start + join + tile / 32 * (double)std::min<int64_t>(a->kc, a->s.max_len);
+    return start * std::ceil(n) + tile / 32 * (n * (len - spread / 2) + (len - spread) / 2);
   };
-  a->keys = rows <= 16 || (rows <= 256 && heads * ((rows + 15) / 16) <= ctx->num_cus);
-  if (a->keys) {
-    plan(16, 2);
-  } else if (a->c.dp > 128) {
-    plan(64, 2);
-  } else {
-    // 64 rows cost 7/8 of what 128 do, with three at once instead of two.
-    const double few = plan(64, 3) * 7, many = plan(128, 2) * 8;
-    if (few < many) plan(64, 3);
-  }
+  // Measured at full use and with few workgroups (int8, D 128): a tile of 32 keys takes one of 16
+  // rows 0.5 us (its four waves have four tiles under way), one of 64 rows 1.8, one of 128 rows
+  // 2.1; heads above 128 have the registers for one workgroup of 16 rows a compute unit, two of 64.
+  // Chosen so against the other two kinds: 256 rows' prompt over 2000 keys, D 64, by 16 rows 24 us,
+  // 64 44, 128 47; 4096 rows of D 96 from none 220, 160 and 205; 2048 rows over 6000 keys, D 128,
+  // 680, 561 and 454.
+  const bool wide = a->c.dp > 128;
+  const double size = a->c.dp / 128.0;
+  const auto by16 = [&] { return plan(16, wide ? 1 : 2, 5, 0.5 * size); };
+  const auto by64 = [&] { return plan(64, wide ? 2 : 3, 9, wide ? 2 : 0.4 + 1.4 * size); };
+  const auto by128 = [&] { return plan(128, 2, 12, 0.5 + 1.6 * size); };
+  const double none = std::numeric_limits<double>::infinity();
+  const double t128 = wide || rows <= 64 ? none : by128(), t64 = rows <= 16 ? none : by64();
+  const double t16 = by16();
+  a->keys = t16 <= std::min(t64, t128);
+  if (!a->keys) t64 <= t128 ? by64() : by128();
   a->parts = heads * rows * a->nsplit;
   return a->nsplit == 1 ? 0 : (size_t)a->parts * (a->c.dp * 4 + sizeof(float2));
 }
