@@ -313,12 +313,13 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
 // One tile's weights for QB blocks of 16 rows: the scores of the lane's eight keys, in units that
 // make its running maximum m current, and from them the digits of the weights times the V scales.
 // l and z are the lane's share of the sum and (INT4) of the sum of weights times middles.
-// masked: only the keys of `seen` count (a branch of the whole wave, or a constant).  `between`
-// is work of the caller's that runs along with the exponentials.
-template <int FMT, int NB, int QB, class Between>
-__device__ inline void weigh(Between between, bool masked, const float4v (&acc)[QB][2], const float (&ksf)[8],
+// masked: only the keys of `seen` count (a branch of the whole wave, or a constant), and the V scales
+// want the factors `unit` of the rows yet (null: none).
+template <int FMT, int NB, int QB>
+__device__ inline void weigh(bool masked, const float4v (&acc)[QB][2], const float (&ksf)[8],
                              const float (&vsn)[8], const float (&kzf)[8], const float (&vz)[8],
-                             const float (&qs)[QB], const uint32_t (&seen)[QB], float (&m)[QB],
+                             const float (&qs)[QB], const uint32_t (&seen)[QB],
+                             const float *unit, float (&m)[QB],
                              float (&l)[QB], float (&z)[QB], float4v (&o)[QB][NB],
                              half8v (&ph)[QB], half8v (&pl)[QB]) {
   float d[QB][8];  // scores less m, of unseen keys too
@@ -360,16 +361,19 @@ __device__ inline void weigh(Between between, bool masked, const float4v (&acc)[
       for (int i = 0; i < NB; i++) o[q][i] *= by;
     }
     scores();
+    // (A score of 2^31 and more is rounded by more than exponents have room for.)
+#pragma unroll
+    for (int q = 0; q < QB; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) d[q][j] = d[q][j] > kSlack ? kSlack : d[q][j];
   }
-  between();
-  float e[QB][8], w[QB][8], zs[QB][8];
+  float e[QB][8], w[QB][8];
 #pragma unroll
   for (int q = 0; q < QB; q++)
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       e[q][j] = exp2_of(d[q][j]);
       w[q][j] = e[q][j] * vsn[j];
-      if (FMT == MG_KV_INT4) zs[q][j] = e[q][j] * vz[j];
     }
   if (masked) {
     // An unseen key counts nothing, whatever its score and scales are.  (The empty statement
@@ -381,9 +385,14 @@ __device__ inline void weigh(Between between, bool masked, const float4v (&acc)[
       for (int j = 0; j < 8; j++) {
         const bool on = seen[q] >> j & 1;
         e[q][j] = on ? e[q][j] : 0.f;
-        w[q][j] = on ? w[q][j] : 0.f;
-        if (FMT == MG_KV_INT4) zs[q][j] = on ? zs[q][j] : 0.f;
+        w[q][j] = on ? (unit ? w[q][j] * unit[256 * q] : w[q][j]) : 0.f;
+        if (FMT == MG_KV_INT4) z[q] += on ? e[q][j] * vz[j] : 0.f;
       }
+  } else if (FMT == MG_KV_INT4) {
+#pragma unroll
+    for (int q = 0; q < QB; q++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) z[q] = fmaf(e[q][j], vz[j], z[q]);
   }
 #pragma unroll
   for (int q = 0; q < QB; q++)
@@ -393,7 +402,6 @@ __device__ inline void weigh(Between between, bool masked, const float4v (&acc)[
   for (int q = 0; q < QB; q++)
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      if (FMT == MG_KV_INT4) z[q] += zs[q][j] + zs[q][j + 1];
       const half2v hi = __builtin_convertvector(float2v{w[q][j], w[q][j + 1]}, half2v);
       ph[q][j] = hi[0];
       ph[q][j + 1] = hi[1];
@@ -418,23 +426,6 @@ __device__ inline uint32_t seen_keys(const mg_kv_attn &a, const kv_seq &sq, int 
   return seen;
 }
 
-// The digits of 16 rows' queries in matrix order from shared memory, times dn.
-template <int FMT, int KS>
-__device__ inline void query_digits(const float *x, float dn, half8v (&qh)[KS], half8v (&ql)[KS],
-                                    float &qs) {
-  float sum = 0.f;
-#pragma unroll
-  for (int s = 0; s < KS; s++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float v = x[8 * s + k_slot<FMT>(j)] * dn;
-      const _Float16 hi = (_Float16)v;
-      qh[s][j] = hi;
-      ql[s][j] = rest_of(v, hi);
-      sum += v;
-    }
-  qs = FMT == MG_KV_INT4 ? row_sum(sum) : 0.f;
-}
 // Largest finite size among n elements.
 __device__ inline float largest(const float *x, int n, float mx) {
 #pragma unroll
@@ -443,6 +434,32 @@ __device__ inline float largest(const float *x, int n, float mx) {
     mx = v < __builtin_inff() ? fmaxf(mx, v) : mx;
   }
   return mx;
+}
+
+// The digits of 16 rows' queries in matrix order from shared memory (x: the lane's run), times a
+// power of two: a row's largest element comes under 2^15, so that a digit pair is exact to 2^-22 of
+// any element down to 2^-17 of the largest, and to 2^-39 of the largest below.  Rows share the
+// power dn of the largest of them all, max; one 2^12 below has its own, and `own` gives its scores
+// the units of the others (1 for those): a row does not see how large another is.
+// row: the row's largest.
+template <int FMT, int KS>
+__device__ inline void query_digits(const float *x, float row, float max, float dn, half8v (&qh)[KS],
+                                    half8v (&ql)[KS], float &qs, float &own) {
+  const bool apart = row != 0.f && row < 0x1p-12f * max;
+  const float mine = apart ? 32768.f * pow2_under(row) : dn;
+  own = apart ? dn / mine : 1.f;
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; s++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float v = x[8 * s + k_slot<FMT>(j)] * mine;
+      const _Float16 hi = (_Float16)v;
+      qh[s][j] = hi;
+      ql[s][j] = rest_of(v, hi);
+      sum += v;
+    }
+  qs = FMT == MG_KV_INT4 ? row_sum(sum) * own : 0.f;
 }
 
 // Which sequence, split, row block and KV head a workgroup has (heads innermost), and its keys.
@@ -510,7 +527,7 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   constexpr int DP = S::DP, KS = S::KS, KW = S::KW, QP = DP + 4, STEP = 128;
   // 16 rows' queries; later the four waves' results.
   __shared__ __attribute__((aligned(16))) float lds[64 * QP];
-  __shared__ float stat[4][2][16];
+  __shared__ float stat[4][2][16], units[4][64];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   Work w;
@@ -536,13 +553,14 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   }
   stage_queries<DP>(a, sq, w.h, w.r0, w.rows, 16, lds);
   __syncthreads();
-  // One power of two for the rows: the largest element under 2^15, so that a digit pair is
-  // exact to 2^-22 of any element down to 2^-17 of it, and to 2^-39 of it below.
   const float *x = lds + c * QP + g * (DP / 4);
-  const float dn = 32768.f * pow2_under(wave_max(largest(x, DP / 4, 0.f))), f = 1.f / dn;
+  const float row = row_max(largest(x, DP / 4, 0.f)), mx = wave_max(row);
+  const float dn = 32768.f * pow2_under(mx), f = 1.f / dn;
   half8v qh[KS], ql[KS];
-  float qs[1];
-  query_digits<FMT, KS>(x, dn, qh, ql, qs[0]);
+  float qs[1], own;
+  query_digits<FMT, KS>(x, row, mx, dn, qh, ql, qs[0], own);
+  const bool uneven = __any(own != 1.f);
+  units[wave][lane] = own;
   const int qi = min(w.r0 + c, w.rows - 1) / a.group;
   const int see = a.tree ? sq.past : sq.past + qi + 1;
   const int64_t word = (int64_t)(sq.start + qi) * a.tree_words;
@@ -588,26 +606,27 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
       spread(kzf, t.kz, f);
       spread(vz, t.vz, 1.f);
     }
-    // V scales relative to the largest seen.
-    {
-      float big = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        if (MASKED && t0 + 16 * (j >> 2) + 4 * g + (j & 3) >= kfin) vsn[j] = 0.f;
-        big = fmaxf(big, vsn[j]);
-      }
-      if (__builtin_expect(__any(big * vn > 16.f), 0)) {
-        const float now = 8.f * pow2_under(wave_max(big)), by = now / vn;
-        vn = now;
-#pragma unroll
-        for (int i = 0; i < NB; i++) o[0][i] *= by;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) vsn[j] *= vn;
-    }
-    half8v ph[1], pl[1];
     const uint32_t seen[1] = {MASKED ? seen_keys(a, sq, t0, g, see, word, kfin) : 0xffu};
-    weigh<FMT, NB, 1>([] {}, MASKED, acc, ksf, vsn, kzf, vz, qs, seen, m, l, z, o, ph, pl);
+    // V scales relative to the largest that the row has seen.
+    float big = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (MASKED) vsn[j] = seen[0] >> j & 1 ? vsn[j] : 0.f;
+      big = fmaxf(big, vsn[j]);
+    }
+    if (__builtin_expect(__any(big * vn > 16.f) || uneven, 0)) {
+      big = row_max(big);
+      const float now = big * vn > 16.f ? 8.f * pow2_under(big) : vn, by = now / vn;
+      vn = now;
+#pragma unroll
+      for (int i = 0; i < NB; i++) o[0][i] *= by;
+      acc[0][0] *= units[wave][lane];
+      acc[0][1] *= units[wave][lane];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) vsn[j] *= vn;
+    half8v ph[1], pl[1];
+    weigh<FMT, NB, 1>(MASKED, acc, ksf, vsn, kzf, vz, qs, seen, nullptr, m, l, z, o, ph, pl);
     if (!AHEAD && more) next.load_scales(a, p, g);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -729,7 +748,7 @@ struct Quarter {
 // code is then converted once for 64 QB rows, not by every wave, and its 16-byte operands cost a
 // quarter of what the products take.
 template <int FMT, int NB, int QB>
-__global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(const mg_kv_attn a) {
+__global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2) void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;
   constexpr int KO = 2 * KS * 64, VO = NB * 64;  // operands of a tile
@@ -740,8 +759,8 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
     } t;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
-  __shared__ __attribute__((aligned(16))) float sc[2][4][32];  // scales of a tile's keys
-  __shared__ float unit[2], size[4];
+  __shared__ __attribute__((aligned(16))) float sc[2][5][32];  // scales of a tile's keys
+  __shared__ float unit[2], size[4], units[QB * 256], mine[QB * 256];  // of a lane's rows
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   Work w;
@@ -770,23 +789,27 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
 
   stage_queries<DP>(a, sq, w.h, w.r0, w.rows, ROWS, sh.q);
   __syncthreads();
-  float mx = 0.f;
+  float row[QB], mx = 0.f;
 #pragma unroll
-  for (int qb = 0; qb < QB; qb++)
-    mx = largest(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), DP / 4, mx);
+  for (int qb = 0; qb < QB; qb++) {
+    row[qb] = row_max(largest(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), DP / 4, 0.f));
+    mx = fmaxf(mx, row[qb]);
+  }
   mx = wave_max(mx);
   if (lane == 0) size[wave] = mx;
   __syncthreads();
-  // One power of two for the workgroup's rows, as in k_kv_keys.
-  const float dn = 32768.f * pow2_under(fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3])));
-  const float f = 1.f / dn;
+  mx = fmaxf(fmaxf(size[0], size[1]), fmaxf(size[2], size[3]));
+  const float dn = 32768.f * pow2_under(mx), f = 1.f / dn;
   half8v qh[QB][KS], ql[QB][KS];
   float qs[QB];
-  int qi[QB];
+  bool uneven = false;
 #pragma unroll
   for (int qb = 0; qb < QB; qb++) {
-    query_digits<FMT, KS>(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), dn, qh[qb], ql[qb], qs[qb]);
-    qi[qb] = min(first + qb * 16 + c, w.rows - 1) / a.group;
+    float own;
+    query_digits<FMT, KS>(sh.q + (wr0 + qb * 16 + c) * QP + g * (DP / 4), row[qb], mx, dn, qh[qb],
+                          ql[qb], qs[qb], own);
+    uneven |= __any(own != 1.f);
+    units[qb * 256 + threadIdx.x] = own;
   }
   __syncthreads();  // the queries' place is the tiles' now
 
@@ -801,12 +824,13 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
       if (lane < 32) {
         sc[at][0][lane] = raw.none ? __builtin_nanf("") : raw.ks * f;
         sc[at][1][lane] = vs * vn;
+        sc[at][4][lane] = vs * 0x1p-20f;
         if (FMT == MG_KV_INT4) {
           sc[at][2][lane] = raw.kz * f;
           sc[at][3][lane] = raw.vz;
         }
       }
-      if (lane == 0) unit[at] = vn;
+      if (lane == 0) unit[at] = vn * 0x1p20f;
     }
   };
 
@@ -819,7 +843,10 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
 #pragma unroll
     for (int i = 0; i < NB; i++) o[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
-  float mine = ldexpf(1.f, 100);  // the unit of this wave's outputs
+  // The units of the wave's outputs, times 2^20: of plain tiles, and (mine) by rows.
+  float last = 0x1p120f;
+#pragma unroll
+  for (int qb = 0; qb < QB; qb++) mine[qb * 256 + threadIdx.x] = last;
   auto tile = [&](int at, int t0) __attribute__((always_inline)) {
     const bool masked = t0 + 32 > plain;  // some row may not see some key
     float4v acc[QB][2];
@@ -842,28 +869,42 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
     for (int k = 0; k < (FMT == MG_KV_INT4 ? 4 : 2); k++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const float4 v = *reinterpret_cast<const float4 *>(&sc[at][k][16 * u + 4 * g]);
+        const float4 v = *reinterpret_cast<const float4 *>(
+            &sc[at][k == 1 && masked ? 4 : k][16 * u + 4 * g]);
         x[k][4 * u] = v.x, x[k][4 * u + 1] = v.y, x[k][4 * u + 2] = v.z, x[k][4 * u + 3] = v.w;
       }
-    const float now = unit[at];
-    if (__builtin_expect(__any(now != mine), 0)) {
-      const float by = now / mine;
-      mine = now;
-#pragma unroll
-      for (int qb = 0; qb < QB; qb++)
-#pragma unroll
-        for (int i = 0; i < NB; i++) o[qb][i] *= by;
-    }
     half8v ph[QB], pl[QB];
     uint32_t seen[QB];
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) {
-      seen[qb] = 0xffu;
-      if (masked)
-        seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi[qb] + 1,
-                             (int64_t)(sq.start + qi[qb]) * a.tree_words, kfin);
+    for (int qb = 0; qb < QB; qb++) seen[qb] = 0xffu;
+    // Units of the V scales: a tile that every row sees has the workgroup's, the rows of a
+    // masked one their own, by the keys that they see.  (Masked tiles come last.)
+    const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit[at])));
+    if (__builtin_expect(masked || now != last || uneven, 0)) {
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++) {
+        const float was = mine[qb * 256 + threadIdx.x];
+        float next = now;
+        if (masked) {
+          const int qi = min(first + qb * 16 + c, w.rows - 1) / a.group;
+          seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi + 1,
+                               (int64_t)(sq.start + qi) * a.tree_words, kfin);
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; j++) big = seen[qb] >> j & 1 ? fmaxf(big, x[1][j]) : big;
+          big = row_max(big);
+          next = big * was > 16.f ? 8.f * pow2_under(big) : was;
+        }
+        const float by = next / was, own = units[qb * 256 + threadIdx.x];
+        mine[qb * 256 + threadIdx.x] = next;
+#pragma unroll
+        for (int i = 0; i < NB; i++) o[qb][i] *= by;
+        acc[qb][0] *= own;
+        acc[qb][1] *= own;
+      }
+      last = now;
     }
-    weigh<FMT, NB, QB>([] {}, masked, acc, x[0], x[1], x[2], x[3], qs, seen, m, l, z, o, ph, pl);
+    weigh<FMT, NB, QB>(masked, acc, x[0], x[1], x[2], x[3], qs, seen, mine + threadIdx.x, m, l, z, o, ph, pl);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const half8v va = __builtin_bit_cast(half8v, sh.t.v[at][i * 64 + lane]);
@@ -889,9 +930,9 @@ __global__ __launch_bounds__(256, NB <= 8 && QB == 1 ? 3 : 2) void k_kv_rows(con
   }
 
   if (refused && lane == 0) atomicOr(a.c.refused, 1);
-  const float iv = 1.f / mine;
 #pragma unroll
   for (int qb = 0; qb < QB; qb++) {
+    const float iv = 0x1p20f / mine[qb * 256 + threadIdx.x];
     const int r = wr0 + qb * 16 + c;
     const float ll = row_sum(l[qb]), zz = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
 #pragma unroll

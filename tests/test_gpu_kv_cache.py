@@ -424,6 +424,98 @@ def test_scales_far_apart(ops, fmt):
     cache.release()
 
 
+# Many short prompts: workgroups of 64 rows; longer ones: of 128 (heads up to 128).
+MANY = [(40, 16), (32, 64)]
+
+
+def many(rng, count, most, page=16, past=100):
+    """A batch of `count` sequences, up to `most` new rows each (some of them none or one)."""
+    new = rng.integers(2, most + 1, count)
+    new[0], new[1], new[2] = most, 0, 1
+    return R.Batch(rng, [int(n) for n in new], rng.integers(0, past, count), page, extra_rows=1)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("d", [33, 64, 128, 160, 256])
+@pytest.mark.parametrize("count, most", MANY)
+def test_many_rows(ops, fmt, d, count, most):
+    rng = np.random.default_rng(d + count)
+    b = many(rng, count, most, past=260)
+    cache, ks, vs = filled(ops, rng, b, 8, d, fmt, 1.5)
+    q = normal(rng, b.rows, 32, d)
+    y = cache.attend(q, **b.args())
+    check_rows(y, q, b, ks, vs, 1 / np.sqrt(d))
+    assert not y[-1:].any()
+    tree = np.zeros((b.rows, 1), np.uint64)
+    for i, n in enumerate(b.new):
+        tree[b.row_start[i]:b.row_start[i + 1]] = tree_words(rng, n, 1)
+    tree[1] = 0
+    cos, sin = tables(rng, 400, d // 2)
+    pos = np.concatenate([p + np.arange(n) for n, p in zip(b.new, b.past)] + [[0]])
+    y = cache.attend(q, **b.args(), tree=tree, rope=(cos, sin, False))
+    check_rows(y, R.rotate(q, cos, sin, pos, False), b, ks, vs, 1 / np.sqrt(d), tree)
+    cache.release()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("kv, group, new, past, d", [(1, 16, 500, 8000, 128), (1, 8, 500, 3000, 256)])
+def test_long_prompt_chunks(ops, fmt, kv, group, new, past, d):
+    # Row blocks and key splits at once; a sample of the rows is compared.
+    rng = np.random.default_rng(past)
+    b = R.Batch(rng, [new], [past], 64)
+    cache, ks, vs = filled(ops, rng, b, kv, d, fmt)
+    q = normal(rng, new, kv * group, d)
+    y = cache.attend(q, **b.args())
+    see = R.visible(new, past)
+    for r in (0, 1, 127, 128, 300, new - 1):
+        want = R.attend(q[r:r + 1], ks[0], vs[0], see[r:r + 1], 1 / np.sqrt(d))
+        assert np.abs(y[r] - want).max() <= R.bound(q[r], ks[0], vs[0], 1 / np.sqrt(d))
+    cache.release()
+
+
+def check_each_row(y, q, b, ks, vs, scale, tree=None):
+    """As check_rows, a row's bound from its own query and what it sees alone."""
+    for i, (k, v) in enumerate(zip(ks, vs)):
+        r = slice(b.row_start[i], b.row_start[i + 1])
+        see = R.visible(b.new[i], int(b.past[i]), None if tree is None else tree[r])
+        want = R.attend(q[r], k, v, see, scale)
+        for j, row in enumerate(range(r.start, r.stop)):
+            for h in range(q.shape[1]):
+                at = (row, slice(h, h + 1))
+                err = np.abs(y[at] - want[j, h]).max()
+                tol = R.bound(q[at], k[see[j]], v[see[j]], scale) if see[j].any() else 0
+                assert err <= tol, (i, j, h, err, tol)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("count, most, d", [(2, 16, 64), (40, 16, 64), (32, 64, 64), (32, 64, 128),
+                                            (2, 16, 256), (40, 16, 256)])
+def test_rows_do_not_feel_one_another(ops, fmt, count, most, d):
+    # Queries and values of neighbouring rows 2^40 and more apart: what a row does not see, and
+    # how large another row's query is, costs it nothing.
+    rng = np.random.default_rng(d + most)
+    new = rng.integers(2, most + 1, count)
+    new[0] = most
+    b = R.Batch(rng, [int(n) for n in new], rng.integers(0, 40, count), 16)
+    n = [int(x) for x in b.past + b.new]
+    k, v = normal(rng, sum(n), 8, d), normal(rng, sum(n), 8, d)
+    v *= np.exp2(rng.choice([-50, 0, 30], sum(n)))[:, None, None].astype(np.float32)
+    cache = ops.KvCache(b.pages, kv_heads=8, head_size=d, page_size=16, fmt=fmt)
+    cache.append(k, v, row_start=np.concatenate([[0], np.cumsum(n)]), past=np.zeros(count),
+                 page_table=b.page_table)
+    cut = np.cumsum(n)[:-1]
+    ks, vs = np.split(R.cached(k, fmt), cut), np.split(R.cached(v, fmt), cut)
+    q = normal(rng, b.rows, 32, d)
+    q[rng.random((b.rows, 32)) < 0.1] *= np.float32(2.0**40)
+    q[rng.random((b.rows, 32)) < 0.1] *= np.float32(2.0**-40)
+    tree = np.zeros((b.rows, 1), np.uint64)
+    for i, m in enumerate(b.new):
+        tree[b.row_start[i]:b.row_start[i + 1]] = tree_words(rng, m, 1)
+    for t in (None, tree):
+        check_each_row(cache.attend(q, **b.args(), tree=t), q, b, ks, vs, 1 / np.sqrt(d), t)
+    cache.release()
+
+
 def test_pages_beyond_32_bit_offsets(ops):
     # A cache of more than 2^32 code bytes, the sequence in its last pages.
     rng = np.random.default_rng(45)
