@@ -12,13 +12,18 @@
 // The alternatives: each wave keeps its 64 largest entries sorted across its lanes, as
 // (key, token) with key the logit's bits in an order that unsigned integers have (NaN
 // above all).  An entry enters when it beats the top-th one, found by one comparison per 16
-// logits and lane; the top-th largest of the lanes' own maxima over the first 16 bounds the
-// row's top-th from below, so that few entries enter only to leave again.  The sorted
-// lists of waves and of a row's runs join by taking the largest head, top times.
+// logits and lane; the top-th largest of the maxima of groups of the first chunk's logits
+// bounds the row's top-th from below, so that few entries enter only to leave again.  Up to ten
+// alternatives: entries enter one by one, and the sorted lists of waves and of a row's runs
+// join by taking the largest head, top times.  More: a chunk's entries are sorted 64 at a time
+// by a bitonic network of register moves, and lists join by its last six stages (1000 rows of
+// 32000, 64 alternatives: 119 us one by one, 68 so; 8 rows of 151936, 64: 61 and 19, 20: 20 and
+// 18, but 1: 9 and 16).
 //
 // The pass over the logits bounds it, 16-byte loads of which every lane has four in flight:
-// 1000 rows of 128256 in 107 us (4.8 TB/s, this card's copy rate; one logit a lane at a time
-// and every entry offered to the list: 358 us).
+// 1000 rows of 128256 with 8 alternatives in 105 us (4.9 TB/s, this card's copy rate; one logit
+// a lane at a time and every entry offered to the list: 358 us).  Few rows are bound by latency:
+// 8 rows of 151936 take 7 us without alternatives.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -128,16 +133,82 @@ __device__ inline void offer(List &l, uint32_t key, int id, bool ok, int top, in
     want &= __ballot(beats(key, id, l.tk, l.ti));
   }
 }
-// A bound from below of the n-th largest (from 1) of the lanes' keys, exact to its upper half: the
-// largest number with zeros in its lower half that n of them reach.
-__device__ inline uint32_t nth_largest(uint32_t x, int n) {
+// A bound from below of the n-th largest (from 1) of the lanes' N keys each, exact to its upper
+// half: the largest number with zeros in its lower half that n of them reach.
+template <int N>
+__device__ inline uint32_t nth_largest(const uint32_t (&x)[N], int n) {
   uint32_t least = 0;
 #pragma unroll
   for (int b = 31; b >= 16; b--) {
     const uint32_t t = least | 1u << b;
-    if (__popcll(__ballot(x >= t)) >= n) least = t;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) count += __popcll(__ballot(x[i] >= t));
+    if (count >= n) least = t;
   }
   return least;
+}
+
+// The value of lane l ^ X.
+template <int X>
+__device__ inline uint32_t across(uint32_t x) {
+  if constexpr (X == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true);
+  if constexpr (X == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true);
+  if constexpr (X == 4) {
+    // Four lanes up in a row's quads 0 and 2, four down in 1 and 3.
+    const int up = __builtin_amdgcn_update_dpp(0, (int)x, 0x104, 0xf, 0x5, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(up, (int)x, 0x114, 0xf, 0xa, false);
+  }
+  if constexpr (X == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true);
+  // (Both results of a swap of x with itself: the even parts' values, the odd parts'.)
+  if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return threadIdx.x & 32 ? r[0] : r[1];
+}
+// Orders entries of lanes l and l ^ X: the better to the lane that has bit X clear, or (up) set.
+template <int X>
+__device__ inline void order(uint32_t &key, int &id, bool up, int lane) {
+  const uint32_t k = across<X>(key);
+  const int i = (int)across<X>((uint32_t)id);
+  const bool first = ((lane & X) == 0) != up;
+  if (beats(k, i, key, id) == first) {  // (no two entries are equal but those of no token)
+    key = k;
+    id = i;
+  }
+}
+// Sorts a bitonic sequence of 2 X entries in every 2 X lanes.
+template <int X>
+__device__ inline void order_all(uint32_t &key, int &id, bool up, int lane) {
+  order<X>(key, id, up, lane);
+  if constexpr (X > 1) order_all<X / 2>(key, id, up, lane);
+}
+// The best 64 of the list, best first, and of entries given worst first.
+__device__ inline void merge(uint32_t &lk, int &li, uint32_t key, int id, int lane) {
+  if (beats(key, id, lk, li)) {
+    lk = key;
+    li = id;
+  }
+  order_all<32>(lk, li, false, lane);
+}
+// Puts 64 entries, one a lane, in any order, into the list.
+__device__ inline void merge_unsorted(List &l, uint32_t key, int id, int top, int lane) {
+  order_all<1>(key, id, (lane & 2) != 0, lane);
+  order_all<2>(key, id, (lane & 4) != 0, lane);
+  order_all<4>(key, id, (lane & 8) != 0, lane);
+  order_all<8>(key, id, (lane & 16) != 0, lane);
+  order_all<16>(key, id, (lane & 32) != 0, lane);
+  order_all<32>(key, id, true, lane);
+  merge(l.key, l.id, key, id, lane);
+  l.tk = lane_value(l.key, top - 1);
+  l.ti = lane_value(l.id, top - 1);
+}
+// The wave's own shared memory: writes before it are there for reads after it.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // Joins up to 64 sorted lists of `top` entries, lane l's at key[l * pitch], id[l * pitch]
@@ -206,10 +277,15 @@ __device__ inline void finish(const mg_logprobs &p, int64_t row, const Sums &t, 
 
 constexpr int kQuads = 4;              // quads of logits a lane takes at a time
 constexpr int kChunk = 64 * 4 * kQuads;  // logits a wave takes at a time
+// Candidates of a chunk put into the list one by one (some 120 cycles each); more are sorted 64 at a
+// time (some 1200).
+constexpr int kFew = 10;
+
+enum { NONE, FEW, MANY };  // alternatives: none, kFew at most, more
 
 // One workgroup a row (nsplit 1) or one of nsplit runs of a row; its waves take chunks of
 // the run in turn.
-template <bool TOP>
+template <int TOP>
 __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -226,6 +302,8 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   float m = kLowest, s = 0.f, a = 0.f;
   List l{0, 0, 0x7fffffff, 0x7fffffff};
   bool first = true;
+  __shared__ uint32_t ck[4][TOP == MANY ? 128 : 1];  // a wave's candidates, 64 to be sorted at once
+  __shared__ int ci[4][TOP == MANY ? 128 : 1];
   for (int64_t c0 = e0 + wave * kChunk; c0 < e1; c0 += 4 * kChunk) {
     float z[kQuads][4];
     const int64_t mine = c0 + lane * 4;
@@ -264,27 +342,71 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
       }
     if (TOP) {
       // (NaN: never the maximum, always a candidate.)
-      uint32_t bk = key_of(big);
-      bool odd = false;
+      uint32_t quad[kQuads];
+      uint32_t bk = 0;
 #pragma unroll
-      for (int q = 0; q < kQuads; q++)
+      for (int q = 0; q < kQuads; q++) {
+        quad[q] = key_of(fmaxf(fmaxf(z[q][0], z[q][1]), fmaxf(z[q][2], z[q][3])));
+        bool odd = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) odd |= z[q][j] != z[q][j];
-      if (odd) bk = 0xffffffffu;
+        if (odd) quad[q] = 0xffffffffu;
+        bk = max(bk, quad[q]);
+      }
       uint32_t least = l.tk;
       if (first) {
-        least = max(least, nth_largest(bk, p.top));
+        const uint32_t one[1] = {bk};
+        least = max(least, TOP == FEW ? nth_largest(one, p.top) : nth_largest(quad, p.top));
         first = false;
       }
       if (__any(bk >= least)) {
+        int count = 0;
+        if (TOP == MANY) {
+#pragma unroll
+          for (int q = 0; q < kQuads; q++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) count += __popcll(__ballot(key_of(z[q][j]) >= least));
+        }
+        int n = 0;
 #pragma unroll
         for (int q = 0; q < kQuads; q++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const int64_t e = mine + q * 256 + j;
+            const int id = (int)(e - off);
             const uint32_t k = key_of(z[q][j]);
-            offer(l, k, (int)(e - off), e >= off && e < e1 && k >= least, p.top, lane);
+            const bool in = e >= off && e < e1 && k >= least;
+            if (TOP == FEW || count <= kFew) {
+              offer(l, k, id, in, p.top, lane);
+              continue;
+            }
+            const bool ok = in && beats(k, id, l.tk, l.ti);
+            const uint64_t who = __ballot(ok);
+            if (!who) continue;
+            if (ok) {
+              const int to = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+              ck[wave][to] = k;
+              ci[wave][to] = id;
+            }
+            n += __popcll(who);
+            wave_sync();
+            if (n < 64) continue;
+            merge_unsorted(l, ck[wave][lane], ci[wave][lane], p.top, lane);
+            n -= 64;
+            const uint32_t rk = ck[wave][64 + lane];
+            const int ri = ci[wave][64 + lane];
+            wave_sync();
+            if (lane < n) {
+              ck[wave][lane] = rk;
+              ci[wave][lane] = ri;
+            }
+            wave_sync();
           }
+        if (TOP == MANY && n)
+          merge_unsorted(l, lane < n ? ck[wave][lane] : 0, lane < n ? ci[wave][lane] : 0x7fffffff, p.top,
+                         lane);
+        wave_sync();
       }
     }
   }
@@ -309,9 +431,11 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
     t.s += y.s;
     t.a += y.a;
   }
-  uint32_t lk = 0;
-  int li = 0x7fffffff;
-  if (TOP) join_lists(sk, si, 64, 4, p.top, lane, lk, li);
+  uint32_t lk = l.key;
+  int li = l.id;
+  if (TOP == FEW) join_lists(sk, si, 64, 4, p.top, lane, lk, li);
+  if (TOP == MANY)
+    for (int w = 1; w < 4; w++) merge(lk, li, sk[w * 64 + 63 - lane], si[w * 64 + 63 - lane], lane);
   if (p.nsplit == 1) {
     finish(p, row, t, lk, li, xt, lane);
     return;
@@ -328,31 +452,42 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   }
 }
 
-// Joins the at most 64 runs of a row: four waves fetch the lists, one joins them.
+// Joins the at most 64 runs of a row: four waves fetch the lists; one joins them, or each merges a
+// quarter of them.
+template <int TOP>
 __global__ __launch_bounds__(256) void k_logprobs_join(const mg_logprobs p) {
-  constexpr int T = MG_LOGPROBS_MAX_TOP, PITCH = T + 1;
-  __shared__ uint32_t sk[64 * PITCH];
-  __shared__ int si[64 * PITCH];
+  constexpr int T = MG_LOGPROBS_MAX_TOP, PITCH = TOP == FEW ? kFew + 1 : T;
+  __shared__ uint32_t sk[TOP ? 64 * PITCH : 1];
+  __shared__ int si[TOP ? 64 * PITCH : 1];
   const int lane = threadIdx.x & 63;
-  const bool last = threadIdx.x < 64;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
   const mg_logprobs_part *o = p.part + row * p.nsplit;
   float xt = 0.f;
   Sums t{kLowest, 0, 0};
-  if (last) {
+  if (wave == 0) {
     xt = given(p, row);
     if (lane < p.nsplit) t = Sums{o[lane].m, o[lane].s, o[lane].a};
   }
+  uint32_t lk = 0;
+  int li = 0x7fffffff;
+  if (TOP) {
 #pragma unroll 4
-  for (int e = threadIdx.x; e < p.nsplit * T; e += 256) {
-    const int r = e / T, j = e % T;
-    if (j < p.top) {
-      sk[r * PITCH + j] = o[r].key[j];
-      si[r * PITCH + j] = o[r].id[j];
+    for (int e = threadIdx.x; e < p.nsplit * PITCH; e += 256) {
+      const int r = e / PITCH, j = e % PITCH;
+      sk[e] = j < p.top ? o[r].key[j] : 0;
+      si[e] = j < p.top ? o[r].id[j] : 0x7fffffff;
     }
+    __syncthreads();
   }
-  __syncthreads();
-  if (!last) return;
+  if (TOP == MANY) {
+    for (int r = wave; r < p.nsplit; r += 4) merge(lk, li, sk[r * T + 63 - lane], si[r * T + 63 - lane], lane);
+    __syncthreads();
+    sk[threadIdx.x] = lk;
+    si[threadIdx.x] = li;
+    __syncthreads();
+  }
+  if (wave) return;
   // (64 bits: the runs' sums may differ by far in size and number.)
   t = moved(t, of_key(wave_max(key_of(t.m))));
 #pragma unroll
@@ -360,10 +495,19 @@ __global__ __launch_bounds__(256) void k_logprobs_join(const mg_logprobs p) {
     t.s += __shfl_xor(t.s, w);
     t.a += __shfl_xor(t.a, w);
   }
-  uint32_t lk = 0;
-  int li = 0x7fffffff;
-  if (p.top) join_lists(sk, si, PITCH, p.nsplit, p.top, lane, lk, li);
+  if (TOP == FEW) join_lists(sk, si, PITCH, p.nsplit, p.top, lane, lk, li);
+  if (TOP == MANY)
+    for (int w = 1; w < 4; w++) merge(lk, li, sk[w * 64 + 63 - lane], si[w * 64 + 63 - lane], lane);
   finish(p, row, t, lk, li, xt, lane);
+}
+
+template <int TOP>
+mg_status launch(mg_ctx *ctx, const mg_logprobs &p) {
+  k_logprobs<TOP><<<dim3((unsigned)(p.rows * p.nsplit)), dim3(256), 0, ctx->stream>>>(p);
+  MG_TRY(mg_launch_check("log probabilities"));
+  if (p.nsplit == 1) return MG_OK;
+  k_logprobs_join<TOP><<<dim3((unsigned)p.rows), dim3(256), 0, ctx->stream>>>(p);
+  return mg_launch_check("log probabilities, join");
 }
 
 }  // namespace
@@ -382,13 +526,5 @@ size_t mg_logprobs_plan(const mg_ctx *ctx, mg_logprobs *p, bool split) {
 }
 
 mg_status mg_logprobs_run(mg_ctx *ctx, const mg_logprobs &p) {
-  const dim3 grid((unsigned)(p.rows * p.nsplit));
-  if (p.top)
-    k_logprobs<true><<<grid, dim3(256), 0, ctx->stream>>>(p);
-  else
-    k_logprobs<false><<<grid, dim3(256), 0, ctx->stream>>>(p);
-  MG_TRY(mg_launch_check("log probabilities"));
-  if (p.nsplit == 1) return MG_OK;
-  k_logprobs_join<<<dim3((unsigned)p.rows), dim3(256), 0, ctx->stream>>>(p);
-  return mg_launch_check("log probabilities, join");
+  return p.top == 0 ? launch<NONE>(ctx, p) : p.top <= kFew ? launch<FEW>(ctx, p) : launch<MANY>(ctx, p);
 }

@@ -69,6 +69,22 @@ def test_ties_go_to_the_lowest_token(ops, rows):
     check(ops, x, rng.integers(0, 3000, rows), 64)
 
 
+@pytest.mark.parametrize("rows", [2, 1030])
+@pytest.mark.parametrize("top", [1, 2, 10, 11, 33, 64])
+def test_alternatives(ops, rows, top):
+    # Few and many of them, of rows of all kinds: ties, rising and falling parts, NaN, nothing.
+    rng = np.random.default_rng(top)
+    v = 6007
+    x = (rng.standard_normal((rows, v)) * 3).astype(np.float32)
+    x[::7] = rng.integers(-2, 3, x[::7].shape)
+    x[1::7] = np.sort(x[1::7], -1)
+    x[2::7, :4000] = np.sort(x[2::7, :4000], -1)[:, ::-1]
+    x[3::7, 50:] = -np.inf
+    x[4::7][:, rng.permutation(v)[:40]] = np.nan
+    x[5::7] = -np.inf
+    check(ops, x, rng.integers(0, v, rows), top)
+
+
 @pytest.mark.parametrize("rows", [3, 1030])
 @pytest.mark.parametrize("order", [1, -1])
 def test_sorted_rows(ops, rows, order):
