@@ -2974,7 +2974,6 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   a.y = y_dev;
   a.q_stride = q_stride;
   a.y_stride = y_stride;
-  a.heads = num_heads;
   a.group = num_heads / cache->kv_heads;
   if (rope) a.rope = *rope;
   a.tree = tree_dev;

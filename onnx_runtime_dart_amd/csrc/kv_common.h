@@ -11,8 +11,8 @@
 //            (the matrix instruction's order for the values); INT4: the dword of a dim pair
 //            (a, a + 1) holds nibbles {t0 a, t2 a, t0 b, t2 b, t1 a, t3 a, t1 b, t3 b};
 //   scales   fp32 [S][token]: K scale, V scale, and for INT4 K middle, V middle.
-// dims are padded to a multiple of 64 with codes of value 0 (INT4: any code; the query
-// is zero there).
+// dims are padded to a multiple of 64 with codes of any value (never NaN): the query is zero there,
+// and what the values give there is not stored.
 struct mg_kv_cache {
   int device = 0;
   int fmt = 0;
@@ -73,7 +73,7 @@ struct mg_kv_attn {
   const float *q;
   float *y;
   int64_t q_stride, y_stride;
-  int heads, group;
+  int group;  // query heads of a KV head
   mg_rope rope;  // half_rot 0: none
   const uint64_t *tree;
   int tree_words;

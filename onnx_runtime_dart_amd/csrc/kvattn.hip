@@ -9,15 +9,24 @@
 //   O^T (16 dims x 16 rows) += V^T . P^T over 32 keys: the lane's eight weights are, as
 //     they are, the B operand of keys {4 g + r, 16 + 4 g + r}; the A operand of row c of tile
 //     i is dim NB c + i (NB = DP / 16) at those keys, and the cache keeps the four keys of a
-//     dim in one dword, NB of them in a row: no transposition, no exchange between lanes,
-//     no shared memory in the loop.
-// Codes are exact in fp16.  q is a pair of fp16 digits (22 bits) under a power of two of its
-// row, and so is a weight times its key's V scale, which is taken relative to the largest
-// power of two seen (vn); the products are exact and summed in fp32.  One digit would round
-// scores and weights to 2^-11, which fp32 callers see; the second costs products
-// that the cached bytes leave idle anyway.
+//     dim in one dword, NB of them in a row: no transposition, no exchange between lanes.
+// Codes are exact in fp16.  q is a pair of fp16 digits (22 bits) under a power of two, and so is
+// a weight times its key's V scale, which is taken relative to a power of two of the largest that
+// its row has seen; the products are exact and summed in fp32.  One digit would round scores and
+// weights to 2^-11, which fp32 callers see; the second doubles the products, which single tokens
+// have room for under the cached bytes and prompts pay for.
 // m moves only when a score exceeds it by 8 (weights up to 2^8 and their sums have room for
 // that), so most tiles rescale nothing and exchange nothing between lanes.
+//
+// Few rows (k_kv_keys): four waves take tiles in turn for the same 16 rows, the next tile's loads
+// in flight under this one's products; long ones are bound by the cached bytes (one token of 64
+// sequences of 2000 to 8000 keys, 8 heads of 128, e4m3: 134 us, 4.9 TB/s; one of 131072 keys,
+// int8: 58 us), short ones by a chain of latencies (about 5 us to the first weights, 4 for the
+// join of key splits).  Many rows (k_kv_rows): bound by the two-digit products and by the
+// exponentials and digits between them (2048 rows over 6000 keys, 32 heads of 128, int8: 460 us,
+// three such chunks 550 TFLOP/s of the product's, 1100 with both digits: what a large fp16
+// product of the library reaches on this card; heads of 64: 420, where the exponentials weigh
+// twice as much).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -746,7 +755,10 @@ struct Quarter {
 // Many rows: each of the four waves has 16 QB rows of its own.  They convert a quarter of each
 // tile each, into shared memory in matrix order (twice, so that one barrier a tile suffices): a
 // code is then converted once for 64 QB rows, not by every wave, and its 16-byte operands cost a
-// quarter of what the products take.
+// quarter of what the products take.  (Each wave converting all of its tiles in registers: 2048
+// rows over 6000 keys, D 128, int8 748 us, not 460; 1500 over 3000, D 256, 502, not 254.)  Pages
+// are looked up a tile ahead by scalar loads, whose wait leaves the codes in flight (by vector
+// loads 489, D 256 333).  The bounds are the waves a SIMD that the registers allow unspilled.
 template <int FMT, int NB, int QB>
 __global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2) void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;

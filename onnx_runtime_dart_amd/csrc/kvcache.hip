@@ -2,7 +2,8 @@
 //
 // A wave takes four aligned positions of one head at a time: lane (t, c) = (l / 16, l % 16)
 // takes NB = padded head size / 16 dims of token t, so a vector's extreme values join within 16
-// lanes (register moves) and loads and stores of full rows are 16 bytes a lane.  Values of four tokens interleave in the cache:
+// lanes (register moves) and loads and stores of full rows are 16 bytes a lane.  Values of four
+// tokens interleave in the cache:
 // their codes change lanes through 16 NB words of shared memory, and one wave alone writes every
 // byte of such a group (so a half-filled one can be read, merged and written).
 //

@@ -16,6 +16,11 @@ defaults and error classes as the reference:
     op_conv_transpose      <- opConvTranspose lib/src/onnx_nn_ops.dart:818
     op_conv_integer        <- opConvInteger   lib/src/onnx_qlinear_ops.dart:299
     op_qlinear_conv        <- opQLinearConv   lib/src/onnx_qlinear_ops.dart:339
+    op_rotary_embedding    <- the rotation in opGroupQueryAttention, as its own op
+
+Beyond the reference: rotary_tables (tables scaled for long contexts), KvCache (a paged
+cache in 8 or 4 bits with attention over it) and op_token_logprobs; their formulas are in
+include/migemm.h.
 
 Tensors are numpy arrays on the host; every op runs on the GPU through the
 C ABI (there is no CPU path).  Weight handles (NBitsWeight, Int8Weight,
