@@ -643,6 +643,14 @@ def _ref(x):
     return None if x is None else C.byref(x)
 
 
+def _int32(x):
+    """Integers as int32; those beyond it as its ends, which nothing takes (not wrapped)."""
+    x = np.asarray(x)
+    if x.dtype.kind not in "iu" and not (x.dtype.kind == "f" and (x == np.rint(x)).all()):
+        raise ArgumentError("expected integers")
+    return np.ascontiguousarray(np.clip(x, -2**31, 2**31 - 1).astype(np.int32))
+
+
 def rotary_tables_dev(cos_ptr: int, sin_ptr: int, first: int, count: int, half_rot: int, *,
                       base: float = 10000.0, scaling: RopeScaling | None = None,
                       ctx: Context | None = None):
@@ -731,8 +739,8 @@ class KvCache:
     # rope = (cos, sin, interleaved) or (cos, sin, interleaved, positions [rows]).
 
     def _host(self, row_start, past, page_table, rows, arrays, out_shapes, rope, call):
-        row_start, past = (np.ascontiguousarray(x, np.int32).ravel() for x in (row_start, past))
-        page_table = np.ascontiguousarray(page_table, np.int32)
+        row_start, past = (_int32(x).ravel() for x in (row_start, past))
+        page_table = _int32(page_table)
         if past.size != max(row_start.size - 1, 0) or page_table.ndim != 2 or \
                 page_table.shape[0] != past.size or row_start.size < 1:
             raise ArgumentError("KvCache: row_start must be [batch + 1], past [batch], page_table "
@@ -753,7 +761,7 @@ class KvCache:
                 bufs += [DeviceBuffer.from_array(cos, self.ctx), DeviceBuffer.from_array(sin, self.ctx)]
                 at = len(bufs) - 2
                 if pos is not None:
-                    pos = np.ascontiguousarray(pos, np.int32).ravel()
+                    pos = _int32(pos).ravel()
                     if pos.size != rows:
                         raise ArgumentError("KvCache: one position a row")
                     bufs.append(DeviceBuffer.from_array(pos, self.ctx))
@@ -807,8 +815,7 @@ def kv_cache_slots(row_start, past, page_table, *, rows: int, max_new: int, max_
                    pages: int, page_size: int):
     """(slots [rows], refused): where the rows of a batch go, by the kernels' own rules
     (host-only)."""
-    row_start, past, page_table = (np.ascontiguousarray(x, np.int32)
-                                   for x in (row_start, past, page_table))
+    row_start, past, page_table = (_int32(x) for x in (row_start, past, page_table))
     if page_table.ndim != 2 or page_table.shape[0] != past.size or row_start.size != past.size + 1:
         raise ArgumentError("KvCache: row_start must be [batch + 1], past [batch], page_table "
                             "[batch, pages]")
@@ -1238,7 +1245,7 @@ def op_rotary_embedding(x, cos_cache, sin_cache, position_ids=None, *, interleav
     ctx = ctx or default_context()
     pos = None
     if position_ids is not None:
-        pos = np.ascontiguousarray(position_ids, np.int32)
+        pos = _int32(position_ids)
         if pos.shape != (batch, seq):
             raise ArgumentError("RotaryEmbedding: position_ids must be [batch, seq]")
     pb = None if pos is None else DeviceBuffer.from_array(pos, ctx)
@@ -1271,6 +1278,8 @@ def op_token_logprobs(logits, tokens=None, *, top: int = 0, ctx: Context | None 
             raise ArgumentError("TokenLogProbs: one integer token a row of logits")
         # (Any token outside the vocabulary is -1: int32 could wrap into it.)
         ins.append(np.where((tokens < 0) | (tokens >= vocab), -1, tokens).astype(np.int32))
+    if not 0 <= top <= min(vocab, 64):
+        raise ArgumentError("TokenLogProbs: top must be 0 .. 64, at most vocab")
     ctx = ctx or default_context()
     bufs = [DeviceBuffer.from_array(a, ctx) for a in ins]
     n = max(rows, 1)

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import kv_reference as R
-from onnx_runtime_dart_amd.errors import UnsupportedError
+from onnx_runtime_dart_amd.errors import ArgumentError, UnsupportedError
 
 pytestmark = pytest.mark.gpu
 
@@ -784,3 +784,26 @@ def test_profile_names(ops):
     assert names == ["KvCacheAttention", "KvCacheRead", "RotaryTables", "TokenLogProbs"]
     cache.release()
     ctx.close()
+
+
+def test_host_numbers_beyond_32_bits(ops):
+    cache = ops.KvCache(2, kv_heads=1, head_size=64, page_size=16)
+    k = np.ones((1, 1, 64), np.float32)
+    with pytest.raises(ArgumentError):
+        cache.append(k, k, row_start=[0, 1], past=[2**32], page_table=[[0]])
+    with pytest.raises(ArgumentError):
+        cache.append(k, k, row_start=[0, 2**32 + 1], past=[0], page_table=[[0]])
+    cache.append(k, k, row_start=[0, 1], past=[0], page_table=[[2**32 + 1]])
+    assert cache.refused()
+    cos = np.ones((4, 8), np.float32)
+    cache.append(k, k, row_start=[0, 1], past=[0], page_table=[[1]],
+                 rope=(cos, 0 * cos, False, [2**32 + 1]))
+    gk, gv = cache.read(1, row_start=[0, 1], past=[0], page_table=[[1]])
+    assert np.isnan(gk).all() and (np.abs(gv - 1) < 0.01).all()
+    # Nothing to write, nothing to read.
+    none = np.zeros((0, 1, 64), np.float32)
+    cache.append(none, none, row_start=[0], past=[], page_table=np.zeros((0, 3), np.int32))
+    cache.append(none, none, row_start=[0, 0], past=[5], page_table=[[1]])
+    assert cache.attend(none, row_start=[0, 0], past=[5], page_table=[[1]]).shape == (0, 1, 64)
+    assert not cache.refused()
+    cache.release()

@@ -167,3 +167,12 @@ def test_more_than_a_launch_takes(ops):
     with pytest.raises(UnsupportedError):
         ops.rotary_tables_dev(x.ptr, x.ptr, 0, 2**31 - 1, 127)
     x.free()
+
+
+def test_positions_beyond_32_bits(ops):
+    rng = np.random.default_rng(9)
+    cos, sin = tables(rng, 5, 8)
+    x = rng.standard_normal((1, 2, 3, 20)).astype(np.float32)  # [batch, heads, seq, head_size]
+    y = ops.op_rotary_embedding(x, cos, sin, np.array([[1, 2**32 + 1, -2**32 + 2]]))
+    assert np.isfinite(y[0, :, 0]).all()
+    assert np.isnan(y[0, :, 1:, :16]).all() and (y[..., 16:] == x[..., 16:]).all()

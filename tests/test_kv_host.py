@@ -259,3 +259,15 @@ def test_host_code_under_sanitizers():
     out = ts._child({"LD_PRELOAD": str(B.asan_runtime()), "MIGEMM_LIBRARY": str(B.SAN_LIB)},
                     ["test_kv_host.py"])
     assert " passed" in out
+
+
+def test_numbers_beyond_32_bits_do_not_wrap():
+    # past 2^32 + 1 is not 1, nor is page 2^32 page 0.
+    slots, refused = ops.kv_cache_slots([0, 1], [2**32 + 1], [[0]], rows=1, max_new=1, max_len=8,
+                                        pages=1, page_size=16)
+    assert refused and (slots == -1).all()
+    slots, refused = ops.kv_cache_slots([0, 1], [1], [[2**32]], rows=1, max_new=1, max_len=8,
+                                        pages=1, page_size=16)
+    assert refused and (slots == -1).all()
+    with pytest.raises(ArgumentError):
+        ops.kv_cache_slots([0, 1], [1.5], [[0]], rows=1, max_new=1, max_len=8, pages=1, page_size=16)
