@@ -55,9 +55,11 @@ __device__ inline bool block_of(const KvRows &a, Block *o) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(a.c.refused, 1);
     return false;
   }
+  // (64 bits: past may be near 2^31 and the grid made for more rows than the sequence has.)
   const int end = o->q.past + o->q.n;
-  o->pos = (o->q.past & ~(SPAN - 1)) + SPAN * (int)blockIdx.x;
-  if (o->pos >= end) return false;
+  const int64_t at = (o->q.past & ~(SPAN - 1)) + (int64_t)SPAN * blockIdx.x;
+  if (o->q.n == 0 || at >= end) return false;
+  o->pos = (int)at;
   o->page = kv_page(a.s, b, o->pos, a.c.plog, a.c.pages);
   o->slot = o->pos & ((1 << a.c.plog) - 1);
   o->first = max(o->q.past - o->pos, 0) >> 2;

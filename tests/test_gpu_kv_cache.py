@@ -786,6 +786,36 @@ def test_profile_names(ops):
     ctx.close()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_sequences_without_rows(ops, fmt):
+    # In a batch that others have rows of, the first and last sequences among them: nothing of
+    # theirs is read, written or refused, wherever their pasts end and whatever their pages are.
+    rng = np.random.default_rng(61)
+    new, past = [0, 2, 0, 0, 1, 0], [5, 6, 31, 1, 3, 2]
+    b = R.Batch(rng, new, past, 16)
+    cache, ks, vs = filled(ops, rng, b, 2, 64, fmt)
+    before = [cache.read(p, row_start=[0, p], past=[0], page_table=b.page_table[i:i + 1])
+              for i, p in enumerate(past)]
+    table = b.page_table.copy()
+    table[2] = -1
+    k, v = normal(rng, b.rows, 2, 64), normal(rng, b.rows, 2, 64)
+    cos, sin = tables(rng, 40, 16)
+    for rope in (None, (cos, sin, False)):
+        cache.append(k, v, row_start=b.row_start, past=past, page_table=table, rope=rope)
+        assert not cache.refused()
+    gk, gv = cache.read(b.rows, row_start=b.row_start, past=past, page_table=table)
+    assert not cache.refused()
+    same(gv, R.cached(v, fmt))
+    q = normal(rng, b.rows, 4, 64)
+    y = cache.attend(q, row_start=b.row_start, past=past, page_table=table)
+    assert np.isfinite(y).all() and not cache.refused()
+    for i, p in enumerate(past):
+        rk, rv = cache.read(p, row_start=[0, p], past=[0], page_table=b.page_table[i:i + 1])
+        same(rk, before[i][0])
+        same(rv, before[i][1])
+    cache.release()
+
+
 def test_host_numbers_beyond_32_bits(ops):
     cache = ops.KvCache(2, kv_heads=1, head_size=64, page_size=16)
     k = np.ones((1, 1, 64), np.float32)
