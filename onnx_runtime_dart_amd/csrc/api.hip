@@ -2669,9 +2669,9 @@ mg_status check_seqs(const char *what, const mg_seq_batch *s) {
   if (!s) return bad_arg(what, "null batch");
   if (s->batch < 0 || s->batch > 65535 || s->rows < 0 || s->rows > MG_KV_MOST || s->max_new < 0 ||
       s->max_new > s->rows || s->max_len < s->max_new || s->max_len > MG_KV_MOST ||
-      s->table_stride < 0)
+      s->table_stride < 0 || s->table_stride > MG_KV_MOST)
     return bad_arg(what, "batch must be 0 .. 65535, 0 <= max_new <= rows, max_new <= max_len, "
-                         "rows and max_len below 2^31 - 256");
+                         "rows, max_len and table_stride below 2^31 - 256");
   if (s->batch > 0 && s->max_new > 0 &&
       (!s->row_start || !s->past || (s->table_stride && !s->page_table)))
     return bad_arg(what, "null row_start, past or page_table");

@@ -471,6 +471,14 @@ __device__ inline void query_digits(const float *x, float row, float max, float 
   qs = FMT == MG_KV_INT4 ? row_sum(sum) * own : 0.f;
 }
 
+// Keys to pass over for rows up to `last`: those that it sees, but no more than one tile past the
+// page table, whose first key reads as NaN like all after it.
+__device__ inline int keys_of(const mg_kv_attn &a, const kv_seq &sq, int last) {
+  const int end = a.tree ? sq.past + sq.n : sq.past + last / a.group + 1;
+  if (a.s.table_stride > end >> a.c.plog) return end;
+  return (int)min((int64_t)end, (a.s.table_stride << a.c.plog) + 32);
+}
+
 // Which sequence, split, row block and KV head a workgroup has (heads innermost), and its keys.
 struct Work {
   kv_seq sq;
@@ -494,8 +502,7 @@ __device__ inline bool work_of(const mg_kv_attn &a, int ROWS, Work *w) {
   w->rows = w->sq.n * a.group;
   w->r0 = blk * ROWS;
   if (w->r0 >= w->rows) return false;
-  w->kend = a.tree ? w->sq.past + w->sq.n
-                   : w->sq.past + (min(w->r0 + ROWS, w->rows) - 1) / a.group + 1;
+  w->kend = keys_of(a, w->sq, min(w->r0 + ROWS, w->rows) - 1);
   w->kbeg = w->split * a.kc;
   return w->kbeg < w->kend || w->split == 0;
 }
@@ -972,7 +979,7 @@ __global__ __launch_bounds__(256) void k_kv_join(const mg_kv_attn a) {
   const kv_seq sq = kv_sequence(a.s, b);
   if (sq.bad || row >= sq.n * a.group) return;
   const int last = min((row / a.rows_wg + 1) * a.rows_wg, sq.n * a.group) - 1;
-  const int kend = a.tree ? sq.past + sq.n : sq.past + last / a.group + 1;
+  const int kend = keys_of(a, sq, last);
   const int n = max(1, min(a.nsplit, (kend + a.kc - 1) / a.kc));
   const int dp = a.c.dp, grp = threadIdx.x / LP, d = 4 * (threadIdx.x % LP);
   const float2 *ml = a.part_ml + at * a.nsplit;

@@ -816,6 +816,49 @@ def test_sequences_without_rows(ops, fmt):
     cache.release()
 
 
+@pytest.mark.parametrize("max_bytes", [0, -1])
+@pytest.mark.parametrize("new, heads", [(1, 2), (30, 2), (60, 32)])
+def test_lengths_beyond_the_page_table(ops, new, heads, max_bytes):
+    # Pasts of 2^31 and a little beyond the table: the rows that see missing pages are NaN, and
+    # the call ends at the table; the sequence beside them is as ever.
+    rng = np.random.default_rng(62)
+    ctx = ops.Context()
+    b = R.Batch(rng, [new] * 33, [100] * 33, 16)
+    cache, ks, vs = filled(ops, rng, b, 8 if heads == 32 else 2, 64, "int8", ctx=ctx)
+    past = b.past.copy()
+    stride = b.page_table.shape[1]
+    past[0], past[2] = 2**31 - 300, 16 * stride  # far and just beyond
+    past[1] = 16 * stride - 1                     # its first row sees the whole table
+    q = normal(rng, b.rows, heads, 64)
+    dev = device(ops, b.row_start, past, b.page_table, q, np.full(q.shape, 7, np.float32))
+    ctx.set_control(max_bytes=max_bytes)
+    s = seq_batch(ops, b, dev, max_len=2**31 - 256)
+    cache.attend_dev(s, dev[3].ptr, dev[4].ptr, heads)
+    ctx.synchronize()
+    y = dev[4].to_array(q.shape, np.float32)
+    assert cache.refused()
+    # (60 rows from 2^31 - 300 pass max_len: refused whole, rows as they were.)
+    assert (np.isnan(y[:new]) if new <= 44 else y[:new] == 7).all()
+    assert np.isnan(y[2 * new:3 * new]).all()
+    assert np.isfinite(y[new]).all() and np.isnan(y[new + 1:2 * new]).all()
+    for i in range(3, 33):
+        r = slice(i * new, (i + 1) * new)
+        want = R.attend(q[r], ks[i], vs[i], R.visible(new, 100), 0.125)
+        assert np.abs(y[r] - want).max() <= R.bound(q[r], ks[i], vs[i], 0.125)
+    ctx.set_control(max_bytes=-1)
+    # Writing there is refused, whatever the bounds.
+    k = normal(rng, b.rows, cache.kv_heads, 64)
+    kd = ops.DeviceBuffer.from_array(k)
+    cache.append_dev(s, kd.ptr, kd.ptr)
+    assert cache.refused()
+    gk, _ = cache.read(b.rows, **b.args())
+    same(gk[3 * new:], R.cached(k, "int8")[3 * new:])
+    for x in dev + [kd]:
+        x.free()
+    cache.release()
+    ctx.close()
+
+
 def test_host_numbers_beyond_32_bits(ops):
     cache = ops.KvCache(2, kv_heads=1, head_size=64, page_size=16)
     k = np.ones((1, 1, 64), np.float32)
