@@ -80,9 +80,10 @@ struct mg_kv_attn {
   float scale2;  // scale * log2(e)
   bool vec;  // q, y and the tables take 16-byte accesses
   // The plan: rows (query, head of the group) a workgroup takes, whether its waves split the
-  // keys of 16 rows (else rows), key splits of kc keys, row blocks a sequence.
+  // keys of 16 rows (else rows), row blocks a sequence, key splits.
   bool keys;
-  int rows_wg, nblk, nsplit, kc;
+  int rows_wg, nblk, nsplit;
+  float share;  // 1 / nsplit
   // Partial results of (row, split): outputs, then (maximum, sum).
   int64_t parts;
   float *part;

@@ -479,11 +479,24 @@ __device__ inline int keys_of(const mg_kv_attn &a, const kv_seq &sq, int last) {
   return (int)min((int64_t)end, (a.s.table_stride << a.c.plog) + 32);
 }
 
+// Keys of a split of the sequence: its own are shared out, so that a bound far above its length
+// costs no more than idle workgroups (one token over 2000 keys, bound 131072: 27 us by the
+// bound's share, 12 so).
+__device__ inline int split_keys(const mg_kv_attn &a, const kv_seq &sq) {
+  if (a.nsplit == 1) return 0x7fffff80;
+  const uint32_t all = (uint32_t)keys_of(a, sq, sq.n * a.group - 1);
+  // (A division on the way to the first loads: by the reciprocal, up to 192 keys short of 2^31.)
+  uint32_t kc = max(128u, ((uint32_t)((float)all * a.share) + 127) & ~127u);
+  if ((uint64_t)kc * a.nsplit < all) kc += 128;
+  if ((uint64_t)kc * a.nsplit < all) kc += 128;
+  return (int)kc;
+}
+
 // Which sequence, split, row block and KV head a workgroup has (heads innermost), and its keys.
 struct Work {
   kv_seq sq;
   int b, h, split, r0, rows;  // rows: of the sequence
-  int kbeg, kend;             // keys that its last row sees, from its split's first on
+  int kbeg, kend, kfin;       // keys that its last row sees, from its split's first on; its split's
 };
 // False: nothing to do.
 __device__ inline bool work_of(const mg_kv_attn &a, int ROWS, Work *w) {
@@ -503,8 +516,13 @@ __device__ inline bool work_of(const mg_kv_attn &a, int ROWS, Work *w) {
   w->r0 = blk * ROWS;
   if (w->r0 >= w->rows) return false;
   w->kend = keys_of(a, w->sq, min(w->r0 + ROWS, w->rows) - 1);
-  w->kbeg = w->split * a.kc;
-  return w->kbeg < w->kend || w->split == 0;
+  // (A split past the last may begin beyond 32 bits.)
+  const int kc = split_keys(a, w->sq);
+  const int64_t kbeg = (int64_t)w->split * kc;
+  if (kbeg >= w->kend && w->split > 0) return false;
+  w->kbeg = (int)kbeg;
+  w->kfin = (int)min((int64_t)w->kend, kbeg + kc);
+  return true;
 }
 
 // Four outputs of row w.r0 + r from dim d, to y (divided by the sum ll) or to the split's
@@ -550,7 +568,7 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   if (!work_of(a, 16, &w)) return;
   const kv_seq &sq = w.sq;
   const int total = sq.past + sq.n;
-  const int kfin = w.kend - w.kbeg > a.kc ? w.kbeg + a.kc : w.kend;
+  const int kfin = w.kfin;
   // Keys below it are seen by every row.
   const int plain = a.tree ? sq.past : sq.past + w.r0 / a.group + 1;
   int t0 = w.kbeg + 32 * wave;
@@ -786,7 +804,7 @@ __global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2
   if (!work_of(a, ROWS, &w)) return;
   const kv_seq &sq = w.sq;
   const int total = sq.past + sq.n;
-  const int kfin = w.kend - w.kbeg > a.kc ? w.kbeg + a.kc : w.kend;  // of the workgroup
+  const int kfin = w.kfin;  // of the workgroup
   const int wr0 = wave * 16 * QB, first = w.r0 + wr0;  // the wave's first row
   // Keys that some row of the wave sees, and those that all of them see.
   const int wfin = first >= w.rows ? 0
@@ -980,7 +998,8 @@ __global__ __launch_bounds__(256) void k_kv_join(const mg_kv_attn a) {
   if (sq.bad || row >= sq.n * a.group) return;
   const int last = min((row / a.rows_wg + 1) * a.rows_wg, sq.n * a.group) - 1;
   const int kend = keys_of(a, sq, last);
-  const int n = max(1, min(a.nsplit, (kend + a.kc - 1) / a.kc));
+  const uint32_t kc = (uint32_t)split_keys(a, sq);
+  const int n = max(1, min(a.nsplit, (int)(((uint32_t)kend + kc - 1) / kc)));
   const int dp = a.c.dp, grp = threadIdx.x / LP, d = 4 * (threadIdx.x % LP);
   const float2 *ml = a.part_ml + at * a.nsplit;
   const float *p = a.part + at * a.nsplit * dp + d;
@@ -1064,14 +1083,13 @@ size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
     int64_t kc = (a->s.max_len + want - 1) / want;
     kc = std::max<int64_t>(128, (kc + 127) / 128 * 128);
     a->nsplit = want == 1 ? 1 : (int)std::max<int64_t>(1, (a->s.max_len + kc - 1) / kc);
-    a->kc = a->nsplit > 1 ? (int)kc : 0x7fffff80;
     // The join writes and reads partial results, at some 4 MB a microsecond.
     const double join = a->nsplit > 1 ? 4 + 2e-6 * (double)(heads * rows * a->nsplit * a->c.dp) : 0;
     // All at once: as long as the longest.  Else the room shares the keys, and at the end half of
     // one of the last, which have fewest, is not shared.
     const double len = (double)a->s.max_len, spread = a->tree ? 0 : (double)a->s.max_new;
     const double n = (double)base / (double)room;
-    if (base * a->nsplit <= room) return start + join + tile / 32 * (double)std::min<int64_t>(a->kc, a->s.max_len);
+    if (base * a->nsplit <= room) return start + join + tile / 32 * (double)(a->nsplit > 1 ? kc : a->s.max_len);
     return start * std::ceil(n) + tile / 32 * (n * (len - spread / 2) + (len - spread) / 2);
   };
   // Measured at full use and with few workgroups (int8, D 128): a tile of 32 keys takes one of 16
@@ -1095,6 +1113,7 @@ size_t mg_kv_attn_plan(const mg_ctx *ctx, mg_kv_attn *a, bool split) {
 }
 
 mg_status mg_kv_attn_run(mg_ctx *ctx, mg_kv_attn a, void *ws) {
+  a.share = 1.f / (float)a.nsplit;
   a.part = static_cast<float *>(ws);
   a.part_ml = reinterpret_cast<float2 *>(a.part + a.parts * a.c.dp);
   const auto odd = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };

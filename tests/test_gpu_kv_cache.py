@@ -816,6 +816,31 @@ def test_sequences_without_rows(ops, fmt):
     cache.release()
 
 
+@pytest.mark.parametrize("past, max_len", [
+    ([0], 131072), ([126], 131072), ([127], 131072), ([128], 131072), ([8191], 8192),
+    ([8192], 131072), ([20000], 20001), ([20001], 131072), ([32766, 1, 0, 300], 32767),
+    ([300, 32768, 4000], 2**31 - 256), ([513, 1023, 1024, 1025, 5000], 700000)])
+def test_splits_share_a_sequence_out(ops, past, max_len):
+    # Whatever the bound, every key counts once.
+    rng = np.random.default_rng(sum(past))
+    b = R.Batch(rng, [1] * len(past), past, 256)
+    cache, ks, vs = filled(ops, rng, b, 2, 64, "int8")
+    q = normal(rng, b.rows, 4, 64)
+    dev = device(ops, b.row_start, b.past, b.page_table, q, np.zeros_like(q))
+    cache.attend_dev(seq_batch(ops, b, dev, max_len=max_len), dev[3].ptr, dev[4].ptr, 4)
+    check_rows(dev[4].to_array(q.shape, np.float32), q, b, ks, vs, 0.125)
+    # All scores alike: a key left out or taken twice shows in the mean, by 1 / t of a value.  (Digits
+    # round to 2^-22, a thousand tiles' sums walk by some 32 roundings of 2^-24.)
+    cache.attend_dev(seq_batch(ops, b, dev, max_len=max_len), dev[3].ptr, dev[4].ptr, 4, scale=0.0)
+    y = dev[4].to_array(q.shape, np.float32)
+    for i, v in enumerate(vs):
+        mean = v.astype(np.float64).mean(0).repeat(2, 0)
+        assert np.abs(y[i] - mean).max() <= 2e-6 * np.abs(v).max()
+    for x in dev:
+        x.free()
+    cache.release()
+
+
 @pytest.mark.parametrize("max_bytes", [0, -1])
 @pytest.mark.parametrize("new, heads", [(1, 2), (30, 2), (60, 32)])
 def test_lengths_beyond_the_page_table(ops, new, heads, max_bytes):
