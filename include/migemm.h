@@ -748,6 +748,7 @@ mg_status mg_kv_cache_info(const mg_kv_cache *cache, int64_t *pages, int64_t *pa
  * replays with what they hold then); the numbers bound them for the launch:
  *   0 <= row_start[b] <= row_start[b + 1] <= rows, at most max_new rows a sequence, and
  *   past[b] + its rows <= max_len.
+ * They may be loose (max_new above rows too; not above max_len).
  * A sequence that breaks a bound is refused: nothing of it is read or written.  A page
  * number outside the cache or the table is refused likewise: not written, and read as NaN.
  * Both are remembered until mg_kv_cache_refused asks.  Rows that belong to no sequence are

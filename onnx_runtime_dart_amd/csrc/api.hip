@@ -2668,9 +2668,9 @@ constexpr int64_t MG_KV_MOST_NEW = 4 * (MG_MOST_GROUPS - 1);
 mg_status check_seqs(const char *what, const mg_seq_batch *s) {
   if (!s) return bad_arg(what, "null batch");
   if (s->batch < 0 || s->batch > 65535 || s->rows < 0 || s->rows > MG_KV_MOST || s->max_new < 0 ||
-      s->max_new > s->rows || s->max_len < s->max_new || s->max_len > MG_KV_MOST ||
+      s->max_len < s->max_new || s->max_len > MG_KV_MOST ||
       s->table_stride < 0 || s->table_stride > MG_KV_MOST)
-    return bad_arg(what, "batch must be 0 .. 65535, 0 <= max_new <= rows, max_new <= max_len, "
+    return bad_arg(what, "batch must be 0 .. 65535, 0 <= max_new <= max_len, rows >= 0, "
                          "rows, max_len and table_stride below 2^31 - 256");
   if (s->batch > 0 && s->max_new > 0 &&
       (!s->row_start || !s->past || (s->table_stride && !s->page_table)))
@@ -2678,11 +2678,15 @@ mg_status check_seqs(const char *what, const mg_seq_batch *s) {
   return MG_OK;
 }
 
+// Also copies the batch, with max_new (a bound: it may be loose) no more than the rows.
 mg_status check_cache(const char *what, const mg_ctx *ctx, const mg_kv_cache *c,
-                      const mg_seq_batch *s) {
+                      const mg_seq_batch *s, mg_seq_batch *own) {
   if (!ctx || !c) return bad_arg(what, "null argument");
   if (c->device != ctx->device) return bad_arg(what, "cache of another device");
-  return check_seqs(what, s);
+  MG_TRY(check_seqs(what, s));
+  *own = *s;
+  own->max_new = std::min(s->max_new, s->rows);
+  return MG_OK;
 }
 
 // A row stride, 0 = the row's own length.
@@ -2920,16 +2924,17 @@ mg_status mg_kv_cache_append_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_s
   const char *what = "KvCacheAppend";
   ProfScope prof_(ctx, what);
   g_last_error.clear();
-  MG_TRY(check_cache(what, ctx, cache, seqs));
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
   MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
   MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
   if (rope) MG_TRY(check_rope(what, *rope, cache->d));
-  if (seqs->max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheAppend: too many rows");
-  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (s.max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheAppend: too many rows");
+  if (s.batch == 0 || s.max_new == 0) return MG_OK;
   if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
   MG_TRY(mg_use_device(ctx));
   MG_TRY(mg_check_control(ctx, 0));
-  return mg_kv_append_run(ctx, *cache, *seqs, k_dev, k_stride, v_dev, v_stride, rope);
+  return mg_kv_append_run(ctx, *cache, s, k_dev, k_stride, v_dev, v_stride, rope);
 }
 
 mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
@@ -2938,15 +2943,16 @@ mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq
   const char *what = "KvCacheRead";
   ProfScope prof_(ctx, what);
   g_last_error.clear();
-  MG_TRY(check_cache(what, ctx, cache, seqs));
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
   MG_TRY(check_stride(what, &k_stride, (int64_t)cache->kv_heads * cache->d));
   MG_TRY(check_stride(what, &v_stride, (int64_t)cache->kv_heads * cache->d));
-  if (seqs->max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheRead: too many rows");
-  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (s.max_new > MG_KV_MOST_NEW) return mg_fail(MG_UNSUPPORTED, "KvCacheRead: too many rows");
+  if (s.batch == 0 || s.max_new == 0) return MG_OK;
   if (!k_dev || !v_dev) return bad_arg(what, "null buffer");
   MG_TRY(mg_use_device(ctx));
   MG_TRY(mg_check_control(ctx, 0));
-  return mg_kv_read_run(ctx, *cache, *seqs, k_dev, k_stride, v_dev, v_stride);
+  return mg_kv_read_run(ctx, *cache, s, k_dev, k_stride, v_dev, v_stride);
 }
 
 mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
@@ -2957,19 +2963,20 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   const char *what = "KvCacheAttention";
   ProfScope prof_(ctx, what);
   g_last_error.clear();
-  MG_TRY(check_cache(what, ctx, cache, seqs));
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
   if (num_heads < 1 || num_heads % cache->kv_heads)
     return bad_arg(what, "num_heads must be a multiple of kv_heads");
   MG_TRY(check_stride(what, &q_stride, (int64_t)num_heads * cache->d));
   MG_TRY(check_stride(what, &y_stride, (int64_t)num_heads * cache->d));
   if (rope) MG_TRY(check_rope(what, *rope, cache->d));
-  if (tree_dev && (tree_words < 1 || (int64_t)tree_words * 64 < seqs->max_new))
+  if (tree_dev && (tree_words < 1 || (int64_t)tree_words * 64 < s.max_new))
     return bad_arg(what, "tree_words must hold a bit for each of max_new rows");
-  if (seqs->batch == 0 || seqs->max_new == 0) return MG_OK;
+  if (s.batch == 0 || s.max_new == 0) return MG_OK;
   if (!q_dev || !y_dev) return bad_arg(what, "null buffer");
   mg_kv_attn a{};
   a.c = *cache;
-  a.s = *seqs;
+  a.s = s;
   a.q = q_dev;
   a.y = y_dev;
   a.q_stride = q_stride;
@@ -2980,7 +2987,7 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   a.tree_words = tree_dev ? tree_words : 0;
   a.scale2 = (float)((has_scale ? (double)scale : 1.0 / std::sqrt((double)cache->d)) *
                      1.44269504088896340736);
-  if (seqs->max_new * (int64_t)a.group > MG_KV_MOST)
+  if (s.max_new * (int64_t)a.group > MG_KV_MOST)
     return mg_fail(MG_UNSUPPORTED, "KvCacheAttention: too many rows");
   size_t need = mg_kv_attn_plan(ctx, &a, true);
   MG_TRY(mg_use_device(ctx));

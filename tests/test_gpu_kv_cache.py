@@ -816,6 +816,33 @@ def test_sequences_without_rows(ops, fmt):
     cache.release()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("new, past", [([1], [0]), ([1], [700]), ([3], [17]), ([20], [40]), ([2, 0, 1], [9, 8, 7])])
+def test_more_new_rows_allowed_than_there_are(ops, fmt, new, past):
+    # max_new above the rows of the whole batch, in all three calls.
+    rng = np.random.default_rng(63)
+    b = R.Batch(rng, new, past, 16)
+    cache, ks, vs = filled(ops, rng, b, 2, 64, fmt)
+    k, v, q = normal(rng, b.rows, 2, 64), normal(rng, b.rows, 2, 64), normal(rng, b.rows, 8, 64)
+    out = np.zeros_like(k)
+    dev = device(ops, b.row_start, b.past, b.page_table, k, v, out, out, q, np.zeros_like(q))
+    for most in (b.rows, b.rows + 1, 33, 600):
+        s = seq_batch(ops, b, dev, max_new=most, max_len=1000)
+        cache.append_dev(s, dev[3].ptr, dev[4].ptr)
+        cache.read_dev(s, dev[5].ptr, dev[6].ptr)
+        same(dev[5].to_array(k.shape, np.float32), R.cached(k, fmt))
+        same(dev[6].to_array(k.shape, np.float32), R.cached(v, fmt))
+        for i in range(len(new)):
+            r = slice(b.row_start[i], b.row_start[i + 1])
+            ks[i][past[i]:], vs[i][past[i]:] = R.cached(k[r], fmt), R.cached(v[r], fmt)
+        cache.attend_dev(s, dev[7].ptr, dev[8].ptr, 8)
+        check_rows(dev[8].to_array(q.shape, np.float32), q, b, ks, vs, 0.125)
+        assert not cache.refused()
+    for x in dev:
+        x.free()
+    cache.release()
+
+
 @pytest.mark.parametrize("past, max_len", [
     ([0], 131072), ([126], 131072), ([127], 131072), ([128], 131072), ([8191], 8192),
     ([8192], 131072), ([20000], 20001), ([20001], 131072), ([32766, 1, 0, 300], 32767),

@@ -38,8 +38,8 @@ def rope(**kw):
     return ops.Rope(**{**base, **kw})
 
 
-BAD_SEQS = [dict(batch=-1), dict(batch=65536), dict(rows=-1), dict(max_new=5), dict(max_new=-1),
-            dict(max_len=3), dict(max_len=2**31), dict(rows=2**31), dict(table_stride=-1),
+BAD_SEQS = [dict(batch=-1), dict(batch=65536), dict(rows=-1), dict(max_new=101), dict(max_new=-1),
+            dict(max_len=3), dict(max_new=2**31, max_len=2**31), dict(max_len=2**31), dict(rows=2**31), dict(table_stride=-1),
             dict(table_stride=2**31),
             dict(row_start_ptr=0), dict(past_ptr=0), dict(page_table_ptr=0)]
 BAD_ROPE = [dict(half_rot=0), dict(half_rot=33), dict(max_pos=0), dict(max_pos=2**31),
@@ -94,7 +94,8 @@ def test_more_rows_than_a_launch_takes():
 def test_nothing_to_do_needs_no_device():
     none = seqs(batch=0, row_start_ptr=0, past_ptr=0, page_table_ptr=0)
     empty = seqs(rows=0, max_new=0, row_start_ptr=0, past_ptr=0, page_table_ptr=0)
-    for s in (none, empty):
+    loose = seqs(rows=0, max_new=7)
+    for s in (none, empty, loose):
         assert append(s, k=None, v=None) == read(s, k=None, v=None) == attend(s, q=None, y=None) == 0
 
 
