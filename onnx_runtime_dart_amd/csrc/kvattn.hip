@@ -785,7 +785,8 @@ struct Quarter {
 // are looked up a tile ahead by scalar loads, whose wait leaves the codes in flight (by vector
 // loads 489, D 256 333).  The bounds are the waves a SIMD that the registers allow unspilled.
 template <int FMT, int NB, int QB>
-__global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2) void k_kv_rows(const mg_kv_attn a) {
+__global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2)
+void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;
   constexpr int KO = 2 * KS * 64, VO = NB * 64;  // operands of a tile

@@ -817,7 +817,8 @@ def test_sequences_without_rows(ops, fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("new, past", [([1], [0]), ([1], [700]), ([3], [17]), ([20], [40]), ([2, 0, 1], [9, 8, 7])])
+@pytest.mark.parametrize("new, past", [
+    ([1], [0]), ([1], [700]), ([3], [17]), ([20], [40]), ([2, 0, 1], [9, 8, 7])])
 def test_more_new_rows_allowed_than_there_are(ops, fmt, new, past):
     # max_new above the rows of the whole batch, in all three calls.
     rng = np.random.default_rng(63)

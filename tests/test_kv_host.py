@@ -39,7 +39,8 @@ def rope(**kw):
 
 
 BAD_SEQS = [dict(batch=-1), dict(batch=65536), dict(rows=-1), dict(max_new=101), dict(max_new=-1),
-            dict(max_len=3), dict(max_new=2**31, max_len=2**31), dict(max_len=2**31), dict(rows=2**31), dict(table_stride=-1),
+            dict(max_len=3), dict(max_new=2**31, max_len=2**31), dict(max_len=2**31),
+            dict(rows=2**31), dict(table_stride=-1),
             dict(table_stride=2**31),
             dict(row_start_ptr=0), dict(past_ptr=0), dict(page_table_ptr=0)]
 BAD_ROPE = [dict(half_rot=0), dict(half_rot=33), dict(max_pos=0), dict(max_pos=2**31),
