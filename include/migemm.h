@@ -724,7 +724,7 @@ mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t b
  *   INT8  s = amax / 127, q = x / s rounded half to even, value q s
  *   E4M3  s = amax / 448, q = x / s rounded half to even to e4m3 (fn), value q s
  *   INT4  m = (max + min) / 2, h = (max - min) / 30, n = ((x - m) / h + 15) / 2 rounded half
- *         to even, value m + (2 n - 15) h
+ *         to even, 0 at least and 15 at most, value m + (2 n - 15) h
  * with s, m, h rounded to fp32 and the quotients not rounded before q or n.  A vector that
  * holds Infinity or NaN reads back as NaN throughout. */
 typedef enum mg_kv_format { MG_KV_INT8 = 0, MG_KV_E4M3 = 1, MG_KV_INT4 = 2 } mg_kv_format;

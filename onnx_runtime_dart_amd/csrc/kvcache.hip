@@ -151,7 +151,8 @@ __device__ inline void quantise(const float (&x)[NB], uint32_t (&code)[NB / 4], 
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       if (FMT == MG_KV_INT4) {
-        const float u = fmaf(x[e + j] - m, 0.5f * r, 7.5f);
+        // (m is rounded: of extremes few units in the last place apart one may lie beyond 15 steps.)
+        const float u = fminf(fmaxf(fmaf(x[e + j] - m, 0.5f * r, 7.5f), 0.f), 15.f);
         a[j] = u - 0x1p-18f;
         b[j] = u + 0x1p-18f;
       } else {

@@ -933,3 +933,26 @@ def test_host_numbers_beyond_32_bits(ops):
     assert cache.attend(none, row_start=[0, 0], past=[5], page_table=[[1]]).shape == (0, 1, 64)
     assert not cache.refused()
     cache.release()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("base", [1.0, -1.0, 1.0000001192, -3e-20, 7e6, 2.0**100])
+def test_nearly_constant_vectors(ops, fmt, base):
+    # Extremes 1 to 40 units in the last place apart, on both parities: the middle's rounding
+    # leaves one of them outside middle +- 15 steps (INT4), where the code is the last one.
+    rng = np.random.default_rng(26)
+    n, d = 80, 64
+    first = np.full((n, 2, 1), np.float32(base)).view(np.int32) + (np.arange(n) % 2)[:, None, None]
+    steps = (1 + np.arange(n) // 2)[:, None, None]
+    b = R.Batch(rng, [n], [3], 16)
+    cache = ops.KvCache(b.pages, kv_heads=2, head_size=d, page_size=16, fmt=fmt)
+    for part in (rng.integers(0, 2, (n, 2, d)), rng.random((n, 2, d))):
+        part[..., :2] = [0, 1]  # (both extremes are there)
+        bits = first + np.rint(rng.permuted(part.astype(np.float64), axis=-1) * steps)
+        k = bits.astype(np.int32).view(np.float32)
+        v = k[..., ::-1].copy()
+        cache.append(k, v, **b.args())
+        gk, gv = cache.read(n, **b.args())
+        same(gk, R.cached(k, fmt))
+        same(gv, R.cached(v, fmt))
+    cache.release()
