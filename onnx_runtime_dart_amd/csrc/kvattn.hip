@@ -471,12 +471,16 @@ __device__ inline void query_digits(const float *x, float row, float max, float 
   qs = FMT == MG_KV_INT4 ? row_sum(sum) * own : 0.f;
 }
 
-// Keys to pass over for rows up to `last`: those that it sees, but no more than one tile past the
-// page table, whose first key reads as NaN like all after it.
+// Keys to pass over for rows up to `last`: those that it sees, but where every row that sees a key
+// past the page table sees the first there, no more than one tile beyond it: that key reads as NaN
+// like all after it.  (Drafts see one another by their tree alone: where the past ends within the table
+// they are all passed over.)
 __device__ inline int keys_of(const mg_kv_attn &a, const kv_seq &sq, int last) {
   const int end = a.tree ? sq.past + sq.n : sq.past + last / a.group + 1;
   if (a.s.table_stride > end >> a.c.plog) return end;
-  return (int)min((int64_t)end, (a.s.table_stride << a.c.plog) + 32);
+  const int64_t held = a.s.table_stride << a.c.plog;
+  if (a.tree && sq.past <= held) return end;
+  return (int)min((int64_t)end, held + 32);
 }
 
 // Keys of a split of the sequence: its own are shared out, so that a bound far above its length

@@ -956,3 +956,49 @@ def test_nearly_constant_vectors(ops, fmt, base):
         same(gk, R.cached(k, fmt))
         same(gv, R.cached(v, fmt))
     cache.release()
+
+
+@pytest.mark.parametrize("max_bytes", [0, -1])
+@pytest.mark.parametrize("count, heads", [(1, 2), (40, 32)])
+@pytest.mark.parametrize("past, stride", [(16, 1), (0, 0), (5, 1), (15, 1), (17, 1), (700, 44), (704, 44),
+                                          (705, 44)])
+def test_drafts_beyond_the_page_table(ops, count, heads, past, stride, max_bytes):
+    # Positions past the table read as NaN, in whatever rows see them: also in those that see
+    # one far behind the table's end and none of the first ones there.
+    rng = np.random.default_rng(past + count)
+    ctx = ops.Context()
+    new, kv, page = 64, 8 if heads == 32 else 2, 16
+    total = past + new
+    pages = -(-total // page)
+    b = R.Batch(rng, [new] * count, [past] * count, page)
+    cache, ks, vs = filled(ops, rng, b, kv, 64, "int8", ctx=ctx)
+    table = np.ascontiguousarray(b.page_table[:, :stride])
+    q = normal(rng, b.rows, heads, 64)
+    tree = np.zeros((b.rows, 1), np.uint64)
+    own = np.uint64(1) << np.arange(new, dtype=np.uint64)
+    for i in range(count):
+        tree[i * new:(i + 1) * new, 0] = own
+    tree[3], tree[5] = 0, 1  # one that sees the past alone, one that sees the first draft
+    dev = device(ops, b.row_start, b.past, table if stride else np.zeros(1, np.int32), q,
+                 np.full(q.shape, 7, np.float32), tree)
+    s = ops.SeqBatch(batch=count, rows=b.rows, max_new=new, max_len=pages * page,
+                     row_start_ptr=dev[0].ptr, past_ptr=dev[1].ptr, page_table_ptr=dev[2].ptr,
+                     table_stride=stride)
+    ctx.set_control(max_bytes=max_bytes)
+    cache.attend_dev(s, dev[3].ptr, dev[4].ptr, heads, tree_ptr=dev[5].ptr, tree_words=1)
+    ctx.synchronize()
+    y = dev[4].to_array(q.shape, np.float32)
+    assert cache.refused()
+    for i in range(min(count, 3)):
+        r = slice(i * new, (i + 1) * new)
+        see = R.visible(new, past, tree[r])
+        lost = see[:, stride * page:].any(-1)
+        assert np.isnan(y[r][lost]).all()
+        want = R.attend(q[r], ks[i], vs[i], see, 0.125)
+        err = np.abs(y[r][~lost] - want[~lost]).max(initial=0)
+        assert err <= R.bound(q[r], ks[i], vs[i], 0.125)
+    ctx.set_control(max_bytes=-1)
+    for x in dev:
+        x.free()
+    cache.release()
+    ctx.close()
