@@ -11,12 +11,17 @@
 //     i is dim NB c + i (NB = DP / 16) at those keys, and the cache keeps the four keys of a
 //     dim in one dword, NB of them in a row: no transposition, no exchange between lanes.
 // Codes are exact in fp16.  q is a pair of fp16 digits (22 bits) under a power of two, and so is
-// a weight times its key's V scale, which is taken relative to a power of two of the largest that
-// its row has seen; the products are exact and summed in fp32.  One digit would round scores and
-// weights to 2^-11, which fp32 callers see; the second doubles the products, which single tokens
-// have room for under the cached bytes and prompts pay for.
-// m moves only when a score exceeds it by 8 (weights up to 2^8 and their sums have room for
-// that), so most tiles rescale nothing and exchange nothing between lanes.
+// a weight times its key's V scale; the products are exact and summed in fp32.  One digit would
+// round scores and weights to 2^-11, which fp32 callers see; the second doubles the products,
+// which single tokens have room for under the cached bytes and prompts pay for.
+// Digits end at 2^-25, so their unit is that of a row's weights times scales, not of its largest weight
+// and its largest scale, which may belong to different keys: 2^(s - m) is kept relative to a
+// reference m of the row, a whole number that puts the sum of these products over a tile at 2^11 (scales
+// in units of the largest, 2^12; an outlier among them moves m down).  What a key contributes is
+// then off by 2^-22 of itself and 2^-35 of the row's sum, however far its weight and its scale lie
+// from the others'.  m moves up only when a product outgrows fp16, so most tiles rescale nothing and
+// exchange nothing between lanes.  (The sum, not the largest product, which a few tiles later is
+// outgrown: 2 x 2048 rows of heads of 64 took 10% longer.)
 //
 // Few rows (k_kv_keys): four waves take tiles in turn for the same 16 rows, the next tile's loads
 // in flight under this one's products; long ones are bound by the cached bytes (one token of 64
@@ -44,8 +49,11 @@ typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
-constexpr float kNoMax = -3.0e38f;  // the running maximum before any score
-constexpr float kSlack = 8.f;       // how far a score may exceed it
+constexpr float kNoMax = -3.0e38f;  // the reference before any score
+constexpr float kTop = 65000.f;     // most of a weight times its scale (fp16 ends at 65504)
+constexpr int kAim = 11;            // log2 of where a tile's sum of them is put
+constexpr int kRoom = 84;           // log2 of a weight so put, at most (their sums have room above)
+constexpr float kScales = 4096.f;   // the largest V scale lies in [2^11, 2^12) of their unit
 
 // Four codes of one dword of K (adjacent dims) or V (four keys of a dim) as fp16.
 template <int FMT>
@@ -158,6 +166,8 @@ __device__ inline float pow2_under(float x) {
   const int e = (int)(__float_as_uint(x) >> 23 & 255u);
   return x == 0.f ? 1.f : ldexpf(1.f, 126 - max(e, 24));
 }
+// floor(log2 x) of a normal x >= 0; -127 below.
+__device__ inline int log2_of(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
 // The second digit of x after the first.  (One mixed fma, exact before its rounding; a -1 that
 // the compiler knows is turned into a conversion and a difference.)
 __device__ inline _Float16 rest_of(float x, _Float16 hi) {
@@ -319,62 +329,77 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
   }
 }
 
-// One tile's weights for QB blocks of 16 rows: the scores of the lane's eight keys, in units that
-// make its running maximum m current, and from them the digits of the weights times the V scales.
-// l and z are the lane's share of the sum and (INT4) of the sum of weights times middles.
-// masked: only the keys of `seen` count (a branch of the whole wave, or a constant), and the V scales
-// want the factors `unit` of the rows yet (null: none).
+// One tile's weights for QB blocks of 16 rows: 2^(s - m) of the lane's eight keys, and the digits of
+// those times the V scales vsn.  l and z are the lane's share of the sum and (INT4) of the sum of
+// weights times middles.  masked: only the keys of `seen` count (a branch of the whole wave, or a constant);
+// limit: kTop, or negative where some row's products have units of their own, the lane's at units[256 q].
 template <int FMT, int NB, int QB>
-__device__ inline void weigh(bool masked, const float4v (&acc)[QB][2], const float (&ksf)[8],
-                             const float (&vsn)[8], const float (&kzf)[8], const float (&vz)[8],
-                             const float (&qs)[QB], const uint32_t (&seen)[QB],
-                             const float *unit, float (&m)[QB],
-                             float (&l)[QB], float (&z)[QB], float4v (&o)[QB][NB],
-                             half8v (&ph)[QB], half8v (&pl)[QB]) {
+__device__ inline void weigh(bool masked, float limit, const float *units, float4v (&acc)[QB][2],
+                             const float (&ksf)[8], const float (&vsn)[8], const float (&kzf)[8],
+                             const float (&vz)[8], const float (&qs)[QB],
+                             const uint32_t (&seen)[QB], float (&m)[QB], float (&l)[QB],
+                             float (&z)[QB], float4v (&o)[QB][NB], half8v (&ph)[QB],
+                             half8v (&pl)[QB]) {
   float d[QB][8];  // scores less m, of unseen keys too
-  auto scores = [&]() __attribute__((always_inline)) {
+  auto scores = [&](int q) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < QB; q++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float base = FMT == MG_KV_INT4 ? fmaf(qs[q], kzf[j], -m[q]) : -m[q];
-        d[q][j] = fmaf(acc[q][j >> 2][j & 3], ksf[j], base);
-      }
+    for (int j = 0; j < 8; j++) {
+      const float base = FMT == MG_KV_INT4 ? fmaf(qs[q], kzf[j], -m[q]) : -m[q];
+      d[q][j] = fmaf(acc[q][j >> 2][j & 3], ksf[j], base);
+    }
   };
   auto top = [&](int q) __attribute__((always_inline)) {
     return fmaxf(fmaxf(fmaxf(d[q][0], d[q][1]), fmaxf(d[q][2], d[q][3])),
                  fmaxf(fmaxf(d[q][4], d[q][5]), fmaxf(d[q][6], d[q][7])));
   };
-  scores();
+#pragma unroll
+  for (int q = 0; q < QB; q++) scores(q);
   float most = top(0);
 #pragma unroll
   for (int q = 1; q < QB; q++) most = fmaxf(most, top(q));
-  // (An unseen key's score may bring a wave here, where only the seen ones count.)
-  if (__builtin_expect(__any(most > kSlack), 0)) {
-    float old[QB];
+  // A bound of the lane's products, and of its weights alone by 2^90.
+  float big = 0x1p-74f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) big = fmaxf(big, vsn[j]);
+  // (An unseen key may bring a wave here, where only the seen ones count; and rows with units of their
+  // own do, whose products d is not yet in.  No branch of their own takes those there: where
+  // paths of different length meet behind a matrix product, the compiler (ROCm 7.2) has left out
+  // the wait for its result.)
+  if (__builtin_expect(__any(exp2_of(most) * big > limit), 0)) {
 #pragma unroll
     for (int q = 0; q < QB; q++) {
-      old[q] = m[q];
+      const float old = m[q];
+      if (limit < 0.f) {
+        acc[q][0] *= units[256 * q];
+        acc[q][1] *= units[256 * q];
+      }
       m[q] = 0.f;
-    }
-    scores();
-#pragma unroll
-    for (int q = 0; q < QB; q++) {
+      scores(q);
 #pragma unroll
       for (int j = 0; j < 8; j++) d[q][j] = seen[q] >> j & 1 ? d[q][j] : -__builtin_inff();
-      m[q] = fmaxf(old[q], row_max(top(q)));
-      const float by = exp2_of(old[q] - m[q]);
+      const float best = row_max(top(q));
+      float p = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float x = exp2_of(d[q][j] - best) * vsn[j];
+        p += x > 0.f ? x : 0.f;
+      }
+      // (Whole numbers: outputs and sums are moved without rounding.)
+      const float aim = rintf(best + (float)max(log2_of(row_sum(p)) - kAim, -kRoom));
+      m[q] = aim > old + 2.f ? aim : old;
+      const float by = ldexpf(1.f, (int)fmaxf(old - m[q], -200.f));
       l[q] *= by;
       z[q] *= by;
 #pragma unroll
       for (int i = 0; i < NB; i++) o[q][i] *= by;
+      scores(q);
+      // (Scores of 2^24 and more are rounded by more than the reference can follow.)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j]));
+        d[q][j] = d[q][j] > lim ? lim : d[q][j];
+      }
     }
-    scores();
-    // (A score of 2^31 and more is rounded by more than exponents have room for.)
-#pragma unroll
-    for (int q = 0; q < QB; q++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) d[q][j] = d[q][j] > kSlack ? kSlack : d[q][j];
   }
   float e[QB][8], w[QB][8];
 #pragma unroll
@@ -394,7 +419,7 @@ __device__ inline void weigh(bool masked, const float4v (&acc)[QB][2], const flo
       for (int j = 0; j < 8; j++) {
         const bool on = seen[q] >> j & 1;
         e[q][j] = on ? e[q][j] : 0.f;
-        w[q][j] = on ? (unit ? w[q][j] * unit[256 * q] : w[q][j]) : 0.f;
+        w[q][j] = on ? w[q][j] : 0.f;
         if (FMT == MG_KV_INT4) z[q] += on ? e[q][j] * vz[j] : 0.f;
       }
   } else if (FMT == MG_KV_INT4) {
@@ -417,6 +442,21 @@ __device__ inline void weigh(bool masked, const float4v (&acc)[QB][2], const flo
       pl[q][j] = rest_of(w[q][j], hi[0]);
       pl[q][j + 1] = rest_of(w[q][j + 1], hi[1]);
     }
+}
+
+// The unit of the row's V scales shrinks to 2^-j of itself: so does what is yet to come, and the
+// reference follows it down, which leaves the outputs as they are.  As far as the sum of the
+// weights has room; they shrink by the rest.
+template <int NB>
+__device__ inline void smaller_unit(int j, float &m, float &l, float &z, float4v (&o)[NB]) {
+  // (A reference of 2^24 and more does not move by small steps.)
+  const int keep = fabsf(m) < 0x1p24f ? max(0, min(j, kRoom - log2_of(row_max(l)))) : 0;
+  m -= (float)keep;
+  l = ldexpf(l, keep);
+  const float by = ldexpf(1.f, keep - j);
+  z *= by;
+#pragma unroll
+  for (int i = 0; i < NB; i++) o[i] *= by;
 }
 
 // Which of the lane's eight keys of the tile at t0 a row sees (bit j: key 16 (j / 4) + 4 g + j % 4),
@@ -529,10 +569,9 @@ __device__ inline bool work_of(const mg_kv_attn &a, int ROWS, Work *w) {
   return true;
 }
 
-// Four outputs of row w.r0 + r from dim d, to y (divided by the sum ll) or to the split's
-// partial results.
+// Four outputs of row w.r0 + r from dim d, to y or to the split's partial results.
 template <int DP>
-__device__ inline void put4(const mg_kv_attn &a, const Work &w, int r, int d, float4 v, float ll) {
+__device__ inline void put4(const mg_kv_attn &a, const Work &w, int r, int d, float4 v) {
   const int row = w.r0 + r;
   if (row >= w.rows) return;
   if (a.nsplit > 1) {
@@ -542,15 +581,22 @@ __device__ inline void put4(const mg_kv_attn &a, const Work &w, int r, int d, fl
   }
   const int qi = row / a.group, j = row - qi * a.group;
   float *y = a.y + (w.sq.start + qi) * a.y_stride + (int64_t)(w.h * a.group + j) * a.c.d + d;
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
   if (a.vec) {
-    if (d < a.c.d) *reinterpret_cast<float4 *>(y) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    if (d < a.c.d) *reinterpret_cast<float4 *>(y) = v;
   } else {
-    if (d < a.c.d) y[0] = v.x * inv;
-    if (d + 1 < a.c.d) y[1] = v.y * inv;
-    if (d + 2 < a.c.d) y[2] = v.z * inv;
-    if (d + 3 < a.c.d) y[3] = v.w * inv;
+    if (d < a.c.d) y[0] = v.x;
+    if (d + 1 < a.c.d) y[1] = v.y;
+    if (d + 2 < a.c.d) y[2] = v.z;
+    if (d + 3 < a.c.d) y[3] = v.w;
   }
+}
+// A part of a row's keys where it is joined with the others: the reference under which the sum l of
+// its weights (kept under m) is below 1, and the sum under a reference that may be higher.
+__device__ inline float part_ref(float m, float l) {
+  return l == 0.f ? kNoMax : m + (float)(log2_of(l) + 1);
+}
+__device__ inline float part_sum(float m, float l, float ref) {
+  return ldexpf(l, (int)fminf(fmaxf(m - ref, -400.f), 400.f));
 }
 __device__ inline void put_stat(const mg_kv_attn &a, const Work &w, int r, float m, float l) {
   if (a.nsplit == 1 || w.r0 + r >= w.rows) return;
@@ -565,7 +611,7 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   constexpr int DP = S::DP, KS = S::KS, KW = S::KW, QP = DP + 4, STEP = 128;
   // 16 rows' queries; later the four waves' results.
   __shared__ __attribute__((aligned(16))) float lds[64 * QP];
-  __shared__ float stat[4][2][16], units[4][64];
+  __shared__ float stat[4][2][16];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   Work w;
@@ -597,8 +643,7 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   half8v qh[KS], ql[KS];
   float qs[1], own;
   query_digits<FMT, KS>(x, row, mx, dn, qh, ql, qs[0], own);
-  const bool uneven = __any(own != 1.f);
-  units[wave][lane] = own;
+  const float fo = f * own;
   const int qi = min(w.r0 + c, w.rows - 1) / a.group;
   const int see = a.tree ? sq.past : sq.past + qi + 1;
   const int64_t word = (int64_t)(sq.start + qi) * a.tree_words;
@@ -638,33 +683,36 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
     }
     if (!AHEAD && more) next.load_k(a, p, g, c);
     float ksf[8], vsn[8], kzf[8], vz[8];
-    spread(ksf, t.ks, f);
+    spread(ksf, t.ks, fo);
     spread(vsn, t.vs, 1.f);
     if (FMT == MG_KV_INT4) {
       spread(kzf, t.kz, f);
       spread(vz, t.vz, 1.f);
     }
     const uint32_t seen[1] = {MASKED ? seen_keys(a, sq, t0, g, see, word, kfin) : 0xffu};
-    // V scales relative to the largest that the row has seen.
-    float big = 0.f;
+    // V scales (INT4: and middles) relative to the largest that the row has seen.
+    float big = 0.f, mid = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       if (MASKED) vsn[j] = seen[0] >> j & 1 ? vsn[j] : 0.f;
+      if (MASKED && FMT == MG_KV_INT4) vz[j] = seen[0] >> j & 1 ? vz[j] : 0.f;
       big = fmaxf(big, vsn[j]);
+      if (FMT == MG_KV_INT4) mid = fmaxf(mid, fabsf(vz[j]));
     }
-    if (__builtin_expect(__any(big * vn > 16.f) || uneven, 0)) {
+    if (FMT == MG_KV_INT4) big = fmaxf(big, 0.0625f * mid);
+    if (__builtin_expect(__any(big * vn > 2.f * kScales), 0)) {
       big = row_max(big);
-      const float now = big * vn > 16.f ? 8.f * pow2_under(big) : vn, by = now / vn;
+      const float now = big * vn > 2.f * kScales ? kScales * pow2_under(big) : vn;
+      smaller_unit<NB>(log2_of(vn) - log2_of(now), m[0], l[0], z[0], o[0]);
       vn = now;
-#pragma unroll
-      for (int i = 0; i < NB; i++) o[0][i] *= by;
-      acc[0][0] *= units[wave][lane];
-      acc[0][1] *= units[wave][lane];
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) vsn[j] *= vn;
+    for (int j = 0; j < 8; j++) {
+      vsn[j] *= vn;
+      if (FMT == MG_KV_INT4) vz[j] *= vn;
+    }
     half8v ph[1], pl[1];
-    weigh<FMT, NB, 1>(MASKED, acc, ksf, vsn, kzf, vz, qs, seen, nullptr, m, l, z, o, ph, pl);
+    weigh<FMT, NB, 1>(MASKED, kTop, nullptr, acc, ksf, vsn, kzf, vz, qs, seen, m, l, z, o, ph, pl);
     if (!AHEAD && more) next.load_scales(a, p, g);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -680,40 +728,40 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
   while (t0 < kfin) tile(std::true_type{});
 
   if (refused && lane == 0) atomicOr(a.c.refused, 1);
-  const float iv = 1.f / vn;
   l[0] = row_sum(l[0]);
   z[0] = FMT == MG_KV_INT4 ? row_sum(z[0]) : 0.f;
-  if (g == 0) {
-    stat[wave][0][c] = m[0];
-    stat[wave][1][c] = l[0];
-  }
+  if (g == 0) stat[wave][0][c] = part_ref(m[0], l[0]);
   __syncthreads();
   const float all = fmaxf(fmaxf(stat[0][0][c], stat[1][0][c]), fmaxf(stat[2][0][c], stat[3][0][c]));
-  const float by = exp2_of(m[0] - all);
+  const float sum = part_sum(m[0], l[0], all), inv = l[0] == 0.f ? 0.f : 1.f / l[0], by = sum / vn;
+  if (g == 0) stat[wave][1][c] = sum;
 #pragma unroll
   for (int e = 0; e < 4; e++)
 #pragma unroll
     for (int i = 0; i < NB; i += 4)
       *reinterpret_cast<float4 *>(lds + (wave * 16 + c) * QP + NB * (4 * g + e) + i) =
-          make_float4((o[0][i][e] * iv + z[0]) * by, (o[0][i + 1][e] * iv + z[0]) * by,
-                      (o[0][i + 2][e] * iv + z[0]) * by, (o[0][i + 3][e] * iv + z[0]) * by);
+          make_float4((o[0][i][e] + z[0]) * inv * by, (o[0][i + 1][e] + z[0]) * inv * by,
+                      (o[0][i + 2][e] + z[0]) * inv * by, (o[0][i + 3][e] + z[0]) * inv * by);
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
     const int r = i / (DP / 4), d = 4 * (i - r * (DP / 4));
-    float mm = stat[0][0][r], ll = 0.f;
+    float mm = stat[0][0][r], ll = stat[0][1][r];
 #pragma unroll
-    for (int k = 1; k < 4; k++) mm = fmaxf(mm, stat[k][0][r]);
+    for (int k = 1; k < 4; k++) {
+      mm = fmaxf(mm, stat[k][0][r]);
+      ll += stat[k][1][r];
+    }
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      ll += stat[k][1][r] * exp2_of(stat[k][0][r] - mm);
       const float4 y = *reinterpret_cast<const float4 *>(lds + (k * 16 + r) * QP + d);
       v.x += y.x;
       v.y += y.y;
       v.z += y.z;
       v.w += y.w;
     }
-    put4<DP>(a, w, r, d, v, ll);
+    const float f1 = a.nsplit > 1 ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
+    put4<DP>(a, w, r, d, make_float4(v.x * f1, v.y * f1, v.z * f1, v.w * f1));
     if (d == 0) put_stat(a, w, r, mm, ll);
   }
 }
@@ -801,8 +849,8 @@ void k_kv_rows(const mg_kv_attn a) {
     } t;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
-  __shared__ __attribute__((aligned(16))) float sc[2][5][32];  // scales of a tile's keys
-  __shared__ float unit[2], size[4], units[QB * 256], mine[QB * 256];  // of a lane's rows
+  __shared__ __attribute__((aligned(16))) float sc[2][4][32];  // scales of a tile's keys
+  __shared__ float unit[2], size[4], units[QB * 256];           // units: of a lane's rows
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   Work w;
@@ -855,24 +903,24 @@ void k_kv_rows(const mg_kv_attn a) {
   }
   __syncthreads();  // the queries' place is the tiles' now
 
-  // Wave 3 keeps the unit of the V scales, 8 under the largest so far.
+  // Wave 3 keeps the unit of the V scales (INT4: and middles), under the largest so far.
   float vn = ldexpf(1.f, 100);
   auto stage = [&](int at, int t0) __attribute__((always_inline)) {
     raw.convert(sh.t.k[at], sh.t.v[at], wave, lane);
     if (wave == 3) {
       const bool in = t0 + (lane & 31) < total;
-      const float vs = in ? raw.vs : 0.f;
-      if (__builtin_expect(__any(vs * vn > 16.f), 0)) vn = 8.f * pow2_under(wave_max(vs));
+      const float vs = in ? raw.vs : 0.f, vz = FMT == MG_KV_INT4 && in ? raw.vz : 0.f;
+      const float big = fmaxf(vs, 0.0625f * fabsf(vz));
+      if (__builtin_expect(__any(big * vn > 2.f * kScales), 0)) vn = kScales * pow2_under(wave_max(big));
       if (lane < 32) {
         sc[at][0][lane] = raw.none ? __builtin_nanf("") : raw.ks * f;
         sc[at][1][lane] = vs * vn;
-        sc[at][4][lane] = vs * 0x1p-20f;
         if (FMT == MG_KV_INT4) {
           sc[at][2][lane] = raw.kz * f;
-          sc[at][3][lane] = raw.vz;
+          sc[at][3][lane] = vz * vn;
         }
       }
-      if (lane == 0) unit[at] = vn * 0x1p20f;
+      if (lane == 0) unit[at] = vn;
     }
   };
 
@@ -885,12 +933,28 @@ void k_kv_rows(const mg_kv_attn a) {
 #pragma unroll
     for (int i = 0; i < NB; i++) o[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
-  // The units of the wave's outputs, times 2^20: of plain tiles, and (mine) by rows.
-  float last = 0x1p120f;
-#pragma unroll
-  for (int qb = 0; qb < QB; qb++) mine[qb * 256 + threadIdx.x] = last;
+  float last = vn;  // the unit of the wave's outputs
   auto tile = [&](int at, int t0) __attribute__((always_inline)) {
     const bool masked = t0 + 32 > plain;  // some row may not see some key
+    half8v ph[QB], pl[QB];
+    uint32_t seen[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) seen[qb] = 0xffu;
+    // (The workgroup's unit for all rows: one that sees far smaller scales has a reference that much
+    // lower, which has room for those 2^84 below the workgroup's largest.)
+    const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit[at])));
+    if (__builtin_expect(masked || now != last, 0)) {
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++) {
+        if (masked) {
+          const int qi = min(first + qb * 16 + c, w.rows - 1) / a.group;
+          seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi + 1,
+                               (int64_t)(sq.start + qi) * a.tree_words, kfin);
+        }
+        if (now != last) smaller_unit<NB>(log2_of(last) - log2_of(now), m[qb], l[qb], z[qb], o[qb]);
+      }
+      last = now;
+    }
     float4v acc[QB][2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -911,42 +975,11 @@ void k_kv_rows(const mg_kv_attn a) {
     for (int k = 0; k < (FMT == MG_KV_INT4 ? 4 : 2); k++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const float4 v = *reinterpret_cast<const float4 *>(
-            &sc[at][k == 1 && masked ? 4 : k][16 * u + 4 * g]);
+        const float4 v = *reinterpret_cast<const float4 *>(&sc[at][k][16 * u + 4 * g]);
         x[k][4 * u] = v.x, x[k][4 * u + 1] = v.y, x[k][4 * u + 2] = v.z, x[k][4 * u + 3] = v.w;
       }
-    half8v ph[QB], pl[QB];
-    uint32_t seen[QB];
-#pragma unroll
-    for (int qb = 0; qb < QB; qb++) seen[qb] = 0xffu;
-    // Units of the V scales: a tile that every row sees has the workgroup's, the rows of a
-    // masked one their own, by the keys that they see.  (Masked tiles come last.)
-    const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit[at])));
-    if (__builtin_expect(masked || now != last || uneven, 0)) {
-#pragma unroll
-      for (int qb = 0; qb < QB; qb++) {
-        const float was = mine[qb * 256 + threadIdx.x];
-        float next = now;
-        if (masked) {
-          const int qi = min(first + qb * 16 + c, w.rows - 1) / a.group;
-          seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi + 1,
-                               (int64_t)(sq.start + qi) * a.tree_words, kfin);
-          float big = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; j++) big = seen[qb] >> j & 1 ? fmaxf(big, x[1][j]) : big;
-          big = row_max(big);
-          next = big * was > 16.f ? 8.f * pow2_under(big) : was;
-        }
-        const float by = next / was, own = units[qb * 256 + threadIdx.x];
-        mine[qb * 256 + threadIdx.x] = next;
-#pragma unroll
-        for (int i = 0; i < NB; i++) o[qb][i] *= by;
-        acc[qb][0] *= own;
-        acc[qb][1] *= own;
-      }
-      last = now;
-    }
-    weigh<FMT, NB, QB>(masked, acc, x[0], x[1], x[2], x[3], qs, seen, mine + threadIdx.x, m, l, z, o, ph, pl);
+    weigh<FMT, NB, QB>(masked, uneven ? -1.f : kTop, units + threadIdx.x, acc, x[0], x[1], x[2], x[3],
+                       qs, seen, m, l, z, o, ph, pl);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const half8v va = __builtin_bit_cast(half8v, sh.t.v[at][i * 64 + lane]);
@@ -974,17 +1007,18 @@ void k_kv_rows(const mg_kv_attn a) {
   if (refused && lane == 0) atomicOr(a.c.refused, 1);
 #pragma unroll
   for (int qb = 0; qb < QB; qb++) {
-    const float iv = 0x1p20f / mine[qb * 256 + threadIdx.x];
     const int r = wr0 + qb * 16 + c;
     const float ll = row_sum(l[qb]), zz = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
+    const float ref = part_ref(m[qb], ll), sum = a.nsplit > 1 ? part_sum(m[qb], ll, ref) : 1.f;
+    const float inv = ll == 0.f ? 0.f : 1.f / ll, by = sum / last;
 #pragma unroll
     for (int e = 0; e < 4; e++)
 #pragma unroll
       for (int i = 0; i < NB; i += 4)
         put4<DP>(a, w, r, NB * (4 * g + e) + i,
-                 make_float4(o[qb][i][e] * iv + zz, o[qb][i + 1][e] * iv + zz,
-                             o[qb][i + 2][e] * iv + zz, o[qb][i + 3][e] * iv + zz), ll);
-    if (g == 0) put_stat(a, w, r, m[qb], ll);
+                 make_float4((o[qb][i][e] + zz) * inv * by, (o[qb][i + 1][e] + zz) * inv * by,
+                             (o[qb][i + 2][e] + zz) * inv * by, (o[qb][i + 3][e] + zz) * inv * by));
+    if (g == 0) put_stat(a, w, r, ref, sum);
   }
 }
 
