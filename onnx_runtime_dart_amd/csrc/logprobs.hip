@@ -5,9 +5,9 @@
 //   log p_t = x_t - m - log S,   H = log S - A / S,
 // both parts of H being >= 0, so nothing cancels.  When m grows to m', S and A become
 // e^(m - m') S and e^(m - m') (A + (m - m') S).  Each lane keeps its own m, S and A over 16
-// logits at a time (fp32 sums of at most a few thousand terms, each at most 1); lanes and
-// waves join in 64 bits.  A NaN or +inf logit makes S NaN, a row of -inf leaves S 0:
-// neither has a distribution.
+// logits at a time: fp32 sums of at most 128 terms, each at most 1, which then go into sums in 64
+// bits, so a long row costs no accuracy; lanes and waves join in 64 bits.  A NaN or +inf logit
+// makes S NaN, a row of -inf leaves S 0: neither has a distribution.
 //
 // The alternatives: each wave keeps its 64 largest entries sorted across its lanes, as
 // (key, token) with key the logit's bits in an order that unsigned integers have (NaN
@@ -277,6 +277,7 @@ __device__ inline void finish(const mg_logprobs &p, int64_t row, const Sums &t, 
 
 constexpr int kQuads = 4;              // quads of logits a lane takes at a time
 constexpr int kChunk = 64 * 4 * kQuads;  // logits a wave takes at a time
+constexpr int kFold = 8;               // chunks of a wave whose sums stay in fp32
 // Candidates of a chunk put into the list one by one (some 120 cycles each); more are sorted 64 at a
 // time (some 1200).
 constexpr int kFew = 10;
@@ -300,11 +301,20 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
   const int64_t e0 = (int64_t)split * p.run, e1 = min(end, e0 + p.run);
   const float xt = wave == 0 && p.nsplit == 1 ? given(p, row) : 0.f;
   float m = kLowest, s = 0.f, a = 0.f;
+  Sums far{kLowest, 0, 0};
   List l{0, 0, 0x7fffffff, 0x7fffffff};
   bool first = true;
   __shared__ uint32_t ck[4][TOP == MANY ? 128 : 1];  // a wave's candidates, 64 to be sorted at once
   __shared__ int ci[4][TOP == MANY ? 128 : 1];
+  int64_t fold = e0 + kFold * 4 * kChunk;
   for (int64_t c0 = e0 + wave * kChunk; c0 < e1; c0 += 4 * kChunk) {
+    if (c0 >= fold) {
+      far = moved(far, m);
+      far.s += s;
+      far.a += a;
+      s = a = 0.f;
+      fold = c0 + kFold * 4 * kChunk;
+    }
     float z[kQuads][4];
     const int64_t mine = c0 + lane * 4;
     if (c0 >= off && c0 + kChunk <= e1) {
@@ -410,7 +420,8 @@ __global__ __launch_bounds__(256) void k_logprobs(const mg_logprobs p) {
       }
     }
   }
-  Sums t = wave_join(m, s, a);
+  far = moved(far, m);
+  Sums t = wave_join(m, (float)far.s + s, (float)far.a + a);
   __shared__ Sums st[4];
   __shared__ uint32_t sk[4 * 64];
   __shared__ int si[4 * 64];

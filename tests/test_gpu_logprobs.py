@@ -187,3 +187,30 @@ def test_repeated_calls_are_equal(ops):
     for _ in range(3):
         for a, b in zip(first, ops.op_token_logprobs(x, np.array([1, 2, 3]), top=16)):
             np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("max_bytes", [0, -1])
+@pytest.mark.parametrize("vocab", [2**20 + 3, 2**26 + 5])
+def test_long_rows(ops, vocab, max_bytes):
+    # All logits but one are alike, and a lane has up to 2^18 of them: the sums do not feel how many.
+    low = np.float32(-0.7)
+    x = np.full(vocab, low)
+    x[7] = 0
+    ctx = ops.Context()
+    dev = [ops.DeviceBuffer.from_array(a) for a in (x, np.array([7], np.int32))]
+    out = [ops.DeviceBuffer(4) for _ in range(2)]
+    ctx.set_control(max_bytes=max_bytes)
+    ops.token_logprobs_dev(dev[0].ptr, 1, vocab, tokens_ptr=dev[1].ptr, logprob_ptr=out[0].ptr,
+                           entropy_ptr=out[1].ptr, ctx=ctx)
+    ctx.synchronize()
+    e = np.exp(np.float64(low))
+    s = 1 + (vocab - 1) * e
+    lp, h = -np.log(s), np.log(s) - (vocab - 1) * e * np.float64(low) / s
+    # A term is off by (0.7 + 4) 2^-23 of itself; sums of 128, and those of the lanes, by 200 roundings.
+    # The entropy's own sum is 0.7 of the other; both results round once.
+    rel = 4.7 * 2.0**-23 + 200 * 2.0**-24
+    assert abs(out[0].to_array((1,), np.float32)[0] - lp) <= rel + abs(lp) * 2.0**-24
+    assert abs(out[1].to_array((1,), np.float32)[0] - h) <= 3 * rel + abs(h) * 2.0**-24
+    for t in dev + out:
+        t.free()
+    ctx.close()
