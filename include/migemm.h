@@ -710,7 +710,8 @@ mg_status mg_rotary_tables_f32_dev(mg_ctx *ctx, int64_t first, int64_t count, in
  * [batch, seq, heads, head_size] contiguous; the elements of a vector are adjacent.
  * rope->positions is [batch, seq], NULL = 0 .. seq - 1 in every batch.  A row whose
  * position lies outside the tables gets NaN in its turned elements.  y may be x (with the
- * same strides); it must not overlap it otherwise. */
+ * same strides); it must not overlap it otherwise.  seq below 2^31, heads at most 2^31 - 4,
+ * 2^38 elements at most. */
 mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t batch, int64_t seq,
                                       int64_t heads, int64_t head_size, const int64_t *x_strides,
                                       const mg_rope *rope, float *y_dev,

@@ -2771,7 +2771,7 @@ mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t b
   if (!ctx || !rope) return bad_arg(what, "null argument");
   constexpr int64_t most = (int64_t)1 << 38;  // elements
   if (batch < 0 || seq < 0 || heads < 0 || head_size < 1 || batch > most || seq > 0x7fffffff ||
-      heads > most || head_size > 65536 || (batch && seq > most / batch) ||
+      heads > 0x7ffffffc || head_size > 65536 || (batch && seq > most / batch) ||
       (batch * seq && heads * head_size > most / (batch * seq)))
     return bad_arg(what, "dimensions out of range");
   MG_TRY(check_rope(what, *rope, head_size));

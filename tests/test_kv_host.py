@@ -274,3 +274,9 @@ def test_numbers_beyond_32_bits_do_not_wrap():
     assert refused and (slots == -1).all()
     with pytest.raises(ArgumentError):
         ops.kv_cache_slots([0, 1], [1.5], [[0]], rows=1, max_new=1, max_len=8, pages=1, page_size=16)
+
+
+def test_rotary_heads_beyond_32_bits():
+    # Within the elements that a call takes, but not within the kernel's index of a head.
+    for heads in (2**31 - 3, 2**31, 2**33):
+        assert rotary(heads=heads, d=16) == 1
