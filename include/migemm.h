@@ -708,6 +708,8 @@ mg_status mg_rotary_tables_f32_dev(mg_ctx *ctx, int64_t first, int64_t count, in
  * (lib/src/onnx_ops.dart:2653-2722), in 64 bits, rounded once.  x and y hold batch x seq x
  * heads vectors of head_size; strides are elements of {batch, seq, head}, NULL =
  * [batch, seq, heads, head_size] contiguous; the elements of a vector are adjacent.
+ * Vectors of y must not overlap: each of its strides, from the smallest, passes all that the
+ * smaller ones span.
  * rope->positions is [batch, seq], NULL = 0 .. seq - 1 in every batch.  A row whose
  * position lies outside the tables gets NaN in its turned elements.  y may be x (with the
  * same strides); it must not overlap it otherwise.  seq below 2^31, heads at most 2^31 - 4,

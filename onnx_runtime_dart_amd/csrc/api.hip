@@ -2778,16 +2778,24 @@ mg_status mg_rotary_embedding_f32_dev(mg_ctx *ctx, const float *x_dev, int64_t b
   if (batch * seq * heads == 0) return MG_OK;
   if (!x_dev || !y_dev) return bad_arg(what, "null buffer");
   mg_rotate_problem p{x_dev, y_dev, batch, seq, heads, head_size, {}, {}, *rope};
+  const int64_t sizes[3] = {batch, seq, heads};
   for (int i = 0; i < 3; i++) {
     const int64_t own = i == 0 ? seq * heads * head_size : i == 1 ? heads * head_size : head_size;
     p.xs[i] = x_strides ? x_strides[i] : own;
     p.ys[i] = y_strides ? y_strides[i] : own;
     if (p.xs[i] < 0 || p.ys[i] < 0 || p.xs[i] > most || p.ys[i] > most)
       return bad_arg(what, "strides out of range");
-    const int64_t n = i == 0 ? batch : i == 1 ? seq : heads;
-    if (n > 1 && p.ys[i] < head_size) return bad_arg(what, "output vectors overlap");
-    if (x_dev == y_dev && n > 1 && p.xs[i] != p.ys[i])
+    if (x_dev == y_dev && sizes[i] > 1 && p.xs[i] != p.ys[i])
       return bad_arg(what, "in place needs equal strides");
+  }
+  // y: each stride, from the smallest, passes all that the smaller ones span.
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return p.ys[a] < p.ys[b]; });
+  __int128 span = head_size;
+  for (int i : order) {
+    if (sizes[i] == 1) continue;
+    if (p.ys[i] < span) return bad_arg(what, "output vectors overlap");
+    span += (__int128)p.ys[i] * (sizes[i] - 1);
   }
   MG_TRY(mg_use_device(ctx));
   MG_TRY(mg_check_control(ctx, 0));

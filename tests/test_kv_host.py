@@ -280,3 +280,15 @@ def test_rotary_heads_beyond_32_bits():
     # Within the elements that a call takes, but not within the kernel's index of a head.
     for heads in (2**31 - 3, 2**31, 2**33):
         assert rotary(heads=heads, d=16) == 1
+
+
+@pytest.mark.parametrize("sizes, ys, ok", [
+    ((2, 2, 1), (64, 64, 64), False), ((2, 2, 2), (128, 64, 64), False), ((2, 3, 1), (128, 64, 64), False),
+    ((3, 2, 2), (128, 4096, 64), True), ((2, 1, 2), (64, 0, 64), False), ((1, 4, 2), (0, 64, 100), False),
+    ((2, 3, 4), (768, 256, 64), True), ((2, 3, 4), (64, 512, 128), True), ((2, 3, 4), (767, 256, 64), False),
+    ((1, 1, 1), (0, 0, 0), True), ((1, 5, 1), (1, 64, 1), True), ((2, 3, 4), (64, 128, 384), True),
+    ((2, 3, 4), (64, 128, 383), False)], ids=str)
+def test_rotary_outputs_that_overlap(sizes, ys, ok):
+    # Vectors of 64: each stride passes all that the smaller ones span.
+    refused = rotary(*sizes, d=64, xs=(1, 1, 1), ys=ys) == 1
+    assert refused != ok
