@@ -1229,10 +1229,12 @@ def op_rotary_embedding(x, cos_cache, sin_cache, position_ids=None, *, interleav
                         num_heads: int = 0, ctx: Context | None = None) -> np.ndarray:
     """RotaryEmbedding (the rotation of lib/src/onnx_ops.dart:2653-2722 as its own node): x
     [batch, seq, hidden] with num_heads heads, or [batch, heads, seq, head_size];
-    caches [max_pos, half_rot]; position_ids [batch, seq], or None for 0 .. seq - 1."""
+    caches [max_pos, half_rot] with position_ids [batch, seq], or None for 0 .. seq - 1;
+    or, without position_ids, caches [batch, seq, half_rot], each row's own."""
     x, cos, sin = (np.ascontiguousarray(a, np.float32) for a in (x, cos_cache, sin_cache))
-    if cos.ndim != 2 or cos.shape != sin.shape:
-        raise ArgumentError("RotaryEmbedding: cos and sin caches must be [max_pos, half_rot]")
+    if cos.ndim not in (2, 3) or cos.shape != sin.shape:
+        raise ArgumentError("RotaryEmbedding: cos and sin caches must be [max_pos, half_rot] or "
+                            "[batch, seq, half_rot]")
     if x.ndim == 4:
         batch, heads, seq, d = x.shape
         strides = (heads * seq * d, d, seq * d)
@@ -1242,6 +1244,13 @@ def op_rotary_embedding(x, cos_cache, sin_cache, position_ids=None, *, interleav
     else:
         raise ArgumentError("RotaryEmbedding: x must be [batch, seq, hidden] of num_heads heads or "
                             "[batch, heads, seq, head_size]")
+    if cos.ndim == 3:
+        if position_ids is not None or cos.shape[:2] != (batch, seq):
+            raise ArgumentError("RotaryEmbedding: caches [batch, seq, half_rot] go without position_ids")
+        if batch * seq == 0:
+            return np.zeros(x.shape, np.float32)
+        position_ids = np.arange(batch * seq).reshape(batch, seq)
+        cos, sin = (t.reshape(batch * seq, -1) for t in (cos, sin))
     ctx = ctx or default_context()
     pos = None
     if position_ids is not None:

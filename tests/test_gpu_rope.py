@@ -176,3 +176,23 @@ def test_positions_beyond_32_bits(ops):
     y = ops.op_rotary_embedding(x, cos, sin, np.array([[1, 2**32 + 1, -2**32 + 2]]))
     assert np.isfinite(y[0, :, 0]).all()
     assert np.isnan(y[0, :, 1:, :16]).all() and (y[..., 16:] == x[..., 16:]).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("batch, seq, heads, d, half", [(1, 1, 1, 2, 1), (3, 7, 4, 64, 32), (2, 5, 3, 80, 16)])
+def test_tables_of_each_row(ops, inter, batch, seq, heads, d, half):
+    # The node without position_ids: caches [batch, seq, half], gathered before.
+    rng = np.random.default_rng(10)
+    x = rng.standard_normal((batch, seq, heads, d)).astype(np.float32)
+    cos, sin = tables(rng, batch * seq, half)
+    want = rotate(x.reshape(batch * seq, heads, d), cos, sin, np.arange(batch * seq), inter).reshape(x.shape)
+    cos, sin = cos.reshape(batch, seq, half), sin.reshape(batch, seq, half)
+    y = ops.op_rotary_embedding(x.reshape(batch, seq, -1), cos, sin, num_heads=heads, interleaved=inter)
+    np.testing.assert_array_equal(y.reshape(x.shape), want)
+    y = ops.op_rotary_embedding(x.transpose(0, 2, 1, 3), cos, sin, interleaved=inter)
+    np.testing.assert_array_equal(y, want.transpose(0, 2, 1, 3))
+
+
+def test_no_rows(ops):
+    cos = np.ones((0, 5, 8), np.float32)
+    assert ops.op_rotary_embedding(np.zeros((0, 5, 32), np.float32), cos, cos, num_heads=2).shape == (0, 5, 32)

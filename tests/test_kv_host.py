@@ -292,3 +292,14 @@ def test_rotary_outputs_that_overlap(sizes, ys, ok):
     # Vectors of 64: each stride passes all that the smaller ones span.
     refused = rotary(*sizes, d=64, xs=(1, 1, 1), ys=ys) == 1
     assert refused != ok
+
+
+def test_rotary_cache_shapes():
+    x = np.zeros((2, 3, 32), np.float32)
+    three = np.ones((2, 3, 8), np.float32)
+    for cos, kw in ((three, dict(position_ids=np.zeros((2, 3), np.int64))), (three[:1], {}), (three[:, :2], {}),
+                    (three[0, 0], {}), (three[None], {})):
+        with pytest.raises(ArgumentError):
+            ops.op_rotary_embedding(x, cos, cos, num_heads=2, ctx=object(), **kw)
+    with pytest.raises(ArgumentError):
+        ops.op_rotary_embedding(x, three, three[..., :4], num_heads=2, ctx=object())
