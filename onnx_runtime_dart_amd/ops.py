@@ -193,6 +193,29 @@ class DeviceBuffer:
             pass
 
 
+class _Buffers(list):
+    """Device buffers of one call, freed at its end however it ends."""
+
+    def __init__(self, ctx):
+        super().__init__()
+        self.ctx = ctx
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        for b in self:
+            b.free()
+
+    def new(self, nbytes: int) -> DeviceBuffer:
+        self.append(DeviceBuffer(nbytes, self.ctx))
+        return self[-1]
+
+    def upload(self, arr) -> DeviceBuffer:
+        self.append(DeviceBuffer.from_array(arr, self.ctx))
+        return self[-1]
+
+
 def default_context() -> Context:
     ctx = getattr(_tls, "ctx", None)
     if ctx is None:
@@ -749,35 +772,31 @@ class KvCache:
         if past.size and (row_start[0] < 0 or (n < 0).any() or row_start[-1] > rows or
                           (past < 0).any()):
             raise ArgumentError("KvCache: row_start must rise from 0 to the rows, past be >= 0")
-        bufs = [DeviceBuffer.from_array(x, self.ctx) for x in [row_start, past, page_table, *arrays]]
-        outs = [DeviceBuffer.from_array(np.zeros(sh, np.float32), self.ctx) for sh in out_shapes]
-        try:
+        with _Buffers(self.ctx) as bufs:
+            where = [bufs.upload(x).ptr for x in (row_start, past, page_table)]
+            ins = [bufs.upload(x).ptr for x in arrays]
+            outs = [bufs.upload(np.zeros(sh, np.float32)) for sh in out_shapes]
             r = None
             if rope is not None:
                 cos, sin = (np.ascontiguousarray(x, np.float32) for x in rope[:2])
                 if cos.ndim != 2 or cos.shape != sin.shape:
                     raise ArgumentError("KvCache: cos and sin must be [max_pos, half_rot]")
                 pos = rope[3] if len(rope) > 3 else None
-                bufs += [DeviceBuffer.from_array(cos, self.ctx), DeviceBuffer.from_array(sin, self.ctx)]
-                at = len(bufs) - 2
                 if pos is not None:
                     pos = _int32(pos).ravel()
                     if pos.size != rows:
                         raise ArgumentError("KvCache: one position a row")
-                    bufs.append(DeviceBuffer.from_array(pos, self.ctx))
-                r = Rope(bufs[at].ptr, bufs[at + 1].ptr, max_pos=cos.shape[0], half_rot=cos.shape[1],
-                         interleaved=rope[2], positions_ptr=0 if pos is None else bufs[-1].ptr)
+                r = Rope(bufs.upload(cos).ptr, bufs.upload(sin).ptr, max_pos=cos.shape[0],
+                         half_rot=cos.shape[1], interleaved=rope[2],
+                         positions_ptr=0 if pos is None else bufs.upload(pos).ptr)
             seqs = SeqBatch(batch=past.size, rows=rows, max_new=int(n.max(initial=0)),
-                            max_len=int((n + past).max(initial=0)), row_start_ptr=bufs[0].ptr,
-                            past_ptr=bufs[1].ptr, page_table_ptr=bufs[2].ptr,
+                            max_len=int((n + past).max(initial=0)), row_start_ptr=where[0],
+                            past_ptr=where[1], page_table_ptr=where[2],
                             table_stride=page_table.shape[1])
-            call(seqs, r, [b.ptr for b in bufs[3:3 + len(arrays)]], [o.ptr for o in outs])
+            call(seqs, r, ins, [o.ptr for o in outs])
             got = [o.to_array(sh, np.float32) for o, sh in zip(outs, out_shapes)]
             self.ctx.synchronize()
             return got
-        finally:
-            for b in bufs + outs:
-                b.free()
 
     def append(self, k, v, *, row_start, past, page_table, rope=None):
         """Writes host rows k, v [rows, kv_heads, head_size]."""
@@ -1257,19 +1276,14 @@ def op_rotary_embedding(x, cos_cache, sin_cache, position_ids=None, *, interleav
         pos = _int32(position_ids)
         if pos.shape != (batch, seq):
             raise ArgumentError("RotaryEmbedding: position_ids must be [batch, seq]")
-    pb = None if pos is None else DeviceBuffer.from_array(pos, ctx)
-
-    def call(px, pc, ps, py):
-        rotary_embedding_dev(px, batch, seq, heads, d,
-                             Rope(pc, ps, max_pos=cos.shape[0], half_rot=cos.shape[1],
-                                  interleaved=interleaved, positions_ptr=pb.ptr if pb else 0),
-                             py, x_strides=strides, y_strides=strides, ctx=ctx)
-
-    try:
-        return _run_dev([x, cos, sin], [x.shape], call, ctx)[0]
-    finally:
-        if pb:
-            pb.free()
+    with _Buffers(ctx) as bufs:
+        ins = [bufs.upload(a).ptr for a in (x, cos, sin)]
+        rope = Rope(ins[1], ins[2], max_pos=cos.shape[0], half_rot=cos.shape[1], interleaved=interleaved,
+                    positions_ptr=0 if pos is None else bufs.upload(pos).ptr)
+        y = bufs.new(x.nbytes)
+        rotary_embedding_dev(ins[0], batch, seq, heads, d, rope, y.ptr, x_strides=strides,
+                             y_strides=strides, ctx=ctx)
+        return y.to_array(x.shape, np.float32)
 
 
 def op_token_logprobs(logits, tokens=None, *, top: int = 0, ctx: Context | None = None):
@@ -1290,19 +1304,16 @@ def op_token_logprobs(logits, tokens=None, *, top: int = 0, ctx: Context | None 
     if not 0 <= top <= min(vocab, 64):
         raise ArgumentError("TokenLogProbs: top must be 0 .. 64, at most vocab")
     ctx = ctx or default_context()
-    bufs = [DeviceBuffer.from_array(a, ctx) for a in ins]
     n = max(rows, 1)
-    outs = [DeviceBuffer(4 * k, ctx) for k in (n, n, n * max(top, 1), n * max(top, 1))]
-    try:
-        token_logprobs_dev(bufs[0].ptr, rows, vocab, tokens_ptr=bufs[1].ptr if tokens is not None else 0,
+    with _Buffers(ctx) as bufs:
+        ins = [bufs.upload(a).ptr for a in ins]
+        outs = [bufs.new(4 * k) for k in (n, n, n * max(top, 1), n * max(top, 1))]
+        token_logprobs_dev(ins[0], rows, vocab, tokens_ptr=ins[1] if tokens is not None else 0,
                            logprob_ptr=outs[0].ptr, entropy_ptr=outs[1].ptr, top=top,
                            top_ids_ptr=outs[2].ptr, top_logprobs_ptr=outs[3].ptr, ctx=ctx)
         return (outs[0].to_array(lead, np.float32) if tokens is not None else None,
                 outs[1].to_array(lead, np.float32), outs[2].to_array(lead + (top,), np.int32),
                 outs[3].to_array(lead + (top,), np.float32))
-    finally:
-        for b in bufs + outs:
-            b.free()
 
 
 # ------------------------------------------------------------ convolution

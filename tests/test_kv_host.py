@@ -303,3 +303,43 @@ def test_rotary_cache_shapes():
             ops.op_rotary_embedding(x, cos, cos, num_heads=2, ctx=object(), **kw)
     with pytest.raises(ArgumentError):
         ops.op_rotary_embedding(x, three, three[..., :4], num_heads=2, ctx=object())
+
+
+class Memory:
+    """Device buffers of which the n-th cannot be had."""
+
+    def __init__(self, n):
+        self.left, self.held = n, []
+
+    def __call__(self, nbytes, ctx=None):
+        self.left -= 1
+        if self.left < 0:
+            raise MemoryError
+        buf = type("Buffer", (), dict(ptr=P, free=lambda b: self.held.remove(b)))()
+        self.held.append(buf)
+        return buf
+
+    def from_array(self, arr, ctx=None):
+        return self(arr.nbytes, ctx)
+
+
+def test_buffers_of_a_call_that_fails_are_freed(monkeypatch):
+    # At once, not when the exception is let go.
+    cache = ops.KvCache.__new__(ops.KvCache)
+    cache.kv_heads, cache.head_size, cache.ctx = 2, 16, object()
+    k = np.zeros((3, 2, 16), np.float32)
+    cos = np.zeros((4, 8), np.float32)
+    where = dict(row_start=[0, 3], past=[0], page_table=[[0]])
+    rope = (cos, cos, False, [0, 1, 2])
+    calls = [(lambda: cache.append(k, k, **where, rope=rope), 8),
+             (lambda: cache.read(3, **where), 5),
+             (lambda: cache.attend(k, **where, tree=np.ones((3, 1), np.uint64), rope=rope), 9),
+             (lambda: ops.op_token_logprobs(k[..., 0], np.zeros(3, np.int64), top=1, ctx=object()), 6),
+             (lambda: ops.op_rotary_embedding(k, cos, cos, np.zeros((3, 2)), num_heads=1, ctx=object()), 5)]
+    for call, most in calls:
+        for n in range(most):
+            memory = Memory(n)
+            monkeypatch.setattr(ops, "DeviceBuffer", memory)
+            with pytest.raises(MemoryError) as held:
+                call()
+            assert memory.held == [], (call, n, held)
