@@ -799,7 +799,7 @@ mg_status mg_kv_cache_read_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq
  * ancestors of a drafted token and itself.  Rows that see nothing get zeros.  q is rotated by
  * rope (may be NULL) as keys are by append.  scale defaults to 1 / sqrt(head_size).  Products
  * are formed from fp16 digit pairs of q (22 bits of a row's largest element) and of the weights
- * times V scales (each off by 2^-22 of itself and 2^-35 of the row's sum of them) against the
+ * times V scales (each off by 2^-22 of itself and 2^-33 of the row's sum of them) against the
  * exact codes, sums in fp32.  Strides: 0 = num_heads * head_size; y must not overlap q.  The call takes workspace
  * for partial results when a sequence's keys are split. */
 mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,

@@ -16,12 +16,12 @@
 // which single tokens have room for under the cached bytes and prompts pay for.
 // Digits end at 2^-25, so their unit is that of a row's weights times scales, not of its largest weight
 // and its largest scale, which may belong to different keys: 2^(s - m) is kept relative to a
-// reference m of the row, a whole number that puts the sum of these products over a tile at 2^11 (scales
+// reference m of the row, a whole number that puts the sum of these products over a tile at 2^9 (scales
 // in units of the largest, 2^12; an outlier among them moves m down).  What a key contributes is
-// then off by 2^-22 of itself and 2^-35 of the row's sum, however far its weight and its scale lie
-// from the others'.  m moves up only when a product outgrows fp16, so most tiles rescale nothing and
-// exchange nothing between lanes.  (The sum, not the largest product, which a few tiles later is
-// outgrown: 2 x 2048 rows of heads of 64 took 10% longer.)
+// then off by 2^-22 of itself and 2^-33 of what its wave sums, however far its weight and its scale
+// lie from the others'.  m moves up only when a product outgrows fp16, so most tiles rescale nothing
+// and exchange nothing between lanes.  (With sums at 2^11, 2 x 2048 rows of heads of 64 meet that
+// often enough to take 2% longer; with the largest product at 2^12, 10%.)
 //
 // Few rows (k_kv_keys): four waves take tiles in turn for the same 16 rows, the next tile's loads
 // in flight under this one's products; long ones are bound by the cached bytes (one token of 64
@@ -51,7 +51,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr float kNoMax = -3.0e38f;  // the reference before any score
 constexpr float kTop = 65000.f;     // most of a weight times its scale (fp16 ends at 65504)
-constexpr int kAim = 11;            // log2 of where a tile's sum of them is put
+constexpr int kAim = 9;             // log2 of where a tile's sum of them is put
 constexpr int kRoom = 84;           // log2 of a weight so put, at most (their sums have room above)
 constexpr float kScales = 4096.f;   // the largest V scale lies in [2^11, 2^12) of their unit
 
@@ -147,14 +147,18 @@ __device__ inline void load_run(uint32_t (&w)[KW], const uint8_t *p) {
   }
 }
 
-// Max and sum over the four lanes that hold one row.
+// Max and sum over the four lanes that hold one row, 16 apart.  (Both results of a swap of x with
+// itself: the even parts' values and the odd parts'.)
+template <class F>
+__device__ inline float row_join(float x, const F &join) {
+  x = join(x, __shfl_xor(x, 16));
+  return join(x, __shfl_xor(x, 32));
+}
 __device__ inline float row_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  return row_join(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ inline float row_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  return row_join(x, [](float a, float b) { return a + b; });
 }
 __device__ inline float wave_max(float x) {
 #pragma unroll
@@ -393,11 +397,13 @@ __device__ inline void weigh(bool masked, float limit, const float *units, float
 #pragma unroll
       for (int i = 0; i < NB; i++) o[q][i] *= by;
       scores(q);
-      // (Scores of 2^24 and more are rounded by more than the reference can follow.)
+      // (Scores of 2^23 and more are rounded by more than the reference can follow.)
+      if (__any(fabsf(best) > 0x1p23f)) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j]));
-        d[q][j] = d[q][j] > lim ? lim : d[q][j];
+        for (int j = 0; j < 8; j++) {
+          const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j]));
+          d[q][j] = d[q][j] > lim ? lim : d[q][j];
+        }
       }
     }
   }
@@ -835,9 +841,10 @@ struct Quarter {
 // quarter of what the products take.  (Each wave converting all of its tiles in registers: 2048
 // rows over 6000 keys, D 128, int8 748 us, not 460; 1500 over 3000, D 256, 502, not 254.)  Pages
 // are looked up a tile ahead by scalar loads, whose wait leaves the codes in flight (by vector
-// loads 489, D 256 333).  The bounds are the waves a SIMD that the registers allow unspilled.
+// loads 489, D 256 333).  Two waves a SIMD from 128 rows of heads of 64 on: three, at 168 registers, took
+// 504 us for 494 (2 x 2048 such rows), and more spill.
 template <int FMT, int NB, int QB>
-__global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2)
+__global__ __launch_bounds__(256, QB * NB < 8 ? 3 : 2)
 void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;

@@ -22,22 +22,23 @@ def softmax(s):
     return w / w.sum()
 
 
-def bound(s, v, roundings):
-    """How far a row's output may be off: s [t] its scores, v [t, d] the values as read back.
+def bound(s, v, tiles):
+    """How far a row's output may be off: s [t] its scores, v [t, d] the values as read back,
+    tiles of 32 keys that one wave sums at most.
 
     Queries and keys have one element each, so a score is one product: the query is a power of
     two, its factor scale log2(e) rounds by 2^-24, its product by 2^-24 and to two digits by
     2^-22, the product with the key's scale and the difference to the reference by 2^-24 each
     (INT4: middle and offset, three times the score's size): 8 2^-24 |s|, INT4 three times.
     A weight: that, and 2^-21 (exp2, the scale, its digits of 22 bits).  Digits end at 2^-25
-    where the weights times scales sum to 2^10.5 at least, so each key may lose 2^-35.5 of the sum.
-    Twice for the sum of weights; the sums round `roundings` times, once every 32 keys of a wave
-    and some at the joins.  A value's terms are at most three times its vector's largest element
-    (INT4: middle and offset apart)."""
+    where the weights times scales of a wave sum to 2^8.5 at least, so each of its keys may lose
+    2^-33.5 of its sum.  Twice for the sum of weights; the sums round once a tile and some 32 times
+    at the joins.  A value's terms are at most three times its vector's largest element (INT4:
+    middle and offset apart)."""
     p, size = softmax(s), np.abs(v).max(-1)
-    each = (p * size) @ (24 * np.abs(s) * 2.0**-24 + 2.0**-21) + \
-        (p * size).sum() * (p @ (24 * np.abs(s) * 2.0**-24 + 2.0**-21))
-    return 3 * (each + (len(s) * 2.0**-35.5 + roundings * 2.0**-24) * (p * size).sum())
+    eps = 24 * np.abs(s) * 2.0**-24 + 2.0**-21
+    each = (p * size) @ eps + (p * size).sum() * (p @ eps)
+    return 3 * (each + (32 * tiles * 2.0**-33.5 + (tiles + 32) * 2.0**-24) * (p * size).sum())
 
 
 class Far:
@@ -57,12 +58,12 @@ class Far:
         self.s = R.cached(k[:, 0], fmt)[:, 0].astype(np.float64)
         self.v = R.cached(vv[:, 0], fmt).astype(np.float64)
 
-    def check(self, roundings, tree=None, rows=None):
+    def check(self, tiles, tree=None, rows=None):
         y = self.cache.attend(self.q, **self.b.args(), scale=1.0, tree=tree)
         see = R.visible(self.new, len(self.s) - self.new, tree)
         for i in range(self.new) if rows is None else rows:
             s, v = self.s[see[i]], self.v[see[i]]
-            want, tol = softmax(s) @ v, bound(s, v, roundings)
+            want, tol = softmax(s) @ v, bound(s, v, tiles)
             err = np.abs(y[i] - want).max()
             assert err <= tol, (i, err, tol)
         self.cache.release()
@@ -89,7 +90,7 @@ def test_large_values_of_little_weight(ops, fmt, shape, larger, place):
     s, v = rng.uniform(-1, 1, t), rng.uniform(0.5, 1.5, (t, 64))
     s[at] = -(40 if larger < 30 else 100) * LN2
     v[at] *= 2.0**larger
-    Far(ops, fmt, s, v, **shape).check(t / 32 + 8, rows=sample(shape["new"]))
+    Far(ops, fmt, s, v, **shape).check(t / 32 + 1, rows=sample(shape["new"]))
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -103,7 +104,7 @@ def test_many_keys_of_little_weight(ops, fmt, low, first):
     s[5] = low * LN2
     v[5] *= first
     # (The keys are split: no wave sums more than 64 tiles.)
-    Far(ops, fmt, s, v).check(64 + 32)
+    Far(ops, fmt, s, v).check(64)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -116,7 +117,7 @@ def test_many_rows_over_keys_of_little_weight(ops, fmt, low, first, shape):
     s, v = np.zeros(t), rng.uniform(0.5, 1.5, (t, 64))
     s[5] = low * LN2
     v[5] *= first
-    Far(ops, fmt, s, v, **shape).check(t / 32 + 8, rows=sample(shape["new"]))
+    Far(ops, fmt, s, v, **shape).check(t / 32 + 1, rows=sample(shape["new"]))
 
 
 ORDERS = {"rising": np.sort, "falling": lambda x: np.sort(x)[::-1], "any": lambda x: x}
@@ -133,7 +134,7 @@ def test_weights_and_values_of_all_sizes(ops, fmt, shape, scores, sizes, d):
     t = 900
     s = ORDERS[scores](rng.uniform(-60, 60, t)) * LN2
     v = rng.uniform(0.5, 1.5, (t, d)) * np.exp2(ORDERS[sizes](rng.uniform(-40, 40, t)))[:, None]
-    Far(ops, fmt, s, v, **shape).check(t / 32 + 8, rows=sample(shape["new"]))
+    Far(ops, fmt, s, v, **shape).check(t / 32 + 1, rows=sample(shape["new"]))
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -148,7 +149,7 @@ def test_zero_values_first(ops, fmt, shape):
     s[:100] += 12
     for late in (0.0, 25.0):
         s[300:] += late
-        Far(ops, fmt, s, v, **shape).check(t / 32 + 8, rows=sample(shape["new"]))
+        Far(ops, fmt, s, v, **shape).check(t / 32 + 1, rows=sample(shape["new"]))
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -163,4 +164,4 @@ def test_trees_over_values_of_all_sizes(ops, fmt, new, heads):
     v[:past] *= 1e-18
     tree = np.uint64(1) << rng.integers(0, new, (new, 1)).astype(np.uint64)
     tree[::3] = 0
-    Far(ops, fmt, s, v, new=new, heads=heads, kv=min(heads, 16), page=16).check(8, tree=tree)
+    Far(ops, fmt, s, v, new=new, heads=heads, kv=min(heads, 16), page=16).check(t / 32 + 1, tree=tree)
