@@ -841,10 +841,11 @@ struct Quarter {
 // quarter of what the products take.  (Each wave converting all of its tiles in registers: 2048
 // rows over 6000 keys, D 128, int8 748 us, not 460; 1500 over 3000, D 256, 502, not 254.)  Pages
 // are looked up a tile ahead by scalar loads, whose wait leaves the codes in flight (by vector
-// loads 489, D 256 333).  Two waves a SIMD from 128 rows of heads of 64 on: three, at 168 registers, took
-// 504 us for 494 (2 x 2048 such rows), and more spill.
+// loads 489, D 256 333).  The bounds are the waves a SIMD that the registers allow unspilled.  (128 rows
+// of heads of 64 with two, not three: 8 x 2048 rows over 1000 keys 800 us, not 680; 2 x 2048 over 6000,
+// which leave the card half empty, 576, not 604.)
 template <int FMT, int NB, int QB>
-__global__ __launch_bounds__(256, QB * NB < 8 ? 3 : 2)
+__global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2)
 void k_kv_rows(const mg_kv_attn a) {
   using S = Shape<FMT, NB>;
   constexpr int DP = S::DP, KS = S::KS, QP = DP + 4, ROWS = 64 * QB;
