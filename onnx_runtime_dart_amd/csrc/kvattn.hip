@@ -26,12 +26,12 @@
 // Few rows (k_kv_keys): four waves take tiles in turn for the same 16 rows, the next tile's loads
 // in flight under this one's products; long ones are bound by the cached bytes (one token of 64
 // sequences of 2000 to 8000 keys, 8 heads of 128, e4m3: 134 us, 4.9 TB/s; one of 131072 keys,
-// int8: 58 us), short ones by a chain of latencies (about 5 us to the first weights, 4 for the
-// join of key splits).  Many rows (k_kv_rows): bound by the two-digit products and by the
-// exponentials and digits between them (2048 rows over 6000 keys, 32 heads of 128, int8: 460 us,
-// three such chunks 550 TFLOP/s of the product's, 1100 with both digits: what a large fp16
-// product of the library reaches on this card; heads of 64: 420, where the exponentials weigh
-// twice as much).
+// int8: 59 us; int4 by its conversions, 153 us for 64 sequences where e4m3 takes 144), short ones by
+// a chain of latencies (about 5 us to the first weights, 4 for the join of key splits).  Many
+// rows (k_kv_rows): bound by the two-digit products and by the exponentials and digits between
+// them (2048 rows over 6000 keys, 32 heads of 128, int8: 460 us, three such chunks 540 TFLOP/s of
+// the product's, 1080 with both digits, near what a large fp16 product of the library reaches on
+// this card; heads of 64: 344 us and 429 TFLOP/s, where the exponentials weigh twice as much).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

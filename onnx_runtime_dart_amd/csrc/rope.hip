@@ -3,9 +3,11 @@
 //
 // Tables: entry (p, i) is value_factor * cos / sin of p f_i.  The angle in turns, p f_i /
 // 2 pi, is formed in 64 bits and its whole part dropped there, so an entry at position
-// 10^6 is as exact as one at 0; what is left, at most half a turn, goes through the fp32
-// sincospi.  One pass of writes bounds it: a thread makes four adjacent entries (one
-// 16-byte store a table) where half_rot is a multiple of four.
+// 10^6 is as exact as one at 0; what is left, at most half a turn, is rounded to fp32 and goes
+// through the fp32 sincospi, then times value_factor in fp32: three roundings, where cosines in
+// 64 bits would round once, for twice the error (4e-8 of the entries' size on average).  One pass
+// of writes bounds it: a thread makes four adjacent entries (one 16-byte store a table) where
+// half_rot is a multiple of four.
 //
 // Rotation: y = (x c - z s, z c + x s) per pair in 64 bits, rounded once, as the
 // rotation inside GroupQueryAttention.  One pass of reads and writes bounds it: a thread
