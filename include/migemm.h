@@ -698,8 +698,8 @@ typedef struct mg_rope_scaling {
 /* cos_dev / sin_dev [count, half_rot] for positions first .. first + count - 1:
  * value_factor * cos(p f_i) with f_i = base^(-i / half_rot) scaled as above (NULL:
  * MG_ROPE_NONE, value_factor 1).  Angles are formed in 64 bits, so far positions are as
- * exact as near ones: within 4e-7 of value_factor up to position 10^8.  These are the cos_cache / sin_cache inputs of
- * GroupQueryAttention.  half_rot <= 128, positions < 2^31. */
+ * exact as near ones: within 4e-7 of value_factor up to position 10^8.  These are the
+ * cos_cache / sin_cache inputs of GroupQueryAttention.  half_rot <= 128, positions < 2^31. */
 mg_status mg_rotary_tables_f32_dev(mg_ctx *ctx, int64_t first, int64_t count, int64_t half_rot,
                                    double base, const mg_rope_scaling *scaling, float *cos_dev,
                                    float *sin_dev);
