@@ -147,18 +147,14 @@ __device__ inline void load_run(uint32_t (&w)[KW], const uint8_t *p) {
   }
 }
 
-// Max and sum over the four lanes that hold one row, 16 apart.  (Both results of a swap of x with
-// itself: the even parts' values and the odd parts'.)
-template <class F>
-__device__ inline float row_join(float x, const F &join) {
-  x = join(x, __shfl_xor(x, 16));
-  return join(x, __shfl_xor(x, 32));
-}
+// Max and sum over the four lanes that hold one row.
 __device__ inline float row_max(float x) {
-  return row_join(x, [](float a, float b) { return fmaxf(a, b); });
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
 }
 __device__ inline float row_sum(float x) {
-  return row_join(x, [](float a, float b) { return a + b; });
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
 }
 __device__ inline float wave_max(float x) {
 #pragma unroll
