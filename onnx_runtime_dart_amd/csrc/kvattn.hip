@@ -331,15 +331,16 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
 
 // One tile's weights for QB blocks of 16 rows: 2^(s - m) of the lane's eight keys, and the digits of
 // those times the V scales vsn.  l and z are the lane's share of the sum and (INT4) of the sum of
-// weights times middles.  masked: only the keys of `seen` count (a branch of the whole wave, or a constant);
-// limit: kTop, or negative where some row's products have units of their own, the lane's at units[256 q].
-template <int FMT, int NB, int QB>
-__device__ inline void weigh(bool masked, float limit, const float *units, float4v (&acc)[QB][2],
-                             const float (&ksf)[8], const float (&vsn)[8], const float (&kzf)[8],
-                             const float (&vz)[8], const float (&qs)[QB],
-                             const uint32_t (&seen)[QB], float (&m)[QB], float (&l)[QB],
-                             float (&z)[QB], float4v (&o)[QB][NB], half8v (&ph)[QB],
-                             half8v (&pl)[QB]) {
+// weights times middles.  masked: only the keys of `seen` count (a branch of the whole wave, or a
+// constant), and with UNITS V scales and middles want the factors unit[256 q] of the rows yet.  own: some
+// row's products do so with units[256 q].  limit: kTop (over the largest such factor); with own negative.
+template <int FMT, int NB, int QB, bool UNITS>
+__device__ inline void weigh(bool masked, const float *unit, bool own, const float *units,
+                             float limit, float4v (&acc)[QB][2], const float (&ksf)[8],
+                             const float (&vsn)[8], const float (&kzf)[8], const float (&vz)[8],
+                             const float (&qs)[QB], const uint32_t (&seen)[QB], float (&m)[QB],
+                             float (&l)[QB], float (&z)[QB], float4v (&o)[QB][NB],
+                             half8v (&ph)[QB], half8v (&pl)[QB]) {
   float d[QB][8];  // scores less m, of unseen keys too
   auto scores = [&](int q) __attribute__((always_inline)) {
 #pragma unroll
@@ -361,15 +362,15 @@ __device__ inline void weigh(bool masked, float limit, const float *units, float
   float big = 0x1p-74f;
 #pragma unroll
   for (int j = 0; j < 8; j++) big = fmaxf(big, vsn[j]);
-  // (An unseen key may bring a wave here, where only the seen ones count; and rows with units of their
-  // own do, whose products d is not yet in.  No branch of their own takes those there: where
-  // paths of different length meet behind a matrix product, the compiler (ROCm 7.2) has left out
-  // the wait for its result.)
+  // (An unseen key may bring a wave here, where only the seen ones count; and a negative limit does, where
+  // products want factors yet.  No branch of their own takes those there: where paths of
+  // different length meet behind a matrix product, the compiler (ROCm 7.2) has left out the wait
+  // for its result.)
   if (__builtin_expect(__any(exp2_of(most) * big > limit), 0)) {
 #pragma unroll
     for (int q = 0; q < QB; q++) {
       const float old = m[q];
-      if (limit < 0.f) {
+      if (own) {
         acc[q][0] *= units[256 * q];
         acc[q][1] *= units[256 * q];
       }
@@ -377,11 +378,11 @@ __device__ inline void weigh(bool masked, float limit, const float *units, float
       scores(q);
 #pragma unroll
       for (int j = 0; j < 8; j++) d[q][j] = seen[q] >> j & 1 ? d[q][j] : -__builtin_inff();
-      const float best = row_max(top(q));
+      const float best = row_max(top(q)), u = UNITS && masked ? unit[256 * q] : 1.f;
       float p = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float x = exp2_of(d[q][j] - best) * vsn[j];
+        const float x = exp2_of(d[q][j] - best) * vsn[j] * u;
         p += x > 0.f ? x : 0.f;
       }
       // (Whole numbers: outputs and sums are moved without rounding.)
@@ -397,7 +398,7 @@ __device__ inline void weigh(bool masked, float limit, const float *units, float
       if (__any(fabsf(best) > 0x1p23f)) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j]));
+          const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j] * u));
           d[q][j] = d[q][j] > lim ? lim : d[q][j];
         }
       }
@@ -416,14 +417,16 @@ __device__ inline void weigh(bool masked, float limit, const float *units, float
     // keeps the selections in their branch; else every tile does them.)
     asm volatile("");
 #pragma unroll
-    for (int q = 0; q < QB; q++)
+    for (int q = 0; q < QB; q++) {
+      const float u = UNITS ? unit[256 * q] : 1.f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const bool on = seen[q] >> j & 1;
         e[q][j] = on ? e[q][j] : 0.f;
-        w[q][j] = on ? w[q][j] : 0.f;
-        if (FMT == MG_KV_INT4) z[q] += on ? e[q][j] * vz[j] : 0.f;
+        w[q][j] = on ? w[q][j] * u : 0.f;
+        if (FMT == MG_KV_INT4) z[q] += on ? e[q][j] * (vz[j] * u) : 0.f;
       }
+    }
   } else if (FMT == MG_KV_INT4) {
 #pragma unroll
     for (int q = 0; q < QB; q++)
@@ -714,7 +717,8 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
       if (FMT == MG_KV_INT4) vz[j] *= vn;
     }
     half8v ph[1], pl[1];
-    weigh<FMT, NB, 1>(MASKED, kTop, nullptr, acc, ksf, vsn, kzf, vz, qs, seen, m, l, z, o, ph, pl);
+    weigh<FMT, NB, 1, false>(MASKED, nullptr, false, nullptr, kTop, acc, ksf, vsn, kzf, vz, qs, seen,
+                             m, l, z, o, ph, pl);
     if (!AHEAD && more) next.load_scales(a, p, g);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -853,8 +857,9 @@ void k_kv_rows(const mg_kv_attn a) {
     } t;
   };
   __shared__ __attribute__((aligned(16))) Shared sh;
-  __shared__ __attribute__((aligned(16))) float sc[2][4][32];  // scales of a tile's keys
-  __shared__ float unit[2], size[4], units[QB * 256];           // units: of a lane's rows
+  // Scales of a tile's keys: K, V, and INT4 their middles; V's in units, and as they are (for masked tiles).
+  __shared__ __attribute__((aligned(16))) float sc[2][2][4][32];
+  __shared__ float unit[2], size[4], units[QB * 256], mine[QB * 256];  // of a lane's rows
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   Work w;
@@ -868,6 +873,7 @@ void k_kv_rows(const mg_kv_attn a) {
                    : a.tree        ? kfin
                         : min(kfin, sq.past + (min(first + 16 * QB, w.rows) - 1) / a.group + 1);
   const int plain = a.tree ? sq.past : sq.past + min(first, w.rows - 1) / a.group + 1;
+  const int all = a.tree ? sq.past : sq.past + w.r0 / a.group + 1;  // of the workgroup
   Quarter<FMT, NB> raw;
   Place p;
   bool refused = false;
@@ -917,11 +923,20 @@ void k_kv_rows(const mg_kv_attn a) {
       const float big = fmaxf(vs, 0.0625f * fabsf(vz));
       if (__builtin_expect(__any(big * vn > 2.f * kScales), 0)) vn = kScales * pow2_under(wave_max(big));
       if (lane < 32) {
-        sc[at][0][lane] = raw.none ? __builtin_nanf("") : raw.ks * f;
-        sc[at][1][lane] = vs * vn;
+        const float ks = raw.none ? __builtin_nanf("") : raw.ks * f, kz = raw.kz * f;
+        sc[at][0][0][lane] = ks;
+        sc[at][0][1][lane] = vs * vn;
         if (FMT == MG_KV_INT4) {
-          sc[at][2][lane] = raw.kz * f;
-          sc[at][3][lane] = vz * vn;
+          sc[at][0][2][lane] = kz;
+          sc[at][0][3][lane] = vz * vn;
+        }
+        if (t0 + 32 > all) {
+          sc[at][1][0][lane] = ks;
+          sc[at][1][1][lane] = vs;
+          if (FMT == MG_KV_INT4) {
+            sc[at][1][2][lane] = kz;
+            sc[at][1][3][lane] = vz;
+          }
         }
       }
       if (lane == 0) unit[at] = vn;
@@ -937,28 +952,14 @@ void k_kv_rows(const mg_kv_attn a) {
 #pragma unroll
     for (int i = 0; i < NB; i++) o[qb][i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
-  float last = vn;  // the unit of the wave's outputs
-  auto tile = [&](int at, int t0) __attribute__((always_inline)) {
-    const bool masked = t0 + 32 > plain;  // some row may not see some key
-    half8v ph[QB], pl[QB];
-    uint32_t seen[QB];
+  // The units of the wave's outputs: of plain tiles, and (mine) by rows.
+  float last = vn;
 #pragma unroll
-    for (int qb = 0; qb < QB; qb++) seen[qb] = 0xffu;
-    // (The workgroup's unit for all rows: one that sees far smaller scales has a reference that much
-    // lower, which has room for those 2^84 below the workgroup's largest.)
-    const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit[at])));
-    if (__builtin_expect(masked || now != last, 0)) {
-#pragma unroll
-      for (int qb = 0; qb < QB; qb++) {
-        if (masked) {
-          const int qi = min(first + qb * 16 + c, w.rows - 1) / a.group;
-          seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi + 1,
-                               (int64_t)(sq.start + qi) * a.tree_words, kfin);
-        }
-        if (now != last) smaller_unit<NB>(log2_of(last) - log2_of(now), m[qb], l[qb], z[qb], o[qb]);
-      }
-      last = now;
-    }
+  for (int qb = 0; qb < QB; qb++) mine[qb * 256 + threadIdx.x] = last;
+  auto tile = [&](int at, int t0, float unit_at) __attribute__((always_inline)) {
+    // Some row may not see some key.  (A number: as a condition, it is made one of each lane.)
+    const uint32_t part = (uint32_t)(plain - (t0 + 32)) >> 31;
+    const bool masked = part;
     float4v acc[QB][2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -979,11 +980,52 @@ void k_kv_rows(const mg_kv_attn a) {
     for (int k = 0; k < (FMT == MG_KV_INT4 ? 4 : 2); k++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const float4 v = *reinterpret_cast<const float4 *>(&sc[at][k][16 * u + 4 * g]);
+        const float4 v = *reinterpret_cast<const float4 *>(&sc[at][part][k][16 * u + 4 * g]);
         x[k][4 * u] = v.x, x[k][4 * u + 1] = v.y, x[k][4 * u + 2] = v.z, x[k][4 * u + 3] = v.w;
       }
-    weigh<FMT, NB, QB>(masked, uneven ? -1.f : kTop, units + threadIdx.x, acc, x[0], x[1], x[2], x[3],
-                       qs, seen, m, l, z, o, ph, pl);
+    // The eight wait states of the last product's result, written out: where paths of different length
+    // meet behind a matrix product, the compiler (ROCm 7.2) has left them out.
+    if constexpr (QB == 1)
+      asm volatile("s_nop 7" : "+v"(acc[0][0]), "+v"(acc[0][1]));
+    else
+      asm volatile("s_nop 7" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]));
+    half8v ph[QB], pl[QB];
+    uint32_t seen[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; qb++) seen[qb] = 0xffu;
+    // Units of the V scales: a tile that every row sees has the workgroup's, the rows of a
+    // masked one their own, by the keys that they see.  (Masked tiles come last.)
+    const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit_at)));
+    float limit = uneven ? -1.f : kTop;
+    if (__builtin_expect(masked || now != last, 0)) {
+      float most = 0.f;
+#pragma unroll
+      for (int qb = 0; qb < QB; qb++) {
+        const float was = mine[qb * 256 + threadIdx.x];
+        float next = now;
+        if (masked) {
+          const int qi = min(first + qb * 16 + c, w.rows - 1) / a.group;
+          seen[qb] = seen_keys(a, sq, t0, g, a.tree ? sq.past : sq.past + qi + 1,
+                               (int64_t)(sq.start + qi) * a.tree_words, kfin);
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const float v = FMT == MG_KV_INT4 ? fmaxf(x[1][j], 0.0625f * fabsf(x[3][j])) : x[1][j];
+            big = seen[qb] >> j & 1 ? fmaxf(big, v) : big;
+          }
+          big = row_max(big);
+          next = big * was > 2.f * kScales ? kScales * pow2_under(big) : was;
+        }
+        smaller_unit<NB>(log2_of(was) - log2_of(next), m[qb], l[qb], z[qb], o[qb]);
+        mine[qb * 256 + threadIdx.x] = next;
+        most = fmaxf(most, next);
+      }
+      // (2^20 at most: the bound of the weights alone has no such factor.)
+      if (masked && !uneven) limit = fminf(kTop / most, 0x1p20f);
+      last = now;
+    }
+    weigh<FMT, NB, QB, true>(masked, mine + threadIdx.x, uneven, units + threadIdx.x, limit, acc, x[0],
+                             x[1], x[2], x[3], qs, seen, m, l, z, o, ph, pl);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const half8v va = __builtin_bit_cast(half8v, sh.t.v[at][i * 64 + lane]);
@@ -1000,11 +1042,12 @@ void k_kv_rows(const mg_kv_attn a) {
   int at = 0;
   for (int t0 = w.kbeg; t0 < kfin; t0 += 32) {
     __syncthreads();  // tile t0 is there, and every wave is done with the one before
+    const float unit_at = unit[at];
     if (t0 + 32 < kfin) {
       stage(at ^ 1, t0 + 32);
       if (t0 + 64 < kfin) fetch(t0 + 64);
     }
-    if (t0 < wfin) tile(at, t0);
+    if (t0 < wfin) tile(at, t0, unit_at);
     at ^= 1;
   }
 
@@ -1014,7 +1057,7 @@ void k_kv_rows(const mg_kv_attn a) {
     const int r = wr0 + qb * 16 + c;
     const float ll = row_sum(l[qb]), zz = FMT == MG_KV_INT4 ? row_sum(z[qb]) : 0.f;
     const float ref = part_ref(m[qb], ll), sum = a.nsplit > 1 ? part_sum(m[qb], ll, ref) : 1.f;
-    const float inv = ll == 0.f ? 0.f : 1.f / ll, by = sum / last;
+    const float inv = ll == 0.f ? 0.f : 1.f / ll, by = sum / mine[qb * 256 + threadIdx.x];
 #pragma unroll
     for (int e = 0; e < 4; e++)
 #pragma unroll

@@ -165,3 +165,29 @@ def test_trees_over_values_of_all_sizes(ops, fmt, new, heads):
     tree = np.uint64(1) << rng.integers(0, new, (new, 1)).astype(np.uint64)
     tree[::3] = 0
     Far(ops, fmt, s, v, new=new, heads=heads, kv=min(heads, 16), page=16).check(t / 32 + 1, tree=tree)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new, heads", [(30, 1), (64, 512), (500, 256)])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_values_of_the_last_size_that_a_row_does_not_see(ops, fmt, d, new, heads, drafts):
+    # Some of the new tokens hold values near the largest of all; rows before them, and drafts beside
+    # them, are as exact as without.
+    rng = np.random.default_rng(10)
+    past = 70
+    t = past + new
+    v = rng.uniform(0.5, 1.5, (t, d)) * np.exp2(rng.choice([-20, 0], t))[:, None]
+    s = rng.uniform(-8, 8, t)
+    far = past + np.array([new // 3, new // 2, new - 1])
+    v[far] = rng.choice([-1, 1], (3, d)) * 1e37
+    tree = None
+    if drafts:
+        words = -(-new // 64)
+        j = rng.integers(0, new, new)
+        j[np.isin(j + past, far)] = 0
+        tree = np.zeros((new, words), np.uint64)
+        tree[np.arange(new), j // 64] = np.uint64(1) << (j % 64).astype(np.uint64)
+    rows = [r for r in range(new) if drafts or r < new // 3]
+    Far(ops, fmt, s, v, new=new, heads=heads, kv=min(heads, 16), page=16).check(
+        t / 32 + 1, tree=tree, rows=rows if new < 100 else rows[::7])
