@@ -21,7 +21,7 @@
 // then off by 2^-22 of itself and 2^-33 of what its wave sums, however far its weight and its scale
 // lie from the others'.  m moves up only when a product outgrows fp16, so most tiles rescale nothing
 // and exchange nothing between lanes.  (With sums at 2^11, 2 x 2048 rows of heads of 64 meet that
-// often enough to take 2% longer; with the largest product at 2^12, 10%.)
+// often enough to take 1% longer; with the largest product at 2^12, 10%.)
 //
 // Few rows (k_kv_keys): four waves take tiles in turn for the same 16 rows, the next tile's loads
 // in flight under this one's products; long ones are bound by the cached bytes (one token of 64
@@ -29,9 +29,9 @@
 // int8: 59 us; int4 by its conversions, 153 us for 64 sequences where e4m3 takes 144), short ones by
 // a chain of latencies (about 5 us to the first weights, 4 for the join of key splits).  Many
 // rows (k_kv_rows): bound by the two-digit products and by the exponentials and digits between
-// them (2048 rows over 6000 keys, 32 heads of 128, int8: 460 us, three such chunks 540 TFLOP/s of
-// the product's, 1080 with both digits, near what a large fp16 product of the library reaches on
-// this card; heads of 64: 344 us and 429 TFLOP/s, where the exponentials weigh twice as much).
+// them (2048 rows over 6000 keys, 32 heads of 128, int8: 468 us, three such chunks 532 TFLOP/s of
+// the product's, 1064 with both digits, near what a large fp16 product of the library reaches on
+// this card; heads of 64: 334 us and 426 TFLOP/s, where the exponentials weigh twice as much).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -842,8 +842,8 @@ struct Quarter {
 // rows over 6000 keys, D 128, int8 748 us, not 460; 1500 over 3000, D 256, 502, not 254.)  Pages
 // are looked up a tile ahead by scalar loads, whose wait leaves the codes in flight (by vector
 // loads 489, D 256 333).  The bounds are the waves a SIMD that the registers allow unspilled.  (128 rows
-// of heads of 64 with two, not three: 8 x 2048 rows over 1000 keys 800 us, not 680; 2 x 2048 over 6000,
-// which leave the card half empty, 576, not 604.)
+// of heads of 64 with two, not three: 8 x 2048 rows over 1000 keys 818 us, not 675; 2 x 2048 over 6000,
+// which leave the card half empty, 580 and 582.)
 template <int FMT, int NB, int QB>
 __global__ __launch_bounds__(256, QB * NB <= (FMT == MG_KV_INT4 ? 4 : 8) ? 3 : 2)
 void k_kv_rows(const mg_kv_attn a) {
