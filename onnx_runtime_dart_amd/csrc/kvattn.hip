@@ -333,10 +333,11 @@ __device__ inline void stage_queries(const mg_kv_attn &a, const kv_seq &sq, int 
 // those times the V scales vsn.  l and z are the lane's share of the sum and (INT4) of the sum of
 // weights times middles.  masked: only the keys of `seen` count (a branch of the whole wave, or a
 // constant), and with UNITS V scales and middles want the factors unit[256 q] of the rows yet.  own: some
-// row's products do so with units[256 q].  limit: kTop (over the largest such factor); with own negative.
+// row's products do so with units[256 q].  limit: kTop (over the largest such factor); negative with own,
+// and with coarse, which is set for good where scores are too large for the reference to follow.
 template <int FMT, int NB, int QB, bool UNITS>
 __device__ inline void weigh(bool masked, const float *unit, bool own, const float *units,
-                             float limit, float4v (&acc)[QB][2], const float (&ksf)[8],
+                             bool &coarse, float limit, float4v (&acc)[QB][2], const float (&ksf)[8],
                              const float (&vsn)[8], const float (&kzf)[8], const float (&vz)[8],
                              const float (&qs)[QB], const uint32_t (&seen)[QB], float (&m)[QB],
                              float (&l)[QB], float (&z)[QB], float4v (&o)[QB][NB],
@@ -388,19 +389,21 @@ __device__ inline void weigh(bool masked, const float *unit, bool own, const flo
       // (Whole numbers: outputs and sums are moved without rounding.)
       const float aim = rintf(best + (float)max(log2_of(row_sum(p)) - kAim, -kRoom));
       m[q] = aim > old + 2.f ? aim : old;
+      // Scores beyond 2^22 go by their fp32 values, the reference is the largest: differences that are
+      // not rounded would tell apart what is equal, and miss the reference.
+      const bool far = fabsf(best) > 0x1p22f && best > -__builtin_inff();
+      coarse |= __any(far);
+      if (far) m[q] = fmaxf(old, best);
       const float by = ldexpf(1.f, (int)fmaxf(old - m[q], -200.f));
       l[q] *= by;
       z[q] *= by;
 #pragma unroll
       for (int i = 0; i < NB; i++) o[q][i] *= by;
-      scores(q);
-      // (Scores of 2^23 and more are rounded by more than the reference can follow.)
-      if (__any(fabsf(best) > 0x1p23f)) {
+      if (coarse) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float lim = fminf(kRoom + 4.f, 15.87f - __builtin_amdgcn_logf(vsn[j] * u));
-          d[q][j] = d[q][j] > lim ? lim : d[q][j];
-        }
+        for (int j = 0; j < 8; j++) d[q][j] -= m[q];
+      } else {
+        scores(q);
       }
     }
   }
@@ -657,6 +660,7 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
 #pragma unroll
   for (int i = 0; i < NB; i++) o[0][i] = float4v{0.f, 0.f, 0.f, 0.f};
   float m[1] = {kNoMax}, l[1] = {0.f}, z[1] = {0.f}, vn = ldexpf(1.f, 100);
+  bool coarse = false;
   // With registers to spare the next tile's loads start before this one's products, else each
   // part's as soon as this one's is used.
   constexpr bool AHEAD = NB <= 8;
@@ -717,8 +721,8 @@ __global__ __launch_bounds__(256, NB <= 8 ? 2 : 1) void k_kv_keys(const mg_kv_at
       if (FMT == MG_KV_INT4) vz[j] *= vn;
     }
     half8v ph[1], pl[1];
-    weigh<FMT, NB, 1, false>(MASKED, nullptr, false, nullptr, kTop, acc, ksf, vsn, kzf, vz, qs, seen,
-                             m, l, z, o, ph, pl);
+    weigh<FMT, NB, 1, false>(MASKED, nullptr, false, nullptr, coarse, coarse ? -1.f : kTop, acc, ksf,
+                             vsn, kzf, vz, qs, seen, m, l, z, o, ph, pl);
     if (!AHEAD && more) next.load_scales(a, p, g);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
@@ -954,6 +958,7 @@ void k_kv_rows(const mg_kv_attn a) {
   }
   // The units of the wave's outputs: of plain tiles, and (mine) by rows.
   float last = vn;
+  bool coarse = false;
 #pragma unroll
   for (int qb = 0; qb < QB; qb++) mine[qb * 256 + threadIdx.x] = last;
   auto tile = [&](int at, int t0, float unit_at) __attribute__((always_inline)) {
@@ -996,7 +1001,7 @@ void k_kv_rows(const mg_kv_attn a) {
     // Units of the V scales: a tile that every row sees has the workgroup's, the rows of a
     // masked one their own, by the keys that they see.  (Masked tiles come last.)
     const float now = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(unit_at)));
-    float limit = uneven ? -1.f : kTop;
+    float limit = uneven || coarse ? -1.f : kTop;
     if (__builtin_expect(masked || now != last, 0)) {
       float most = 0.f;
 #pragma unroll
@@ -1021,11 +1026,11 @@ void k_kv_rows(const mg_kv_attn a) {
         most = fmaxf(most, next);
       }
       // (2^20 at most: the bound of the weights alone has no such factor.)
-      if (masked && !uneven) limit = fminf(kTop / most, 0x1p20f);
+      if (masked && limit > 0.f) limit = fminf(kTop / most, 0x1p20f);
       last = now;
     }
-    weigh<FMT, NB, QB, true>(masked, mine + threadIdx.x, uneven, units + threadIdx.x, limit, acc, x[0],
-                             x[1], x[2], x[3], qs, seen, m, l, z, o, ph, pl);
+    weigh<FMT, NB, QB, true>(masked, mine + threadIdx.x, uneven, units + threadIdx.x, coarse, limit, acc,
+                             x[0], x[1], x[2], x[3], qs, seen, m, l, z, o, ph, pl);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
       const half8v va = __builtin_bit_cast(half8v, sh.t.v[at][i * 64 + lane]);

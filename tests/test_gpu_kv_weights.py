@@ -191,3 +191,23 @@ def test_values_of_the_last_size_that_a_row_does_not_see(ops, fmt, d, new, heads
     rows = [r for r in range(new) if drafts or r < new // 3]
     Far(ops, fmt, s, v, new=new, heads=heads, kv=min(heads, 16), page=16).check(
         t / 32 + 1, tree=tree, rows=rows if new < 100 else rows[::7])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("size", [2.0**22, 2.0**24, 2.0**27, 2.0**34, -(2.0**34)])
+def test_scores_beyond_what_their_digits_tell_apart(ops, fmt, shape, size):
+    # Equal keys share the weight, however large their scores; all others are far below.
+    rng = np.random.default_rng(11)
+    t = 900
+    top = rng.random(t) < 0.3
+    top[:2] = [False, True]
+    s, v = np.where(top, size, size - 0.5 * abs(size)), rng.uniform(0.5, 1.5, (t, 64))
+    far = Far(ops, fmt, s, v, **shape)
+    y = far.cache.attend(far.q, **far.b.args(), scale=1.0)
+    past = t - far.new
+    for i in sample(far.new):
+        seen = far.v[:past + i + 1][top[:past + i + 1]]
+        tol = bound(np.zeros(len(seen)), seen, t / 32 + 1)
+        assert np.abs(y[i] - seen.mean(0)).max() <= tol, i
+    far.cache.release()
