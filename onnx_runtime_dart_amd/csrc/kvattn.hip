@@ -599,9 +599,10 @@ __device__ inline void put4(const mg_kv_attn &a, const Work &w, int r, int d, fl
   }
 }
 // A part of a row's keys where it is joined with the others: the reference under which the sum l of
-// its weights (kept under m) is below 1, and the sum under a reference that may be higher.
+// its weights (kept under m) is below 1/4, so that a workgroup's four parts of the largest values have
+// a finite sum; and l under a reference that may be higher.
 __device__ inline float part_ref(float m, float l) {
-  return l == 0.f ? kNoMax : m + (float)(log2_of(l) + 1);
+  return l == 0.f ? kNoMax : m + (float)(log2_of(l) + 3);
 }
 __device__ inline float part_sum(float m, float l, float ref) {
   return ldexpf(l, (int)fminf(fmaxf(m - ref, -400.f), 400.f));
@@ -1105,7 +1106,8 @@ __global__ __launch_bounds__(256) void k_kv_join(const mg_kv_attn a) {
     for (int i = grp; i < n; i += G) {
       const float2 s = ml[i];
       const float4 x = *reinterpret_cast<const float4 *>(p + (int64_t)i * dp);
-      const float by = exp2_of(s.x - all);
+      // (2^-10: a row has fewer splits, whose sum then is finite too.)
+      const float by = exp2_of(s.x - all - 10.f);
       l += s.y * by;
       v.x += x.x * by;
       v.y += x.y * by;

@@ -211,3 +211,15 @@ def test_scores_beyond_what_their_digits_tell_apart(ops, fmt, shape, size):
         tol = bound(np.zeros(len(seen)), seen, t / 32 + 1)
         assert np.abs(y[i] - seen.mean(0)).max() <= tol, i
     far.cache.release()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("t, shape", [(9, SHAPES[0]), (300, SHAPES[0]), (40000, SHAPES[0]), (900, SHAPES[1]),
+                                      (6000, dict(new=64, heads=256, kv=16))], ids=str)
+def test_values_of_the_last_size(ops, fmt, t, shape):
+    # Means of values near the largest of all are finite, also where waves and splits are joined.
+    rng = np.random.default_rng(12)
+    v = rng.uniform(0.9, 1, (t, 64)) * 3.3e38
+    new = min(shape["new"], t)
+    Far(ops, fmt, rng.uniform(-0.1, 0.1, t), v, **dict(shape, new=new)).check(
+        64 if t == 40000 else t / 32 + 1, rows=sample(new))
