@@ -808,6 +808,56 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
                                         int32_t tree_words, int32_t has_scale, float scale,
                                         float *y_dev, int64_t y_stride);
 
+/* Pages of a cache, moved and shared.  All of it is asynchronous on the context's stream, reads
+ * its arrays on the device, and what it refuses is remembered as above (mg_kv_cache_refused).
+ *
+ * refs_dev, where taken, is int32 [pages], the caller's, zeros at the start: how many table
+ * entries hold a page (0: free).  Entries of tables under these calls: a sequence's pages in
+ * order, then -1.
+ *
+ * Copies pages: page dst_dev[i] becomes what page src_dev[i] holds, for i < n.  Pairs whose
+ * numbers are both negative, or equal, are passed over.  A pair is refused (its dst left as it
+ * was) where a number lies outside the cache, where its dst is the dst of another pair, or
+ * where its dst is another's src or its src another's dst.  More than 1024 pairs take
+ * workspace. */
+mg_status mg_kv_cache_copy_pages_dev(mg_ctx *ctx, mg_kv_cache *cache, const int32_t *src_dev,
+                                     const int32_t *dst_dev, int64_t n);
+/* Of each sequence's new rows, count_dev[b] stay: row kept_dev[row_start[b] + j] of it (indices
+ * within the sequence, rising) moves to row j, codes and scales as they are (keys keep the
+ * positions that they were rotated at).  What mg_verify_drafts_f32_dev writes.  Rows from
+ * count_dev[b] on hold any finite values afterwards.  The pages that rows move into must be the
+ * sequence's own.  A sequence whose list is not of that form is refused: left as it was; a row
+ * from or to a missing page does not move.  past_out_dev (may be NULL, may be seqs->past):
+ * past[b] + count_dev[b], past[b] for a refused sequence. */
+mg_status mg_kv_cache_compact_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                  const int32_t *kept_dev, const int32_t *count_dev,
+                                  int32_t *past_out_dev);
+/* A new batch of out_batch sequences, each a continuation of sequence parent_dev[i] of seqs (-1:
+ * an empty one), by shared pages: past_out_dev[i] = past[parent], table_out_dev row i [out_stride]
+ * the pages that hold those positions.  The old sequences' pages are no longer held by them:
+ * refs_dev loses their entries and gains the new ones, so that a sequence without a
+ * continuation is freed.  Of seqs batch, max_len, past and page_table are read.  A parent outside
+ * the batch, a past outside 0 .. max_len, or more pages than out_stride: refused, the new
+ * sequence empty.  table_out_dev and past_out_dev must not overlap what is read. */
+mg_status mg_kv_cache_fork_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                               const int32_t *parent_dev, int64_t out_batch,
+                               int32_t *past_out_dev, int32_t *table_out_dev, int64_t out_stride,
+                               int32_t *refs_dev);
+/* Makes each sequence's pages those that its past and new rows need, in seqs->page_table (which
+ * this call writes):
+ *   pages behind them are let go (so past 0 without rows frees a sequence), and those behind the
+ *   past from the first on that others hold too;
+ *   where the first new row falls into the middle of a page that others hold too, the sequence
+ *   gets a copy of its own (the last of the batch that shares it keeps it, if nobody else does);
+ *   missing pages are taken from the free ones.
+ * Free pages go by number, lowest first, to the sequences in order (a sequence's copy before
+ * its new pages).  From the first one for which they do not suffice on, a sequence that needs any
+ * gets none; neither does one that shares its page with such a sequence.  granted_dev[b]: whether
+ * sequence b can be written now.  A sequence that breaks a bound, whose table has not all pages
+ * of its past or is too short, is refused: left as it was, not granted.  Takes workspace. */
+mg_status mg_kv_cache_fit_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                              int32_t *refs_dev, int32_t *granted_dev);
+
 /* -------------------------------------------------------- log probabilities */
 
 /* Of each row of logits [rows, vocab] (row r at r * row_stride, 0 = vocab): the log
@@ -821,6 +871,85 @@ mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_
                                     int64_t vocab, int64_t row_stride, const int32_t *tokens_dev,
                                     float *logprob_dev, float *entropy_dev, int32_t top,
                                     int32_t *top_ids_dev, float *top_logprobs_dev);
+
+/* ------------------------------------------------------ verification of drafts */
+
+/* Drafted tokens of a batch of sequences and the logits to verify them against.  Rows are packed
+ * as in mg_seq_batch: row 0 of a sequence is its last emitted token, the others are drafted,
+ * row i after row parent[i] < i of its sequence (NULL: after row i - 1).  target row r [vocab]
+ * are the logits of what follows row r's token; draft row r those that the token after it was
+ * drawn from, or draft NULL: nothing is known of how tokens were drafted.  Device pointers; the
+ * struct itself is read during the call. */
+typedef struct mg_drafts {
+  int64_t batch;
+  int64_t rows;
+  int64_t max_new;            /* rows a sequence, 1024 at most (a bound: it may exceed rows) */
+  int64_t vocab;
+  const int32_t *row_start;   /* [batch + 1] */
+  const int32_t *tokens;      /* [rows] */
+  const int32_t *parent;      /* [rows] or NULL; with draft: NULL */
+  const float *target;
+  int64_t target_stride;      /* of rows, 0 = vocab */
+  const float *draft;
+  int64_t draft_stride;
+  const float *temperature;   /* [batch], NULL = 1 */
+  const float *uniform;       /* [rows], in [0, 1) */
+} mg_drafts;
+
+/* Which drafted tokens stay, so that what a sequence emits is distributed as if each token had been
+ * drawn from p = softmax(target / temperature) in turn.  From row c = 0 on, in order, the rows i
+ * drafted after row c are tried:
+ *   with draft (q = softmax(draft / temperature)): token x stays if uniform[i] q_c(x) < p_c(x);
+ *   a rejected one leaves the weights max(p_c - q_c, 0), or p_c where these sum to 2^-40 or less;
+ *   without: x stays if uniform[i] (1 - the p_c of the tokens rejected here) < p_c(x); a rejected
+ *   one loses its weight.
+ * Tokens outside the vocabulary and those with p_c(x) = 0 are rejected.  A row that stays becomes
+ * c.  At the end one more token is drawn by the weights left at c: the first whose running sum
+ * exceeds uniform[row 0] of the whole.  A temperature that is not above 0: x stays if it is the
+ * largest logit (the lowest of equal ones), which is also the last token.  Weights, sums and
+ * comparisons are in 64 bits.  Where target row c has no distribution (NaN, +inf, only -inf),
+ * or nothing is left, the last token is -1; a token drafted from a draft row that has none is
+ * rejected and leaves p_c.
+ * out_tokens_dev / kept_dev [rows], from row_start[b] on: the count_dev[b] tokens emitted, and as
+ * many rows that stay (0 first), what mg_kv_cache_compact_dev takes; -1 behind them.  Rows of no
+ * sequence are left as they were.  A sequence that breaks the bounds, or without rows, has count 0
+ * and nothing else written.  Takes workspace. */
+mg_status mg_verify_drafts_f32_dev(mg_ctx *ctx, const mg_drafts *drafts, int32_t *out_tokens_dev,
+                                   int32_t *kept_dev, int32_t *count_dev);
+
+/* ------------------------------------------------------------ low-rank adapters */
+
+/* Low-rank adapters of up to 4 projections of one input (q/k/v, gate/up), for requests that share
+ * the projections but not the adapters.  Slot s of a handle holds an adapter of rank r_s: for
+ * each projection i A_i [r_s, K] and B_i [N_i, r_s], and a factor f_s. */
+typedef enum mg_adapter_format { MG_ADAPTER_F32 = 0, MG_ADAPTER_F16 = 1 } mg_adapter_format;
+typedef struct mg_adapters mg_adapters;
+
+/* slots empty slots (rank 0) for ranks up to max_rank (1 .. 256), n projections K -> N[i].  Values
+ * are held in fp32, or rounded once to fp16 (those beyond its range become infinite).  Memory:
+ * slots * max_rank * (n K + sum N) values, K and N padded to multiples of 8. */
+mg_status mg_adapters_create(mg_ctx *ctx, int64_t K, int32_t n, const int64_t *N, int64_t slots,
+                             int64_t max_rank, int32_t format, mg_adapters **out);
+/* Waits for the device, then frees.  NULL: MG_INVALID_ARGUMENT. */
+mg_status mg_adapters_release(mg_adapters *adapters);
+mg_status mg_adapters_info(const mg_adapters *adapters, int64_t *K, int32_t *n, int64_t *slots,
+                           int64_t *max_rank, int64_t *device_bytes);
+/* Fills a slot: a[i] [rank, K] and b[i] [N_i, rank] in host memory (waits for the stream), or in
+ * device memory (_dev, asynchronous on the context's stream).  rank 0 empties it (a and b are not
+ * read).  Later calls on the context, graphs captured before among them, use what the slot holds
+ * then; calls on other contexts that may run at the same time are the caller's to order. */
+mg_status mg_adapters_set(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,
+                          const float *const *a, const float *const *b, float factor);
+mg_status mg_adapters_set_dev(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,
+                              const float *const *a_dev, const float *const *b_dev, float factor);
+/* y_i[r] = base_i[r] + f_s B_i (A_i x[r]) for rows r of x [rows, K], s = slot_dev[r] (int32, device
+ * memory): what each request's adapter adds to the shared projections' outputs base_i [rows, N_i]
+ * (mg_matmul_nbits_group_dev and its like).  A negative slot or an empty one: y_i[r] = base_i[r].  A
+ * slot beyond the handle's: NaN.  y_i may be base_i; it must not overlap it otherwise, nor x.
+ * Products are fp32, sums in fp32.  Takes workspace. */
+mg_status mg_adapters_apply_f32_dev(mg_ctx *ctx, mg_adapters *adapters, const float *x_dev,
+                                    int64_t rows, const int32_t *slot_dev,
+                                    const float *const *base_dev, float *const *y_dev);
 
 /* ----------------------------------------------------------------- weights */
 

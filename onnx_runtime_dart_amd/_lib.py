@@ -121,6 +121,17 @@ SIGNATURES = {
     "mg_kv_cache_read_f32_dev": [_P, _P, _P, _P, _I64, _P, _I64],
     "mg_kv_cache_attention_f32_dev": [_P, _P, _P, _P, _I64, _I32, _P, _P, _I32, _I32, _F, _P,
                                       _I64],
+    "mg_kv_cache_copy_pages_dev": [_P, _P, _P, _P, _I64],
+    "mg_kv_cache_compact_dev": [_P, _P, _P, _P, _P, _P],
+    "mg_kv_cache_fork_dev": [_P, _P, _P, _P, _I64, _P, _P, _I64, _P],
+    "mg_kv_cache_fit_dev": [_P, _P, _P, _P, _P],
+    "mg_verify_drafts_f32_dev": [_P, _P, _P, _P, _P],
+    "mg_adapters_create": [_P, _I64, _I32, _P, _I64, _I64, _I32, _PP],
+    "mg_adapters_release": [_P],
+    "mg_adapters_info": [_P, _P, _P, _P, _P, _P],
+    "mg_adapters_set": [_P, _P, _I64, _I64, _P, _P, _F],
+    "mg_adapters_set_dev": [_P, _P, _I64, _I64, _P, _P, _F],
+    "mg_adapters_apply_f32_dev": [_P, _P, _P, _I64, _P, _P, _P],
     "mg_token_logprobs_f32_dev": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _I32, _P, _P],
     "mg_weight_release": [_P],
     "mg_weight_info": [_P, C.POINTER(_I64), C.POINTER(_I64), C.POINTER(_I64)],

@@ -13,10 +13,12 @@
 #include <string>
 #include <vector>
 
+#include "adapters_common.h"
 #include "kv_common.h"
 #include "logprobs_common.h"
 #include "mg_internal.h"
 #include "rope_common.h"
+#include "verify_common.h"
 
 // Defined in int8.hip.
 mg_status mg_int8_run_batched(mg_ctx *ctx, const void *a_dev, int32_t a_signed,
@@ -2697,6 +2699,15 @@ mg_status check_stride(const char *what, int64_t *stride, int64_t len) {
   return MG_OK;
 }
 
+// A workspace that a call cannot do without.
+mg_status take_workspace(const char *what, mg_ctx *ctx, size_t bytes) {
+  MG_TRY(mg_check_control(ctx, (int64_t)bytes));
+  if (bytes > ctx->ws_bytes && mg_capturing(ctx))
+    return mg_fail(MG_UNSUPPORTED, std::string(what) + ": the workspace does not grow under stream "
+                                                       "capture; make the call once before it");
+  return mg_ws_reserve(ctx, bytes);
+}
+
 // The frequencies of scaled tables (half values).
 mg_status rope_frequencies(const char *what, int64_t half, double base, const mg_rope_scaling &s,
                            double *f) {
@@ -3008,6 +3019,82 @@ mg_status mg_kv_cache_attention_f32_dev(mg_ctx *ctx, mg_kv_cache *cache, const m
   return mg_kv_attn_run(ctx, a, ctx->ws);
 }
 
+mg_status mg_kv_cache_copy_pages_dev(mg_ctx *ctx, mg_kv_cache *cache, const int32_t *src_dev,
+                                     const int32_t *dst_dev, int64_t n) {
+  const char *what = "KvCacheCopyPages";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx || !cache) return bad_arg(what, "null argument");
+  if (cache->device != ctx->device) return bad_arg(what, "cache of another device");
+  if (n < 0 || n > MG_KV_MOST) return bad_arg(what, "n must be 0 .. 2^31 - 257");
+  if (n == 0) return MG_OK;
+  if (!src_dev || !dst_dev) return bad_arg(what, "null buffer");
+  if (mg_kv_copy_groups(*cache, n) > MG_MOST_GROUPS)
+    return mg_fail(MG_UNSUPPORTED, "KvCacheCopyPages: too many pages");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(take_workspace(what, ctx, mg_kv_copy_ws(n)));
+  return mg_kv_copy_run(ctx, *cache, src_dev, dst_dev, n, ctx->ws);
+}
+
+mg_status mg_kv_cache_compact_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                                  const int32_t *kept_dev, const int32_t *count_dev,
+                                  int32_t *past_out_dev) {
+  const char *what = "KvCacheCompact";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
+  if (s.batch == 0 || (s.max_new == 0 && !past_out_dev)) return MG_OK;
+  if (!s.row_start || !s.past || !count_dev || (s.max_new && !kept_dev))
+    return bad_arg(what, "null buffer");
+  if (2 * s.batch * cache->kv_heads > MG_MOST_GROUPS)
+    return mg_fail(MG_UNSUPPORTED, "KvCacheCompact: too many sequences");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_kv_compact_run(ctx, *cache, s, kept_dev, count_dev, past_out_dev);
+}
+
+mg_status mg_kv_cache_fork_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                               const int32_t *parent_dev, int64_t out_batch,
+                               int32_t *past_out_dev, int32_t *table_out_dev, int64_t out_stride,
+                               int32_t *refs_dev) {
+  const char *what = "KvCacheFork";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
+  if (out_batch < 0 || out_batch > 65535 || out_stride < 0 || out_stride > MG_KV_MOST)
+    return bad_arg(what, "out_batch must be 0 .. 65535, out_stride below 2^31 - 256");
+  if (s.batch + out_batch == 0) return MG_OK;
+  if (!refs_dev || (s.batch && (!s.past || (s.table_stride && !s.page_table))) ||
+      (out_batch && (!parent_dev || !past_out_dev || (out_stride && !table_out_dev))))
+    return bad_arg(what, "null buffer");
+  if (out_batch && s.batch &&
+      (past_out_dev == s.past || (out_stride && table_out_dev == s.page_table)))
+    return bad_arg(what, "the new batch cannot be written over the old one");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_kv_fork_run(ctx, *cache, s, parent_dev, out_batch, past_out_dev, table_out_dev,
+                        out_stride, refs_dev);
+}
+
+mg_status mg_kv_cache_fit_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
+                              int32_t *refs_dev, int32_t *granted_dev) {
+  const char *what = "KvCacheFit";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  mg_seq_batch s;
+  MG_TRY(check_cache(what, ctx, cache, seqs, &s));
+  if (s.batch == 0) return MG_OK;
+  if (!s.row_start || !s.past || (s.table_stride && !s.page_table) || !refs_dev || !granted_dev)
+    return bad_arg(what, "null buffer");
+  if (mg_kv_copy_groups(*cache, s.batch) > MG_MOST_GROUPS)
+    return mg_fail(MG_UNSUPPORTED, "KvCacheFit: too many sequences");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(take_workspace(what, ctx, mg_kv_fit_ws(*cache, s.batch)));
+  return mg_kv_fit_run(ctx, *cache, s, refs_dev, granted_dev, ctx->ws);
+}
+
 mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_t rows,
                                     int64_t vocab, int64_t row_stride, const int32_t *tokens_dev,
                                     float *logprob_dev, float *entropy_dev, int32_t top,
@@ -3043,6 +3130,213 @@ mg_status mg_token_logprobs_f32_dev(mg_ctx *ctx, const float *logits_dev, int64_
   MG_TRY(mg_check_control(ctx, (int64_t)need));
   p.part = need ? static_cast<mg_logprobs_part *>(ctx->ws) : nullptr;
   return mg_logprobs_run(ctx, p);
+}
+
+mg_status mg_verify_drafts_f32_dev(mg_ctx *ctx, const mg_drafts *drafts, int32_t *out_tokens_dev,
+                                   int32_t *kept_dev, int32_t *count_dev) {
+  const char *what = "VerifyDrafts";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx || !drafts) return bad_arg(what, "null argument");
+  mg_verify v{};
+  v.d = *drafts;
+  mg_drafts &d = v.d;
+  if (d.batch < 0 || d.batch > 65535 || d.rows < 0 || d.rows > MG_KV_MOST || d.max_new < 0 ||
+      d.vocab < 1 || d.vocab > 0x7fffd000)
+    return bad_arg(what, "batch must be 0 .. 65535, rows and max_new >= 0, vocab 1 .. 2^31 - 12288");
+  d.max_new = std::min(d.max_new, d.rows);
+  MG_TRY(check_stride(what, &d.target_stride, d.vocab));
+  if (d.draft) MG_TRY(check_stride(what, &d.draft_stride, d.vocab));
+  if (d.max_new > MG_DRAFTS_MOST)
+    return mg_fail(MG_UNSUPPORTED, "VerifyDrafts: at most 1024 rows a sequence");
+  if (d.draft && d.parent)
+    return mg_fail(MG_UNSUPPORTED, "VerifyDrafts: trees are verified without draft logits");
+  if (d.batch == 0) return MG_OK;
+  if (!d.row_start || !count_dev ||
+      (d.max_new && (!d.tokens || !d.target || !d.uniform || !out_tokens_dev || !kept_dev)))
+    return bad_arg(what, "null buffer");
+  const int64_t runs = (d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN;
+  if ((runs + 3) / 4 * d.batch > MG_MOST_GROUPS / (2 * d.max_new + 1) ||
+      d.rows > ((int64_t)1 << 36) / runs)
+    return mg_fail(MG_UNSUPPORTED, "VerifyDrafts: too many logits");
+  v.out = out_tokens_dev;
+  v.kept = kept_dev;
+  v.count = count_dev;
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(take_workspace(what, ctx, mg_verify_plan(&v, nullptr)));
+  mg_verify_plan(&v, ctx->ws);
+  return mg_verify_run(ctx, v);
+}
+
+mg_status mg_adapters_create(mg_ctx *ctx, int64_t K, int32_t n, const int64_t *N, int64_t slots,
+                             int64_t max_rank, int32_t format, mg_adapters **out) {
+  const char *what = "Adapters";
+  g_last_error.clear();
+  if (!ctx || !out || !N) return bad_arg(what, "null argument");
+  *out = nullptr;
+  if (format < MG_ADAPTER_F32 || format > MG_ADAPTER_F16) return bad_arg(what, "unknown format");
+  constexpr int64_t most = (int64_t)1 << 24;
+  if (n < 1 || n > MG_ADAPTER_MOST || K < 1 || K > most || slots < 1 || slots > MG_ADAPTER_SLOTS ||
+      max_rank < 1 || max_rank > 256)
+    return bad_arg(what, "1 .. 4 projections, K 1 .. 2^24, slots 1 .. 4096, max_rank 1 .. 256");
+  mg_adapters h;
+  h.device = ctx->device;
+  h.fmt = format;
+  h.n = n;
+  h.max_rank = (int)max_rank;
+  h.K = K;
+  h.kp = (K + 7) / 8 * 8;
+  h.slots = slots;
+  for (int i = 0; i < n; i++) {
+    if (N[i] < 1 || N[i] > most) return bad_arg(what, "N must be 1 .. 2^24");
+    h.N[i] = N[i];
+    h.np[i] = (N[i] + 7) / 8 * 8;
+    h.b_off[i] = h.b_slot;
+    h.b_slot += max_rank * h.np[i];
+  }
+  h.a_slot = n * max_rank * h.kp;
+  const size_t el = format == MG_ADAPTER_F16 ? 2 : 4;
+  const size_t a = mg_align((size_t)(slots * h.a_slot) * el), b = mg_align((size_t)(slots * h.b_slot) * el);
+  const size_t each = mg_align((size_t)slots * 4), total = a + b + 2 * each;
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, (int64_t)total));
+  mg_adapters *p = new (std::nothrow) mg_adapters(h);
+  if (!p) return mg_fail(MG_OUT_OF_MEMORY, "Adapters: out of host memory");
+  void *base = nullptr;
+  const hipError_t e = hipMalloc(&base, total);
+  if (e != hipSuccess) {
+    delete p;
+    (void)hipGetLastError();
+    return mg_fail(e == hipErrorOutOfMemory ? MG_OUT_OF_MEMORY : MG_DEVICE_ERROR,
+                   std::string("Adapters: hipMalloc: ") + hipGetErrorString(e));
+  }
+  char *at = static_cast<char *>(base);
+  p->a = at;
+  p->b = at + a;
+  p->rank = reinterpret_cast<int32_t *>(at + a + b);
+  p->factor = reinterpret_cast<float *>(at + a + b + each);
+  p->bytes = (int64_t)total;
+  // (Waited for: another context's stream may use them next.)
+  mg_status st = mg_adapters_clear(ctx, *p);
+  if (st == MG_OK && hipStreamSynchronize(ctx->stream) != hipSuccess)
+    st = mg_fail(MG_DEVICE_ERROR, "Adapters: clearing failed");
+  if (st != MG_OK) {
+    (void)hipFree(base);
+    delete p;
+    return st;
+  }
+  *out = p;
+  return MG_OK;
+}
+
+mg_status mg_adapters_release(mg_adapters *adapters) {
+  g_last_error.clear();
+  if (!adapters) return bad_arg("Adapters", "null adapters");
+  int was = 0;
+  const bool known = hipGetDevice(&was) == hipSuccess;
+  MG_HIP(hipSetDevice(adapters->device));
+  const hipError_t e = hipFree(adapters->a);  // (waits for the device)
+  delete adapters;
+  if (known) (void)hipSetDevice(was);
+  if (e != hipSuccess)
+    return mg_fail(MG_DEVICE_ERROR, std::string("Adapters: hipFree: ") + hipGetErrorString(e));
+  return MG_OK;
+}
+
+mg_status mg_adapters_info(const mg_adapters *adapters, int64_t *K, int32_t *n, int64_t *slots,
+                           int64_t *max_rank, int64_t *device_bytes) {
+  g_last_error.clear();
+  if (!adapters) return bad_arg("Adapters", "null adapters");
+  if (K) *K = adapters->K;
+  if (n) *n = adapters->n;
+  if (slots) *slots = adapters->slots;
+  if (max_rank) *max_rank = adapters->max_rank;
+  if (device_bytes) *device_bytes = adapters->bytes;
+  return MG_OK;
+}
+
+namespace {
+mg_status check_adapter(const mg_ctx *ctx, const mg_adapters *h, int64_t slot, int64_t rank,
+                        const float *const *a, const float *const *b, float factor) {
+  const char *what = "Adapters";
+  if (!ctx || !h) return bad_arg(what, "null argument");
+  if (h->device != ctx->device) return bad_arg(what, "adapters of another device");
+  if (slot < 0 || slot >= h->slots || rank < 0 || rank > h->max_rank)
+    return bad_arg(what, "no such slot, or rank above max_rank");
+  if (!std::isfinite(factor)) return bad_arg(what, "factor must be finite");
+  if (rank && (!a || !b)) return bad_arg(what, "null buffer");
+  for (int i = 0; i < h->n && rank; i++)
+    if (!a[i] || !b[i]) return bad_arg(what, "null buffer");
+  return MG_OK;
+}
+}  // namespace
+
+mg_status mg_adapters_set(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,
+                          const float *const *a, const float *const *b, float factor) {
+  ProfScope prof_(ctx, "Adapters.upload");
+  g_last_error.clear();
+  MG_TRY(check_adapter(ctx, adapters, slot, rank, a, b, factor));
+  MG_TRY(mg_use_device(ctx));
+  const mg_adapters &h = *adapters;
+  size_t need = 0;
+  const float *a_dev[MG_ADAPTER_MOST] = {}, *b_dev[MG_ADAPTER_MOST] = {};
+  for (int i = 0; i < h.n; i++)
+    need += mg_align((size_t)(rank * h.K) * 4) + mg_align((size_t)(rank * h.N[i]) * 4);
+  MG_TRY(take_workspace("Adapters", ctx, need));
+  char *at = static_cast<char *>(ctx->ws);
+  for (int i = 0; i < h.n && rank; i++) {
+    for (const bool first : {true, false}) {
+      const size_t bytes = (size_t)(rank * (first ? h.K : h.N[i])) * 4;
+      MG_HIP(hipMemcpyAsync(at, first ? a[i] : b[i], bytes, hipMemcpyHostToDevice, ctx->stream));
+      (first ? a_dev : b_dev)[i] = reinterpret_cast<const float *>(at);
+      at += mg_align(bytes);
+    }
+  }
+  MG_TRY(mg_adapters_fill(ctx, h, slot, rank, a_dev, b_dev, factor));
+  MG_HIP(hipStreamSynchronize(ctx->stream));
+  return MG_OK;
+}
+
+mg_status mg_adapters_set_dev(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,
+                              const float *const *a_dev, const float *const *b_dev, float factor) {
+  ProfScope prof_(ctx, "Adapters.upload");
+  g_last_error.clear();
+  MG_TRY(check_adapter(ctx, adapters, slot, rank, a_dev, b_dev, factor));
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(mg_check_control(ctx, 0));
+  return mg_adapters_fill(ctx, *adapters, slot, rank, a_dev, b_dev, factor);
+}
+
+mg_status mg_adapters_apply_f32_dev(mg_ctx *ctx, mg_adapters *adapters, const float *x_dev,
+                                    int64_t rows, const int32_t *slot_dev,
+                                    const float *const *base_dev, float *const *y_dev) {
+  const char *what = "Adapters";
+  ProfScope prof_(ctx, what);
+  g_last_error.clear();
+  if (!ctx || !adapters) return bad_arg(what, "null argument");
+  if (adapters->device != ctx->device) return bad_arg(what, "adapters of another device");
+  if (rows < 0 || rows > MG_KV_MOST) return bad_arg(what, "rows must be 0 .. 2^31 - 257");
+  if (rows == 0) return MG_OK;
+  mg_adapt p{};
+  p.h = *adapters;
+  if (!x_dev || !slot_dev || !base_dev || !y_dev) return bad_arg(what, "null buffer");
+  for (int i = 0; i < p.h.n; i++)
+    if (!base_dev[i] || !y_dev[i]) return bad_arg(what, "null buffer");
+  if (mg_adapt_groups(p.h, rows) > MG_MOST_GROUPS)
+    return mg_fail(MG_UNSUPPORTED, "Adapters: too many outputs");
+  MG_TRY(mg_use_device(ctx));
+  MG_TRY(take_workspace(what, ctx, mg_adapt_ws(ctx, p.h, rows)));
+  for (int64_t r = 0; r < rows; r += MG_ADAPT_ROWS) {
+    p.rows = std::min(rows - r, MG_ADAPT_ROWS);
+    p.x = x_dev + r * p.h.K;
+    p.slot = slot_dev + r;
+    for (int i = 0; i < p.h.n; i++) {
+      p.base[i] = base_dev[i] + r * p.h.N[i];
+      p.y[i] = y_dev[i] + r * p.h.N[i];
+    }
+    MG_TRY(mg_adapt_run(ctx, p, ctx->ws));
+  }
+  return MG_OK;
 }
 
 }  // extern "C"

@@ -30,7 +30,7 @@ LIB = PKG / "lib" / "libmigemm.so"
 
 SOURCES = ["api.hip", "nbits.hip", "nbits_f8.hip", "int8.hip", "f32.hip", "pair.hip", "dql.hip",
            "attn.hip", "conv.hip", "conv_pair.hip", "elem.hip", "rope.hip", "kvcache.hip", "kvattn.hip",
-           "logprobs.hip"]
+           "kvpages.hip", "logprobs.hip", "verify.hip", "adapters.hip"]
 
 # Packed fp32 VALU forms are disabled (-packed-fp32-ops); the compiler still
 # schedules plain fp32 and the MFMA units.

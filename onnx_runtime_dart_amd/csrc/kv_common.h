@@ -67,6 +67,19 @@ mg_status mg_kv_append_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch
                            const mg_rope *rope);
 mg_status mg_kv_read_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s, float *k,
                          int64_t ks, float *v, int64_t vs);
+// Pages (kvpages.hip); workspaces, and workgroups of the largest launch.
+size_t mg_kv_copy_ws(int64_t n);
+int64_t mg_kv_copy_groups(const mg_kv_cache &c, int64_t n);
+mg_status mg_kv_copy_run(mg_ctx *ctx, const mg_kv_cache &c, const int32_t *src, const int32_t *dst,
+                         int64_t n, void *ws);
+mg_status mg_kv_compact_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
+                            const int32_t *kept, const int32_t *count, int32_t *past_out);
+mg_status mg_kv_fork_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
+                         const int32_t *parent, int64_t out_batch, int32_t *past_out,
+                         int32_t *table_out, int64_t out_stride, int32_t *refs);
+size_t mg_kv_fit_ws(const mg_kv_cache &c, int64_t batch);
+mg_status mg_kv_fit_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s, int32_t *refs,
+                        int32_t *granted, void *ws);
 struct mg_kv_attn {
   mg_kv_cache c;
   mg_seq_batch s;

@@ -1,0 +1,456 @@
+// Verification of drafted tokens against the target's distributions.
+//
+// With m the largest of a row's logits and c = log2(e) / temperature, its weights are
+// 2^((x - m) c) and their sum s; the drafted tokens need the weights of single logits only, the
+// last token of a sequence a running sum over one row.  Tokens of a large vocabulary have borders
+// closer than 1e-5 of each other in that running sum, so weights and sums are in 64 bits: with
+// 32 one draw in a hundred would take a neighbour.
+//
+//   k_stats   (m, s) of every run of 2048 logits, one wave each: the pass over all logits
+//   k_walk    a sequence's rows joined, its drafted tokens tried in order (a workgroup each)
+//   k_masses  the weights left in each run of the one row that the last token is drawn from
+//   k_pick    the run, and the token in it, that the random number falls into
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "mg_internal.h"
+#include "verify_common.h"
+
+namespace {
+
+constexpr double kLog2e = 1.44269504088896340736;
+constexpr int kLane = MG_DRAFTS_RUN / 64;  // logits of a lane
+constexpr float kInf = __builtin_inff();
+
+// 2^t, t at most 0 and a few units above; NaN counts as far below.  The series of e^(f ln 2) for
+// |f| <= 1/2: 14 terms, off by (ln 2 / 2)^14 / 14! = 4e-18.
+__device__ inline double exp2_of(double t) {
+  t = fmax(t, -1100.0);
+  const double n = rint(t), f = t - n;
+  double y = 1.3691488853904124e-12;
+  y = fma(y, f, 2.5678435993488196e-11);
+  y = fma(y, f, 4.44553827187081e-10);
+  y = fma(y, f, 7.054911620801121e-09);
+  y = fma(y, f, 1.0178086009239696e-07);
+  y = fma(y, f, 1.3215486790144305e-06);
+  y = fma(y, f, 1.5252733804059838e-05);
+  y = fma(y, f, 0.00015403530393381606);
+  y = fma(y, f, 0.0013333558146428441);
+  y = fma(y, f, 0.009618129107628477);
+  y = fma(y, f, 0.055504108664821576);
+  y = fma(y, f, 0.2402265069591007);
+  y = fma(y, f, 0.6931471805599453);
+  y = fma(y, f, 1.0);
+  return ldexp(y, (int)n);
+}
+__device__ inline double weight(float x, float m, double c) {
+  return exp2_of(((double)x - (double)m) * c);
+}
+
+struct Seq {
+  int start, n;
+};
+// Sequence b's rows; n = 0 where it breaks a bound.
+__device__ inline Seq sequence(const mg_drafts &d, int64_t b) {
+  const int64_t r0 = d.row_start[b], r1 = d.row_start[b + 1];
+  const bool bad = r0 < 0 || r1 < r0 || r1 > d.rows || r1 - r0 > d.max_new;
+  return bad ? Seq{0, 0} : Seq{(int)r0, (int)(r1 - r0)};
+}
+__device__ inline float temperature(const mg_drafts &d, int64_t b) {
+  return d.temperature ? d.temperature[b] : 1.f;
+}
+
+// (Rows need not begin at 16 bytes; the loads may be of four all the same.)
+struct __attribute__((packed, aligned(4))) Four {
+  float x[4];
+};
+// The lane's logits of a run: four adjacent ones of every 256.  Past the row's end: -inf.
+__device__ inline void load(float (&x)[kLane], const float *row, int64_t first, int64_t vocab,
+                            int lane) {
+  const float *p = row + first;
+  if (first + MG_DRAFTS_RUN <= vocab) {
+#pragma unroll
+    for (int j = 0; j < kLane / 4; j++) {
+      const Four v = *reinterpret_cast<const Four *>(p + 256 * j + 4 * lane);
+#pragma unroll
+      for (int k = 0; k < 4; k++) x[4 * j + k] = v.x[k];
+    }
+  } else {
+    const int n = (int)(vocab - first);
+#pragma unroll
+    for (int j = 0; j < kLane; j++) {
+      const int i = 256 * (j / 4) + 4 * lane + j % 4;
+      x[j] = i < n ? p[i] : -kInf;
+    }
+  }
+}
+
+__device__ inline double wave_sum(double x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+__device__ inline int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = min(x, __shfl_xor(x, o));
+  return x;
+}
+
+__global__ __launch_bounds__(256) void k_stats(const mg_verify v) {
+  const mg_drafts &d = v.d;
+  const int lane = threadIdx.x & 63;
+  const int run = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t b = blockIdx.z;
+  const Seq q = sequence(d, b);
+  const bool drafted = blockIdx.y >= (unsigned)d.max_new;
+  const int i = (int)blockIdx.y - (drafted ? (int)d.max_new : 0);
+  const float temp = temperature(d, b);
+  // (Nothing was drafted after the last row; the largest logit needs no draft.)
+  if (run >= v.nrun || i >= q.n || (drafted && (i + 1 == q.n || !(temp > 0.f)))) return;
+  const int64_t row = q.start + i;
+  float x[kLane];
+  load(x, drafted ? d.draft + row * d.draft_stride : d.target + row * d.target_stride,
+       (int64_t)run * MG_DRAFTS_RUN, d.vocab, lane);
+  float m = -kInf;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < kLane; j++) {
+    m = fmaxf(m, x[j]);
+    bad |= !(x[j] < kInf);
+  }
+  m = __any(bad) ? kInf : wave_max(m);
+  double s = 0.0;
+  if (temp > 0.f && m < kInf) {
+    const double c = kLog2e / (double)temp;
+#pragma unroll
+    for (int j = 0; j < kLane; j++) s += weight(x[j], m, c);
+    s = wave_sum(s);
+  }
+  if (lane == 0) v.part[((drafted ? d.rows : 0) + row) * v.nrun + run] = mg_drafts_part{s, m, 0.f};
+}
+
+// A row's maximum and sum from its runs', by a wave; *at: the first run with the maximum.
+__device__ inline void join(const mg_drafts_part *p, int nrun, double c, int lane, float *m, double *s,
+                            int *at) {
+  float top = -kInf;
+  int first = 0x7fffffff;
+  for (int r = lane; r < nrun; r += 64) {
+    const float y = p[r].m;
+    if (y > top || first == 0x7fffffff) first = r;
+    top = fmaxf(top, y);
+  }
+  const float all = wave_max(top);
+  *at = wave_min(top == all ? first : 0x7fffffff);
+  double sum = 0.0;
+  for (int r = lane; r < nrun; r += 64) sum += p[r].s * exp2_of(((double)p[r].m - (double)all) * c);
+  *m = all;
+  *s = wave_sum(sum);
+}
+
+__global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
+  constexpr int kMost = MG_DRAFTS_MOST;
+  __shared__ double s[kMost], qs[kMost], ep[kMost], eq[kMost];  // rows' sums; tokens' weights
+  __shared__ float m[kMost], qm[kMost];
+  __shared__ int token[kMost], parent[kMost], best[kMost];
+  __shared__ bool again[kMost];  // a token that an earlier row after the same one has too
+  __shared__ int kept_n;
+  const mg_drafts &d = v.d;
+  const int64_t b = blockIdx.x;
+  const Seq q = sequence(d, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  mg_drafts_last &last = v.last[b];
+  if (q.n == 0) {
+    if (threadIdx.x == 0) {
+      v.count[b] = 0;
+      last.mode = 0;
+    }
+    return;
+  }
+  const float temp = temperature(d, b);
+  const bool greedy = !(temp > 0.f);
+  const double c = greedy ? 0.0 : kLog2e / (double)temp;
+  for (int i = threadIdx.x; i < q.n; i += 1024) {
+    token[i] = d.tokens[q.start + i];
+    parent[i] = d.parent ? d.parent[q.start + i] : i - 1;
+  }
+  for (int i = wave; i < q.n; i += 16) {
+    const int64_t row = q.start + i;
+    float top;
+    double sum;
+    int at, ignored;
+    join(v.part + row * v.nrun, v.nrun, c, lane, &top, &sum, &at);
+    if (greedy) {
+      // The first logit that is the largest: in its run.
+      const int64_t first = (int64_t)at * MG_DRAFTS_RUN;
+      const float *x = d.target + row * d.target_stride;
+      int here = 0x7fffffff;
+      for (int j = 0; j < kLane; j++) {
+        const int64_t e = first + 64 * j + lane;
+        if (e < d.vocab && here == 0x7fffffff && x[e] == top) here = (int)e;
+      }
+      here = wave_min(here);
+      if (lane == 0) best[i] = here;
+    }
+    if (lane == 0) {
+      m[i] = top;
+      s[i] = sum;
+    }
+    if (d.draft && !greedy && i + 1 < q.n) {
+      join(v.part + (d.rows + row) * v.nrun, v.nrun, c, lane, &top, &sum, &ignored);
+      if (lane == 0) {
+        qm[i] = top;
+        qs[i] = sum;
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < q.n; i += 1024) {
+    const int t = token[i], up = parent[i];
+    double p = 0.0, w = 0.0;
+    bool same = false;
+    if (i > 0 && up >= 0 && up < i && t >= 0 && t < d.vocab && !greedy) {
+      const int64_t row = q.start + up;
+      p = weight(d.target[row * d.target_stride + t], m[up], c);
+      if (d.draft) w = weight(d.draft[row * d.draft_stride + t], qm[up], c);
+      if (d.parent)
+        for (int j = 1; j < i; j++) same |= parent[j] == up && token[j] == t;
+    }
+    ep[i] = p;
+    eq[i] = w;
+    again[i] = same;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int cur = 0, n = 1, rejected = 0;
+    double left = 1.0;
+    bool rest = false;
+    v.kept[q.start] = 0;
+    for (int i = 1; i < q.n; i++) {
+      if (parent[i] != cur) continue;
+      const bool has = fabsf(m[cur]) < kInf;
+      const double u = (double)d.uniform[q.start + i], p = ep[i] / s[cur];
+      bool stays = has && ep[i] > 0.0;
+      if (greedy) {
+        stays = has && token[i] == best[cur];
+      } else if (d.draft) {
+        const bool known = fabsf(qm[cur]) < kInf;
+        stays = stays && known && u * (eq[i] / qs[cur]) < p;
+        rest = known && !stays;
+      } else {
+        stays = stays && !again[i];
+        if (stays && !(u * left < p)) {
+          stays = false;
+          left -= p;
+          v.rej[q.start + rejected++] = token[i];
+        }
+      }
+      if (stays) {
+        v.out[q.start + n - 1] = token[i];
+        v.kept[q.start + n++] = i;
+        cur = i;
+        left = 1.0;
+        rejected = 0;
+        rest = false;
+      }
+    }
+    const bool has = fabsf(m[cur]) < kInf;
+    const bool drawn = greedy || !has;
+    if (drawn) v.out[q.start + n - 1] = has ? best[cur] : -1;
+    last.s = s[cur];
+    last.qs = rest ? qs[cur] : 1.0;
+    last.c = c;
+    last.u = (double)d.uniform[q.start];
+    last.m = m[cur];
+    last.qm = rest ? qm[cur] : 0.f;
+    last.row = q.start + cur;
+    last.mode = drawn ? 0 : rest ? 2 : 1;
+    last.rejected = rejected;
+    last.first = q.start;
+    last.out = q.start + n - 1;
+    v.count[b] = n;
+    kept_n = n;
+  }
+  __syncthreads();
+  for (int i = kept_n + (int)threadIdx.x; i < q.n; i += 1024) {
+    v.out[q.start + i] = -1;
+    v.kept[q.start + i] = -1;
+  }
+}
+
+// The weight left of a token with logits x and (mode 2) y.
+__device__ inline double left_of(const mg_drafts_last &l, int mode, float x, float y) {
+  const double p = weight(x, l.m, l.c) / l.s;
+  return mode == 2 ? fmax(p - weight(y, l.qm, l.c) / l.qs, 0.0) : p;
+}
+
+__global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
+  const mg_drafts &d = v.d;
+  const int64_t b = blockIdx.y;
+  const mg_drafts_last l = v.last[b];
+  const int lane = threadIdx.x & 63;
+  const int run = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (l.mode == 0 || run >= v.nrun) return;
+  const int64_t first = (int64_t)run * MG_DRAFTS_RUN;
+  float x[kLane], y[kLane] = {};
+  load(x, d.target + l.row * d.target_stride, first, d.vocab, lane);
+  if (l.mode == 2) load(y, d.draft + l.row * d.draft_stride, first, d.vocab, lane);
+  for (int r = 0; r < l.rejected; r++) {
+    const int64_t t = v.rej[l.first + r] - first;
+    if (t < 0 || t >= MG_DRAFTS_RUN) continue;
+#pragma unroll
+    for (int j = 0; j < kLane; j++)
+      if (256 * (j / 4) + 4 * lane + j % 4 == t) x[j] = -kInf;
+  }
+  double w = 0.0;
+#pragma unroll
+  for (int j = 0; j < kLane; j++) w += left_of(l, l.mode, x[j], y[j]);
+  w = wave_sum(w);
+  if (lane == 0) v.mass[b * v.nrun + run] = w;
+}
+
+// The running sum over the workgroup's 256 threads before this one and up to it (the next one's
+// before is this one's up to, bit for bit), and the whole.
+struct Sums {
+  double before, upto, all;
+};
+__device__ inline Sums scan(double x, double *part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  double before = 0.0;
+  for (int k = 0; k < wave; k++) before += part[k];
+  const double y = __shfl_up(x, 1);
+  return Sums{lane ? before + y : before, before + x, part[0] + part[1] + part[2] + part[3]};
+}
+
+__global__ __launch_bounds__(256) void k_pick(const mg_verify v) {
+  constexpr int kOne = MG_DRAFTS_RUN / 256;
+  __shared__ double part[4], below;
+  __shared__ int run, pick, highest;
+  const mg_drafts &d = v.d;
+  const int64_t b = blockIdx.x;
+  const mg_drafts_last l = v.last[b];
+  if (l.mode == 0) return;
+  int mode = l.mode;
+  const int per = (v.nrun + 255) / 256, r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
+  const mg_drafts_part *parts = v.part + l.row * v.nrun;
+  // (mode 1 after the residual came out empty: p's own sums.)
+  auto mass = [&](int r) {
+    return mode == l.mode ? v.mass[b * v.nrun + r]
+                          : parts[r].s * exp2_of(((double)parts[r].m - (double)l.m) * l.c) / l.s;
+  };
+  Sums sum;
+  for (;;) {
+    double mine = 0.0;
+    for (int r = r0; r < r1; r++) mine += mass(r);
+    sum = scan(mine, part);
+    if (mode == 1 || sum.all > 0x1p-40) break;
+    mode = 1;
+  }
+  const double want = l.u * sum.all;
+  if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff;
+  __syncthreads();
+  // The first run whose running sum exceeds it, else (rounding) the last one that has any.
+  if (sum.upto > want && sum.before <= want) {
+    double at = sum.before, base = at;
+    int found = -1;
+    for (int r = r0; r < r1 && at <= want; r++) {
+      const double w = mass(r);
+      if (w > 0.0) found = r, base = at;
+      at += w;
+    }
+    run = found;
+    below = base;
+  }
+  __syncthreads();
+  if (run < 0) {
+    for (int r = r0; r < r1; r++)
+      if (mass(r) > 0.0) atomicMax(&highest, r);
+    __syncthreads();
+    if (threadIdx.x == 0) run = highest, below = 0.0;
+    __syncthreads();
+  }
+  if (run < 0) {
+    if (threadIdx.x == 0) v.out[l.out] = -1;
+    return;
+  }
+  const bool end = highest >= 0;
+  const int64_t first = (int64_t)run * MG_DRAFTS_RUN + kOne * threadIdx.x;
+  const float *x = d.target + l.row * d.target_stride;
+  const float *y = mode == 2 ? d.draft + l.row * d.draft_stride : x;
+  double w[kOne], own = 0.0;
+#pragma unroll
+  for (int j = 0; j < kOne; j++) {
+    const int64_t e = first + j;
+    w[j] = e < d.vocab ? left_of(l, mode, x[e], y[e]) : 0.0;
+  }
+  for (int r = 0; r < l.rejected; r++) {
+    const int64_t t = v.rej[l.first + r] - first;
+#pragma unroll
+    for (int j = 0; j < kOne; j++)
+      if (t == j) w[j] = 0.0;
+  }
+#pragma unroll
+  for (int j = 0; j < kOne; j++) own += w[j];
+  __syncthreads();
+  if (threadIdx.x == 0) highest = -1;
+  double at = below + scan(own, part).before;
+#pragma unroll
+  for (int j = 0; j < kOne; j++) {
+    at += w[j];
+    if (w[j] > 0.0) {
+      atomicMax(&highest, kOne * (int)threadIdx.x + j);
+      if (!end && at > want) atomicMin(&pick, kOne * (int)threadIdx.x + j);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int in = pick < 0x7fffffff ? pick : highest;
+    v.out[l.out] = in < 0 ? -1 : run * MG_DRAFTS_RUN + in;
+  }
+}
+
+}  // namespace
+
+size_t mg_verify_plan(mg_verify *v, void *ws) {
+  v->nrun = (int)((v->d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN);
+  const size_t parts = mg_align((size_t)v->d.rows * v->nrun * (v->d.draft ? 2 : 1) * sizeof(mg_drafts_part));
+  const size_t masses = mg_align((size_t)v->d.batch * v->nrun * 8);
+  const size_t lasts = mg_align((size_t)v->d.batch * sizeof(mg_drafts_last));
+  char *p = static_cast<char *>(ws);
+  if (p) {
+    v->part = reinterpret_cast<mg_drafts_part *>(p);
+    v->mass = reinterpret_cast<double *>(p + parts);
+    v->last = reinterpret_cast<mg_drafts_last *>(p + parts + masses);
+    v->rej = reinterpret_cast<int32_t *>(p + parts + masses + lasts);
+  }
+  return parts + masses + lasts + mg_align((size_t)v->d.rows * 4);
+}
+
+mg_status mg_verify_run(mg_ctx *ctx, const mg_verify &v) {
+  const mg_drafts &d = v.d;
+  const unsigned runs = (unsigned)((v.nrun + 3) / 4);
+  hipStream_t st = ctx->stream;
+  if (d.max_new == 0) {  // (no sequence has rows: their counts)
+    k_walk<<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
+    return mg_launch_check("VerifyDrafts");
+  }
+  k_stats<<<dim3(runs, (unsigned)(d.max_new * (d.draft ? 2 : 1)), (unsigned)d.batch), dim3(256), 0, st>>>(v);
+  k_walk<<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
+  k_masses<<<dim3(runs, (unsigned)d.batch), dim3(256), 0, st>>>(v);
+  k_pick<<<dim3((unsigned)d.batch), dim3(256), 0, st>>>(v);
+  return mg_launch_check("VerifyDrafts");
+}

@@ -758,6 +758,31 @@ class KvCache:
             tree_ptr or None, tree_words, int(scale is not None),
             0.0 if scale is None else scale, y_ptr, y_stride))
 
+    def copy_pages_dev(self, src_ptr: int, dst_ptr: int, n: int):
+        """Page dst[i] becomes what page src[i] holds (int32 lists of n)."""
+        check(lib.mg_kv_cache_copy_pages_dev(self.ctx.handle, self.handle, src_ptr or None,
+                                             dst_ptr or None, n))
+
+    def compact_dev(self, seqs: SeqBatch, kept_ptr: int, count_ptr: int, *, past_out_ptr: int = 0):
+        """Of each sequence's new rows those that stay move together (kept [rows], count
+        [batch] as verify_drafts_dev writes them); past_out = past + count if wanted."""
+        check(lib.mg_kv_cache_compact_dev(self.ctx.handle, self.handle, C.byref(seqs),
+                                          kept_ptr or None, count_ptr or None,
+                                          past_out_ptr or None))
+
+    def fork_dev(self, seqs: SeqBatch, parent_ptr: int, out_batch: int, past_out_ptr: int,
+                 table_out_ptr: int, out_stride: int, refs_ptr: int):
+        """A batch of continuations of seqs' sequences on shared pages (refs int32 [pages])."""
+        check(lib.mg_kv_cache_fork_dev(self.ctx.handle, self.handle, C.byref(seqs),
+                                       parent_ptr or None, out_batch, past_out_ptr or None,
+                                       table_out_ptr or None, out_stride, refs_ptr or None))
+
+    def fit_dev(self, seqs: SeqBatch, refs_ptr: int, granted_ptr: int):
+        """Writes seqs' page table: pages for the past and new rows of each sequence, a copy of a
+        shared page that is written into, nothing behind; granted int32 [batch]."""
+        check(lib.mg_kv_cache_fit_dev(self.ctx.handle, self.handle, C.byref(seqs), refs_ptr or None,
+                                      granted_ptr or None))
+
     # Host arrays: row_start [batch + 1], past [batch], page_table [batch, n] as in SeqBatch;
     # rope = (cos, sin, interleaved) or (cos, sin, interleaved, positions [rows]).
 
@@ -797,6 +822,86 @@ class KvCache:
             got = [o.to_array(sh, np.float32) for o, sh in zip(outs, out_shapes)]
             self.ctx.synchronize()
             return got
+
+    def _lists(self, arrays, outs, call):
+        """Runs call(pointers of the uploaded int32 arrays, of the outputs); outs are shapes
+        (zeros before the call) or arrays (uploaded, written in place)."""
+        with _Buffers(self.ctx) as bufs:
+            ins = [bufs.upload(_int32(x)).ptr for x in arrays]
+            outs = [_int32(x) if isinstance(x, np.ndarray) else np.zeros(x, np.int32) for x in outs]
+            dev = [bufs.upload(x) for x in outs]
+            call(ins, [d.ptr for d in dev])
+            return [d.to_array(x.shape, np.int32) for d, x in zip(dev, outs)]
+
+    @staticmethod
+    def _table(past, page_table):
+        past, page_table = _int32(past).ravel(), _int32(page_table)
+        if page_table.ndim != 2 or page_table.shape[0] != past.size:
+            raise ArgumentError("KvCache: past must be [batch], page_table [batch, pages]")
+        return past, page_table
+
+    def _refs(self, refs):
+        refs = _int32(refs).ravel()
+        if refs.size != self.pages:
+            raise ArgumentError("KvCache: refs must be [pages]")
+        return refs
+
+    def copy_pages(self, src, dst):
+        """Page dst[i] becomes what page src[i] holds."""
+        src, dst = _int32(src).ravel(), _int32(dst).ravel()
+        if src.size != dst.size:
+            raise ArgumentError("KvCache: as many src pages as dst pages")
+        self._lists([src, dst], [], lambda p, _: self.copy_pages_dev(p[0], p[1], src.size))
+        self.ctx.synchronize()
+
+    def compact(self, kept, count, *, row_start, past, page_table):
+        """Moves the rows that stay together; returns past + count [batch]."""
+        past, page_table = self._table(past, page_table)
+        row_start, kept, count = (_int32(x).ravel() for x in (row_start, kept, count))
+        n = np.diff(row_start.astype(np.int64))
+        if row_start.size != past.size + 1 or count.size != past.size or kept.size != row_start[-1] or \
+                row_start[0] != 0 or (n < 0).any() or (past < 0).any():
+            raise ArgumentError("KvCache: row_start must rise from 0 to the rows, kept be [rows], count [batch]")
+
+        def call(p, out):
+            self.compact_dev(SeqBatch(
+                batch=past.size, rows=kept.size, max_new=int(n.max(initial=0)),
+                max_len=int((n + past).max(initial=0)), row_start_ptr=p[0], past_ptr=p[1],
+                page_table_ptr=p[2], table_stride=page_table.shape[1]), p[3], p[4], past_out_ptr=out[0])
+
+        return self._lists([row_start, past, page_table, kept, count], [past.shape], call)[0]
+
+    def fork(self, parent, *, past, page_table, refs, width=None):
+        """(past, page_table [., width], refs) of the continuations parent [out_batch] (-1: an
+        empty sequence) of a batch; width None: the old table's."""
+        past, page_table = self._table(past, page_table)
+        parent, refs = _int32(parent).ravel(), self._refs(refs)
+        width = page_table.shape[1] if width is None else int(width)
+
+        def call(p, out):
+            self.fork_dev(SeqBatch(batch=past.size, rows=0, max_new=0,
+                                   max_len=max(int(past.max(initial=0)), 0), row_start_ptr=0, past_ptr=p[1],
+                                   page_table_ptr=p[2], table_stride=page_table.shape[1]),
+                          p[0], parent.size, out[0], out[1], width, out[2])
+
+        return self._lists([parent, past, page_table], [parent.shape, (parent.size, width), refs], call)
+
+    def fit(self, *, row_start, past, page_table, refs):
+        """(page_table, refs, granted [batch]): each sequence's pages made those that its past and
+        new rows need."""
+        past, page_table = self._table(past, page_table)
+        row_start, refs = _int32(row_start).ravel(), self._refs(refs)
+        n = np.diff(row_start.astype(np.int64))
+        if row_start.size != past.size + 1 or row_start[0] != 0 or (n < 0).any() or (past < 0).any():
+            raise ArgumentError("KvCache: row_start must rise from 0 to the rows, past be >= 0")
+
+        def call(p, out):
+            self.fit_dev(SeqBatch(
+                batch=past.size, rows=int(row_start[-1]), max_new=int(n.max(initial=0)),
+                max_len=int((n + past).max(initial=0)), row_start_ptr=p[0], past_ptr=p[1],
+                page_table_ptr=out[0], table_stride=page_table.shape[1]), out[1], out[2])
+
+        return self._lists([row_start, past], [page_table, refs, past.shape], call)
 
     def append(self, k, v, *, row_start, past, page_table, rope=None):
         """Writes host rows k, v [rows, kv_heads, head_size]."""
@@ -858,6 +963,115 @@ def token_logprobs_dev(logits_ptr: int, rows: int, vocab: int, *, tokens_ptr: in
                                         tokens_ptr or None, logprob_ptr or None,
                                         entropy_ptr or None, top, top_ids_ptr or None,
                                         top_logprobs_ptr or None))
+
+
+class Drafts(C.Structure):
+    """mg_drafts: drafted tokens of a batch of sequences and the logits to verify them against.
+    Pointers are device memory; 0 for those that are not given."""
+    _fields_ = [("batch", C.c_int64), ("rows", C.c_int64), ("max_new", C.c_int64),
+                ("vocab", C.c_int64), ("row_start", C.c_void_p), ("tokens", C.c_void_p),
+                ("parent", C.c_void_p), ("target", C.c_void_p), ("target_stride", C.c_int64),
+                ("draft", C.c_void_p), ("draft_stride", C.c_int64), ("temperature", C.c_void_p),
+                ("uniform", C.c_void_p)]
+
+    def __init__(self, *, batch: int, rows: int, max_new: int, vocab: int, row_start_ptr: int,
+                 tokens_ptr: int, target_ptr: int, uniform_ptr: int, parent_ptr: int = 0,
+                 draft_ptr: int = 0, temperature_ptr: int = 0, target_stride: int = 0,
+                 draft_stride: int = 0):
+        super().__init__(batch, rows, max_new, vocab, row_start_ptr or None, tokens_ptr or None,
+                         parent_ptr or None, target_ptr or None, target_stride, draft_ptr or None,
+                         draft_stride, temperature_ptr or None, uniform_ptr or None)
+
+
+def verify_drafts_dev(drafts: Drafts, out_tokens_ptr: int, kept_ptr: int, count_ptr: int,
+                      ctx: Context | None = None):
+    """Which drafted tokens stay: emitted tokens and rows that stay [rows], how many [batch]."""
+    ctx = ctx or default_context()
+    check(lib.mg_verify_drafts_f32_dev(ctx.handle, C.byref(drafts), out_tokens_ptr or None,
+                                       kept_ptr or None, count_ptr or None))
+
+
+class Adapters:
+    """Low-rank adapters in HBM (mg_adapters) of the projections k -> ns[i] of one input, one in
+    each slot."""
+
+    FORMATS = {"f32": 0, "f16": 1}
+    handle = None
+
+    def __init__(self, k: int, ns, *, slots: int, max_rank: int, fmt: str = "f32",
+                 ctx: Context | None = None):
+        if fmt not in self.FORMATS:
+            raise ArgumentError(f"Adapters: unknown format {fmt}")
+        self.ctx = ctx or default_context()
+        self.k, self.ns, self.slots, self.max_rank = int(k), [int(n) for n in ns], int(slots), int(max_rank)
+        h = C.c_void_p()
+        check(lib.mg_adapters_create(self.ctx.handle, self.k, len(self.ns),
+                                     (C.c_int64 * max(len(self.ns), 1))(*self.ns), self.slots,
+                                     self.max_rank, self.FORMATS[fmt], C.byref(h)))
+        self.handle = h
+
+    def release(self):
+        if self.handle:
+            lib.mg_adapters_release(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+    @property
+    def device_bytes(self) -> int:
+        n = C.c_int64(0)
+        check(lib.mg_adapters_info(self.handle, None, None, None, None, C.byref(n)))
+        return n.value
+
+    def _pointers(self, ptrs):
+        ptrs = list(ptrs)
+        if len(ptrs) != len(self.ns):
+            raise ArgumentError("Adapters: one for each projection expected")
+        return (C.c_void_p * len(ptrs))(*[p or None for p in ptrs])
+
+    def set(self, slot: int, a, b, *, scale: float = 1.0):
+        """Fills a slot: a[i] [rank, k] and b[i] [ns[i], rank] for each projection (or one of each,
+        where there is one); a and b None empty it."""
+        if a is None and b is None:
+            check(lib.mg_adapters_set(self.ctx.handle, self.handle, slot, 0, None, None, 1.0))
+            return
+        a, b = ([np.ascontiguousarray(y, np.float32) for y in ([x] if isinstance(x, np.ndarray) else x)]
+                for x in (a, b))
+        rank = a[0].shape[0] if a and a[0].ndim == 2 else -1
+        if len(a) != len(self.ns) or len(b) != len(self.ns) or rank < 1 or any(
+                x.shape != (rank, self.k) for x in a) or any(y.shape != (n, rank) for y, n in zip(b, self.ns)):
+            raise ArgumentError("Adapters: a[i] must be [rank, k], b[i] [ns[i], rank]")
+        check(lib.mg_adapters_set(self.ctx.handle, self.handle, slot, rank,
+                                  self._pointers(x.ctypes.data for x in a),
+                                  self._pointers(x.ctypes.data for x in b), scale))
+
+    def set_dev(self, slot: int, rank: int, a_ptrs, b_ptrs, *, scale: float = 1.0):
+        """Fills a slot from device memory (asynchronous)."""
+        check(lib.mg_adapters_set_dev(self.ctx.handle, self.handle, slot, rank, self._pointers(a_ptrs),
+                                      self._pointers(b_ptrs), scale))
+
+    def apply_dev(self, x_ptr: int, rows: int, slot_ptr: int, base_ptrs, y_ptrs):
+        """y_i = base_i + scale B_i (A_i x), each row by its own slot (int32; negative: none)."""
+        check(lib.mg_adapters_apply_f32_dev(self.ctx.handle, self.handle, x_ptr or None, rows,
+                                            slot_ptr or None, self._pointers(base_ptrs),
+                                            self._pointers(y_ptrs)))
+
+    def apply(self, x, slots, bases):
+        """apply_dev on host arrays x [..., k], slots [...], bases[i] [..., ns[i]]: the y_i."""
+        x = np.ascontiguousarray(x, np.float32)
+        slots, bases = _int32(slots), [np.ascontiguousarray(y, np.float32) for y in bases]
+        if x.ndim < 1 or x.shape[-1] != self.k or slots.shape != x.shape[:-1] or \
+                [y.shape for y in bases] != [x.shape[:-1] + (n,) for n in self.ns]:
+            raise ArgumentError("Adapters: x must be [..., k], slots [...], bases[i] [..., ns[i]]")
+        with _Buffers(self.ctx) as bufs:
+            ins = [bufs.upload(v).ptr for v in (x, slots)]
+            ys = [bufs.upload(y) for y in bases]
+            self.apply_dev(ins[0], slots.size, ins[1], [y.ptr for y in ys], [y.ptr for y in ys])
+            return [y.to_array(b.shape, np.float32) for y, b in zip(ys, bases)]
 
 
 # ---------------------------------------------------------------------- ops
@@ -1314,6 +1528,52 @@ def op_token_logprobs(logits, tokens=None, *, top: int = 0, ctx: Context | None 
         return (outs[0].to_array(lead, np.float32) if tokens is not None else None,
                 outs[1].to_array(lead, np.float32), outs[2].to_array(lead + (top,), np.int32),
                 outs[3].to_array(lead + (top,), np.float32))
+
+
+def op_verify_drafts(target, tokens, uniform, row_start, *, parent=None, draft=None, temperature=None,
+                     ctx: Context | None = None):
+    """(emitted tokens [rows], rows that stay [rows], how many of each [batch]) of drafted tokens
+    [rows] verified against target logits [rows, vocab]: rows of sequence b are row_start[b] ..
+    row_start[b + 1] - 1, the first its last emitted token; parent [rows] (indices within the
+    sequence; None: chains), draft logits [rows, vocab] or None, temperature [batch] (None: 1),
+    uniform [rows] random numbers in [0, 1).  -1 behind what a sequence emits."""
+    x = np.ascontiguousarray(target, np.float32)
+    if x.ndim != 2 or x.shape[1] < 1:
+        raise ArgumentError("VerifyDrafts: target must be [rows, vocab]")
+    rows, vocab = x.shape
+    start = _int32(row_start).ravel()
+    n = np.diff(start.astype(np.int64))
+    if start.size < 1 or (start.size > 1 and (start[0] != 0 or start[-1] != rows or (n < 0).any())):
+        raise ArgumentError("VerifyDrafts: row_start must rise from 0 to the rows")
+    u = np.ascontiguousarray(uniform, np.float32).ravel()
+    tokens = np.asarray(tokens).ravel()
+    if tokens.dtype.kind not in "iu" or tokens.size != rows or u.size != rows:
+        raise ArgumentError("VerifyDrafts: one integer token and one random number a row")
+    if not ((u >= 0) & (u < 1)).all():
+        raise ArgumentError("VerifyDrafts: random numbers must be in [0, 1)")
+    # (Any token outside the vocabulary is -1: int32 could wrap into it.)
+    tokens = np.where((tokens < 0) | (tokens >= vocab), -1, tokens).astype(np.int32)
+    if parent is not None:
+        parent = _int32(parent).ravel()
+        if parent.size != rows:
+            raise ArgumentError("VerifyDrafts: one parent a row")
+    if draft is not None:
+        draft = np.ascontiguousarray(draft, np.float32)
+        if draft.shape != x.shape:
+            raise ArgumentError("VerifyDrafts: draft must be [rows, vocab] as target")
+    if temperature is not None:
+        temperature = np.ascontiguousarray(temperature, np.float32).ravel()
+        if temperature.size != n.size:
+            raise ArgumentError("VerifyDrafts: one temperature a sequence")
+    ctx = ctx or default_context()
+    with _Buffers(ctx) as bufs:
+        p = [0 if a is None else bufs.upload(a).ptr for a in (start, tokens, x, u, parent, draft, temperature)]
+        outs = [bufs.upload(np.full(max(k, 1), -1, np.int32)) for k in (rows, rows, n.size)]
+        verify_drafts_dev(Drafts(batch=n.size, rows=rows, max_new=int(n.max(initial=0)), vocab=vocab,
+                                 row_start_ptr=p[0], tokens_ptr=p[1], target_ptr=p[2], uniform_ptr=p[3],
+                                 parent_ptr=p[4], draft_ptr=p[5], temperature_ptr=p[6]),
+                          *[o.ptr for o in outs], ctx=ctx)
+        return tuple(o.to_array((k,), np.int32) for o, k in zip(outs, (rows, rows, n.size)))
 
 
 # ------------------------------------------------------------ convolution
