@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "adapters_common.h"
 
@@ -154,15 +155,12 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
   __shared__ int part[16];
   const int buckets = (int)p.h.slots + 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rows = (int)p.rows;
-  auto bucket = [&](int r) {
-    const int s = slot_of(p, r);
-    return s >= 0 ? s : buckets - 1 + (s == -2 ? 0 : -1);
-  };
+  auto bucket = [&](int s) { return s < 0 ? buckets - 2 : s >= buckets - 2 ? buckets - 1 : s; };
   for (int i = threadIdx.x; i < buckets; i += 1024) lds[i] = 0;
   __syncthreads();
   // (Rows of a prompt lie together: a wave of one bucket counts them at once.)
-  auto places = [&](int r, bool in) {
-    const int b = in ? bucket(r) : -1;
+  auto places = [&](int s, bool in) {
+    const int b = in ? bucket(s) : -1;
     const int lead = __builtin_amdgcn_readfirstlane(b);
     int at = 0;
     if (__all(b == lead)) {
@@ -175,7 +173,21 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
     }
     return at;
   };
-  for (int r0 = 0; r0 < rows; r0 += 1024) places(r0 + threadIdx.x, r0 + (int)threadIdx.x < rows);
+  // (Eight loads ahead: their latency bounds this.)
+  constexpr int kAhead = 8;
+  auto each = [&](auto place) {
+    for (int r0 = threadIdx.x; r0 - (int)threadIdx.x < rows; r0 += 1024 * kAhead) {
+      int s[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) s[i] = p.slot[min(r0 + 1024 * i, rows - 1)];
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) {
+        const int r = r0 + 1024 * i, to = places(s[i], r < rows);
+        if (r < rows) place(r, to);
+      }
+    }
+  };
+  each([](int, int) {});
   __syncthreads();
   // First places and tiles, in the buckets' order.
   int at = 0, tiles = 0;
@@ -205,25 +217,22 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
     }
     const int start = before + x - n;
     next += y - m;
+    const int slot = b >= buckets - 1 ? -2 : b == buckets - 2 || n == 0 || p.h.rank[b] == 0 ? -1 : b;
     for (int k = 0; k < m; k++)
-      o.tile[next + k] = Tile{b < buckets - 2 ? b : b == buckets - 2 ? -1 : -2, start + k * kTile,
-                              min(kTile, n - k * kTile), 0};
+      o.tile[next + k] = Tile{slot, start + k * kTile, min(kTile, n - k * kTile), 0};
     if (b < buckets) lds[b] = start;
   }
   if (threadIdx.x == 0) *o.tiles = tiles;
   __syncthreads();
-  for (int r0 = 0; r0 < rows; r0 += 1024) {
-    const int r = r0 + threadIdx.x;
-    const int to = places(r, r < rows);
-    if (r < rows) o.row[to] = r;
-  }
+  each([&](int r, int to) { o.row[to] = r; });
 }
 
 // Part of t[sorted row][rank * projection + value] of a tile: K's share of blockIdx.y, values
-// from kCols * blockIdx.z on.
-template <class T>
-__global__ __launch_bounds__(256) void k_down(const mg_adapt p, const Order o, float *t, int64_t share,
-                                              int64_t cols) {
+// from kCols * blockIdx.z on.  VEC: K is a multiple of four.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256, 2) void k_down(const mg_adapt p, const Order o, float *t, int64_t share,
+                                                 int64_t cols) {
+  constexpr int kDeep = 4;  // steps of eight k that are loaded ahead
   __shared__ float sums[4][64][64];
   if ((int)blockIdx.x >= *o.tiles) return;
   const Tile tile = o.tile[blockIdx.x];
@@ -232,37 +241,64 @@ __global__ __launch_bounds__(256) void k_down(const mg_adapt p, const Order o, f
   if (c0 >= all) return;
   const int lane = threadIdx.x & 63, hi = lane >> 5, l = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const bool wide = c0 + 32 < all;  // a second block of values
+  const int K = (int)p.h.K;
   const float *x[2];
   const T *a[2];
 #pragma unroll
   for (int u = 0; u < 2; u++) {
-    x[u] = p.x + (int64_t)o.row[tile.start + min(32 * u + l, tile.count - 1)] * p.h.K;
+    x[u] = p.x + (int64_t)o.row[tile.start + min(32 * u + l, tile.count - 1)] * K;
     const int c = min(c0 + 32 * u + l, all - 1), i = c / rank;
     a[u] = static_cast<const T *>(p.h.a) + tile.slot * p.h.a_slot +
            ((int64_t)i * p.h.max_rank + c - i * rank) * p.h.kp;
   }
   f32x16 acc[2][2] = {};
-  const int64_t first = share * blockIdx.y, end = std::min(first + share, p.h.kp);
-  // Steps of eight k: four for each half of the wave, two waves' k never alike.
-#pragma unroll 4
-  for (int64_t k0 = first + 8 * wave; k0 < end; k0 += 32) {
-    const int64_t k = k0 + 4 * hi;
-    f32x4 xv[2], av[2];
+  const int first = (int)(share * blockIdx.y), end = (int)std::min(first + share, p.h.kp);
+  // WIDE: a second block of 32 values.  A step is eight k, four for each half of the wave; the four
+  // waves take steps in turn.
+  auto products = [&](auto wide) {
+    constexpr int W = decltype(wide)::value;
+#pragma unroll 1
+    for (int k0 = first + 8 * wave; k0 < end; k0 += 32 * kDeep) {
+      f32x4 xv[kDeep][2], av[kDeep][W];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      xv[u] = load_row(x[u], k, p.h.K);
-      av[u] = u == 0 || wide ? weights(a[u] + k) : f32x4{};
-    }
+      for (int i = 0; i < kDeep; i++) {
+        // (Steps past the end read the last one; x and A count as 0 there.)
+        const int k = min(k0 + 32 * i, end - 8) + 4 * hi;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+        for (int u = 0; u < 2; u++) {
+          if (VEC) {
+            xv[i][u] = load4(x[u] + min(k, K - 4));
+          } else {
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        acc[u][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[u][e], av[0][e], acc[u][0], 0, 0, 0);
-        if (wide) acc[u][1] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[u][e], av[1][e], acc[u][1], 0, 0, 0);
+            for (int e = 0; e < 4; e++) xv[i][u][e] = x[u][min(k + e, K - 1)];
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < W; w++) av[i][w] = weights(a[w] + k);
+      }
+#pragma unroll
+      for (int i = 0; i < kDeep; i++) {
+        const int k = k0 + 32 * i + 4 * hi;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float xe[2], ae[W];
+#pragma unroll
+          for (int u = 0; u < 2; u++) xe[u] = k + e < K && k < end ? xv[i][u][e] : 0.f;
+#pragma unroll
+          for (int w = 0; w < W; w++) ae[w] = k < end ? av[i][w][e] : 0.f;
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int w = 0; w < W; w++)
+              acc[u][w] = __builtin_amdgcn_mfma_f32_32x32x2f32(xe[u], ae[w], acc[u][w], 0, 0, 0);
+        }
       }
     }
-  }
+  };
+  if (c0 + 32 < all)
+    products(std::integral_constant<int, 2>());
+  else
+    products(std::integral_constant<int, 1>());
 #pragma unroll
   for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -280,73 +316,78 @@ __global__ __launch_bounds__(256) void k_down(const mg_adapt p, const Order o, f
   }
 }
 
-// Outputs of a tile: kOuts of them of projection blockIdx.z.
+// Outputs of a tile: kOuts of them of projection blockIdx.z, in blocks of 32 a wave.  stride: of the
+// tile's values in shared memory (odd; kHeld of them at a time, rounded up to 32 with zeros).
+constexpr int kHeld = 128;
 template <class T>
-__global__ __launch_bounds__(256) void k_up(const mg_adapt p, const Order o, const float *t, int parts,
-                                            int64_t cols) {
-  constexpr int kStep = 64, kPad = kStep + 1;
-  __shared__ float low[kTile][kPad];
+__global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, const float *t, int parts,
+                                               int64_t cols, int stride) {
+  extern __shared__ float low[];
   __shared__ int row_of[kTile];
   if ((int)blockIdx.x >= *o.tiles) return;
   const Tile tile = o.tile[blockIdx.x];
   const int z = blockIdx.z;
-  const int64_t N = p.h.N[z], n0 = (int64_t)kOuts * blockIdx.y;
-  if (n0 >= N || (tile.slot == -1 && p.base[z] == p.y[z])) return;
+  const int64_t N = p.h.N[z], np = p.h.np[z], n0 = (int64_t)kOuts * blockIdx.y;
+  const float *base = p.base[z];
+  float *y = p.y[z];
+  if (n0 >= N || (tile.slot == -1 && base == y)) return;
   const int lane = threadIdx.x & 63, hi = lane >> 5, l = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int rank = tile.slot >= 0 ? p.h.rank[tile.slot] : 0;
+  const int rank = tile.slot >= 0 ? p.h.rank[tile.slot] : 0, steps = (rank + 31) / 32;
   if (threadIdx.x < kTile) row_of[threadIdx.x] = o.row[tile.start + min((int)threadIdx.x, tile.count - 1)];
-  const T *b = static_cast<const T *>(p.h.b) + (int64_t)std::max(tile.slot, 0) * p.h.b_slot + p.h.b_off[z];
-  constexpr int kBlocks = kOuts / 128;
-  f32x16 acc[kBlocks][2] = {};
-  for (int j0 = 0; j0 < rank; j0 += kStep) {
-    const int n = min(kStep, rank - j0);
+  auto stage = [&](int j1) {
+    const int n = min(kHeld, 32 * steps - j1);
     __syncthreads();
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      const int r = i / kStep, j = i % kStep;
+    for (int i = threadIdx.x; i < kTile * n; i += 256) {
+      const int r = i / n, j = i % n;
       float v = 0.f;
-      if (r < tile.count && j < n)
+      if (r < tile.count && j1 + j < rank)
         for (int part = 0; part < parts; part++)
-          v += t[((int64_t)part * p.rows + tile.start + r) * cols + z * rank + j0 + j];
-      low[r][j] = v;
+          v += t[((int64_t)part * p.rows + tile.start + r) * cols + z * rank + j1 + j];
+      low[r * stride + j] = v;
     }
     __syncthreads();
+  };
+  stage(0);
+  const T *b = static_cast<const T *>(p.h.b) + (int64_t)std::max(tile.slot, 0) * p.h.b_slot + p.h.b_off[z];
+  const float *own = low + l * stride + hi;
+#pragma unroll 1
+  for (int q = 0; q < kOuts / 128; q++) {
+    const int64_t at = n0 + 128 * q + 32 * wave, n = std::min(at + l, N - 1);
+    if (at >= N && rank <= kHeld) break;  // (else it takes part in what follows)
+    float v[2][16];
 #pragma unroll
-    for (int q = 0; q < kBlocks; q++) {
-      const int64_t at = n0 + 128 * q + 32 * wave;
-      if (at >= N) break;
-      const T *col = b + std::min(at + l, p.h.np[z] - 1);
-#pragma unroll 8
-      for (int j = 0; j < n; j += 2) {
-        const int own = j + hi;
-        // (Past an odd rank's end: its last row, times 0.)
-        const float w = (float)col[(int64_t)(j0 + min(own, n - 1)) * p.h.np[z]];
-        const float v = own < n ? w : 0.f;
-        acc[q][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(low[l][own], v, acc[q][0], 0, 0, 0);
-        acc[q][1] = __builtin_amdgcn_mfma_f32_32x32x2f32(low[32 + l][own], v, acc[q][1], 0, 0, 0);
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        v[u][e] = base[(int64_t)row_of[32 * u + 8 * (e / 4) + 4 * hi + e % 4] * N + n];
+    f32x16 acc[2] = {};
+#pragma unroll 1
+    for (int j0 = 0; j0 < 32 * steps; j0 += 32) {
+      if (rank > kHeld && j0 % kHeld == 0) stage(j0);
+      float w[16];
+      // (Past the rank: its last row, then 0, which no infinity of B turns into NaN.)
+#pragma unroll
+      for (int j = 0; j < 16; j++) w[j] = (float)b[(int64_t)min(j0 + 2 * j + hi, rank - 1) * np + n];
+      if (j0 + 32 > rank) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) w[j] = j0 + 2 * j + hi < rank ? w[j] : 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+          acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(own[32 * u * stride + j0 % kHeld + 2 * j], w[j], acc[u], 0, 0, 0);
     }
-  }
-  __syncthreads();
+    if (at + l >= N) continue;
 #pragma unroll
-  for (int q = 0; q < kBlocks; q++) {
-    const int64_t n = n0 + 128 * q + 32 * wave + l;
-    if (n >= N) continue;
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      float v[16];
+    for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         const int r = 32 * u + 8 * (e / 4) + 4 * hi + e % 4;
-        v[e] = p.base[z][(int64_t)row_of[r] * N + n];
+        const float sum = tile.slot == -2 ? __builtin_nanf("") : rank ? v[u][e] + acc[u][e] : v[u][e];
+        if (r < tile.count) y[(int64_t)row_of[r] * N + n] = sum;
       }
-#pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int r = 32 * u + 8 * (e / 4) + 4 * hi + e % 4;
-        const float y = tile.slot == -2 ? __builtin_nanf("") : rank ? v[e] + acc[q][u][e] : v[e];
-        if (r < tile.count) p.y[z][(int64_t)row_of[r] * N + n] = y;
-      }
-    }
   }
 }
 
@@ -388,10 +429,14 @@ void run(mg_ctx *ctx, const mg_adapt &p, void *ws) {
   w += mg_align((size_t)tiles * sizeof(Tile));
   float *t = reinterpret_cast<float *>(w);
   k_sort<<<dim3(1), dim3(1024), (size_t)(h.slots + 2) * 4, st>>>(p, o);
-  k_down<T><<<dim3((unsigned)tiles, (unsigned)parts, (unsigned)((cols + kCols - 1) / kCols)), dim3(256), 0, st>>>(
-      p, o, t, share, cols);
-  k_up<T><<<dim3((unsigned)tiles, (unsigned)((most + kOuts - 1) / kOuts), (unsigned)h.n), dim3(256), 0, st>>>(
-      p, o, t, parts, cols);
+  const dim3 grid((unsigned)tiles, (unsigned)parts, (unsigned)((cols + kCols - 1) / kCols));
+  if (h.K % 4 == 0)
+    k_down<T, true><<<grid, dim3(256), 0, st>>>(p, o, t, share, cols);
+  else
+    k_down<T, false><<<grid, dim3(256), 0, st>>>(p, o, t, share, cols);
+  const int stride = std::min((h.max_rank + 31) / 32 * 32, kHeld) + 1;
+  k_up<T><<<dim3((unsigned)tiles, (unsigned)((most + kOuts - 1) / kOuts), (unsigned)h.n), dim3(256),
+            (size_t)kTile * stride * 4, st>>>(p, o, t, parts, cols, stride);
 }
 
 template <class T>

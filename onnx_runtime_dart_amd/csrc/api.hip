@@ -3050,8 +3050,11 @@ mg_status mg_kv_cache_compact_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_
   if (2 * s.batch * cache->kv_heads > MG_MOST_GROUPS)
     return mg_fail(MG_UNSUPPORTED, "KvCacheCompact: too many sequences");
   MG_TRY(mg_use_device(ctx));
-  MG_TRY(mg_check_control(ctx, 0));
-  return mg_kv_compact_run(ctx, *cache, s, kept_dev, count_dev, past_out_dev);
+  // Without the workspace (byte budget, stream capture) long lists move in order too.
+  size_t need = mg_kv_compact_ws(*cache, s);
+  if (need && !mg_ws_optional(ctx, need)) need = 0;
+  MG_TRY(mg_check_control(ctx, (int64_t)need));
+  return mg_kv_compact_run(ctx, *cache, s, kept_dev, count_dev, past_out_dev, need ? ctx->ws : nullptr);
 }
 
 mg_status mg_kv_cache_fork_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,
@@ -3156,7 +3159,7 @@ mg_status mg_verify_drafts_f32_dev(mg_ctx *ctx, const mg_drafts *drafts, int32_t
       (d.max_new && (!d.tokens || !d.target || !d.uniform || !out_tokens_dev || !kept_dev)))
     return bad_arg(what, "null buffer");
   const int64_t runs = (d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN;
-  if ((runs + 3) / 4 * d.batch > MG_MOST_GROUPS / (2 * d.max_new + 1) ||
+  if (runs * d.batch > MG_MOST_GROUPS / (2 * d.max_new + 1) * 4 || runs * d.batch > MG_MOST_GROUPS ||
       d.rows > ((int64_t)1 << 36) / runs)
     return mg_fail(MG_UNSUPPORTED, "VerifyDrafts: too many logits");
   v.out = out_tokens_dev;

@@ -72,8 +72,9 @@ size_t mg_kv_copy_ws(int64_t n);
 int64_t mg_kv_copy_groups(const mg_kv_cache &c, int64_t n);
 mg_status mg_kv_copy_run(mg_ctx *ctx, const mg_kv_cache &c, const int32_t *src, const int32_t *dst,
                          int64_t n, void *ws);
+size_t mg_kv_compact_ws(const mg_kv_cache &c, const mg_seq_batch &s);
 mg_status mg_kv_compact_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
-                            const int32_t *kept, const int32_t *count, int32_t *past_out);
+                            const int32_t *kept, const int32_t *count, int32_t *past_out, void *ws);
 mg_status mg_kv_fork_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
                          const int32_t *parent, int64_t out_batch, int32_t *past_out,
                          int32_t *table_out, int64_t out_stride, int32_t *refs);

@@ -3,8 +3,9 @@
 //
 // A page's codes of keys, of values and its scales are three runs of memory, so a copy is one read
 // and one write of them.  Rows that move within a sequence only ever move down, in order: a
-// workgroup per head takes them 128 at a time, reads all before it writes any, and nothing that
-// it writes is read later (row j comes from kept[j] >= j, later rows from beyond it).
+// workgroup per head takes them 32 or 128 at a time, reads all before it writes any, and nothing
+// that it writes is read later (row j comes from kept[j] >= j, later rows from beyond it).  Long
+// lists go through the workspace, twice the traffic but all workgroups at once.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -92,44 +93,45 @@ __global__ __launch_bounds__(256) void k_copy_pages(const Pairs a) {
 
 // ------------------------------------------------------------------- compact
 
+// A sequence's rows to move: j0 .. count - 1 (rows before j0 stay where they are).
+struct Moves {
+  int j0, count;
+  int bad, unused;  // bad: the sequence is refused (count is 0)
+};
 struct Compact {
   mg_kv_cache c;
   mg_seq_batch s;
   const int32_t *kept, *count;
   int32_t *past_out;
+  // Staged (long lists): the sequences' moves, and rows on their way [sequence][head][keys or
+  // values][chunk], then their scales.
+  Moves *moves;
+  uint8_t *rows;
+  float *scales;
+  int chunks;
 };
 
-constexpr int kRows = 128;  // rows moved at a time
-
-// A sequence's rows to move: j0 .. count - 1 (rows before j0 stay where they are).
-struct Moves {
-  kv_seq q;
-  int j0, count;
-};
-// By the whole workgroup; false: nothing to move.  *bad: the sequence is refused.
-__device__ inline bool moves_of(const Compact &a, int64_t b, Moves *o, bool *bad) {
-  o->q = kv_sequence(a.s, b);
-  o->count = a.count[b];
-  *bad = o->q.bad || o->count < 0 || o->count > o->q.n;
-  if (*bad) return false;
-  const int32_t *kept = a.kept + o->q.start;
+// By the whole workgroup.
+__device__ inline Moves moves_of(const Compact &a, const kv_seq &q, int64_t b) {
+  const int count = a.count[b];
+  bool bad = q.bad || count < 0 || count > q.n;
   int same = 0;
-  bool wrong = false;
-  for (int j = threadIdx.x; j < o->count; j += 256) {
-    const int k = kept[j];
-    wrong |= k < 0 || k >= o->q.n || (j > 0 && k <= kept[j - 1]);
-    same += k == j;
+  if (!bad) {
+    const int32_t *kept = a.kept + q.start;
+#pragma unroll 4
+    for (int j = threadIdx.x; j < count; j += 256) {
+      const int k = kept[j], before = kept[max(j - 1, 0)];
+      bad |= k < 0 || k >= q.n || (j > 0 && k <= before);
+      same += k == j;
+    }
   }
-  *bad = __syncthreads_or(wrong);
-  if (*bad) return false;
   // (Rising numbers from 0 on: once one is beyond its place, all are.)
   __shared__ int sum;
   if (threadIdx.x == 0) sum = 0;
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   if (same) atomicAdd(&sum, same);
   __syncthreads();
-  o->j0 = sum;
-  return o->j0 < o->count;
+  return bad ? Moves{0, 0, 1, 0} : Moves{sum, count, 0, 0};
 }
 
 // Nibbles of a token's values in the dword of a pair of dims (see kv_common.h).
@@ -143,18 +145,23 @@ __device__ inline uint32_t token_to(uint32_t x, int t) {
   return INT4 ? x << v4_shift(t) : x << 8 * t;
 }
 
-// blockIdx: head, sequence, keys or values.
-template <bool INT4>
+// IN_ORDER: a workgroup takes all of a sequence's rows of a head, ROWS at a time.  GATHER and
+// SCATTER: one such chunk a workgroup, through the workspace.  blockIdx: head, sequence, keys or
+// values (and twice the chunk).
+enum { IN_ORDER, GATHER, SCATTER };
+template <bool INT4, int ROWS, int PHASE>
 __global__ __launch_bounds__(256) void k_compact(const Compact a) {
-  __shared__ int64_t from[kRows + 4], to[kRows + 4];  // places in the cache, -1: none
+  constexpr int kUnits = ROWS / 16;  // vectors of 16 bytes a thread: rows are at most 256 bytes
+  __shared__ int64_t from[ROWS], to[ROWS];  // places in the cache, -1: none
   const int64_t b = blockIdx.y;
-  const int h = blockIdx.x;
-  Moves m;
-  bool bad;
-  const bool any = moves_of(a, b, &m, &bad);
-  const bool first = threadIdx.x == 0 && h == 0 && blockIdx.z == 0;
-  if (bad && first) atomicOr(a.c.refused, 1);
-  if (!any) return;
+  const int h = blockIdx.x, kind = blockIdx.z & 1, chunk = blockIdx.z >> 1;
+  const kv_seq q = kv_sequence(a.s, b);
+  const Moves m = PHASE == IN_ORDER ? moves_of(a, q, b) : a.moves[b];
+  if (PHASE == IN_ORDER && h == 0 && kind == 0 && threadIdx.x == 0) {
+    if (m.bad) atomicOr(a.c.refused, 1);
+    if (a.past_out) a.past_out[b] = a.s.past[b] + m.count;
+  }
+  if (m.j0 >= m.count) return;
   const int page = 1 << a.c.plog, mask = page - 1, heads = a.c.kv_heads;
   const int rb = a.c.dp * (INT4 ? 4 : 8) / 8;  // bytes of a vector's codes
   auto place = [&](int64_t pos) {
@@ -162,95 +169,116 @@ __global__ __launch_bounds__(256) void k_compact(const Compact a) {
     return id < 0 ? (int64_t)-1 : ((id * heads + h) << a.c.plog) + (pos & mask);
   };
   // Groups of four places, from the first that changes on.
-  const int64_t g0 = (m.q.past + m.j0) >> 2, g1 = ((int64_t)m.q.past + m.count + 3) >> 2;
-  for (int64_t g = g0; g < g1; g += kRows / 4) {
-    __syncthreads();
-    bool missing = false;
-    if (threadIdx.x < kRows) {
-      const int64_t pos = 4 * g + threadIdx.x, j = pos - m.q.past;
+  const int64_t g1 = ((int64_t)q.past + m.count + 3) >> 2;
+  int64_t g = ((q.past + m.j0) >> 2) + (PHASE == IN_ORDER ? 0 : (int64_t)chunk * (ROWS / 4));
+  const int64_t staged = ((b * heads + h) * 2 + kind) * a.chunks + chunk;
+  for (; g < g1; g += ROWS / 4) {
+    if (PHASE == IN_ORDER) __syncthreads();
+    if (threadIdx.x < ROWS) {
+      const int64_t pos = 4 * g + threadIdx.x, j = pos - q.past;
       int64_t t = -1, f = -1;
       if (j >= m.j0 && j < m.count) {
         t = place(pos);
-        f = place((int64_t)m.q.past + a.kept[m.q.start + j]);
-        missing = t < 0 || f < 0;
+        f = place((int64_t)q.past + a.kept[q.start + j]);
+        if (t < 0 || f < 0) {
+          t = f = -1;
+          atomicOr(a.c.refused, 1);
+        }
       }
-      to[threadIdx.x] = missing ? -1 : t;
-      from[threadIdx.x] = missing ? -1 : f;
+      to[threadIdx.x] = t;
+      from[threadIdx.x] = f;
     }
-    if (missing) atomicOr(a.c.refused, 1);
     __syncthreads();
-    // Scales, read now and written behind the barrier.
-    const int sc = (int)blockIdx.z + 2 * ((int)threadIdx.x / kRows), row = threadIdx.x % kRows;
-    const bool scaled = (INT4 || threadIdx.x < kRows) && to[row] >= 0;
-    // The scale of a place: (page, head) block, kind, token.
+    const int rows = (int)std::min<int64_t>(ROWS, 4 * (g1 - g)), units = rows * rb / 16;
+    // Scales: (page, head) block, kind, token.
+    const int sc = kind + 2 * ((int)threadIdx.x / ROWS), row = threadIdx.x % ROWS;
+    const bool scaled = (int)threadIdx.x < (INT4 ? 2 * ROWS : ROWS) && to[row] >= 0;
     auto scale = [&](int64_t at) {
       return a.c.sc + ((at >> a.c.plog) * kv_scales(a.c.fmt) + sc) * page + (at & mask);
     };
+    float *scale_ws = a.scales + staged * 2 * ROWS + threadIdx.x;
+    u32x4 *row_ws = reinterpret_cast<u32x4 *>(a.rows + staged * ROWS * rb) + threadIdx.x;
     float s = 0.f;
-    if (scaled) s = *scale(from[row]);
-    if (blockIdx.z == 0) {
-      const int vec = rb / 16;  // 2 .. 16
-      u32x4 x[8];
-      // (At most 2048 vectors of 16 bytes; rows that do not move read the cache's first.)
+    if (scaled) s = PHASE == SCATTER ? *scale_ws : *scale(from[row]);
+    u32x4 x[kUnits];
+    if (PHASE == SCATTER) {
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int i = 256 * u + threadIdx.x, r = i / vec;
-        const int64_t at = r < kRows && to[r] >= 0 ? from[r] * rb + 16 * (i - r * vec) : 0;
+      for (int u = 0; u < kUnits; u++)
+        if (256 * u < units) x[u] = row_ws[256 * u];
+    } else if (kind == 0) {
+      const int vec = rb / 16;
+#pragma unroll
+      for (int u = 0; u < kUnits; u++) {
+        if (256 * u >= units) break;
+        const int i = 256 * u + threadIdx.x, r = min(i / vec, ROWS - 1);
+        // (Rows that do not move read the cache's first.)
+        const int64_t at = to[r] >= 0 ? from[r] * rb + 16 * (i % vec) : 0;
         x[u] = *reinterpret_cast<const u32x4 *>(a.c.k + at);
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+    }
+    // Values: dwords of four tokens, those of rows that move from where they are, the others kept.
+    const int vec = rb / 4;  // vectors of four dwords of a group
+    // The group (four places lie together) that gets rows in this call, -1: none.
+    auto group = [&](int k) {
+      int64_t g4 = -1;
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int i = 256 * u + threadIdx.x, r = i / vec;
-        if (r < kRows && to[r] >= 0)
-          *reinterpret_cast<u32x4 *>(a.c.k + to[r] * rb + 16 * (i - r * vec)) = x[u];
-      }
-    } else {
-      // Dwords of four tokens: those of rows that move from where they are, the others kept.
-      const int vec = rb / 4;  // vectors of four dwords of a group: 8 .. 64
-      u32x4 x[8];
-      // The group (four places lie together) that gets rows in this call, -1: none.
-      auto group = [&](int q) {
-        int64_t g4 = -1;
+      for (int t = 0; t < 4; t++) g4 = std::max(g4, to[4 * k + t] >> 2);
+      return g4;
+    };
+    if (PHASE != SCATTER && kind == 1) {
 #pragma unroll
-        for (int t = 0; t < 4; t++) g4 = std::max(g4, to[4 * q + t] >> 2);
-        return g4;
-      };
-#pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int i = 256 * u + threadIdx.x, q = std::min(i / vec, kRows / 4 - 1), o = i % vec;
-        const int64_t own = std::max<int64_t>(group(q), 0);
+      for (int u = 0; u < kUnits; u++) {
+        if (256 * u >= units) break;
+        const int i = 256 * u + threadIdx.x, k = min(i / vec, ROWS / 4 - 1), o = i % vec;
+        const int64_t own = std::max<int64_t>(group(k), 0);
         x[u] = 0;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-          const int64_t at = to[4 * q + t] >= 0 ? from[4 * q + t] : 4 * own + t;
+          const int64_t at = to[4 * k + t] >= 0 ? from[4 * k + t] : 4 * own + t;
           const u32x4 w = *reinterpret_cast<const u32x4 *>(a.c.v + (at >> 2) * 4 * rb + 16 * o);
-          const int k = (int)(at & 3);
+          const int n = (int)(at & 3);
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[u][e] |= token_to<INT4>(token_of<INT4>(w[e], k), t);
+          for (int e = 0; e < 4; e++) x[u][e] |= token_to<INT4>(token_of<INT4>(w[e], n), t);
         }
       }
+    }
+    if (PHASE == GATHER) {
+      if (scaled) *scale_ws = s;
+#pragma unroll
+      for (int u = 0; u < kUnits; u++)
+        if (256 * u < units) row_ws[256 * u] = x[u];
+      return;
+    }
+    if (PHASE == IN_ORDER) {  // all read before any is written
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
+    }
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int i = 256 * u + threadIdx.x, q = i / vec, o = i % vec;
-        const int64_t own = q < kRows / 4 ? group(q) : -1;
-        if (own >= 0) *reinterpret_cast<u32x4 *>(a.c.v + own * 4 * rb + 16 * o) = x[u];
+    for (int u = 0; u < kUnits; u++) {
+      if (256 * u >= units) break;
+      const int i = 256 * u + threadIdx.x;
+      if (i >= units) break;
+      if (kind == 0) {
+        const int r = i / (rb / 16);
+        if (to[r] >= 0) *reinterpret_cast<u32x4 *>(a.c.k + to[r] * rb + 16 * (i % (rb / 16))) = x[u];
+      } else {
+        const int64_t own = group(i / vec);
+        if (own >= 0) *reinterpret_cast<u32x4 *>(a.c.v + own * 4 * rb + 16 * (i % vec)) = x[u];
       }
     }
     if (scaled) *scale(to[row]) = s;
+    if (PHASE == SCATTER) return;
   }
 }
 
-// (Its own launch: past_out may be the past that the moves read.)
-__global__ __launch_bounds__(256) void k_past(const Compact a) {
-  Moves m;
-  bool bad;
-  moves_of(a, blockIdx.x, &m, &bad);
-  if (threadIdx.x == 0)
-    a.past_out[blockIdx.x] = a.s.past[blockIdx.x] + (bad ? 0 : m.count);
+// The sequences' moves for the staged form, and their new lengths.
+__global__ __launch_bounds__(256) void k_moves(const Compact a) {
+  const int64_t b = blockIdx.x;
+  const Moves m = moves_of(a, kv_sequence(a.s, b), b);
+  if (threadIdx.x) return;
+  if (m.bad) atomicOr(a.c.refused, 1);
+  if (a.moves) a.moves[b] = m;
+  if (a.past_out) a.past_out[b] = a.s.past[b] + m.count;
 }
 
 // ---------------------------------------------------------- shared and free pages
@@ -482,6 +510,133 @@ __global__ __launch_bounds__(256) void k_fit_give(const Fit a) {
   }
 }
 
+// All of it but the copies by one workgroup: what few sequences and pages need, without the waits
+// between launches (4 sequences of 64 pages: 17 us in five launches, 12 so).
+constexpr int kOneBatch = 1024, kOnePages = 65536, kOneNeed = 8192;
+// A count that other waves change in this launch.
+__device__ inline int count_of(const int32_t *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
+  __shared__ int held[kOneBatch], mid[kOneBatch], need[kOneBatch], first[kOneBatch], free[kOneNeed];
+  __shared__ uint8_t copies[kOneBatch];  // as Fit's copy
+  __shared__ int64_t part[16];
+  __shared__ int count[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, batch = (int)a.s.batch;
+  const int64_t stride = a.s.table_stride;
+  // What is kept, a wave a sequence (as k_fit_held).
+  for (int b = wave; b < batch; b += 16) {
+    const kv_seq q = kv_sequence(a.s, b);
+    const int64_t want = wanted(a, q), full = ((int64_t)q.past + (1 << a.c.plog) - 1) >> a.c.plog;
+    const int32_t *row = a.table + b * stride;
+    bool bad = q.bad || want > stride, gap = false, shared = false;
+    int has = 0, keep = 0;  // pages before the first gap; before the first shared one behind the past
+    for (int64_t e0 = 0; !bad && e0 < want; e0 += 64) {
+      const int64_t e = e0 + lane;
+      const int id = e < want ? row[e] : -1;
+      const bool other = id >= 0 && id < a.c.pages && e >= full && a.refs[id] > 1;
+      const uint64_t no = __ballot(id < 0 && e < want), more = __ballot(other);
+      const int n = (int)std::min<int64_t>(64, want - e0);
+      bad = __any(id >= a.c.pages) || (gap && __any(id >= 0));
+      if (!gap) {
+        has += no ? __builtin_ctzll(no) : n;
+        // (None behind the gap.)
+        bad |= no && __any(id >= 0 && lane > __builtin_ctzll(no));
+      }
+      if (!shared) keep += more ? __builtin_ctzll(more) : n;
+      gap |= no != 0;
+      shared |= more != 0;
+    }
+    bad |= has < full;
+    if (lane == 0) {
+      held[b] = bad ? -1 : min(has, keep);
+      if (bad) atomicOr(a.c.refused, 1);
+    }
+  }
+  __syncthreads();
+  // What is let go.
+  for (int b = wave; b < batch; b += 16) {
+    int32_t *row = a.table + b * stride;
+    for (int64_t e = held[b] + lane; held[b] >= 0 && e < stride; e += 64) {
+      const int id = row[e];
+      if (id >= 0 && id < a.c.pages) atomicSub(a.refs + id, 1);
+      row[e] = -1;
+    }
+    if (lane == 0) {
+      const kv_seq q = kv_sequence(a.s, b);
+      const bool writes = held[b] >= 0 && q.n > 0 && (q.past & ((1 << a.c.plog) - 1)) != 0;
+      mid[b] = writes ? row[q.past >> a.c.plog] : -1;
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  // What is needed, in all and before each.
+  for (int b = wave; b < batch; b += 16) {
+    const int page = mid[b];
+    int earlier = 0;
+    for (int o0 = 0; page >= 0 && o0 < b; o0 += 64)
+      earlier += __popcll(__ballot(o0 + lane < b && mid[min(o0 + lane, b)] == page));
+    const int refs = page >= 0 ? count_of(a.refs + page) : 0;
+    const bool copy = page >= 0 && earlier + 1 < refs;
+    if (lane == 0) {
+      copies[b] = copy ? 1 : refs > 1 ? 2 : 0;
+      need[b] = held[b] < 0 ? 0 : (int)(wanted(a, kv_sequence(a.s, b)) - held[b]) + copy;
+    }
+  }
+  __syncthreads();
+  const int total = (int)scan_all(need, first, batch, part);
+  // The free pages that are needed, lowest first: four a thread.
+  int found = 0;
+  for (int64_t p0 = 0; p0 < a.c.pages && found < total; p0 += 4096) {
+    int is = 0, n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int64_t p = p0 + 4 * (int)threadIdx.x + k;
+      if (p < a.c.pages && count_of(a.refs + p) == 0) is |= 1 << k, n++;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) count[wave] = x;
+    __syncthreads();
+    int at = found + x - n;
+    for (int k = 0; k < 16; k++) {
+      if (k < wave) at += count[k];
+      found += count[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (is >> k & 1) {
+        if (at < total) free[at] = (int)(p0 + 4 * (int)threadIdx.x + k);
+        at++;
+      }
+  }
+  __syncthreads();
+  for (int b = wave; b < batch; b += 16) {
+    const int n = need[b], at = first[b], copy = copies[b] == 1;
+    const bool given = held[b] >= 0 && ((n == 0 && copies[b] == 0) || at + n <= found);
+    int32_t *row = a.table + b * stride;
+    if (lane == 0) {
+      a.granted[b] = given;
+      a.own[b] = given && copy ? free[at] : -1;
+      a.old[b] = mid[b];
+      if (given && copy) {
+        row[kv_sequence(a.s, b).past >> a.c.plog] = free[at];
+        a.refs[free[at]] = 1;
+        atomicSub(a.refs + mid[b], 1);
+      }
+    }
+    for (int i = copy + lane; given && i < n; i += 64) {
+      row[held[b] + i - copy] = free[at + i];
+      a.refs[free[at + i]] = 1;
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void k_fit_copy(const Fit a) {
   const int64_t b = blockIdx.y;
   const int own = a.own[b];
@@ -505,17 +660,58 @@ mg_status mg_kv_copy_run(mg_ctx *ctx, const mg_kv_cache &c, const int32_t *src, 
 }
 int64_t mg_kv_copy_groups(const mg_kv_cache &c, int64_t n) { return n * page_pieces(c); }
 
-mg_status mg_kv_compact_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
-                            const int32_t *kept, const int32_t *count, int32_t *past_out) {
-  const Compact a{c, s, kept, count, past_out};
-  const dim3 grid((unsigned)c.kv_heads, (unsigned)s.batch, 2);
-  if (s.max_new > 0) {
-    if (c.fmt == MG_KV_INT4)
-      k_compact<true><<<grid, dim3(256), 0, ctx->stream>>>(a);
+// Chunks of a sequence in the staged form.
+constexpr int kLong = 128;
+static int64_t compact_chunks(const mg_seq_batch &s) { return (s.max_new + 3 + kLong - 1) / kLong + 1; }
+size_t mg_kv_compact_ws(const mg_kv_cache &c, const mg_seq_batch &s) {
+  // Lists of up to 256 rows move in order, and what is beyond a launch.
+  const int64_t chunks = compact_chunks(s);
+  if (s.max_new <= 2 * kLong || chunks > 32767 || s.batch * c.kv_heads * 2 > MG_MOST_GROUPS / chunks) return 0;
+  const size_t parts = (size_t)s.batch * c.kv_heads * 2 * chunks;
+  return mg_align((size_t)s.batch * sizeof(Moves)) + parts * kLong * (c.dp * kv_bits(c.fmt) / 8 + 8);
+}
+
+template <bool INT4>
+static void compact(mg_ctx *ctx, Compact a, void *ws) {
+  const unsigned heads = (unsigned)a.c.kv_heads, batch = (unsigned)a.s.batch;
+  hipStream_t st = ctx->stream;
+  int32_t *past_out = a.past_out;
+  const bool alias = past_out == a.s.past;  // (written once nothing reads the past any more)
+  if (alias) a.past_out = nullptr;
+  if (a.s.max_new == 0) {
+    // No rows: the lengths alone.
+  } else if (!ws) {
+    const dim3 grid(heads, batch, 2);
+    if (a.s.max_new <= 32)
+      k_compact<INT4, 32, IN_ORDER><<<grid, dim3(256), 0, st>>>(a);
     else
-      k_compact<false><<<grid, dim3(256), 0, ctx->stream>>>(a);
+      k_compact<INT4, kLong, IN_ORDER><<<grid, dim3(256), 0, st>>>(a);
+  } else {
+    a.chunks = (int)compact_chunks(a.s);
+    char *p = static_cast<char *>(ws);
+    a.moves = reinterpret_cast<Moves *>(p);
+    p += mg_align((size_t)a.s.batch * sizeof(Moves));
+    a.scales = reinterpret_cast<float *>(p);
+    p += (size_t)a.s.batch * heads * 2 * a.chunks * kLong * 8;
+    a.rows = reinterpret_cast<uint8_t *>(p);
+    const dim3 grid(heads, batch, 2 * (unsigned)a.chunks);
+    k_moves<<<dim3(batch), dim3(256), 0, st>>>(a);
+    k_compact<INT4, kLong, GATHER><<<grid, dim3(256), 0, st>>>(a);
+    k_compact<INT4, kLong, SCATTER><<<grid, dim3(256), 0, st>>>(a);
   }
-  if (past_out) k_past<<<dim3((unsigned)s.batch), dim3(256), 0, ctx->stream>>>(a);
+  if (past_out && (alias || a.s.max_new == 0)) {
+    a.past_out = past_out;
+    k_moves<<<dim3(batch), dim3(256), 0, st>>>(a);
+  }
+}
+
+mg_status mg_kv_compact_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s,
+                            const int32_t *kept, const int32_t *count, int32_t *past_out, void *ws) {
+  const Compact a{c, s, kept, count, past_out, nullptr, nullptr, nullptr, 1};
+  if (c.fmt == MG_KV_INT4)
+    compact<true>(ctx, a, ws);
+  else
+    compact<false>(ctx, a, ws);
   return mg_launch_check("KV cache compact");
 }
 
@@ -544,6 +740,11 @@ mg_status mg_kv_fit_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s
   }
   const unsigned batch = (unsigned)s.batch;
   hipStream_t st = ctx->stream;
+  if (s.batch <= kOneBatch && c.pages <= kOnePages && s.batch * (s.table_stride + 1) <= kOneNeed) {
+    k_fit_one<<<dim3(1), dim3(1024), 0, st>>>(a);
+    k_fit_copy<<<dim3((unsigned)page_pieces(c), batch), dim3(256), 0, st>>>(a);
+    return mg_launch_check("KV cache fit");
+  }
   k_fit_held<<<dim3(batch), dim3(256), 0, st>>>(a);
   k_fit_release<<<dim3(batch), dim3(256), 0, st>>>(a);
   k_fit_need<<<dim3(batch + (unsigned)a.nrun), dim3(256), 0, st>>>(a);

@@ -157,7 +157,7 @@ __device__ inline void join(const mg_drafts_part *p, int nrun, double c, int lan
 __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   constexpr int kMost = MG_DRAFTS_MOST;
   __shared__ double s[kMost], qs[kMost], ep[kMost], eq[kMost];  // rows' sums; tokens' weights
-  __shared__ float m[kMost], qm[kMost];
+  __shared__ float m[kMost], qm[kMost], u01[kMost];
   __shared__ int token[kMost], parent[kMost], best[kMost];
   __shared__ bool again[kMost];  // a token that an earlier row after the same one has too
   __shared__ int kept_n;
@@ -179,6 +179,7 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   for (int i = threadIdx.x; i < q.n; i += 1024) {
     token[i] = d.tokens[q.start + i];
     parent[i] = d.parent ? d.parent[q.start + i] : i - 1;
+    u01[i] = d.uniform[q.start + i];
   }
   for (int i = wave; i < q.n; i += 16) {
     const int64_t row = q.start + i;
@@ -189,12 +190,12 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     if (greedy) {
       // The first logit that is the largest: in its run.
       const int64_t first = (int64_t)at * MG_DRAFTS_RUN;
-      const float *x = d.target + row * d.target_stride;
+      float x[kLane];
+      load(x, d.target + row * d.target_stride, first, d.vocab, lane);
       int here = 0x7fffffff;
-      for (int j = 0; j < kLane; j++) {
-        const int64_t e = first + 64 * j + lane;
-        if (e < d.vocab && here == 0x7fffffff && x[e] == top) here = (int)e;
-      }
+#pragma unroll
+      for (int j = kLane - 1; j >= 0; j--)
+        if (x[j] == top) here = (int)first + 256 * (j / 4) + 4 * lane + j % 4;
       here = wave_min(here);
       if (lane == 0) best[i] = here;
     }
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     for (int i = 1; i < q.n; i++) {
       if (parent[i] != cur) continue;
       const bool has = fabsf(m[cur]) < kInf;
-      const double u = (double)d.uniform[q.start + i], p = ep[i] / s[cur];
+      const double u = (double)u01[i], p = ep[i] / s[cur];
       bool stays = has && ep[i] > 0.0;
       if (greedy) {
         stays = has && token[i] == best[cur];
@@ -263,10 +264,10 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     const bool has = fabsf(m[cur]) < kInf;
     const bool drawn = greedy || !has;
     if (drawn) v.out[q.start + n - 1] = has ? best[cur] : -1;
-    last.s = s[cur];
-    last.qs = rest ? qs[cur] : 1.0;
+    last.s = 1.0 / s[cur];
+    last.qs = rest ? 1.0 / qs[cur] : 1.0;
     last.c = c;
-    last.u = (double)d.uniform[q.start];
+    last.u = (double)u01[0];
     last.m = m[cur];
     last.qm = rest ? qm[cur] : 0.f;
     last.row = q.start + cur;
@@ -286,36 +287,64 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
 
 // The weight left of a token with logits x and (mode 2) y.
 __device__ inline double left_of(const mg_drafts_last &l, int mode, float x, float y) {
-  const double p = weight(x, l.m, l.c) / l.s;
-  return mode == 2 ? fmax(p - weight(y, l.qm, l.c) / l.qs, 0.0) : p;
+  const double p = weight(x, l.m, l.c) * l.s;
+  return mode == 2 ? fmax(p - weight(y, l.qm, l.c) * l.qs, 0.0) : p;
 }
+// Of the runs' sums those of p without a rejected token are there already.
+__device__ inline double mass_of(const mg_drafts_part &p, const mg_drafts_last &l) {
+  return p.s * exp2_of(((double)p.m - (double)l.m) * l.c) * l.s;
+}
+
+constexpr int kOne = MG_DRAFTS_RUN / 256;  // logits of a thread of k_masses
 
 __global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
+  __shared__ double part[4];
+  __shared__ int list[MG_DRAFTS_MOST], listed;
   const mg_drafts &d = v.d;
   const int64_t b = blockIdx.y;
-  const mg_drafts_last l = v.last[b];
-  const int lane = threadIdx.x & 63;
-  const int run = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  if (l.mode == 0 || run >= v.nrun) return;
+  const mg_drafts_last &l = v.last[b];
+  const int mode = l.mode, rejected = l.rejected, run = blockIdx.x, lane = threadIdx.x & 63;
+  if (mode == 0 || (mode == 1 && rejected == 0)) return;
   const int64_t first = (int64_t)run * MG_DRAFTS_RUN;
-  float x[kLane], y[kLane] = {};
-  load(x, d.target + l.row * d.target_stride, first, d.vocab, lane);
-  if (l.mode == 2) load(y, d.draft + l.row * d.draft_stride, first, d.vocab, lane);
-  for (int r = 0; r < l.rejected; r++) {
-    const int64_t t = v.rej[l.first + r] - first;
-    if (t < 0 || t >= MG_DRAFTS_RUN) continue;
-#pragma unroll
-    for (int j = 0; j < kLane; j++)
-      if (256 * (j / 4) + 4 * lane + j % 4 == t) x[j] = -kInf;
+  const float *xr = d.target + l.row * d.target_stride, *yr = xr;
+  if (mode == 2) yr = d.draft + l.row * d.draft_stride;
+  if (mode == 1) {
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < rejected; r += 256) {
+      const int64_t t = v.rej[l.first + r] - first;
+      if (t >= 0 && t < MG_DRAFTS_RUN) list[atomicAdd(&listed, 1)] = (int)t;
+    }
+    __syncthreads();
+    if (listed == 0) {
+      if (threadIdx.x == 0) v.mass[b * v.nrun + run] = mass_of(v.part[l.row * v.nrun + run], l);
+      return;
+    }
   }
+  float x[kOne], y[kOne];
+#pragma unroll
+  for (int j = 0; j < kOne; j++) {
+    const int64_t e = first + 1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4;
+    x[j] = e < d.vocab ? xr[e] : -kInf;
+    y[j] = mode == 2 && e < d.vocab ? yr[e] : -kInf;
+  }
+  if (mode == 1)
+    for (int r = 0; r < listed; r++)
+#pragma unroll
+      for (int j = 0; j < kOne; j++)
+        if (1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4 == list[r]) x[j] = -kInf;
   double w = 0.0;
 #pragma unroll
-  for (int j = 0; j < kLane; j++) w += left_of(l, l.mode, x[j], y[j]);
+  for (int j = 0; j < kOne; j++) w += left_of(l, mode, x[j], y[j]);
   w = wave_sum(w);
-  if (lane == 0) v.mass[b * v.nrun + run] = w;
+  if (lane == 0) part[threadIdx.x >> 6] = w;
+  __syncthreads();
+  if (threadIdx.x == 0) v.mass[b * v.nrun + run] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-// The running sum over the workgroup's 256 threads before this one and up to it (the next one's
+constexpr int kPick = 1024;  // threads of k_pick
+
+// The running sum over the workgroup's threads before this one and up to it (the next one's
 // before is this one's up to, bit for bit), and the whole.
 struct Sums {
   double before, upto, all;
@@ -330,27 +359,32 @@ __device__ inline Sums scan(double x, double *part) {
   __syncthreads();
   if (lane == 63) part[wave] = x;
   __syncthreads();
-  double before = 0.0;
-  for (int k = 0; k < wave; k++) before += part[k];
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPick / 64; k++) {
+    if (k == wave) before = all;
+    all += part[k];
+  }
   const double y = __shfl_up(x, 1);
-  return Sums{lane ? before + y : before, before + x, part[0] + part[1] + part[2] + part[3]};
+  return Sums{lane ? before + y : before, before + x, all};
 }
 
-__global__ __launch_bounds__(256) void k_pick(const mg_verify v) {
-  constexpr int kOne = MG_DRAFTS_RUN / 256;
-  __shared__ double part[4], below;
+__global__ __launch_bounds__(kPick) void k_pick(const mg_verify v) {
+  constexpr int kEach = MG_DRAFTS_RUN / kPick;
+  __shared__ double part[kPick / 64], below;
   __shared__ int run, pick, highest;
+  __shared__ bool gone[MG_DRAFTS_RUN];
   const mg_drafts &d = v.d;
   const int64_t b = blockIdx.x;
-  const mg_drafts_last l = v.last[b];
+  const mg_drafts_last &l = v.last[b];
   if (l.mode == 0) return;
   int mode = l.mode;
-  const int per = (v.nrun + 255) / 256, r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
+  const int rejected = l.rejected;
+  const int per = (v.nrun + kPick - 1) / kPick;
+  const int r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
   const mg_drafts_part *parts = v.part + l.row * v.nrun;
-  // (mode 1 after the residual came out empty: p's own sums.)
   auto mass = [&](int r) {
-    return mode == l.mode ? v.mass[b * v.nrun + r]
-                          : parts[r].s * exp2_of(((double)parts[r].m - (double)l.m) * l.c) / l.s;
+    return mode == 1 && rejected == 0 ? mass_of(parts[r], l) : v.mass[b * v.nrun + r];
   };
   Sums sum;
   for (;;) {
@@ -362,6 +396,8 @@ __global__ __launch_bounds__(256) void k_pick(const mg_verify v) {
   }
   const double want = l.u * sum.all;
   if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) gone[kPick * j + threadIdx.x] = false;
   __syncthreads();
   // The first run whose running sum exceeds it, else (rounding) the last one that has any.
   if (sum.upto > want && sum.before <= want) {
@@ -388,34 +424,41 @@ __global__ __launch_bounds__(256) void k_pick(const mg_verify v) {
     return;
   }
   const bool end = highest >= 0;
-  const int64_t first = (int64_t)run * MG_DRAFTS_RUN + kOne * threadIdx.x;
+  const int64_t first = (int64_t)run * MG_DRAFTS_RUN;
+  for (int r = threadIdx.x; r < rejected; r += kPick) {
+    const int64_t t = v.rej[l.first + r] - first;
+    if (t >= 0 && t < MG_DRAFTS_RUN) gone[t] = true;
+  }
   const float *x = d.target + l.row * d.target_stride;
   const float *y = mode == 2 ? d.draft + l.row * d.draft_stride : x;
-  double w[kOne], own = 0.0;
+  double w[kEach], own = 0.0;
 #pragma unroll
-  for (int j = 0; j < kOne; j++) {
-    const int64_t e = first + j;
+  for (int j = 0; j < kEach; j++) {
+    const int64_t e = first + kEach * (int)threadIdx.x + j;
     w[j] = e < d.vocab ? left_of(l, mode, x[e], y[e]) : 0.0;
   }
-  for (int r = 0; r < l.rejected; r++) {
-    const int64_t t = v.rej[l.first + r] - first;
-#pragma unroll
-    for (int j = 0; j < kOne; j++)
-      if (t == j) w[j] = 0.0;
-  }
-#pragma unroll
-  for (int j = 0; j < kOne; j++) own += w[j];
   __syncthreads();
   if (threadIdx.x == 0) highest = -1;
-  double at = below + scan(own, part).before;
 #pragma unroll
-  for (int j = 0; j < kOne; j++) {
+  for (int j = 0; j < kEach; j++) {
+    if (gone[kEach * threadIdx.x + j]) w[j] = 0.0;
+    own += w[j];
+  }
+  double at = below + scan(own, part).before;
+  int top = -1, here = 0x7fffffff;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
     at += w[j];
     if (w[j] > 0.0) {
-      atomicMax(&highest, kOne * (int)threadIdx.x + j);
-      if (!end && at > want) atomicMin(&pick, kOne * (int)threadIdx.x + j);
+      top = kEach * (int)threadIdx.x + j;
+      if (!end && at > want) here = min(here, top);
     }
   }
+  // (Tokens rise with the lanes: the last lane that has any, the first that is beyond.)
+  const uint64_t any = __ballot(top >= 0), beyond = __ballot(here < 0x7fffffff);
+  const int lane = threadIdx.x & 63;
+  if (any && lane == 63 - __builtin_clzll(any)) atomicMax(&highest, top);
+  if (beyond && lane == __builtin_ctzll(beyond)) atomicMin(&pick, here);
   __syncthreads();
   if (threadIdx.x == 0) {
     const int in = pick < 0x7fffffff ? pick : highest;
@@ -450,7 +493,7 @@ mg_status mg_verify_run(mg_ctx *ctx, const mg_verify &v) {
   }
   k_stats<<<dim3(runs, (unsigned)(d.max_new * (d.draft ? 2 : 1)), (unsigned)d.batch), dim3(256), 0, st>>>(v);
   k_walk<<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
-  k_masses<<<dim3(runs, (unsigned)d.batch), dim3(256), 0, st>>>(v);
-  k_pick<<<dim3((unsigned)d.batch), dim3(256), 0, st>>>(v);
+  k_masses<<<dim3((unsigned)v.nrun, (unsigned)d.batch), dim3(256), 0, st>>>(v);
+  k_pick<<<dim3((unsigned)d.batch), dim3(kPick), 0, st>>>(v);
   return mg_launch_check("VerifyDrafts");
 }

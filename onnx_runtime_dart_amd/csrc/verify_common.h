@@ -13,7 +13,7 @@ struct mg_drafts_part {
 };
 // Where a sequence's last token is drawn, and by what.
 struct mg_drafts_last {
-  double s, qs, c, u;  // sums of p's and q's row, log2(e) / temperature, the random number
+  double s, qs, c, u;  // 1 / the sums of p's and q's row, log2(e) / temperature, the random number
   float m, qm;         // maxima of the rows
   int64_t row;
   int32_t mode;     // 0: it is drawn already; 1: by p without the rejected tokens; 2: max(p - q, 0)
