@@ -927,7 +927,8 @@ typedef struct mg_adapters mg_adapters;
 
 /* slots empty slots (rank 0) for ranks up to max_rank (1 .. 256), n projections K -> N[i].  Values
  * are held in fp32, or rounded once to fp16 (those beyond its range become infinite).  Memory:
- * slots * max_rank * (n K + sum N) values, K and N padded to multiples of 8. */
+ * slots * max_rank * (n K + sum N) values, K and N padded to multiples of 8 and, of sum N,
+ * max_rank to one of 32. */
 mg_status mg_adapters_create(mg_ctx *ctx, int64_t K, int32_t n, const int64_t *N, int64_t slots,
                              int64_t max_rank, int32_t format, mg_adapters **out);
 /* Waits for the device, then frees.  NULL: MG_INVALID_ARGUMENT. */

@@ -21,8 +21,15 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;   // rows of a tile
 constexpr int kCols = 64;   // values of A's rows that a workgroup takes
-constexpr int kOuts = 512;  // outputs that a workgroup takes
-constexpr int64_t kFew = 96;
+constexpr int kOuts = 256;  // outputs that a workgroup takes at least
+// Few rows: up to 512, and 1.2 10^8 multiply-adds.  Measured where both take as long (all rows of one
+// slot / of 64 slots in turn): 2048 -> 2048 by 64, 450 and 384 rows (9 and 9 us at 32 against 25 and 26
+// sorted); 2048 -> 2 x 8192 by 64, 105 and 200; by 16, 300 and 350; 1024 -> 4096 by 8, beyond 512.
+inline bool few_rows(const mg_adapters &h, int64_t rows) {
+  int64_t out = 0;
+  for (int i = 0; i < h.n; i++) out += h.N[i];
+  return rows <= 512 && rows * h.max_rank <= (int64_t)120000000 / (h.n * h.K + out);
+}
 
 // Four adjacent floats at any address of 4 bytes.
 struct __attribute__((packed, aligned(4))) Four {
@@ -54,23 +61,33 @@ __device__ inline f32x4 weights<_Float16>(const _Float16 *p) {
 
 // ------------------------------------------------------------- filling slots
 
+struct Fill {
+  mg_adapters h;
+  const float *a[MG_ADAPTER_MOST], *b[MG_ADAPTER_MOST];
+  int64_t slot;
+  int rank;
+  float factor;
+};
+// blockIdx.z: A [rank, K], as it is, and B [N, rank] to [rank][np] with zeros up to a multiple of 32
+// ranks, of each projection in turn; blockIdx.y: the rank.
 template <class T>
-__global__ __launch_bounds__(256) void k_fill_a(const float *src, T *dst, int64_t K, int64_t kp) {
-  const int64_t j = blockIdx.y;
-  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < kp; k += (int64_t)gridDim.x * 256)
-    dst[j * kp + k] = (T)(k < K ? src[j * K + k] : 0.f);
-}
-// B [N, rank] to [rank][np].
-template <class T>
-__global__ __launch_bounds__(256) void k_fill_b(const float *src, T *dst, int64_t N, int64_t np, int rank) {
-  const int64_t j = blockIdx.y;
-  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < np; n += (int64_t)gridDim.x * 256)
-    dst[j * np + n] = (T)(n < N ? src[n * rank + j] : 0.f);
-}
-// (Behind the values, on the same stream: nothing reads a rank without them.)
-__global__ void k_fill_slot(int32_t *rank, float *factor, int32_t r, float f) {
-  *rank = r;
-  *factor = f;
+__global__ __launch_bounds__(256) void k_fill(const Fill f) {
+  const int i = blockIdx.z >> 1, j = blockIdx.y;
+  const mg_adapters &h = f.h;
+  if (blockIdx.x + blockIdx.y + blockIdx.z == 0 && threadIdx.x == 0) {
+    h.rank[f.slot] = f.rank;
+    h.factor[f.slot] = f.factor;
+  }
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  if (blockIdx.z & 1) {
+    if (j >= (f.rank + 31) / 32 * 32) return;
+    T *dst = static_cast<T *>(h.b) + f.slot * h.b_slot + h.b_off[i] + j * h.np[i];
+    for (int64_t n = first; n < h.np[i]; n += step)
+      dst[n] = (T)(n < h.N[i] && j < f.rank ? f.b[i][n * f.rank + j] : 0.f);
+  } else if (j < f.rank) {
+    T *dst = static_cast<T *>(h.a) + f.slot * h.a_slot + ((int64_t)i * h.max_rank + j) * h.kp;
+    for (int64_t k = first; k < h.kp; k += step) dst[k] = (T)(k < h.K ? f.a[i][j * h.K + k] : 0.f);
+  }
 }
 __global__ __launch_bounds__(256) void k_empty(int32_t *rank, float *factor, int64_t n) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -142,8 +159,14 @@ __global__ __launch_bounds__(64) void k_up_few(const mg_adapt p, const float *t)
 
 // Rows in the order of their slots, and tiles of it.  Buckets: the slots, none, beyond.
 struct Tile {
-  int slot, start, count, unused;
+  int slot, start, count, rank;
 };
+// (Loads of what stores might change are not scalar by themselves: a tile is made so, and with it
+// every address that begins at its adapter.)
+__device__ inline Tile uniform(const Tile &t) {
+  return Tile{__builtin_amdgcn_readfirstlane(t.slot), __builtin_amdgcn_readfirstlane(t.start),
+              __builtin_amdgcn_readfirstlane(t.count), __builtin_amdgcn_readfirstlane(t.rank)};
+}
 struct Order {
   int32_t *row;  // [rows]
   Tile *tile;    // [most_tiles]
@@ -175,14 +198,21 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
   };
   // (Eight loads ahead: their latency bounds this.)
   constexpr int kAhead = 8;
+  int s[kAhead];
+  bool there = false;
   auto each = [&](auto place) {
     for (int r0 = threadIdx.x; r0 - (int)threadIdx.x < rows; r0 += 1024 * kAhead) {
-      int s[kAhead];
+      // (The second time they are there, if these are all.)
+      if (!there || rows > 1024 * kAhead) {
 #pragma unroll
-      for (int i = 0; i < kAhead; i++) s[i] = p.slot[min(r0 + 1024 * i, rows - 1)];
+        for (int i = 0; i < kAhead; i++) s[i] = p.slot[min(r0 + 1024 * i, rows - 1)];
+      }
+      there = true;
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
-        const int r = r0 + 1024 * i, to = places(s[i], r < rows);
+        const int r = r0 + 1024 * i;
+        if (r - (int)threadIdx.x >= rows) break;
+        const int to = places(s[i], r < rows);
         if (r < rows) place(r, to);
       }
     }
@@ -217,9 +247,10 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
     }
     const int start = before + x - n;
     next += y - m;
-    const int slot = b >= buckets - 1 ? -2 : b == buckets - 2 || n == 0 || p.h.rank[b] == 0 ? -1 : b;
+    const int rank = n && b < buckets - 2 ? p.h.rank[b] : 0;
+    const int slot = b >= buckets - 1 ? -2 : rank == 0 ? -1 : b;
     for (int k = 0; k < m; k++)
-      o.tile[next + k] = Tile{slot, start + k * kTile, min(kTile, n - k * kTile), 0};
+      o.tile[next + k] = Tile{slot, start + k * kTile, min(kTile, n - k * kTile), rank};
     if (b < buckets) lds[b] = start;
   }
   if (threadIdx.x == 0) *o.tiles = tiles;
@@ -228,179 +259,272 @@ __global__ __launch_bounds__(1024) void k_sort(const mg_adapt p, const Order o) 
 }
 
 // Part of t[sorted row][rank * projection + value] of a tile: K's share of blockIdx.y, values
-// from kCols * blockIdx.z on.  VEC: K is a multiple of four.
+// from kCols * blockIdx.z on.  VEC: K is a multiple of four.  Rows and values pass through shared
+// memory 32 k at a time (read from memory by the lines: with operands straight from it every
+// instruction touches 64 lines, 110 us and not 65 for 8191 rows of 2048 by 128 values); the
+// next 32 k are on their way meanwhile.
 template <class T, bool VEC>
-__global__ __launch_bounds__(256, 2) void k_down(const mg_adapt p, const Order o, float *t, int64_t share,
+__global__ __launch_bounds__(256, 4) void k_down(const mg_adapt p, const Order o, float *t, int64_t share,
                                                  int64_t cols) {
-  constexpr int kDeep = 4;  // steps of eight k that are loaded ahead
-  __shared__ float sums[4][64][64];
-  if ((int)blockIdx.x >= *o.tiles) return;
-  const Tile tile = o.tile[blockIdx.x];
-  if (tile.slot < 0) return;
-  const int rank = p.h.rank[tile.slot], all = rank * p.h.n, c0 = kCols * blockIdx.z;
+  constexpr int kK = 32, kPad = kK + 4;  // (rows 4 banks apart from each other's multiples: no conflicts)
+  __shared__ float xs[kTile * kPad], as[kCols * kPad];
+  const int tiles = *o.tiles;  // (asked for with the tile: there is one in the list for every workgroup)
+  const Tile tile = uniform(o.tile[blockIdx.x]);
+  if ((int)blockIdx.x >= tiles || tile.slot < 0) return;
+  const int rank = tile.rank, all = rank * p.h.n, c0 = kCols * blockIdx.z;
   if (c0 >= all) return;
   const int lane = threadIdx.x & 63, hi = lane >> 5, l = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int K = (int)p.h.K;
-  const float *x[2];
-  const T *a[2];
+  const int K = (int)p.h.K, first = (int)(share * blockIdx.y), end = (int)std::min(first + share, p.h.kp);
+  // A thread brings four k of rows and of values r + 32 u.
+  constexpr int kU = kTile / 32;
+  const int r = threadIdx.x >> 3, part = 4 * (threadIdx.x & 7);
+  const float *x[kU];
+  const T *a[kU];
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    x[u] = p.x + (int64_t)o.row[tile.start + min(32 * u + l, tile.count - 1)] * K;
-    const int c = min(c0 + 32 * u + l, all - 1), i = c / rank;
+  for (int u = 0; u < kU; u++) {
+    x[u] = p.x + (int64_t)o.row[tile.start + min(32 * u + r, tile.count - 1)] * K;
+    const int c = min(c0 + 32 * u + r, all - 1), i = c / rank;
     a[u] = static_cast<const T *>(p.h.a) + tile.slot * p.h.a_slot +
            ((int64_t)i * p.h.max_rank + c - i * rank) * p.h.kp;
   }
-  f32x16 acc[2][2] = {};
-  const int first = (int)(share * blockIdx.y), end = (int)std::min(first + share, p.h.kp);
-  // WIDE: a second block of 32 values.  A step is eight k, four for each half of the wave; the four
-  // waves take steps in turn.
-  auto products = [&](auto wide) {
-    constexpr int W = decltype(wide)::value;
-#pragma unroll 1
-    for (int k0 = first + 8 * wave; k0 < end; k0 += 32 * kDeep) {
-      f32x4 xv[kDeep][2], av[kDeep][W];
+  f32x4 xv[kU], av[kU];
+  auto load = [&](int k0) {
+    const int k = k0 + part;
 #pragma unroll
-      for (int i = 0; i < kDeep; i++) {
-        // (Steps past the end read the last one; x and A count as 0 there.)
-        const int k = min(k0 + 32 * i, end - 8) + 4 * hi;
+    for (int u = 0; u < kU; u++) {
+      // (Past the end: the last ones, where x and A count as 0.)
+      if (VEC) {
+        xv[u] = load4(x[u] + min(k, K - 4));
+      } else {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          if (VEC) {
-            xv[i][u] = load4(x[u] + min(k, K - 4));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) xv[i][u][e] = x[u][min(k + e, K - 1)];
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < W; w++) av[i][w] = weights(a[w] + k);
+        for (int e = 0; e < 4; e++) xv[u][e] = x[u][min(k + e, K - 1)];
       }
+      av[u] = weights(a[u] + min(k, end - 4));
+    }
+    if (k0 + kK > std::min(end, K)) {
 #pragma unroll
-      for (int i = 0; i < kDeep; i++) {
-        const int k = k0 + 32 * i + 4 * hi;
+      for (int u = 0; u < kU; u++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          float xe[2], ae[W];
-#pragma unroll
-          for (int u = 0; u < 2; u++) xe[u] = k + e < K && k < end ? xv[i][u][e] : 0.f;
-#pragma unroll
-          for (int w = 0; w < W; w++) ae[w] = k < end ? av[i][w][e] : 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int w = 0; w < W; w++)
-              acc[u][w] = __builtin_amdgcn_mfma_f32_32x32x2f32(xe[u], ae[w], acc[u][w], 0, 0, 0);
+          xv[u][e] = k + e < K && k < end ? xv[u][e] : 0.f;
+          av[u][e] = k < end ? av[u][e] : 0.f;
         }
-      }
     }
   };
-  if (c0 + 32 < all)
-    products(std::integral_constant<int, 2>());
-  else
-    products(std::integral_constant<int, 1>());
+  // More than 32 values: a wave takes one block of 32 rows by 32 values; else half of the k of one.
+  const bool wide = c0 + 32 < all;
+  const int rows0 = 32 * (wave & 1), cols0 = wide ? 32 * (wave >> 1) : 0;
+  // (A wave whose rows the tile does not have only brings operands.)
+  const int s0 = wide ? 0 : 2 * (wave >> 1), s1 = rows0 >= tile.count ? 0 : wide ? 4 : s0 + 2;
+  const float *xl = xs + (rows0 + l) * kPad + 4 * hi, *al = as + (cols0 + l) * kPad + 4 * hi;
+  f32x16 acc = {};
+  load(first);
+  for (int k0 = first; k0 < end; k0 += kK) {
+    __syncthreads();
 #pragma unroll
-  for (int u = 0; u < 2; u++)
+    for (int u = 0; u < kU; u++) {
+      *reinterpret_cast<f32x4 *>(xs + (32 * u + r) * kPad + part) = xv[u];
+      *reinterpret_cast<f32x4 *>(as + (32 * u + r) * kPad + part) = av[u];
+    }
+    __syncthreads();
+    if (k0 + kK < end) load(k0 + kK);
 #pragma unroll
-    for (int w = 0; w < 2; w++)
+    for (int s = 0; s < 4; s++) {
+      if (s < s0 || s >= s1) continue;
+      const f32x4 xe = *reinterpret_cast<const f32x4 *>(xl + 8 * s);
+      const f32x4 ae = *reinterpret_cast<const f32x4 *>(al + 8 * s);
 #pragma unroll
-      for (int e = 0; e < 16; e++) sums[wave][(2 * u + w) * 16 + e][lane] = acc[u][w][e];
-  __syncthreads();
+      for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(xe[e], ae[e], acc, 0, 0, 0);
+    }
+  }
   const float f = p.h.factor[tile.slot];
   t += (int64_t)blockIdx.y * p.rows * cols;
-  for (int r = wave; r < 64; r += 4) {
-    const int u = r / 32, w = r / 16 % 2, e = r % 16;
-    const int row = 32 * u + 8 * (e / 4) + 4 * hi + e % 4, c = c0 + 32 * w + l;
-    const float v = (sums[0][r][lane] + sums[1][r][lane]) + (sums[2][r][lane] + sums[3][r][lane]);
-    if (row < tile.count && c < all) t[(tile.start + row) * cols + c] = v * f;
+  if (!wide) {
+    __syncthreads();
+    if (wave >= 2) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) xs[((wave & 1) * 16 + e) * 64 + lane] = acc[e];
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] += xs[(wave * 16 + e) * 64 + lane];
+  }
+  const int c = c0 + cols0 + l;
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+    const int row = rows0 + 8 * (e / 4) + 4 * hi + e % 4;
+    if (row < tile.count && c < all) t[(tile.start + row) * cols + c] = acc[e] * f;
   }
 }
 
-// Outputs of a tile: kOuts of them of projection blockIdx.z, in blocks of 32 a wave.  stride: of the
-// tile's values in shared memory (odd; kHeld of them at a time, rounded up to 32 with zeros).
-constexpr int kHeld = 128;
+// Outputs of a tile: `outs` of them of projection blockIdx.z, 32 a wave at a time.  Products change
+// lanes through the wave's own part of shared memory, so that base and y are read and written 16
+// bytes a lane and a line of a row at once; waves wait for each other only at the start.  The base
+// of the next block is on its way during a block's products.  stride: of the tile's values in
+// shared memory (odd; kHeld of them at a time, rounded up to 32 with zeros).
+constexpr int kHeld = 128, kTurn = 36;
 template <class T>
 __global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, const float *t, int parts,
-                                               int64_t cols, int stride) {
+                                               int64_t cols, int stride, int outs) {
   extern __shared__ float low[];
-  __shared__ int row_of[kTile];
-  if ((int)blockIdx.x >= *o.tiles) return;
-  const Tile tile = o.tile[blockIdx.x];
-  const int z = blockIdx.z;
-  const int64_t N = p.h.N[z], np = p.h.np[z], n0 = (int64_t)kOuts * blockIdx.y;
+  __shared__ float turns[4][32 * kTurn];
+  __shared__ int64_t row_of[kTile];  // where the rows' outputs begin
+  const int tiles = *o.tiles;
+  const Tile tile = uniform(o.tile[blockIdx.y]);
+  // The projection and its outputs (all chunks of all projections side by side: a grid with empty
+  // places gives some XCDs less to do).
+  int z = 0, chunk = blockIdx.x;
+  while (z + 1 < p.h.n && chunk >= (int)((p.h.N[z] + outs - 1) / outs)) chunk -= (int)((p.h.N[z++] + outs - 1) / outs);
+  const int64_t N = p.h.N[z], np = p.h.np[z], n0 = (int64_t)outs * chunk;
   const float *base = p.base[z];
   float *y = p.y[z];
-  if (n0 >= N || (tile.slot == -1 && base == y)) return;
+  if ((int)blockIdx.y >= tiles || (tile.slot == -1 && base == y)) return;
+  const int64_t last = std::min(n0 + outs, N);  // of the workgroup's outputs
   const int lane = threadIdx.x & 63, hi = lane >> 5, l = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int rank = tile.slot >= 0 ? p.h.rank[tile.slot] : 0, steps = (rank + 31) / 32;
-  if (threadIdx.x < kTile) row_of[threadIdx.x] = o.row[tile.start + min((int)threadIdx.x, tile.count - 1)];
-  auto stage = [&](int j1) {
-    const int n = min(kHeld, 32 * steps - j1);
+  if (threadIdx.x < kTile)
+    row_of[threadIdx.x] = o.row[tile.start + min((int)threadIdx.x, tile.count - 1)] * N;
+  if (tile.slot < 0) {
     __syncthreads();
-    for (int i = threadIdx.x; i < kTile * n; i += 256) {
-      const int r = i / n, j = i % n;
-      float v = 0.f;
-      if (r < tile.count && j1 + j < rank)
-        for (int part = 0; part < parts; part++)
-          v += t[((int64_t)part * p.rows + tile.start + r) * cols + z * rank + j1 + j];
-      low[r * stride + j] = v;
-    }
-    __syncthreads();
+    for (int r = wave; r < tile.count; r += 4)
+      for (int64_t n = n0 + lane; n < last; n += 64)
+        y[row_of[r] + n] = tile.slot == -1 ? base[row_of[r] + n] : __builtin_nanf("");
+    return;
+  }
+  const int rank = tile.rank;
+  const T *b = static_cast<const T *>(p.h.b) + tile.slot * p.h.b_slot + p.h.b_off[z];
+  // A lane's outputs of a block: four of rows r8 + 8 i.
+  const int r8 = lane >> 3, part4 = 4 * (lane & 7);
+  struct Block {
+    f32x4 v[8];
   };
-  stage(0);
-  const T *b = static_cast<const T *>(p.h.b) + (int64_t)std::max(tile.slot, 0) * p.h.b_slot + p.h.b_off[z];
-  const float *own = low + l * stride + hi;
-#pragma unroll 1
-  for (int q = 0; q < kOuts / 128; q++) {
-    const int64_t at = n0 + 128 * q + 32 * wave, n = std::min(at + l, N - 1);
-    if (at >= N && rank <= kHeld) break;  // (else it takes part in what follows)
-    float v[2][16];
+  auto load_base = [&](const float *from, int64_t at) {
+    Block v;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int i = 0; i < 8; i++) v.v[i] = load4(from + row_of[r8 + 8 * i] + at + part4);
+    return v;
+  };
+  struct Weights {
+    float w[16];
+  };
+  // Weights of 32 ranks from j0 on (past the rank: zeros), by one address a lane and 16 scalar ones.
+  auto load_weights = [&](int n, int j0) {
+    Weights w;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T *>(b + j0 * np), (short)0, (int)(uint32_t)std::min<int64_t>(32 * np * (int)sizeof(T), 0x7ffffff0),
+        0x00020000);
+    const unsigned at = (unsigned)(hi * (int)np + n) * (unsigned)sizeof(T);
 #pragma unroll
-      for (int e = 0; e < 16; e++)
-        v[u][e] = base[(int64_t)row_of[32 * u + 8 * (e / 4) + 4 * hi + e % 4] * N + n];
-    f32x16 acc[2] = {};
-#pragma unroll 1
-    for (int j0 = 0; j0 < 32 * steps; j0 += 32) {
-      if (rank > kHeld && j0 % kHeld == 0) stage(j0);
-      float w[16];
-      // (Past the rank: its last row, then 0, which no infinity of B turns into NaN.)
-#pragma unroll
-      for (int j = 0; j < 16; j++) w[j] = (float)b[(int64_t)min(j0 + 2 * j + hi, rank - 1) * np + n];
-      if (j0 + 32 > rank) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) w[j] = j0 + 2 * j + hi < rank ? w[j] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 16; j++)
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-          acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(own[32 * u * stride + j0 % kHeld + 2 * j], w[j], acc[u], 0, 0, 0);
+    for (int j = 0; j < 16; j++) {
+      const unsigned row = (unsigned)(2 * j) * (unsigned)np * (unsigned)sizeof(T);
+      if (sizeof(T) == 4)
+        w.w[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, row, 0));
+      else
+        w.w[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, row, 0));
     }
-    if (at + l >= N) continue;
+    return w;
+  };
+  const float *own = low + l * stride + hi;
+  auto products = [&](const Weights &w, int j0, f32x16 (&acc)[2]) {
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int j = 0; j < 16; j++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int r = 32 * u + 8 * (e / 4) + 4 * hi + e % 4;
-        const float sum = tile.slot == -2 ? __builtin_nanf("") : rank ? v[u][e] + acc[u][e] : v[u][e];
-        if (r < tile.count) y[(int64_t)row_of[r] * N + n] = sum;
+      for (int u = 0; u < 2; u++)
+        acc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(own[32 * u * stride + j0 + 2 * j], w.w[j], acc[u], 0, 0, 0);
+  };
+  float *turn = turns[wave];
+  // (Ranks beyond kHeld are added in rounds: to the base, then to what a lane wrote itself.)
+#pragma unroll 1
+  for (int j1 = 0; j1 < rank; j1 += kHeld) {
+    const int j2 = min(j1 + kHeld, rank);
+    __syncthreads();
+    // The tile's values: 32 of each row at a time, eight a thread.
+#pragma unroll 1
+    for (int j0 = j1; j0 < j2; j0 += 32) {
+      const int j = j0 + l;
+      float v[8] = {};
+#pragma unroll 2
+      for (int part = 0; part < parts; part++) {
+        const float *from = t + ((int64_t)part * p.rows + tile.start) * cols + z * rank;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          v[i] += from[(uint32_t)(min(2 * wave + hi + 8 * i, tile.count - 1) * (int)cols + min(j, rank - 1))];
       }
+#pragma unroll
+      for (int i = 0; i < 8; i++) low[(2 * wave + hi + 8 * i) * stride + j - j1] = j < rank ? v[i] : 0.f;
+    }
+    __syncthreads();
+    const float *from = j1 ? y : base;
+    int64_t at = n0 + 32 * wave;
+    // (A block of less than 32 outputs, the last one, reads its base at the end.)
+    Block v = {};
+    if (at + 32 <= last) v = load_base(from, at);
+#pragma unroll 1
+    for (; at < last; at += 128) {
+      asm volatile("" ::: "memory");  // (the tile's values stay in shared memory: registers are for loads)
+      const int col = (int)std::min(at + l, N - 1);
+      const Weights w0 = load_weights(col, j1);
+      Weights w1 = w0;
+      if (j1 + 32 < j2) w1 = load_weights(col, j1 + 32);
+      Block next = v;
+      if (at + 160 <= last) next = load_base(from, at + 128);
+      f32x16 acc[2] = {};
+      products(w0, 0, acc);
+      if (j1 + 32 < j2) products(w1, 32, acc);
+#pragma unroll 1
+      for (int j0 = j1 + 64; j0 < j2; j0 += 32) products(load_weights(col, j0), j0 - j1, acc);
+      const int64_t n = at + part4;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < 16; e++) turn[(8 * (e / 4) + 4 * hi + e % 4) * kTurn + l] = acc[u][e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (at + 32 <= last) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int r = 32 * u + r8 + 8 * i;
+            const f32x4 s = v.v[4 * u + i] + *reinterpret_cast<const f32x4 *>(turn + (r8 + 8 * i) * kTurn + part4);
+            if (r < tile.count)
+              *reinterpret_cast<Four *>(y + row_of[r] + n) = Four{{s[0], s[1], s[2], s[3]}};
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 16; i++) {
+            const int r = 32 * u + 2 * i + hi;
+            const int64_t e = row_of[r] + at + l;
+            if (r < tile.count && at + l < last) y[e] = from[e] + turn[(2 * i + hi) * kTurn + l];
+          }
+        }
+      }
+      v = next;
+    }
   }
 }
 
 int64_t most_tiles(const mg_adapters &h, int64_t rows) {
   return rows / kTile + std::min<int64_t>(h.slots + 2, rows);
 }
-// The share of K of a workgroup, so that tiles fill the card twice over.
+// The share of K of a workgroup: as many as are at work together (four a CU), 256 at least.
 int64_t k_share(const mg_ctx *ctx, const mg_adapters &h, int64_t rows, int *parts) {
   const int64_t groups = (rows + kTile - 1) / kTile * ((h.n * h.max_rank + kCols - 1) / kCols);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * ctx->num_cus / groups, h.kp / 256));
-  const int64_t share = ((h.kp + want - 1) / want + 31) / 32 * 32;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(4 * ctx->num_cus / groups, h.kp / 256));
+  const int64_t share = ((h.kp + want - 1) / want + 127) / 128 * 128;
   *parts = (int)((h.kp + share - 1) / share);
   return share;
+}
+
+// The outputs of a workgroup: so many that its start (its rows and their values) costs little, so
+// few that there are workgroups enough (three a CU at work together).
+int64_t up_outs(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
+  int64_t all = 0;
+  for (int i = 0; i < h.n; i++) all += (h.N[i] + 127) / 128;
+  const int64_t blocks = (rows + kTile - 1) / kTile * all / (3 * ctx->num_cus);
+  return 128 * std::max<int64_t>(2, std::min<int64_t>(blocks, 16));
 }
 
 template <class T>
@@ -410,7 +534,7 @@ void run(mg_ctx *ctx, const mg_adapt &p, void *ws) {
   const unsigned rows = (unsigned)p.rows;
   int64_t most = 0;
   for (int i = 0; i < h.n; i++) most = std::max(most, h.N[i]);
-  if (p.rows <= kFew) {
+  if (few_rows(h, p.rows)) {
     float *t = static_cast<float *>(ws);
     k_down_few<T><<<dim3((unsigned)((h.n * h.max_rank + 3) / 4), rows), dim3(256), 0, st>>>(p, t);
     k_up_few<T><<<dim3((unsigned)((most + 255) / 256), rows, (unsigned)h.n), dim3(64), 0, st>>>(p, t);
@@ -435,22 +559,11 @@ void run(mg_ctx *ctx, const mg_adapt &p, void *ws) {
   else
     k_down<T, false><<<grid, dim3(256), 0, st>>>(p, o, t, share, cols);
   const int stride = std::min((h.max_rank + 31) / 32 * 32, kHeld) + 1;
-  k_up<T><<<dim3((unsigned)tiles, (unsigned)((most + kOuts - 1) / kOuts), (unsigned)h.n), dim3(256),
-            (size_t)kTile * stride * 4, st>>>(p, o, t, parts, cols, stride);
-}
-
-template <class T>
-void fill(mg_ctx *ctx, const mg_adapters &h, int64_t slot, int64_t rank, const float *const *a,
-          const float *const *b) {
-  for (int i = 0; i < h.n; i++) {
-    T *ad = static_cast<T *>(h.a) + slot * h.a_slot + (int64_t)i * h.max_rank * h.kp;
-    T *bd = static_cast<T *>(h.b) + slot * h.b_slot + h.b_off[i];
-    const auto grid = [&](int64_t n) {
-      return dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1024), (unsigned)rank);
-    };
-    k_fill_a<T><<<grid(h.kp), dim3(256), 0, ctx->stream>>>(a[i], ad, h.K, h.kp);
-    k_fill_b<T><<<grid(h.np[i]), dim3(256), 0, ctx->stream>>>(b[i], bd, h.N[i], h.np[i], (int)rank);
-  }
+  const int64_t outs = up_outs(ctx, h, p.rows);
+  int64_t chunks = 0;
+  for (int i = 0; i < h.n; i++) chunks += (h.N[i] + outs - 1) / outs;
+  k_up<T><<<dim3((unsigned)chunks, (unsigned)tiles), dim3(256),
+            (size_t)kTile * stride * 4, st>>>(p, o, t, parts, cols, stride, (int)outs);
 }
 
 }  // namespace
@@ -465,7 +578,7 @@ size_t mg_adapt_ws(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
   rows = std::min(rows, MG_ADAPT_ROWS);
   const size_t cols = (size_t)h.n * h.max_rank;
   // (A last round of few rows needs no more than a whole one.)
-  if (rows <= kFew) return mg_align((size_t)rows * cols * 4);
+  if (few_rows(h, rows)) return mg_align((size_t)rows * cols * 4);
   int parts;
   k_share(ctx, h, rows, &parts);
   return mg_align((size_t)rows * 4) + 256 + mg_align((size_t)most_tiles(h, rows) * sizeof(Tile)) +
@@ -482,13 +595,19 @@ mg_status mg_adapt_run(mg_ctx *ctx, const mg_adapt &p, void *ws) {
 
 mg_status mg_adapters_fill(mg_ctx *ctx, const mg_adapters &h, int64_t slot, int64_t rank,
                            const float *const *a, const float *const *b, float factor) {
-  if (rank) {
-    if (h.fmt == MG_ADAPTER_F16)
-      fill<_Float16>(ctx, h, slot, rank, a, b);
-    else
-      fill<float>(ctx, h, slot, rank, a, b);
+  Fill f{h, {}, {}, slot, (int)rank, factor};
+  int64_t most = h.kp;
+  for (int i = 0; i < h.n; i++) {
+    f.a[i] = rank ? a[i] : nullptr;
+    f.b[i] = rank ? b[i] : nullptr;
+    most = std::max(most, h.np[i]);
   }
-  k_fill_slot<<<dim3(1), dim3(1), 0, ctx->stream>>>(h.rank + slot, h.factor + slot, (int32_t)rank, factor);
+  const dim3 grid((unsigned)std::min<int64_t>((most + 255) / 256, 64), (unsigned)std::max<int64_t>(1, (rank + 31) / 32 * 32),
+                  (unsigned)(2 * h.n));
+  if (h.fmt == MG_ADAPTER_F16)
+    k_fill<_Float16><<<grid, dim3(256), 0, ctx->stream>>>(f);
+  else
+    k_fill<float><<<grid, dim3(256), 0, ctx->stream>>>(f);
   return mg_launch_check("Adapters fill");
 }
 

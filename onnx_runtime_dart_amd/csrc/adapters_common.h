@@ -9,7 +9,8 @@ constexpr int64_t MG_ADAPTER_SLOTS = 4096;
 
 // Values are fp32 or fp16; per slot A [projection][rank][kp] and, per projection, B transposed
 // [rank][np] (so that neighbouring outputs are neighbours), K and N padded to multiples of 8 with
-// zeros.  Rows from a slot's own rank on hold anything.
+// zeros.  Beyond a slot's own rank A's rows hold anything; B has room for ranks up to a multiple
+// of 32, and zeros up to the one that the slot's own reaches.
 struct mg_adapters {
   int device = 0, fmt = 0, n = 0, max_rank = 0;
   int64_t K = 0, kp = 0, slots = 0, bytes = 0;

@@ -3191,11 +3191,12 @@ mg_status mg_adapters_create(mg_ctx *ctx, int64_t K, int32_t n, const int64_t *N
   h.kp = (K + 7) / 8 * 8;
   h.slots = slots;
   for (int i = 0; i < n; i++) {
-    if (N[i] < 1 || N[i] > most) return bad_arg(what, "N must be 1 .. 2^24");
+    // (32 ranks of fp32 stay below 2^31 bytes.)
+    if (N[i] < 1 || N[i] > most / 2) return bad_arg(what, "N must be 1 .. 2^23");
     h.N[i] = N[i];
     h.np[i] = (N[i] + 7) / 8 * 8;
     h.b_off[i] = h.b_slot;
-    h.b_slot += max_rank * h.np[i];
+    h.b_slot += (max_rank + 31) / 32 * 32 * h.np[i];
   }
   h.a_slot = n * max_rank * h.kp;
   const size_t el = format == MG_ADAPTER_F16 ? 2 : 4;

@@ -139,17 +139,30 @@ __global__ __launch_bounds__(256) void k_stats(const mg_verify v) {
 // A row's maximum and sum from its runs', by a wave; *at: the first run with the maximum.
 __device__ inline void join(const mg_drafts_part *p, int nrun, double c, int lane, float *m, double *s,
                             int *at) {
-  float top = -kInf;
+  constexpr int kHeld = 2;  // runs that a lane keeps: vocabularies of up to 262144 are read once
+  float top = -kInf, hm[kHeld];
+  double hs[kHeld];
   int first = 0x7fffffff;
-  for (int r = lane; r < nrun; r += 64) {
-    const float y = p[r].m;
+  auto with = [&](int r, float y) {
     if (y > top || first == 0x7fffffff) first = r;
     top = fmaxf(top, y);
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) {
+    const mg_drafts_part q = p[min(lane + 64 * i, nrun - 1)];
+    hm[i] = q.m;
+    hs[i] = lane + 64 * i < nrun ? q.s : 0.0;
   }
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (lane + 64 * i < nrun) with(lane + 64 * i, hm[i]);
+  for (int r = lane + 64 * kHeld; r < nrun; r += 64) with(r, p[r].m);
   const float all = wave_max(top);
   *at = wave_min(top == all ? first : 0x7fffffff);
   double sum = 0.0;
-  for (int r = lane; r < nrun; r += 64) sum += p[r].s * exp2_of(((double)p[r].m - (double)all) * c);
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) sum += hs[i] * exp2_of(((double)hm[i] - (double)all) * c);
+  for (int r = lane + 64 * kHeld; r < nrun; r += 64) sum += p[r].s * exp2_of(((double)p[r].m - (double)all) * c);
   *m = all;
   *s = wave_sum(sum);
 }
@@ -321,21 +334,43 @@ __global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
       return;
     }
   }
-  float x[kOne], y[kOne];
+  float x[kOne], y[kOne] = {};
+  if (first + MG_DRAFTS_RUN <= d.vocab) {
+    const int64_t at = first + 4 * (int)threadIdx.x;
+    Four v4[kOne / 4], u4[kOne / 4];
 #pragma unroll
-  for (int j = 0; j < kOne; j++) {
-    const int64_t e = first + 1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4;
-    x[j] = e < d.vocab ? xr[e] : -kInf;
-    y[j] = mode == 2 && e < d.vocab ? yr[e] : -kInf;
+    for (int j = 0; j < kOne / 4; j++) v4[j] = *reinterpret_cast<const Four *>(xr + at + 1024 * j);
+    if (mode == 2) {
+#pragma unroll
+      for (int j = 0; j < kOne / 4; j++) u4[j] = *reinterpret_cast<const Four *>(yr + at + 1024 * j);
+#pragma unroll
+      for (int j = 0; j < kOne; j++) y[j] = u4[j / 4].x[j % 4];
+    }
+#pragma unroll
+    for (int j = 0; j < kOne; j++) x[j] = v4[j / 4].x[j % 4];
+  } else {
+#pragma unroll
+    for (int j = 0; j < kOne; j++) {
+      const int64_t e = first + 1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4;
+      x[j] = e < d.vocab ? xr[e] : -kInf;
+      y[j] = e < d.vocab ? yr[e] : -kInf;
+    }
   }
   if (mode == 1)
     for (int r = 0; r < listed; r++)
 #pragma unroll
       for (int j = 0; j < kOne; j++)
         if (1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4 == list[r]) x[j] = -kInf;
+  // (The sequence's numbers once: its record is not read again for every logit.)
+  const mg_drafts_last one = l;
   double w = 0.0;
+  if (mode == 2) {
 #pragma unroll
-  for (int j = 0; j < kOne; j++) w += left_of(l, mode, x[j], y[j]);
+    for (int j = 0; j < kOne; j++) w += left_of(one, 2, x[j], y[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kOne; j++) w += left_of(one, 1, x[j], y[j]);
+  }
   w = wave_sum(w);
   if (lane == 0) part[threadIdx.x >> 6] = w;
   __syncthreads();

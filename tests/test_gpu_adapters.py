@@ -72,7 +72,7 @@ def inputs(rng, h, rows):
 @pytest.mark.parametrize("fmt", ["f32", "f16"])
 @pytest.mark.parametrize("k, ns, max_rank", [(1, [1], 1), (7, [5, 9], 3), (64, [64], 8), (130, [33, 100, 7], 16),
                                              (1024, [256, 130], 33), (515, [513], 64), (96, [40], 256)])
-@pytest.mark.parametrize("rows", [1, 3, 96, 97, 160, 700])
+@pytest.mark.parametrize("rows", [1, 3, 160, 512, 513, 700])
 def test_sizes(ops, fmt, k, ns, max_rank, rows):
     rng = np.random.default_rng(k + rows)
     h, held = adapters(ops, rng, k, ns, 6, max_rank, fmt)
@@ -81,7 +81,7 @@ def test_sizes(ops, fmt, k, ns, max_rank, rows):
     check(h.apply(x, slots, bases), x, slots, bases, held)
 
 
-@pytest.mark.parametrize("rows", [40, 64, 65, 127, 128, 129, 1025])
+@pytest.mark.parametrize("rows", [40, 65, 513, 575, 576, 577, 640, 1025])
 def test_prompts_and_tokens(ops, rows):
     # Runs of one slot, single rows between, all rows of one slot, none.
     rng = np.random.default_rng(rows)
@@ -90,6 +90,17 @@ def test_prompts_and_tokens(ops, rows):
     for slots in (np.sort(rng.integers(-1, 12, rows)), rng.integers(0, 12, rows), np.full(rows, 5),
                   np.full(rows, -1), np.where(np.arange(rows) % 64 == 63, 3, 7), np.full(rows, 12)):
         check(h.apply(x, slots, bases), x, slots, bases, held)
+
+
+@pytest.mark.parametrize("k, ns, rank, rows", [(2048, [2048], 59, 490), (2048, [2048], 61, 490),
+                                               (4096, [5000, 5000], 128, 60)])
+def test_wide_adapters(ops, k, ns, rank, rows):
+    # Few rows of many multiply-adds: on both sides of where they are sorted.
+    rng = np.random.default_rng(rank)
+    h, held = adapters(ops, rng, k, ns, 3, rank, ranks=[rank, rank - 1, 1])
+    x, bases = inputs(rng, h, rows)
+    slots = rng.integers(-1, 3, rows)
+    check(h.apply(x, slots, bases), x, slots, bases, held)
 
 
 def test_many_slots(ops):
@@ -118,7 +129,7 @@ def test_rounds_of_rows(ops):
     np.testing.assert_array_equal(got[none], bases[0][none])
 
 
-@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("rows", [5, 600])
 def test_rows_without_an_adapter_are_the_base(ops, rows):
     rng = np.random.default_rng(3)
     h, held = adapters(ops, rng, 64, [100], 2, 4, ranks=[4, 0])
@@ -132,7 +143,7 @@ def test_rows_without_an_adapter_are_the_base(ops, rows):
     assert np.isnan(got[~none]).all()
 
 
-@pytest.mark.parametrize("rows", [7, 200])
+@pytest.mark.parametrize("rows", [7, 520])
 def test_values_that_are_not_finite_stay_with_their_rows(ops, rows):
     rng = np.random.default_rng(4)
     h, held = adapters(ops, rng, 50, [40], 3, 5, ranks=[5, 3, 4])
@@ -153,7 +164,7 @@ def test_values_that_are_not_finite_stay_with_their_rows(ops, rows):
 
 
 @pytest.mark.parametrize("fmt", ["f32", "f16"])
-@pytest.mark.parametrize("rows", [9, 150])
+@pytest.mark.parametrize("rows", [9, 550])
 def test_slots_filled_anew(ops, fmt, rows):
     # Of larger and smaller ranks than before, Infinity among what is left behind.
     rng = np.random.default_rng(5)
@@ -180,7 +191,7 @@ def test_rounding_to_fp16(ops):
     np.testing.assert_array_equal(got[0], [1, 1 + 2.0**-9, 65504, np.inf, 0, 2.0**-23])
 
 
-@pytest.mark.parametrize("rows", [6, 400])
+@pytest.mark.parametrize("rows", [6, 600])
 def test_device_calls(ops, rows):
     # In place, apart, from device weights, at odd addresses, rows behind left alone.
     rng = np.random.default_rng(6)
@@ -208,7 +219,7 @@ def test_device_calls(ops, rows):
     check(h.apply(x, slots, bases), x, slots, bases, held)
 
 
-@pytest.mark.parametrize("rows", [12, 333])
+@pytest.mark.parametrize("rows", [12, 1560])
 def test_captured_graph(ops, rows):
     # Slots, rows' slots and inputs change between replays; another graph shares the workspace.
     rng = np.random.default_rng(7)
@@ -251,7 +262,7 @@ def test_beside_a_shared_projection(ops):
         ws.append(ops.NBitsWeight(q, rng.uniform(0.002, 0.02, (n, k // 32)).astype(np.float32), k=k, n=n,
                                   block_size=32))
     h, held = adapters(ops, rng, k, ns, 5, 8)
-    for rows in (4, 130):
+    for rows in (4, 530):
         x = rng.standard_normal((rows, k)).astype(np.float32)
         slots = rng.integers(-1, 5, rows)
         shared = [w(x) for w in ws]
@@ -264,7 +275,7 @@ def test_beside_a_shared_projection(ops):
         check(got, x, slots, shared, held)
 
 
-@pytest.mark.parametrize("rows", [20, 500])
+@pytest.mark.parametrize("rows", [20, 800])
 def test_repeated_calls_are_equal(ops, rows):
     rng = np.random.default_rng(9)
     h, held = adapters(ops, rng, 300, [200], 7, 16)

@@ -105,7 +105,7 @@ def apply(x=P, rows=3, slot=P, base=pointers(P, P), y=pointers(P, P), h=ADAPTERS
 
 def test_adapters_out_of_bounds():
     assert create(k=0) == create(k=2**24 + 1) == create(n=0) == create(n=5, ns=[8] * 5) == create(ns=[0]) == 1
-    assert create(ns=[2**24 + 1]) == create(slots=0) == create(slots=4097) == create(rank=0) == 1
+    assert create(ns=[2**23 + 1]) == create(slots=0) == create(slots=4097) == create(rank=0) == 1
     assert create(rank=257) == create(fmt=2) == create(fmt=-1) == create(ctx=None) == 1
     for call in (lib.mg_adapters_set, lib.mg_adapters_set_dev):
         assert put(slot=-1, call=call) == put(slot=4, call=call) == put(rank=-1, call=call) == 1
