@@ -511,64 +511,89 @@ __global__ __launch_bounds__(256) void k_fit_give(const Fit a) {
 }
 
 // All of it but the copies by one workgroup: what few sequences and pages need, without the waits
-// between launches (4 sequences of 64 pages: 17 us in five launches, 12 so).
-constexpr int kOneBatch = 1024, kOnePages = 65536, kOneNeed = 8192;
+// between launches, every table entry in a register of its own (64 sequences of 64 pages: 15
+// us, 21 in the kernels of their own and as many waits; 4 sequences: 11 and 17).
+constexpr int kOneBatch = 1024, kOnePages = 65536, kOneNeed = 8192, kOneEach = kOneNeed / 1024;
 // A count that other waves change in this launch.
 __device__ inline int count_of(const int32_t *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
-  __shared__ int held[kOneBatch], mid[kOneBatch], need[kOneBatch], first[kOneBatch], free[kOneNeed];
-  __shared__ uint8_t copies[kOneBatch];  // as Fit's copy
+  // Of each sequence: its page of the first new row, if that falls into the middle, else -1; pages
+  // wanted, full of the past (the last one too), held; the first gap and the first shared page.
+  __shared__ int mid[kOneBatch], want[kOneBatch], full[kOneBatch], gap[kOneBatch], other[kOneBatch];
+  __shared__ int need[kOneBatch], first[kOneBatch], free[kOneNeed];
+  __shared__ uint8_t bad[kOneBatch], copies[kOneBatch];  // copies: as Fit's copy
   __shared__ int64_t part[16];
   __shared__ int count[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, batch = (int)a.s.batch;
-  const int64_t stride = a.s.table_stride;
-  // What is kept, a wave a sequence (as k_fit_held).
-  for (int b = wave; b < batch; b += 16) {
-    const kv_seq q = kv_sequence(a.s, b);
-    const int64_t want = wanted(a, q), full = ((int64_t)q.past + (1 << a.c.plog) - 1) >> a.c.plog;
-    const int32_t *row = a.table + b * stride;
-    bool bad = q.bad || want > stride, gap = false, shared = false;
-    int has = 0, keep = 0;  // pages before the first gap; before the first shared one behind the past
-    for (int64_t e0 = 0; !bad && e0 < want; e0 += 64) {
-      const int64_t e = e0 + lane;
-      const int id = e < want ? row[e] : -1;
-      const bool other = id >= 0 && id < a.c.pages && e >= full && a.refs[id] > 1;
-      const uint64_t no = __ballot(id < 0 && e < want), more = __ballot(other);
-      const int n = (int)std::min<int64_t>(64, want - e0);
-      bad = __any(id >= a.c.pages) || (gap && __any(id >= 0));
-      if (!gap) {
-        has += no ? __builtin_ctzll(no) : n;
-        // (None behind the gap.)
-        bad |= no && __any(id >= 0 && lane > __builtin_ctzll(no));
-      }
-      if (!shared) keep += more ? __builtin_ctzll(more) : n;
-      gap |= no != 0;
-      shared |= more != 0;
-    }
-    bad |= has < full;
-    if (lane == 0) {
-      held[b] = bad ? -1 : min(has, keep);
-      if (bad) atomicOr(a.c.refused, 1);
-    }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, me = threadIdx.x;
+  const int batch = (int)a.s.batch, stride = (int)a.s.table_stride;
+  // The table's entries, eight a thread.
+  int id[kOneEach], refs[kOneEach];
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) {
+    const int at = me + 1024 * i;
+    id[i] = at < batch * stride ? a.table[at] : -1;
+  }
+  // A sequence a thread.
+  kv_seq q = {};
+  if (me < batch) {
+    q = kv_sequence(a.s, me);
+    const int64_t w = wanted(a, q);
+    bad[me] = q.bad || w > stride;
+    want[me] = bad[me] ? 0 : (int)w;
+    full[me] = bad[me] ? 0 : (int)(((int64_t)q.past + (1 << a.c.plog) - 1) >> a.c.plog);
+    gap[me] = other[me] = want[me];
+    // (For now the entry, which a sequence that is not refused keeps.)
+    mid[me] = q.n > 0 && (q.past & ((1 << a.c.plog) - 1)) != 0 ? q.past >> a.c.plog : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) refs[i] = id[i] >= 0 && id[i] < a.c.pages ? a.refs[id[i]] : 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) {
+    const int at = me + 1024 * i;
+    if (at >= batch * stride) break;
+    const int b = at / stride, e = at - b * stride;
+    if (e >= want[b]) continue;
+    if (id[i] < 0) atomicMin(gap + b, e);
+    if (id[i] >= a.c.pages) bad[b] = 1;
+    if (e >= full[b] && refs[i] > 1) atomicMin(other + b, e);
   }
   __syncthreads();
-  // What is let go.
-  for (int b = wave; b < batch; b += 16) {
-    int32_t *row = a.table + b * stride;
-    for (int64_t e = held[b] + lane; held[b] >= 0 && e < stride; e += 64) {
-      const int id = row[e];
-      if (id >= 0 && id < a.c.pages) atomicSub(a.refs + id, 1);
-      row[e] = -1;
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) {  // (nothing behind a gap)
+    const int at = me + 1024 * i;
+    if (at >= batch * stride) break;
+    const int b = at / stride, e = at - b * stride;
+    if (e < want[b] && e > gap[b] && id[i] >= 0) bad[b] = 1;
+  }
+  __syncthreads();
+  if (me < batch) {
+    if (gap[me] < full[me]) bad[me] = 1;
+    if (bad[me]) atomicOr(a.c.refused, 1);
+    gap[me] = bad[me] ? -1 : min(gap[me], other[me]);  // what it keeps
+    need[me] = -1;
+  }
+  __syncthreads();
+  const int *held = gap;
+  // What is let go; the pages in whose middle rows begin.
+#pragma unroll
+  for (int i = 0; i < kOneEach; i++) {
+    const int at = me + 1024 * i;
+    if (at >= batch * stride) break;
+    const int b = at / stride, e = at - b * stride;
+    if (held[b] < 0) continue;
+    if (e < held[b]) {
+      if (e == mid[b]) need[b] = id[i];
+      continue;
     }
-    if (lane == 0) {
-      const kv_seq q = kv_sequence(a.s, b);
-      const bool writes = held[b] >= 0 && q.n > 0 && (q.past & ((1 << a.c.plog) - 1)) != 0;
-      mid[b] = writes ? row[q.past >> a.c.plog] : -1;
-    }
+    if (id[i] >= 0 && id[i] < a.c.pages) atomicSub(a.refs + id[i], 1);
+    a.table[at] = -1;
   }
   __threadfence();
+  __syncthreads();
+  if (me < batch) mid[me] = need[me];  // the page
   __syncthreads();
   // What is needed, in all and before each.
   for (int b = wave; b < batch; b += 16) {
@@ -576,24 +601,29 @@ __global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
     int earlier = 0;
     for (int o0 = 0; page >= 0 && o0 < b; o0 += 64)
       earlier += __popcll(__ballot(o0 + lane < b && mid[min(o0 + lane, b)] == page));
-    const int refs = page >= 0 ? count_of(a.refs + page) : 0;
-    const bool copy = page >= 0 && earlier + 1 < refs;
-    if (lane == 0) {
-      copies[b] = copy ? 1 : refs > 1 ? 2 : 0;
-      need[b] = held[b] < 0 ? 0 : (int)(wanted(a, kv_sequence(a.s, b)) - held[b]) + copy;
-    }
+    if (lane == 0) need[b] = earlier;
+  }
+  __syncthreads();
+  if (me < batch) {
+    const int r = mid[me] >= 0 ? count_of(a.refs + mid[me]) : 0;
+    const bool copy = mid[me] >= 0 && need[me] + 1 < r;
+    copies[me] = copy ? 1 : r > 1 ? 2 : 0;
+    need[me] = held[me] < 0 ? 0 : want[me] - held[me] + copy;
   }
   __syncthreads();
   const int total = (int)scan_all(need, first, batch, part);
   // The free pages that are needed, lowest first: four a thread.
   int found = 0;
   for (int64_t p0 = 0; p0 < a.c.pages && found < total; p0 += 4096) {
-    int is = 0, n = 0;
+    int is = 0, n = 0, c[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const int64_t p = p0 + 4 * (int)threadIdx.x + k;
-      if (p < a.c.pages && count_of(a.refs + p) == 0) is |= 1 << k, n++;
+      const int64_t p = p0 + 4 * me + k;
+      c[k] = p < a.c.pages ? count_of(a.refs + p) : 1;
     }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (c[k] == 0) is |= 1 << k, n++;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -611,29 +641,35 @@ __global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
 #pragma unroll
     for (int k = 0; k < 4; k++)
       if (is >> k & 1) {
-        if (at < total) free[at] = (int)(p0 + 4 * (int)threadIdx.x + k);
+        if (at < total) free[at] = (int)(p0 + 4 * me + k);
         at++;
       }
   }
   __syncthreads();
-  for (int b = wave; b < batch; b += 16) {
-    const int n = need[b], at = first[b], copy = copies[b] == 1;
-    const bool given = held[b] >= 0 && ((n == 0 && copies[b] == 0) || at + n <= found);
-    int32_t *row = a.table + b * stride;
-    if (lane == 0) {
-      a.granted[b] = given;
-      a.own[b] = given && copy ? free[at] : -1;
-      a.old[b] = mid[b];
-      if (given && copy) {
-        row[kv_sequence(a.s, b).past >> a.c.plog] = free[at];
-        a.refs[free[at]] = 1;
-        atomicSub(a.refs + mid[b], 1);
-      }
+  if (me < batch) {
+    const bool copy = copies[me] == 1;
+    const bool given = held[me] >= 0 && ((need[me] == 0 && copies[me] == 0) || first[me] + need[me] <= found);
+    a.granted[me] = given;
+    a.own[me] = given && copy ? free[first[me]] : -1;
+    a.old[me] = mid[me];
+    bad[me] = !given;
+    if (given && copy) atomicSub(a.refs + mid[me], 1);
+  }
+  __syncthreads();
+  for (int g = me; g < min(total, found); g += 1024) {
+    // The last sequence whose pages begin at g or before.
+    int lo = 0, hi = batch;
+    while (hi - lo > 1) {
+      const int at = (lo + hi) / 2;
+      if (first[at] <= g) lo = at;
+      else hi = at;
     }
-    for (int i = copy + lane; given && i < n; i += 64) {
-      row[held[b] + i - copy] = free[at + i];
-      a.refs[free[at + i]] = 1;
-    }
+    const int at = g - first[lo];
+    if (bad[lo] || at >= need[lo]) continue;
+    const bool copy = copies[lo] == 1;
+    const int e = copy && at == 0 ? full[lo] - 1 : held[lo] + at - copy;
+    a.table[(int64_t)lo * stride + e] = free[g];
+    a.refs[free[g]] = 1;
   }
 }
 

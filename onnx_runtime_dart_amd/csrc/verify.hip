@@ -7,9 +7,10 @@
 // 32 one draw in a hundred would take a neighbour.
 //
 //   k_stats   (m, s) of every run of 2048 logits, one wave each: the pass over all logits
-//   k_walk    a sequence's rows joined, its drafted tokens tried in order (a workgroup each)
-//   k_masses  the weights left in each run of the one row that the last token is drawn from
-//   k_pick    the run, and the token in it, that the random number falls into
+//   k_walk    a sequence's rows joined, its drafted tokens tried in order (a workgroup each); without
+//             draft logits it also draws the last token, from the runs' sums that are there
+//   k_masses  with them: the weights left in each run of the one row that it is drawn from
+//   k_pick    and the run, and the token in it, that the random number falls into
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -87,20 +88,54 @@ __device__ inline void load(float (&x)[kLane], const float *row, int64_t first, 
   }
 }
 
-__device__ inline double wave_sum(double x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+// x of another lane by a register move (`none` where there is none, or the row takes no part).
+template <int CTRL, int ROWS = 0xf>
+__device__ inline int moved(int x, int none) {
+  return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false);
 }
+template <int CTRL, int ROWS = 0xf>
+__device__ inline double moved(double x) {
+  const uint64_t u = __double_as_longlong(x);
+  const uint32_t lo = (uint32_t)moved<CTRL, ROWS>((int)(uint32_t)u, 0);
+  const uint32_t hi = (uint32_t)moved<CTRL, ROWS>((int)(uint32_t)(u >> 32), 0);
+  return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+// Running sums over the wave: within rows of 16 lanes, then across them (0x142, 0x143: a row's last
+// lane to the next row's, the second row's to the last two).
+__device__ inline double wave_scan(double x) {
+  x += moved<0x111>(x);
+  x += moved<0x112>(x);
+  x += moved<0x114>(x);
+  x += moved<0x118>(x);
+  x += moved<0x142, 0xa>(x);
+  return x + moved<0x143, 0xc>(x);
+}
+__device__ inline double lane63(double x) {
+  const uint64_t u = __double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+  return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+__device__ inline double wave_sum(double x) { return lane63(wave_scan(x)); }
 __device__ inline float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+  const int none = (int)__float_as_uint(-kInf);
+  auto with = [&](int y) { x = fmaxf(x, __uint_as_float((uint32_t)y)); };
+  with(moved<0x111>((int)__float_as_uint(x), none));
+  with(moved<0x112>((int)__float_as_uint(x), none));
+  with(moved<0x114>((int)__float_as_uint(x), none));
+  with(moved<0x118>((int)__float_as_uint(x), none));
+  with(moved<0x142>((int)__float_as_uint(x), none));
+  with(moved<0x143>((int)__float_as_uint(x), none));
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
 }
 __device__ inline int wave_min(int x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = min(x, __shfl_xor(x, o));
-  return x;
+  x = min(x, moved<0x111>(x, 0x7fffffff));
+  x = min(x, moved<0x112>(x, 0x7fffffff));
+  x = min(x, moved<0x114>(x, 0x7fffffff));
+  x = min(x, moved<0x118>(x, 0x7fffffff));
+  x = min(x, moved<0x142>(x, 0x7fffffff));
+  x = min(x, moved<0x143>(x, 0x7fffffff));
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 __global__ __launch_bounds__(256) void k_stats(const mg_verify v) {
@@ -167,22 +202,191 @@ __device__ inline void join(const mg_drafts_part *p, int nrun, double c, int lan
   *s = wave_sum(sum);
 }
 
+// The weight left of a token with logits x and (mode 2) y.
+__device__ inline double left_of(const mg_drafts_last &l, int mode, float x, float y) {
+  const double p = weight(x, l.m, l.c) * l.s;
+  return mode == 2 ? fmax(p - weight(y, l.qm, l.c) * l.qs, 0.0) : p;
+}
+// A run's sum of p's weights.
+__device__ inline double mass_of(const mg_drafts_part &p, const mg_drafts_last &l) {
+  return p.s * exp2_of(((double)p.m - (double)l.m) * l.c) * l.s;
+}
+
+constexpr int kPick = 1024;  // threads that draw a token
+
+// The running sum over the workgroup's threads before this one and up to it (the next one's
+// before is this one's up to, bit for bit), and the whole.
+struct Sums {
+  double before, upto, all;
+};
+__device__ inline Sums scan(double x, double *part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x = wave_scan(x);
+  __syncthreads();
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int k = 0; k < kPick / 64; k++) {
+    if (k == wave) before = all;
+    all += part[k];
+  }
+  // (0x138: the value of the lane before, 0 for the first.)
+  return Sums{before + moved<0x138>(x), before + x, all};
+}
+
+// Tokens without weight (shared memory), and room for the sums of their runs without them.
+struct Gone {
+  const int *token;
+  int *run;
+  double (*mass)[MG_DRAFTS_MOST];  // of each quarter of the run
+  int n;
+};
+// The last token of a sequence, by the whole workgroup (kPick threads).
+__device__ inline void draw_token(const mg_verify &v, const mg_drafts_last &l, int64_t b, const Gone &gone) {
+  constexpr int kEach = MG_DRAFTS_RUN / kPick;
+  __shared__ double part[kPick / 64], below;
+  __shared__ int run, pick, highest;
+  const mg_drafts &d = v.d;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float *x = d.target + l.row * d.target_stride;
+  // Runs of tokens without weight are summed again, a wave a quarter (of tokens of one run: by the
+  // first).
+  for (int part4 = wave; part4 < 4 * gone.n; part4 += kPick / 64) {
+    const int k = part4 >> 2, g = part4 & 3;
+    const int own = __builtin_amdgcn_readfirstlane(gone.token[k]) / MG_DRAFTS_RUN;
+    const int64_t first = (int64_t)own * MG_DRAFTS_RUN + 512 * g;
+    float z[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t e = first + 64 * j + lane;
+      z[j] = e < d.vocab ? x[e] : -kInf;
+    }
+    bool again = false;
+    for (int i0 = 0; i0 < gone.n; i0 += 64) {
+      const int t = i0 + lane < gone.n ? gone.token[i0 + lane] : -1;
+      uint64_t here = __ballot(t >= 0 && t / MG_DRAFTS_RUN == own);
+      again |= here && i0 + __builtin_ctzll(here) < k;
+      for (; here; here &= here - 1) {
+        const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(here)) - (int)first;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (at == 64 * j + lane) z[j] = -kInf;
+      }
+    }
+    double w = 0.0;
+    if (!again) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) w += weight(z[j], l.m, l.c) * l.s;
+    }
+    w = wave_sum(w);
+    if (lane == 0) {
+      if (g == 0) gone.run[k] = again ? -1 : own;
+      gone.mass[g][k] = w;
+    }
+  }
+  if (gone.n) __syncthreads();
+  int mode = l.mode;
+  const int per = (v.nrun + kPick - 1) / kPick;
+  const int r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
+  const mg_drafts_part *parts = v.part + l.row * v.nrun;
+  auto mass = [&](int r) {
+    if (mode == 2) return v.mass[b * v.nrun + r];
+    int k = -1;
+    for (int i = 0; i < gone.n; i++) k = gone.run[i] == r ? i : k;
+    if (k < 0) return mass_of(parts[r], l);
+    return (gone.mass[0][k] + gone.mass[1][k]) + (gone.mass[2][k] + gone.mass[3][k]);
+  };
+  Sums sum;
+  for (;;) {
+    double mine = 0.0;
+    for (int r = r0; r < r1; r++) mine += mass(r);
+    sum = scan(mine, part);
+    if (mode == 1 || sum.all > 0x1p-40) break;
+    mode = 1;
+  }
+  const double want = l.u * sum.all;
+  if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff;
+  __syncthreads();
+  // The first run whose running sum exceeds it, else (rounding) the last one that has any.
+  if (sum.upto > want && sum.before <= want) {
+    double at = sum.before, base = at;
+    int found = -1;
+    for (int r = r0; r < r1 && at <= want; r++) {
+      const double w = mass(r);
+      if (w > 0.0) found = r, base = at;
+      at += w;
+    }
+    run = found;
+    below = base;
+  }
+  __syncthreads();
+  if (run < 0) {
+    for (int r = r0; r < r1; r++)
+      if (mass(r) > 0.0) atomicMax(&highest, r);
+    __syncthreads();
+    if (threadIdx.x == 0) run = highest, below = 0.0;
+    __syncthreads();
+  }
+  if (run < 0) {
+    if (threadIdx.x == 0) v.out[l.out] = -1;
+    return;
+  }
+  const bool end = highest >= 0;
+  const float *y = mode == 2 ? d.draft + l.row * d.draft_stride : x;
+  double w[kEach], own = 0.0;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    const int64_t e = (int64_t)run * MG_DRAFTS_RUN + kEach * (int)threadIdx.x + j;
+    bool none = e >= d.vocab;
+    for (int k = 0; k < gone.n; k++) none |= gone.token[k] == e;
+    w[j] = none ? 0.0 : left_of(l, mode, x[e], y[e]);
+    own += w[j];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) highest = -1;
+  double at = below + scan(own, part).before;
+  int top = -1, here = 0x7fffffff;
+#pragma unroll
+  for (int j = 0; j < kEach; j++) {
+    at += w[j];
+    if (w[j] > 0.0) {
+      top = kEach * (int)threadIdx.x + j;
+      if (!end && at > want) here = min(here, top);
+    }
+  }
+  // (Tokens rise with the lanes: the last lane that has any, the first that is beyond.)
+  const uint64_t any = __ballot(top >= 0), beyond = __ballot(here < 0x7fffffff);
+  if (any && lane == 63 - __builtin_clzll(any)) atomicMax(&highest, top);
+  if (beyond && lane == __builtin_ctzll(beyond)) atomicMin(&pick, here);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int in = pick < 0x7fffffff ? pick : highest;
+    v.out[l.out] = in < 0 ? -1 : run * MG_DRAFTS_RUN + in;
+  }
+}
+
+// DRAFT: the last token is drawn by later launches; else here.
+template <bool DRAFT>
 __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   constexpr int kMost = MG_DRAFTS_MOST;
-  __shared__ double s[kMost], qs[kMost], ep[kMost], eq[kMost];  // rows' sums; tokens' weights
+  // Rows' sums of weights, tokens' probabilities after their parents (0: never, and for a token
+  // that an earlier row after the same one has too).
+  __shared__ double sums[4][kMost];
+  double *s = sums[0], *qs = sums[1], *pt = sums[2], *qt = sums[3];
   __shared__ float m[kMost], qm[kMost], u01[kMost];
-  __shared__ int token[kMost], parent[kMost], best[kMost];
-  __shared__ bool again[kMost];  // a token that an earlier row after the same one has too
+  __shared__ int token[kMost], parent[kMost], best[kMost];  // best of greedy rows, else rejected tokens
+  __shared__ uint16_t child[kMost], next[kMost];  // the first row after a row, the next one after the same; 0: none
   __shared__ int kept_n;
   const mg_drafts &d = v.d;
   const int64_t b = blockIdx.x;
   const Seq q = sequence(d, b);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  mg_drafts_last &last = v.last[b];
+  __shared__ mg_drafts_last last;
   if (q.n == 0) {
     if (threadIdx.x == 0) {
       v.count[b] = 0;
-      last.mode = 0;
+      if (DRAFT) v.last[b].mode = 0;
     }
     return;
   }
@@ -216,7 +420,7 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
       m[i] = top;
       s[i] = sum;
     }
-    if (d.draft && !greedy && i + 1 < q.n) {
+    if (DRAFT && !greedy && i + 1 < q.n) {
       join(v.part + (d.rows + row) * v.nrun, v.nrun, c, lane, &top, &sum, &ignored);
       if (lane == 0) {
         qm[i] = top;
@@ -227,18 +431,26 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   __syncthreads();
   for (int i = threadIdx.x; i < q.n; i += 1024) {
     const int t = token[i], up = parent[i];
-    double p = 0.0, w = 0.0;
+    const bool hangs = i > 0 && up >= 0 && up < i, inside = hangs && t >= 0 && t < d.vocab && !greedy;
+    float x = -kInf, y = -kInf;
+    if (inside) x = d.target[(q.start + up) * d.target_stride + t];
+    if (DRAFT && inside) y = d.draft[(q.start + up) * d.draft_stride + t];
     bool same = false;
-    if (i > 0 && up >= 0 && up < i && t >= 0 && t < d.vocab && !greedy) {
-      const int64_t row = q.start + up;
-      p = weight(d.target[row * d.target_stride + t], m[up], c);
-      if (d.draft) w = weight(d.draft[row * d.draft_stride + t], qm[up], c);
-      if (d.parent)
-        for (int j = 1; j < i; j++) same |= parent[j] == up && token[j] == t;
+    int below = 0, beside = 0;
+    if (d.parent) {
+      for (int j = 1; j < i; j++) same |= parent[j] == up && token[j] == t;
+      for (int j = q.n - 1; j > i; j--) {
+        if (parent[j] == i) below = j;
+        if (hangs && parent[j] == up) beside = j;
+      }
+    } else {
+      below = i + 1 < q.n ? i + 1 : 0;
     }
-    ep[i] = p;
-    eq[i] = w;
-    again[i] = same;
+    // (A token of weight 0 stays so: the sum is 1 at least.)
+    pt[i] = inside && !same ? weight(x, m[up], c) / s[up] : 0.0;
+    qt[i] = DRAFT && inside ? weight(y, qm[up], c) / qs[up] : 0.0;
+    child[i] = (uint16_t)below;
+    next[i] = (uint16_t)beside;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -246,33 +458,33 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     double left = 1.0;
     bool rest = false;
     v.kept[q.start] = 0;
-    for (int i = 1; i < q.n; i++) {
-      if (parent[i] != cur) continue;
+    // (Rows after a row come behind it: children in order are rows in order.)
+    for (int i = child[0]; i;) {
       const bool has = fabsf(m[cur]) < kInf;
-      const double u = (double)u01[i], p = ep[i] / s[cur];
-      bool stays = has && ep[i] > 0.0;
+      const double u = (double)u01[i], p = pt[i];
+      bool stays = has && p > 0.0;
       if (greedy) {
         stays = has && token[i] == best[cur];
-      } else if (d.draft) {
+      } else if (DRAFT) {
         const bool known = fabsf(qm[cur]) < kInf;
-        stays = stays && known && u * (eq[i] / qs[cur]) < p;
+        stays = stays && known && u * qt[i] < p;
         rest = known && !stays;
-      } else {
-        stays = stays && !again[i];
-        if (stays && !(u * left < p)) {
-          stays = false;
-          left -= p;
-          v.rej[q.start + rejected++] = token[i];
-        }
+      } else if (stays && !(u * left < p)) {
+        stays = false;
+        left -= p;
+        best[rejected++] = token[i];
       }
-      if (stays) {
-        v.out[q.start + n - 1] = token[i];
-        v.kept[q.start + n++] = i;
-        cur = i;
-        left = 1.0;
-        rejected = 0;
-        rest = false;
+      if (!stays) {
+        i = next[i];
+        continue;
       }
+      v.out[q.start + n - 1] = token[i];
+      v.kept[q.start + n++] = i;
+      cur = i;
+      left = 1.0;
+      rejected = 0;
+      rest = false;
+      i = child[i];
     }
     const bool has = fabsf(m[cur]) < kInf;
     const bool drawn = greedy || !has;
@@ -286,8 +498,8 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     last.row = q.start + cur;
     last.mode = drawn ? 0 : rest ? 2 : 1;
     last.rejected = rejected;
-    last.first = q.start;
     last.out = q.start + n - 1;
+    if (DRAFT) v.last[b] = last;
     v.count[b] = n;
     kept_n = n;
   }
@@ -296,58 +508,35 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     v.out[q.start + i] = -1;
     v.kept[q.start + i] = -1;
   }
-}
-
-// The weight left of a token with logits x and (mode 2) y.
-__device__ inline double left_of(const mg_drafts_last &l, int mode, float x, float y) {
-  const double p = weight(x, l.m, l.c) * l.s;
-  return mode == 2 ? fmax(p - weight(y, l.qm, l.c) * l.qs, 0.0) : p;
-}
-// Of the runs' sums those of p without a rejected token are there already.
-__device__ inline double mass_of(const mg_drafts_part &p, const mg_drafts_last &l) {
-  return p.s * exp2_of(((double)p.m - (double)l.m) * l.c) * l.s;
+  // (parent and the sums have been read: they take the runs of rejected tokens.)
+  if (!DRAFT && last.mode) draw_token(v, last, b, Gone{best, parent, sums, last.rejected});
 }
 
 constexpr int kOne = MG_DRAFTS_RUN / 256;  // logits of a thread of k_masses
 
+// The sums of the weights max(p - q, 0) of a run.
 __global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
   __shared__ double part[4];
-  __shared__ int list[MG_DRAFTS_MOST], listed;
   const mg_drafts &d = v.d;
   const int64_t b = blockIdx.y;
-  const mg_drafts_last &l = v.last[b];
-  const int mode = l.mode, rejected = l.rejected, run = blockIdx.x, lane = threadIdx.x & 63;
-  if (mode == 0 || (mode == 1 && rejected == 0)) return;
-  const int64_t first = (int64_t)run * MG_DRAFTS_RUN;
-  const float *xr = d.target + l.row * d.target_stride, *yr = xr;
-  if (mode == 2) yr = d.draft + l.row * d.draft_stride;
-  if (mode == 1) {
-    if (threadIdx.x == 0) listed = 0;
-    __syncthreads();
-    for (int r = threadIdx.x; r < rejected; r += 256) {
-      const int64_t t = v.rej[l.first + r] - first;
-      if (t >= 0 && t < MG_DRAFTS_RUN) list[atomicAdd(&listed, 1)] = (int)t;
-    }
-    __syncthreads();
-    if (listed == 0) {
-      if (threadIdx.x == 0) v.mass[b * v.nrun + run] = mass_of(v.part[l.row * v.nrun + run], l);
-      return;
-    }
-  }
-  float x[kOne], y[kOne] = {};
+  if (v.last[b].mode != 2) return;
+  const mg_drafts_last l = v.last[b];
+  const int64_t first = (int64_t)blockIdx.x * MG_DRAFTS_RUN;
+  const float *xr = d.target + l.row * d.target_stride, *yr = d.draft + l.row * d.draft_stride;
+  float x[kOne], y[kOne];
   if (first + MG_DRAFTS_RUN <= d.vocab) {
     const int64_t at = first + 4 * (int)threadIdx.x;
     Four v4[kOne / 4], u4[kOne / 4];
 #pragma unroll
-    for (int j = 0; j < kOne / 4; j++) v4[j] = *reinterpret_cast<const Four *>(xr + at + 1024 * j);
-    if (mode == 2) {
-#pragma unroll
-      for (int j = 0; j < kOne / 4; j++) u4[j] = *reinterpret_cast<const Four *>(yr + at + 1024 * j);
-#pragma unroll
-      for (int j = 0; j < kOne; j++) y[j] = u4[j / 4].x[j % 4];
+    for (int j = 0; j < kOne / 4; j++) {
+      v4[j] = *reinterpret_cast<const Four *>(xr + at + 1024 * j);
+      u4[j] = *reinterpret_cast<const Four *>(yr + at + 1024 * j);
     }
 #pragma unroll
-    for (int j = 0; j < kOne; j++) x[j] = v4[j / 4].x[j % 4];
+    for (int j = 0; j < kOne; j++) {
+      x[j] = v4[j / 4].x[j % 4];
+      y[j] = u4[j / 4].x[j % 4];
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < kOne; j++) {
@@ -356,179 +545,49 @@ __global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
       y[j] = e < d.vocab ? yr[e] : -kInf;
     }
   }
-  if (mode == 1)
-    for (int r = 0; r < listed; r++)
-#pragma unroll
-      for (int j = 0; j < kOne; j++)
-        if (1024 * (j / 4) + 4 * (int)threadIdx.x + j % 4 == list[r]) x[j] = -kInf;
-  // (The sequence's numbers once: its record is not read again for every logit.)
-  const mg_drafts_last one = l;
   double w = 0.0;
-  if (mode == 2) {
 #pragma unroll
-    for (int j = 0; j < kOne; j++) w += left_of(one, 2, x[j], y[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kOne; j++) w += left_of(one, 1, x[j], y[j]);
-  }
+  for (int j = 0; j < kOne; j++) w += left_of(l, 2, x[j], y[j]);
   w = wave_sum(w);
-  if (lane == 0) part[threadIdx.x >> 6] = w;
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = w;
   __syncthreads();
-  if (threadIdx.x == 0) v.mass[b * v.nrun + run] = (part[0] + part[1]) + (part[2] + part[3]);
-}
-
-constexpr int kPick = 1024;  // threads of k_pick
-
-// The running sum over the workgroup's threads before this one and up to it (the next one's
-// before is this one's up to, bit for bit), and the whole.
-struct Sums {
-  double before, upto, all;
-};
-__device__ inline Sums scan(double x, double *part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) part[wave] = x;
-  __syncthreads();
-  double before = 0.0, all = 0.0;
-#pragma unroll
-  for (int k = 0; k < kPick / 64; k++) {
-    if (k == wave) before = all;
-    all += part[k];
-  }
-  const double y = __shfl_up(x, 1);
-  return Sums{lane ? before + y : before, before + x, all};
+  if (threadIdx.x == 0) v.mass[b * v.nrun + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 __global__ __launch_bounds__(kPick) void k_pick(const mg_verify v) {
-  constexpr int kEach = MG_DRAFTS_RUN / kPick;
-  __shared__ double part[kPick / 64], below;
-  __shared__ int run, pick, highest;
-  __shared__ bool gone[MG_DRAFTS_RUN];
-  const mg_drafts &d = v.d;
-  const int64_t b = blockIdx.x;
-  const mg_drafts_last &l = v.last[b];
-  if (l.mode == 0) return;
-  int mode = l.mode;
-  const int rejected = l.rejected;
-  const int per = (v.nrun + kPick - 1) / kPick;
-  const int r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
-  const mg_drafts_part *parts = v.part + l.row * v.nrun;
-  auto mass = [&](int r) {
-    return mode == 1 && rejected == 0 ? mass_of(parts[r], l) : v.mass[b * v.nrun + r];
-  };
-  Sums sum;
-  for (;;) {
-    double mine = 0.0;
-    for (int r = r0; r < r1; r++) mine += mass(r);
-    sum = scan(mine, part);
-    if (mode == 1 || sum.all > 0x1p-40) break;
-    mode = 1;
-  }
-  const double want = l.u * sum.all;
-  if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff;
-#pragma unroll
-  for (int j = 0; j < kEach; j++) gone[kPick * j + threadIdx.x] = false;
-  __syncthreads();
-  // The first run whose running sum exceeds it, else (rounding) the last one that has any.
-  if (sum.upto > want && sum.before <= want) {
-    double at = sum.before, base = at;
-    int found = -1;
-    for (int r = r0; r < r1 && at <= want; r++) {
-      const double w = mass(r);
-      if (w > 0.0) found = r, base = at;
-      at += w;
-    }
-    run = found;
-    below = base;
-  }
-  __syncthreads();
-  if (run < 0) {
-    for (int r = r0; r < r1; r++)
-      if (mass(r) > 0.0) atomicMax(&highest, r);
-    __syncthreads();
-    if (threadIdx.x == 0) run = highest, below = 0.0;
-    __syncthreads();
-  }
-  if (run < 0) {
-    if (threadIdx.x == 0) v.out[l.out] = -1;
-    return;
-  }
-  const bool end = highest >= 0;
-  const int64_t first = (int64_t)run * MG_DRAFTS_RUN;
-  for (int r = threadIdx.x; r < rejected; r += kPick) {
-    const int64_t t = v.rej[l.first + r] - first;
-    if (t >= 0 && t < MG_DRAFTS_RUN) gone[t] = true;
-  }
-  const float *x = d.target + l.row * d.target_stride;
-  const float *y = mode == 2 ? d.draft + l.row * d.draft_stride : x;
-  double w[kEach], own = 0.0;
-#pragma unroll
-  for (int j = 0; j < kEach; j++) {
-    const int64_t e = first + kEach * (int)threadIdx.x + j;
-    w[j] = e < d.vocab ? left_of(l, mode, x[e], y[e]) : 0.0;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) highest = -1;
-#pragma unroll
-  for (int j = 0; j < kEach; j++) {
-    if (gone[kEach * threadIdx.x + j]) w[j] = 0.0;
-    own += w[j];
-  }
-  double at = below + scan(own, part).before;
-  int top = -1, here = 0x7fffffff;
-#pragma unroll
-  for (int j = 0; j < kEach; j++) {
-    at += w[j];
-    if (w[j] > 0.0) {
-      top = kEach * (int)threadIdx.x + j;
-      if (!end && at > want) here = min(here, top);
-    }
-  }
-  // (Tokens rise with the lanes: the last lane that has any, the first that is beyond.)
-  const uint64_t any = __ballot(top >= 0), beyond = __ballot(here < 0x7fffffff);
-  const int lane = threadIdx.x & 63;
-  if (any && lane == 63 - __builtin_clzll(any)) atomicMax(&highest, top);
-  if (beyond && lane == __builtin_ctzll(beyond)) atomicMin(&pick, here);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int in = pick < 0x7fffffff ? pick : highest;
-    v.out[l.out] = in < 0 ? -1 : run * MG_DRAFTS_RUN + in;
-  }
+  const mg_drafts_last l = v.last[blockIdx.x];
+  if (l.mode) draw_token(v, l, blockIdx.x, Gone{nullptr, nullptr, nullptr, 0});
 }
+
 
 }  // namespace
 
 size_t mg_verify_plan(mg_verify *v, void *ws) {
   v->nrun = (int)((v->d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN);
   const size_t parts = mg_align((size_t)v->d.rows * v->nrun * (v->d.draft ? 2 : 1) * sizeof(mg_drafts_part));
-  const size_t masses = mg_align((size_t)v->d.batch * v->nrun * 8);
-  const size_t lasts = mg_align((size_t)v->d.batch * sizeof(mg_drafts_last));
+  const size_t masses = v->d.draft ? mg_align((size_t)v->d.batch * v->nrun * 8) : 0;
+  const size_t lasts = v->d.draft ? mg_align((size_t)v->d.batch * sizeof(mg_drafts_last)) : 0;
   char *p = static_cast<char *>(ws);
   if (p) {
     v->part = reinterpret_cast<mg_drafts_part *>(p);
     v->mass = reinterpret_cast<double *>(p + parts);
     v->last = reinterpret_cast<mg_drafts_last *>(p + parts + masses);
-    v->rej = reinterpret_cast<int32_t *>(p + parts + masses + lasts);
   }
-  return parts + masses + lasts + mg_align((size_t)v->d.rows * 4);
+  return parts + masses + lasts;
 }
 
 mg_status mg_verify_run(mg_ctx *ctx, const mg_verify &v) {
   const mg_drafts &d = v.d;
   const unsigned runs = (unsigned)((v.nrun + 3) / 4);
   hipStream_t st = ctx->stream;
-  if (d.max_new == 0) {  // (no sequence has rows: their counts)
-    k_walk<<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
-    return mg_launch_check("VerifyDrafts");
+  if (d.max_new > 0)
+    k_stats<<<dim3(runs, (unsigned)(d.max_new * (d.draft ? 2 : 1)), (unsigned)d.batch), dim3(256), 0, st>>>(v);
+  if (d.draft) {
+    k_walk<true><<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
+    k_masses<<<dim3((unsigned)v.nrun, (unsigned)d.batch), dim3(256), 0, st>>>(v);
+    k_pick<<<dim3((unsigned)d.batch), dim3(kPick), 0, st>>>(v);
+  } else {
+    k_walk<false><<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
   }
-  k_stats<<<dim3(runs, (unsigned)(d.max_new * (d.draft ? 2 : 1)), (unsigned)d.batch), dim3(256), 0, st>>>(v);
-  k_walk<<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
-  k_masses<<<dim3((unsigned)v.nrun, (unsigned)d.batch), dim3(256), 0, st>>>(v);
-  k_pick<<<dim3((unsigned)d.batch), dim3(kPick), 0, st>>>(v);
   return mg_launch_check("VerifyDrafts");
 }

@@ -17,19 +17,18 @@ struct mg_drafts_last {
   float m, qm;         // maxima of the rows
   int64_t row;
   int32_t mode;     // 0: it is drawn already; 1: by p without the rejected tokens; 2: max(p - q, 0)
-  int32_t rejected; // tokens, from rej[first row of the sequence] on
-  int32_t first;    // first row of the sequence
+  int32_t rejected; // tokens
   int32_t out;      // row that the token goes to
 };
 struct mg_verify {
   mg_drafts d;
   int32_t *out, *kept, *count;
   int nrun;  // runs of a row
-  // Workspace: parts [2][rows][nrun], masses [batch][nrun], lasts [batch], rejected tokens [rows].
+  // Workspace: parts [rows][nrun]; with draft logits as many again, masses [batch][nrun] and lasts
+  // [batch].
   mg_drafts_part *part;
   double *mass;
   mg_drafts_last *last;
-  int32_t *rej;
 };
 // The workspace of a problem (its pointers set from ws, where not null).
 size_t mg_verify_plan(mg_verify *v, void *ws);
