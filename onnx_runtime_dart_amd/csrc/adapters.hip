@@ -361,9 +361,9 @@ __global__ __launch_bounds__(256, 4) void k_down(const mg_adapt p, const Order o
 
 // Outputs of a tile: `outs` of them of projection blockIdx.z, 32 a wave at a time.  Products change
 // lanes through the wave's own part of shared memory, so that base and y are read and written 16
-// bytes a lane and a line of a row at once; waves wait for each other only at the start.  The base
-// of the next block is on its way during a block's products.  stride: of the tile's values in
-// shared memory (odd; kHeld of them at a time, rounded up to 32 with zeros).
+// bytes a lane and a line of a row at once; waves wait for each other only at the start.  Weights
+// and base of the next block are asked for between a block's products and its stores.  stride: of
+// the tile's values in shared memory (odd; kHeld of them at a time, rounded up to 32 with zeros).
 constexpr int kHeld = 128, kTurn = 36;
 template <class T>
 __global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, const float *t, int parts,
@@ -386,13 +386,6 @@ __global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (threadIdx.x < kTile)
     row_of[threadIdx.x] = o.row[tile.start + min((int)threadIdx.x, tile.count - 1)] * N;
-  if (tile.slot < 0) {
-    __syncthreads();
-    for (int r = wave; r < tile.count; r += 4)
-      for (int64_t n = n0 + lane; n < last; n += 64)
-        y[row_of[r] + n] = tile.slot == -1 ? base[row_of[r] + n] : __builtin_nanf("");
-    return;
-  }
   const int rank = tile.rank;
   const T *b = static_cast<const T *>(p.h.b) + tile.slot * p.h.b_slot + p.h.b_off[z];
   // A lane's outputs of a block: four of rows r8 + 8 i.
@@ -406,6 +399,30 @@ __global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, 
     for (int i = 0; i < 8; i++) v.v[i] = load4(from + row_of[r8 + 8 * i] + at + part4);
     return v;
   };
+  if (tile.slot < 0) {
+    // No adapter: the base, beyond the slots: NaN.
+    __syncthreads();
+    const bool none = tile.slot == -1;
+    const float nan = __builtin_nanf("");
+#pragma unroll 2
+    for (int64_t at = n0 + 32 * wave; at < last; at += 128) {
+      if (at + 32 <= last) {
+        Block v;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v.v[i] = nan;
+        if (none) v = load_base(base, at);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (r8 + 8 * i < tile.count)
+            *reinterpret_cast<Four *>(y + row_of[r8 + 8 * i] + at + part4) =
+                Four{{v.v[i][0], v.v[i][1], v.v[i][2], v.v[i][3]}};
+      } else {
+        for (int r = hi; r < tile.count; r += 2)
+          if (at + l < last) y[row_of[r] + at + l] = none ? base[row_of[r] + at + l] : nan;
+      }
+    }
+    return;
+  }
   struct Weights {
     float w[16];
   };
@@ -460,21 +477,27 @@ __global__ __launch_bounds__(256, 3) void k_up(const mg_adapt p, const Order o, 
     int64_t at = n0 + 32 * wave;
     // (A block of less than 32 outputs, the last one, reads its base at the end.)
     Block v = {};
+    Weights w0, w1;
+    auto load_both = [&](int64_t to) {
+      const int col = (int)std::min(to + l, N - 1);
+      w0 = load_weights(col, j1);
+      if (j1 + 32 < j2) w1 = load_weights(col, j1 + 32);
+    };
+    load_both(at);
     if (at + 32 <= last) v = load_base(from, at);
 #pragma unroll 1
     for (; at < last; at += 128) {
       asm volatile("" ::: "memory");  // (the tile's values stay in shared memory: registers are for loads)
-      const int col = (int)std::min(at + l, N - 1);
-      const Weights w0 = load_weights(col, j1);
-      Weights w1 = w0;
-      if (j1 + 32 < j2) w1 = load_weights(col, j1 + 32);
-      Block next = v;
-      if (at + 160 <= last) next = load_base(from, at + 128);
       f32x16 acc[2] = {};
       products(w0, 0, acc);
       if (j1 + 32 < j2) products(w1, 32, acc);
 #pragma unroll 1
-      for (int j0 = j1 + 64; j0 < j2; j0 += 32) products(load_weights(col, j0), j0 - j1, acc);
+      for (int j0 = j1 + 64; j0 < j2; j0 += 32)
+        products(load_weights((int)std::min(at + l, N - 1), j0), j0 - j1, acc);
+      // (Before this block's stores: what comes behind them is waited for with them.)
+      Block next = v;
+      if (at + 128 < last) load_both(at + 128);
+      if (at + 160 <= last) next = load_base(from, at + 128);
       const int64_t n = at + part4;
 #pragma unroll
       for (int u = 0; u < 2; u++) {
