@@ -547,7 +547,7 @@ int64_t up_outs(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
   int64_t all = 0;
   for (int i = 0; i < h.n; i++) all += (h.N[i] + 127) / 128;
   const int64_t blocks = (rows + kTile - 1) / kTile * all / (3 * ctx->num_cus);
-  return 128 * std::max<int64_t>(2, std::min<int64_t>(blocks, 16));
+  return 128 * std::max<int64_t>(2, std::min<int64_t>(blocks, 8));
 }
 
 template <class T>
