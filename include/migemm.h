@@ -935,10 +935,11 @@ mg_status mg_adapters_create(mg_ctx *ctx, int64_t K, int32_t n, const int64_t *N
 mg_status mg_adapters_release(mg_adapters *adapters);
 mg_status mg_adapters_info(const mg_adapters *adapters, int64_t *K, int32_t *n, int64_t *slots,
                            int64_t *max_rank, int64_t *device_bytes);
-/* Fills a slot: a[i] [rank, K] and b[i] [N_i, rank] in host memory (waits for the stream), or in
- * device memory (_dev, asynchronous on the context's stream).  rank 0 empties it (a and b are not
- * read).  Later calls on the context, graphs captured before among them, use what the slot holds
- * then; calls on other contexts that may run at the same time are the caller's to order. */
+/* Fills a slot: a[i] [rank, K] and b[i] [N_i, rank] in host memory (waits for the stream, so not
+ * under its capture: MG_UNSUPPORTED), or in device memory (_dev, asynchronous on the context's
+ * stream).  rank 0 empties it (a and b are not read).  Later calls on the context, graphs captured
+ * before among them, use what the slot holds then; calls on other contexts that may run at the
+ * same time are the caller's to order. */
 mg_status mg_adapters_set(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,
                           const float *const *a, const float *const *b, float factor);
 mg_status mg_adapters_set_dev(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int64_t rank,

@@ -3032,7 +3032,7 @@ mg_status mg_kv_cache_copy_pages_dev(mg_ctx *ctx, mg_kv_cache *cache, const int3
   if (mg_kv_copy_groups(*cache, n) > MG_MOST_GROUPS)
     return mg_fail(MG_UNSUPPORTED, "KvCacheCopyPages: too many pages");
   MG_TRY(mg_use_device(ctx));
-  MG_TRY(take_workspace(what, ctx, mg_kv_copy_ws(n)));
+  MG_TRY(take_workspace(what, ctx, mg_kv_copy_ws(*cache, n)));
   return mg_kv_copy_run(ctx, *cache, src_dev, dst_dev, n, ctx->ws);
 }
 
@@ -3281,6 +3281,8 @@ mg_status mg_adapters_set(mg_ctx *ctx, mg_adapters *adapters, int64_t slot, int6
   g_last_error.clear();
   MG_TRY(check_adapter(ctx, adapters, slot, rank, a, b, factor));
   MG_TRY(mg_use_device(ctx));
+  if (mg_capturing(ctx))
+    return mg_fail(MG_UNSUPPORTED, "Adapters: host memory is not read under stream capture");
   const mg_adapters &h = *adapters;
   size_t need = 0;
   const float *a_dev[MG_ADAPTER_MOST] = {}, *b_dev[MG_ADAPTER_MOST] = {};

@@ -68,7 +68,7 @@ mg_status mg_kv_append_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch
 mg_status mg_kv_read_run(mg_ctx *ctx, const mg_kv_cache &c, const mg_seq_batch &s, float *k,
                          int64_t ks, float *v, int64_t vs);
 // Pages (kvpages.hip); workspaces, and workgroups of the largest launch.
-size_t mg_kv_copy_ws(int64_t n);
+size_t mg_kv_copy_ws(const mg_kv_cache &c, int64_t n);
 int64_t mg_kv_copy_groups(const mg_kv_cache &c, int64_t n);
 mg_status mg_kv_copy_run(mg_ctx *ctx, const mg_kv_cache &c, const int32_t *src, const int32_t *dst,
                          int64_t n, void *ws);

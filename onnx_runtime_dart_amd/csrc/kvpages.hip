@@ -53,14 +53,25 @@ struct Pairs {
   const int32_t *src, *dst;
   int64_t n;
   int pieces;
-  uint8_t *ok;  // [n], or null: each workgroup sees for itself
+  uint32_t *marks;  // [pages], or null (up to 1024 pairs): each workgroup looks through them
 };
+// Of a page: a pair's src (its dst another page), a pair's dst (its src another), and how many pairs'
+// dst in all.
+constexpr uint32_t kIsSrc = 1, kIsDst = 2, kOneDst = 4;
 // Whether pair i is to be copied, by the whole workgroup; *bad: it is refused.
 __device__ inline bool pair_ok(const Pairs &a, int64_t i, bool *bad) {
   const int s = a.src[i], d = a.dst[i];
   *bad = false;
   if ((s < 0 && d < 0) || s == d) return false;
   bool clash = s < 0 || d < 0 || s >= a.c.pages || d >= a.c.pages;
+  if (a.marks) {
+    if (!clash) {
+      const uint32_t on = a.marks[d];
+      clash = on / kOneDst > 1 || (on & kIsSrc) || (a.marks[s] & kIsDst);
+    }
+    *bad = clash;
+    return !clash;
+  }
   for (int64_t j = threadIdx.x; j < a.n; j += 256) {
     const int sj = a.src[j], dj = a.dst[j];
     if (j != i && !(sj < 0 && dj < 0)) clash |= dj == d || (sj != dj && (sj == d || dj == s));
@@ -69,26 +80,26 @@ __device__ inline bool pair_ok(const Pairs &a, int64_t i, bool *bad) {
   return !*bad;
 }
 
-__global__ __launch_bounds__(256) void k_check_pairs(const Pairs a) {
-  bool bad;
-  const bool ok = pair_ok(a, blockIdx.x, &bad);
-  if (threadIdx.x == 0) {
-    a.ok[blockIdx.x] = ok;
-    if (bad) atomicOr(a.c.refused, 1);
-  }
+__global__ __launch_bounds__(256) void k_clear_marks(const Pairs a) {
+  const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (p < a.c.pages) a.marks[p] = 0;
+}
+__global__ __launch_bounds__(256) void k_mark(const Pairs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.n) return;
+  const int s = a.src[i], d = a.dst[i];
+  if (s < 0 && d < 0) return;
+  if (s != d && s >= 0 && s < a.c.pages) atomicOr(a.marks + s, kIsSrc);
+  if (s != d && d >= 0 && d < a.c.pages) atomicOr(a.marks + d, kIsDst);
+  if (d >= 0 && d < a.c.pages) atomicAdd(a.marks + d, kOneDst);
 }
 __global__ __launch_bounds__(256) void k_copy_pages(const Pairs a) {
   const int64_t i = blockIdx.x / a.pieces;
   const int piece = blockIdx.x % a.pieces;
-  if (a.ok) {
-    if (!a.ok[i]) return;
-  } else {
-    bool bad;
-    const bool ok = pair_ok(a, i, &bad);
-    if (bad && piece == 0 && threadIdx.x == 0) atomicOr(a.c.refused, 1);
-    if (!ok) return;
-  }
-  copy_piece(a.c, a.src[i], a.dst[i], piece);
+  bool bad;
+  const bool ok = pair_ok(a, i, &bad);
+  if (bad && piece == 0 && threadIdx.x == 0) atomicOr(a.c.refused, 1);
+  if (ok) copy_piece(a.c, a.src[i], a.dst[i], piece);
 }
 
 // ------------------------------------------------------------------- compact
@@ -681,15 +692,18 @@ __global__ __launch_bounds__(256) void k_fit_copy(const Fit a) {
 
 }  // namespace
 
-size_t mg_kv_copy_ws(int64_t n) { return n > 1024 ? mg_align((size_t)n) : 0; }
+size_t mg_kv_copy_ws(const mg_kv_cache &c, int64_t n) {
+  return n > 1024 ? mg_align((size_t)c.pages * 4) : 0;
+}
 
 mg_status mg_kv_copy_run(mg_ctx *ctx, const mg_kv_cache &c, const int32_t *src, const int32_t *dst,
                          int64_t n, void *ws) {
   Pairs a{c, src, dst, n, page_pieces(c), nullptr};
-  // Each workgroup reads the whole list for its pair: for long ones once, not for every piece.
+  // Each workgroup reads the whole list for its pair; long ones leave their marks at the pages first.
   if (n > 1024) {
-    a.ok = static_cast<uint8_t *>(ws);
-    k_check_pairs<<<dim3((unsigned)n), dim3(256), 0, ctx->stream>>>(a);
+    a.marks = static_cast<uint32_t *>(ws);
+    k_clear_marks<<<dim3((unsigned)((c.pages + 255) / 256)), dim3(256), 0, ctx->stream>>>(a);
+    k_mark<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, ctx->stream>>>(a);
   }
   k_copy_pages<<<dim3((unsigned)(n * a.pieces)), dim3(256), 0, ctx->stream>>>(a);
   return mg_launch_check("KV cache copy");

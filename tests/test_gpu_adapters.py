@@ -252,6 +252,27 @@ def test_captured_graph(ops, rows):
         h.release()
 
 
+def test_host_weights_are_refused_under_capture(ops):
+    from onnx_runtime_dart_amd.errors import UnsupportedError
+    rng = np.random.default_rng(9)
+    with Captured(ops) as g:
+        h, held = adapters(ops, rng, 16, [8], 2, 4, ranks=[4, 2], ctx=g.ctx)
+        x, bases = inputs(rng, h, 5)
+        slots = np.array([0, 1, -1, 1, 0], np.int32)
+        d = [g.buffer(v) for v in (x, slots, bases[0], np.zeros((5, 8), np.float32))]
+
+        def call():
+            with pytest.raises(UnsupportedError):
+                h.set(0, [np.ones((4, 16), np.float32)], [np.ones((8, 4), np.float32)])
+            h.apply_dev(d[0].ptr, 5, d[1].ptr, [d[2].ptr], [d[3].ptr])
+
+        h.apply_dev(d[0].ptr, 5, d[1].ptr, [d[2].ptr], [d[3].ptr])
+        g.capture(call)()
+        g.wait()
+        check([d[3].to_array((5, 8), np.float32)], x, slots, bases, held)
+        h.release()
+
+
 def test_beside_a_shared_projection(ops):
     # int4 q and v projections of all requests, their adapters added in place.
     rng = np.random.default_rng(8)

@@ -150,6 +150,41 @@ def test_compact_long(ops, fmt):
         c.now = c.read()
 
 
+@pytest.mark.parametrize("budget", [False, True])
+def test_compact_long_in_place(ops, budget):
+    # The new lengths over the old ones; without room for a workspace rows move in order.  The graph
+    # is captured before the context has any workspace, then again after a call.
+    rng = np.random.default_rng(28)
+    with Captured(ops) as g:
+        c = Cache(ops, rng, 40, 64, "int8", 2, 48, ctx=g.ctx)
+        past = np.array([70, 0], np.int32)
+        kept, counts = lists(rng, [700, 901], 0.6)
+        table = rng.permutation(40)[:32].reshape(2, 16).astype(np.int32)
+        d = [g.buffer(v) for v in (np.array([0, 700, 1601], np.int32), past, table, kept, counts)]
+        s = ops.SeqBatch(batch=2, rows=1601, max_new=901, max_len=1024, row_start_ptr=d[0].ptr,
+                         past_ptr=d[1].ptr, page_table_ptr=d[2].ptr, table_stride=16)
+
+        def step():
+            g.ctx.set_control(max_bytes=1000 if budget else -1)
+            c.c.compact_dev(s, d[3].ptr, d[4].ptr, past_out_ptr=d[1].ptr)
+            g.ctx.set_control(max_bytes=-1)
+
+        for call in (g.capture(step), step, None):
+            call = call or g.capture(step)
+            for _ in range(3):
+                b = K.Batch(rng, [700, 901], past, 64)
+                b.page_table = table
+                call()
+                g.wait()
+                free = moved(c, b, kept, counts)
+                np.testing.assert_array_equal(d[1].to_array((2,), np.int32), past + counts)
+                c.check(free)
+                c.now = c.read()
+                g.put(d[1], past)
+                assert not c.c.refused()
+        c.c.release()
+
+
 def test_compact_without_moves_writes_nothing(ops):
     rng = np.random.default_rng(4)
     b = K.Batch(rng, [20, 30], [3, 50], 16)
