@@ -235,11 +235,13 @@ __device__ inline Sums scan(double x, double *part) {
   return Sums{before + moved<0x138>(x), before + x, all};
 }
 
-// Tokens without weight (shared memory), and room for the sums of their runs without them.
+// Tokens without weight and their probabilities (shared memory), and room for the sums of their runs
+// without them.
 struct Gone {
   const int *token;
+  const double *p;
   int *run;
-  double (*mass)[MG_DRAFTS_MOST];  // of each quarter of the run
+  double *mass;
   int n;
 };
 // The last token of a sequence, by the whole workgroup (kPick threads).
@@ -250,52 +252,54 @@ __device__ inline void draw_token(const mg_verify &v, const mg_drafts_last &l, i
   const mg_drafts &d = v.d;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float *x = d.target + l.row * d.target_stride;
-  // Runs of tokens without weight are summed again, a wave a quarter (of tokens of one run: by the
-  // first).
-  for (int part4 = wave; part4 < 4 * gone.n; part4 += kPick / 64) {
-    const int k = part4 >> 2, g = part4 & 3;
+  const mg_drafts_part *parts = v.part + l.row * v.nrun;
+  // Runs of tokens without weight, a wave each (of tokens of one run: the first).  Where 2^-20 of the
+  // run is left or more, that is the difference (sums of 2048 weights are right to 2^-47, so it is to
+  // 2^-27); else the run is summed again.
+  for (int k = wave; k < gone.n; k += kPick / 64) {
     const int own = __builtin_amdgcn_readfirstlane(gone.token[k]) / MG_DRAFTS_RUN;
-    const int64_t first = (int64_t)own * MG_DRAFTS_RUN + 512 * g;
-    float z[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int64_t e = first + 64 * j + lane;
-      z[j] = e < d.vocab ? x[e] : -kInf;
-    }
+    const double whole = mass_of(parts[own], l);
     bool again = false;
-    for (int i0 = 0; i0 < gone.n; i0 += 64) {
-      const int t = i0 + lane < gone.n ? gone.token[i0 + lane] : -1;
-      uint64_t here = __ballot(t >= 0 && t / MG_DRAFTS_RUN == own);
-      again |= here && i0 + __builtin_ctzll(here) < k;
-      for (; here; here &= here - 1) {
-        const int at = __builtin_amdgcn_readlane(t, __builtin_ctzll(here)) - (int)first;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (at == 64 * j + lane) z[j] = -kInf;
-      }
-    }
     double w = 0.0;
-    if (!again) {
-#pragma unroll
-      for (int j = 0; j < 8; j++) w += weight(z[j], l.m, l.c) * l.s;
+    for (int i0 = 0; i0 < gone.n; i0 += 64) {
+      const int i = min(i0 + lane, gone.n - 1);
+      const bool in = i0 + lane < gone.n && gone.token[i] / MG_DRAFTS_RUN == own;
+      const uint64_t here = __ballot(in);
+      again |= here && i0 + __builtin_ctzll(here) < k;
+      if (in) w += gone.p[i];
     }
-    w = wave_sum(w);
+    w = whole - wave_sum(w);
+    if (!again && !(w > whole * 0x1p-20)) {
+      w = 0.0;
+      for (int j0 = 0; j0 < MG_DRAFTS_RUN; j0 += 512) {
+        const int64_t first = (int64_t)own * MG_DRAFTS_RUN + j0 + lane;
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] = first + 64 * j < d.vocab ? x[first + 64 * j] : -kInf;
+        for (int i = 0; i < gone.n; i++) {
+          const int64_t at = gone.token[i] - first;
+#pragma unroll
+          for (int j = 0; j < 8; j++) z[j] = at == 64 * j ? -kInf : z[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) w += weight(z[j], l.m, l.c) * l.s;
+      }
+      w = wave_sum(w);
+    }
     if (lane == 0) {
-      if (g == 0) gone.run[k] = again ? -1 : own;
-      gone.mass[g][k] = w;
+      gone.run[k] = again ? -1 : own;
+      gone.mass[k] = w;
     }
   }
   if (gone.n) __syncthreads();
   int mode = l.mode;
   const int per = (v.nrun + kPick - 1) / kPick;
   const int r0 = min((int)threadIdx.x * per, v.nrun), r1 = min(r0 + per, v.nrun);
-  const mg_drafts_part *parts = v.part + l.row * v.nrun;
   auto mass = [&](int r) {
     if (mode == 2) return v.mass[b * v.nrun + r];
     int k = -1;
     for (int i = 0; i < gone.n; i++) k = gone.run[i] == r ? i : k;
-    if (k < 0) return mass_of(parts[r], l);
-    return (gone.mass[0][k] + gone.mass[1][k]) + (gone.mass[2][k] + gone.mass[3][k]);
+    return k < 0 ? mass_of(parts[r], l) : gone.mass[k];
   };
   Sums sum;
   for (;;) {
@@ -372,8 +376,7 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   constexpr int kMost = MG_DRAFTS_MOST;
   // Rows' sums of weights, tokens' probabilities after their parents (0: never, and for a token
   // that an earlier row after the same one has too).
-  __shared__ double sums[4][kMost];
-  double *s = sums[0], *qs = sums[1], *pt = sums[2], *qt = sums[3];
+  __shared__ double s[kMost], qs[kMost], pt[kMost], qt[kMost];
   __shared__ float m[kMost], qm[kMost], u01[kMost];
   __shared__ int token[kMost], parent[kMost], best[kMost];  // best of greedy rows, else rejected tokens
   __shared__ uint16_t child[kMost], next[kMost];  // the first row after a row, the next one after the same; 0: none
@@ -393,12 +396,40 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
   const float temp = temperature(d, b);
   const bool greedy = !(temp > 0.f);
   const double c = greedy ? 0.0 : kLog2e / (double)temp;
-  for (int i = threadIdx.x; i < q.n; i += 1024) {
-    token[i] = d.tokens[q.start + i];
-    parent[i] = d.parent ? d.parent[q.start + i] : i - 1;
-    u01[i] = d.uniform[q.start + i];
+  // A row a thread.  Its token's logits are asked for before the rows' parts.
+  static_assert(kMost <= 1024, "rows of a sequence");
+  const int me = threadIdx.x;
+  const int t = me < q.n ? d.tokens[q.start + me] : -1;
+  const int up = me < q.n && d.parent ? d.parent[q.start + me] : me - 1;
+  const bool hangs = me > 0 && me < q.n && up >= 0 && up < me;
+  const bool inside = hangs && t >= 0 && t < d.vocab && !greedy;
+  float x = -kInf, y = -kInf;
+  if (inside) x = d.target[(q.start + up) * d.target_stride + t];
+  if (DRAFT && inside) y = d.draft[(q.start + up) * d.draft_stride + t];
+  if (me < q.n) {
+    token[me] = t;
+    parent[me] = up;
+    u01[me] = d.uniform[q.start + me];
   }
-  for (int i = wave; i < q.n; i += 16) {
+  bool same = false;
+  int below = 0, beside = 0;
+  if (d.parent) {
+    __syncthreads();
+    if (wave * 64 < q.n) {
+#pragma unroll 4
+      for (int j = q.n - 1; j > 0; j--) {
+        const int pj = parent[j], tj = token[j];
+        same |= j < me && pj == up && tj == t;
+        if (j > me && pj == me) below = j;
+        if (j > me && pj == up) beside = j;
+      }
+    }
+    if (!hangs) beside = 0;
+  } else {
+    below = me + 1 < q.n ? me + 1 : 0;
+  }
+  // (The first waves have the rows' threads too.)
+  for (int i = 15 - wave; i < q.n; i += 16) {
     const int64_t row = q.start + i;
     float top;
     double sum;
@@ -407,12 +438,12 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     if (greedy) {
       // The first logit that is the largest: in its run.
       const int64_t first = (int64_t)at * MG_DRAFTS_RUN;
-      float x[kLane];
-      load(x, d.target + row * d.target_stride, first, d.vocab, lane);
+      float z[kLane];
+      load(z, d.target + row * d.target_stride, first, d.vocab, lane);
       int here = 0x7fffffff;
 #pragma unroll
       for (int j = kLane - 1; j >= 0; j--)
-        if (x[j] == top) here = (int)first + 256 * (j / 4) + 4 * lane + j % 4;
+        if (z[j] == top) here = (int)first + 256 * (j / 4) + 4 * lane + j % 4;
       here = wave_min(here);
       if (lane == 0) best[i] = here;
     }
@@ -429,28 +460,12 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < q.n; i += 1024) {
-    const int t = token[i], up = parent[i];
-    const bool hangs = i > 0 && up >= 0 && up < i, inside = hangs && t >= 0 && t < d.vocab && !greedy;
-    float x = -kInf, y = -kInf;
-    if (inside) x = d.target[(q.start + up) * d.target_stride + t];
-    if (DRAFT && inside) y = d.draft[(q.start + up) * d.draft_stride + t];
-    bool same = false;
-    int below = 0, beside = 0;
-    if (d.parent) {
-      for (int j = 1; j < i; j++) same |= parent[j] == up && token[j] == t;
-      for (int j = q.n - 1; j > i; j--) {
-        if (parent[j] == i) below = j;
-        if (hangs && parent[j] == up) beside = j;
-      }
-    } else {
-      below = i + 1 < q.n ? i + 1 : 0;
-    }
+  if (me < q.n) {
     // (A token of weight 0 stays so: the sum is 1 at least.)
-    pt[i] = inside && !same ? weight(x, m[up], c) / s[up] : 0.0;
-    qt[i] = DRAFT && inside ? weight(y, qm[up], c) / qs[up] : 0.0;
-    child[i] = (uint16_t)below;
-    next[i] = (uint16_t)beside;
+    pt[me] = inside && !same ? weight(x, m[up], c) / s[up] : 0.0;
+    qt[me] = DRAFT && inside ? weight(y, qm[up], c) / qs[up] : 0.0;
+    child[me] = (uint16_t)below;
+    next[me] = (uint16_t)beside;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -459,8 +474,8 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     bool rest = false;
     v.kept[q.start] = 0;
     // (Rows after a row come behind it: children in order are rows in order.)
+    bool has = fabsf(m[0]) < kInf;
     for (int i = child[0]; i;) {
-      const bool has = fabsf(m[cur]) < kInf;
       const double u = (double)u01[i], p = pt[i];
       bool stays = has && p > 0.0;
       if (greedy) {
@@ -472,6 +487,7 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
       } else if (stays && !(u * left < p)) {
         stays = false;
         left -= p;
+        qs[rejected] = p;
         best[rejected++] = token[i];
       }
       if (!stays) {
@@ -481,12 +497,12 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
       v.out[q.start + n - 1] = token[i];
       v.kept[q.start + n++] = i;
       cur = i;
+      has = fabsf(m[cur]) < kInf;
       left = 1.0;
       rejected = 0;
       rest = false;
       i = child[i];
     }
-    const bool has = fabsf(m[cur]) < kInf;
     const bool drawn = greedy || !has;
     if (drawn) v.out[q.start + n - 1] = has ? best[cur] : -1;
     last.s = 1.0 / s[cur];
@@ -508,8 +524,8 @@ __global__ __launch_bounds__(1024) void k_walk(const mg_verify v) {
     v.out[q.start + i] = -1;
     v.kept[q.start + i] = -1;
   }
-  // (parent and the sums have been read: they take the runs of rejected tokens.)
-  if (!DRAFT && last.mode) draw_token(v, last, b, Gone{best, parent, sums, last.rejected});
+  // (parent and pt have been read: they take the runs of rejected tokens.)
+  if (!DRAFT && last.mode) draw_token(v, last, b, Gone{best, qs, parent, pt, last.rejected});
 }
 
 constexpr int kOne = MG_DRAFTS_RUN / 256;  // logits of a thread of k_masses
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(256) void k_masses(const mg_verify v) {
 
 __global__ __launch_bounds__(kPick) void k_pick(const mg_verify v) {
   const mg_drafts_last l = v.last[blockIdx.x];
-  if (l.mode) draw_token(v, l, blockIdx.x, Gone{nullptr, nullptr, nullptr, 0});
+  if (l.mode) draw_token(v, l, blockIdx.x, Gone{nullptr, nullptr, nullptr, nullptr, 0});
 }
 
 
