@@ -6,6 +6,12 @@
 // rows are sorted by slot into tiles of 64 rows of one adapter, and both products are made of
 // 32 x 32 x 2 fp32 matrix instructions: operands as they are, sums in fp32.  Rows of a tile do
 // not touch each other's results, so the order within a slot does not matter.
+//
+// 8191 rows of 3 prompts, 2048 -> 2 x 8192 by 64 in fp32: order 10 us, down 60 to 69 (by the matrix
+// instructions, whose rate alone asks for 28, and the latency of the loads between them), up 253 to 284
+// (by bytes of base and y: 1.08 GB, 3.8 to 4.3 TB/s).  2494 rows of 5 prompts and 48 tokens, 2048 ->
+// 2048, 512, 512 by 16 in fp16: 5.5, 20 and 20 (latencies: 8 steps of 32 k a workgroup, 2 blocks of 128
+// outputs).  64 rows with adapters of their own, 2048 -> 2048 by 32 in fp32: 4.2 and 4.9 us, 35 MB.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

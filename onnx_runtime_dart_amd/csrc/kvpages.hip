@@ -6,6 +6,11 @@
 // workgroup per head takes them 32 or 128 at a time, reads all before it writes any, and nothing
 // that it writes is read later (row j comes from kept[j] >= j, later rows from beyond it).  Long
 // lists go through the workspace, twice the traffic but all workgroups at once.
+//
+// Bound by bytes where there are many: pages of 4 sequences of 7001 to 8192 e4m3 tokens of 8 heads of
+// 128 copied in 28 us (4.9 TB/s, read and written), half of their tokens moved in 15 + 13 us and 5 for
+// the lists (in order, without the workspace: 118); else by chains of loads: 25 rows of 64 sequences
+// 6.4 us, a fork 2.3 to 2.8, 64 copies of pages 4.4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -522,8 +527,9 @@ __global__ __launch_bounds__(256) void k_fit_give(const Fit a) {
 }
 
 // All of it but the copies by one workgroup: what few sequences and pages need, without the waits
-// between launches, every table entry in a register of its own (64 sequences of 64 pages: 15
-// us, 21 in the kernels of their own and as many waits; 4 sequences: 11 and 17).
+// between launches, every table entry in a register of its own (64 sequences of 64 pages: 13
+// us, 21 in the kernels of their own and as many waits; 4 sequences: 9 and 17).  A chain: the entries, their
+// counts, what is let go, what is free, the entries written: 7 us of waits.
 constexpr int kOneBatch = 1024, kOnePages = 65536, kOneNeed = 8192, kOneEach = kOneNeed / 1024;
 // A count that other waves change in this launch.
 __device__ inline int count_of(const int32_t *p) {
@@ -602,8 +608,19 @@ __global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
     if (id[i] >= 0 && id[i] < a.c.pages) atomicSub(a.refs + id[i], 1);
     a.table[at] = -1;
   }
-  __threadfence();
+  // (The counts are kept by the L2 that this workgroup's atomics and count_of go to: waiting is enough.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  // The first pages' counts, on their way while the need is added up.
+  int c[4];
+  auto counts = [&](int64_t p0) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int64_t p = p0 + 4 * me + k;
+      c[k] = p < a.c.pages ? count_of(a.refs + p) : 1;
+    }
+  };
+  counts(0);
   if (me < batch) mid[me] = need[me];  // the page
   __syncthreads();
   // What is needed, in all and before each.
@@ -626,12 +643,8 @@ __global__ __launch_bounds__(1024) void k_fit_one(const Fit a) {
   // The free pages that are needed, lowest first: four a thread.
   int found = 0;
   for (int64_t p0 = 0; p0 < a.c.pages && found < total; p0 += 4096) {
-    int is = 0, n = 0, c[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int64_t p = p0 + 4 * me + k;
-      c[k] = p < a.c.pages ? count_of(a.refs + p) : 1;
-    }
+    int is = 0, n = 0;
+    if (p0) counts(p0);
 #pragma unroll
     for (int k = 0; k < 4; k++)
       if (c[k] == 0) is |= 1 << k, n++;
