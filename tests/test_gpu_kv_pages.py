@@ -294,6 +294,19 @@ def test_freeing_sequences(ops):
     assert (past == 0).all() and (table == -1).all() and (refs == 0).all()
 
 
+def test_forks_from_and_to_nothing(ops):
+    rng = np.random.default_rng(29)
+    c = Cache(ops, rng, 20, 16)
+    past = np.array([40, 0, 17])
+    table, refs = holdings(rng, past, 16, 20, 4)
+    got = c.c.fork([-1, -1, 0], past=[], page_table=np.zeros((0, 4)), refs=refs, width=2)
+    assert (got[0] == 0).all() and (got[1] == -1).all()
+    np.testing.assert_array_equal(got[2], refs)
+    assert c.c.refused()  # (the third: there is no such parent)
+    got = c.c.fork([], past=past, page_table=table, refs=refs)
+    assert got[0].size == 0 and (got[2] == 0).all() and not c.c.refused()
+
+
 @pytest.mark.parametrize("n", [900, 1500])
 def test_many_pages_and_sequences(ops, n):
     # More pages than one run of the search for free ones; sequences of one workgroup and of many.

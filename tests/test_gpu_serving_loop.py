@@ -1,10 +1,13 @@
 """The serving operators together, as a program runs them: prompts and drafted trees written
 to the paged cache, attended to, verified, the rows that stay moved together, sequences forked and
 fitted with pages, against a cache that only ever held what was emitted."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import drafts_reference as R
+from hip_graph import Captured
 
 pytestmark = pytest.mark.gpu
 KV, HEADS, D, PAGE, VOCAB, RANK = 2, 4, 64, 16, 300, 4
@@ -130,3 +133,53 @@ def test_speculative_decoding(ops, fmt, tree):
     assert (refs > 0).sum() == sum(-(-int(past[i]) // PAGE) for i in (0, 1))
     table, refs, granted = cache.fit(row_start=[0, 0, 0, 0], past=[0, 0, 0], page_table=table, refs=refs)
     assert (refs == 0).all() and (table == -1).all() and granted.all()
+
+
+def test_contexts_at_once(ops):
+    # Two contexts with streams of their own use the same adapters and cache; nothing of one call waits
+    # for the other's.
+    rng = np.random.default_rng(31)
+    ad = ops.Adapters(200, [300], slots=4, max_rank=8)
+    for s in range(4):
+        ad.set(s, *([rng.standard_normal(sh).astype(np.float32)] for sh in ((8, 200), (300, 8))))
+    rows, seqs, n = 1200, 12, 6
+    x, base = (rng.standard_normal((rows, k)).astype(np.float32) for k in (200, 300))
+    slot = rng.integers(-1, 4, rows).astype(np.int32)
+    want = ad.apply(x, slot, [base])[0]
+    logits = rng.standard_normal((seqs * n, 4000)).astype(np.float32)
+    start, tokens = np.arange(0, seqs * n + 1, n), rng.integers(0, 4000, seqs * n)
+    uniform = rng.random(seqs * n).astype(np.float32)
+    drawn = R.verify(target=logits, tokens=tokens, uniform=uniform, row_start=start, parent=None, draft=None)
+    cache = ops.KvCache(8, kv_heads=2, head_size=64, page_size=64, fmt="int8")
+    k, v = rng.standard_normal((2, 512, 2, 64)).astype(np.float32)
+    where = dict(row_start=64 * np.arange(9), past=np.zeros(8), page_table=np.arange(8)[:, None])
+    cache.append(k, v, **where)
+    held = cache.read(512, **where)
+    with Captured(ops) as one, Captured(ops) as two:
+        sides = []
+        for g, src, dst in ((one, [0, 1], [2, 3]), (two, [4, 5], [6, 7])):
+            d = {name: g.buffer(a) for name, a in dict(
+                x=x, base=base, slot=slot, y=np.zeros_like(base), logits=logits, start=start.astype(np.int32),
+                tokens=tokens.astype(np.int32), uniform=uniform, out=np.zeros(seqs * n, np.int32),
+                kept=np.zeros(seqs * n, np.int32), count=np.zeros(seqs, np.int32),
+                src=np.array(src, np.int32), dst=np.array(dst, np.int32)).items()}
+            # (The handles are the default context's: calls on others go by the C entries.)
+            sides.append((g, d, ops.Drafts(
+                batch=seqs, rows=seqs * n, max_new=n, vocab=4000, row_start_ptr=d["start"].ptr,
+                tokens_ptr=d["tokens"].ptr, target_ptr=d["logits"].ptr, uniform_ptr=d["uniform"].ptr)))
+        from onnx_runtime_dart_amd._lib import check, lib
+        for _ in range(6):
+            for g, d, drafts in sides:
+                check(lib.mg_adapters_apply_f32_dev(g.ctx.handle, ad.handle, d["x"].ptr, rows, d["slot"].ptr,
+                                                    (C.c_void_p * 1)(d["base"].ptr), (C.c_void_p * 1)(d["y"].ptr)))
+                ops.verify_drafts_dev(drafts, d["out"].ptr, d["kept"].ptr, d["count"].ptr, ctx=g.ctx)
+                check(lib.mg_kv_cache_copy_pages_dev(g.ctx.handle, cache.handle, d["src"].ptr, d["dst"].ptr, 2))
+        for g, d, _ in sides:
+            g.wait()
+            np.testing.assert_array_equal(d["y"].to_array(want.shape, np.float32), want)
+            for name, w in zip(("out", "kept", "count"), drawn):
+                np.testing.assert_array_equal(d[name].to_array(w.shape, np.int32), w)
+    for got, was in zip(cache.read(512, **where), held):
+        pages = was.reshape((8, 64) + was.shape[1:]).copy()
+        pages[[2, 3, 6, 7]] = pages[[0, 1, 4, 5]]
+        np.testing.assert_array_equal(got.reshape(pages.shape), pages)

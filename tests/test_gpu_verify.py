@@ -178,6 +178,24 @@ def test_large_and_small_values(ops):
     check(ops, **a, temperature=temp)
 
 
+@pytest.mark.parametrize("gap", [12.0, 18.0, 23.0])
+def test_rejected_tokens_that_hold_most_of_their_runs(ops, gap):
+    # A tree's root offers the largest tokens of the first three runs, each but 3400 e^-gap of its run; all
+    # are rejected (fp32 has random numbers up to 1 - 2^-24), and the last token is drawn from the rest.
+    rng = np.random.default_rng(17)
+    seqs, vocab = 48, 7000
+    row = rng.standard_normal(vocab).astype(np.float32)
+    tops = [40, 2048 + 2047, 2 * 2048]
+    row[tops] = [gap, gap - 0.5, gap + 1]
+    row[[50, 2 * 2048 + 900]] = -np.inf
+    uniform = np.full((seqs, 4), 1 - 2.0**-24, np.float32)
+    uniform[:, 0] = rng.random(seqs)
+    got = check(ops, target=np.tile(row, (4 * seqs, 1)), tokens=np.tile([7] + tops, seqs).astype(np.int32),
+                parent=np.tile([-1, 0, 0, 0], seqs).astype(np.int32), row_start=4 * np.arange(seqs + 1),
+                uniform=uniform.ravel(), draft=None)
+    assert (got[2] == 1).all() and not np.isin(got[0], tops).any() and len(np.unique(got[0])) > 30
+
+
 def test_greedy_ties_go_to_the_lowest_token(ops):
     rng = np.random.default_rng(9)
     a = batch(rng, [4] * 20, 7000, draft=False)
