@@ -254,7 +254,7 @@ struct Gone {
 __device__ inline void draw_token(const mg_verify &v, const mg_drafts_last &l, int64_t b, const Gone &gone) {
   constexpr int kEach = MG_DRAFTS_RUN / kPick;
   __shared__ double part[kPick / 64], below;
-  __shared__ int run, pick, highest;
+  __shared__ int run, pick, highest, lowest;
   const mg_drafts &d = v.d;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float *x = d.target + l.row * d.target_stride;
@@ -308,24 +308,33 @@ __device__ inline void draw_token(const mg_verify &v, const mg_drafts_last &l, i
     return k < 0 ? mass_of(parts[r], l) : gone.mass[k];
   };
   Sums sum;
+  double mine;
   for (;;) {
-    double mine = 0.0;
+    mine = 0.0;
     for (int r = r0; r < r1; r++) mine += mass(r);
     sum = scan(mine, part);
     if (mode == 1 || sum.all > 0x1p-40) break;
     mode = 1;
   }
   const double want = l.u * sum.all;
-  if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff;
+  if (threadIdx.x == 0) run = -1, highest = -1, pick = 0x7fffffff, lowest = kPick;
   __syncthreads();
-  // The first run whose running sum exceeds it, else (rounding) the last one that has any.
-  if (sum.upto > want && sum.before <= want) {
+  // The first run whose running sum exceeds it, else (rounding) the last one that has any.  Lanes add
+  // the same weights in orders of their own, so sums may fall by a rounding from one to the next, and
+  // rise where there is no weight: the first of those with weight counts.
+  const uint64_t over = __ballot(mine > 0.0 && sum.upto > want);
+  if (over && lane == __builtin_ctzll(over)) atomicMin(&lowest, (int)threadIdx.x);
+  __syncthreads();
+  if ((int)threadIdx.x == lowest) {
     double at = sum.before, base = at;
     int found = -1;
-    for (int r = r0; r < r1 && at <= want; r++) {
+    for (int r = r0; r < r1; r++) {
       const double w = mass(r);
-      if (w > 0.0) found = r, base = at;
+      if (!(w > 0.0)) continue;
+      found = r;
+      base = at;
       at += w;
+      if (at > want) break;
     }
     run = found;
     below = base;

@@ -145,6 +145,35 @@ def test_masked_and_non_finite_rows(ops):
         assert out[0] == out[4] == out[8] == -1
 
 
+# Weights of 1 in each run of 2048 logits; the half of them ends with a run, and runs without any follow.
+HALVES = [[0, 43, 0, 10, 29, 0, 0, 7, 0, 19, 35, 18, 0, 0, 17, 0],
+          [1, 14, 17, 0, 0, 0, 0, 4, 34, 0, 0, 11, 0, 3, 0, 56],
+          [0, 41, 0, 0, 30, 20, 0, 0, 0, 7, 17, 0, 38, 29, 0, 0],
+          [0, 0, 0, 0, 0, 10, 0, 31, 8, 37, 7, 33, 0, 18, 0, 108],
+          [34, 36, 0, 25, 10, 0, 0, 0, 4, 27, 0, 0, 0, 0, 37, 37],
+          [0, 7, 38, 0, 7, 0, 0, 23, 0, 6, 18, 15, 0, 0, 36, 0],
+          [0, 0, 0, 17, 29, 0, 27, 0, 0, 23, 0, 10, 0, 86, 0, 0],
+          [2, 37, 0, 0, 0, 0, 0, 0, 17, 0, 0, 27, 0, 0, 0, 29]]
+
+
+def test_borders_among_runs_without_weight(ops):
+    # The random number 1/2 falls onto the border between two tokens, where sums in 64 bits may decide for
+    # either of them; lanes that add the same weights in other orders must not make it a third one.
+    target = np.full((len(HALVES), 2048 * 16), -np.inf, np.float32)
+    beside = []
+    for row, k in zip(target, HALVES):
+        for run, n in enumerate(k):
+            row[2048 * run:2048 * run + n] = 3.0
+        tokens = np.nonzero(row == 3.0)[0]
+        assert tokens.size % 2 == 0
+        beside.append(tokens[tokens.size // 2 - 1:tokens.size // 2 + 1])
+    n = len(HALVES)
+    out, _, count = ops.op_verify_drafts(target, np.zeros(n, np.int32), np.full(n, 0.5, np.float32),
+                                         np.arange(n + 1))
+    assert (count == 1).all()
+    assert all(t in two for t, two in zip(out, beside)), (out, beside)
+
+
 def test_tokens_outside_the_vocabulary_and_parents(ops):
     rng = np.random.default_rng(6)
     a = batch(rng, [8, 8, 8], 50, tree=True, size=0.1)
