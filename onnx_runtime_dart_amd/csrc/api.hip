@@ -3158,9 +3158,8 @@ mg_status mg_verify_drafts_f32_dev(mg_ctx *ctx, const mg_drafts *drafts, int32_t
   if (!d.row_start || !count_dev ||
       (d.max_new && (!d.tokens || !d.target || !d.uniform || !out_tokens_dev || !kept_dev)))
     return bad_arg(what, "null buffer");
-  const int64_t runs = (d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN;
-  if (runs * d.batch > MG_MOST_GROUPS / (2 * d.max_new + 1) * 4 || runs * d.batch > MG_MOST_GROUPS ||
-      d.rows > ((int64_t)1 << 36) / runs)
+  if (mg_verify_groups(d) > MG_MOST_GROUPS ||
+      d.rows > ((int64_t)1 << 36) / ((d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN))
     return mg_fail(MG_UNSUPPORTED, "VerifyDrafts: too many logits");
   v.out = out_tokens_dev;
   v.kept = kept_dev;

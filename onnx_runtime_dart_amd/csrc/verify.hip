@@ -590,7 +590,6 @@ __global__ __launch_bounds__(kPick) void k_pick(const mg_verify v) {
   if (l.mode) draw_token(v, l, blockIdx.x, Gone{nullptr, nullptr, nullptr, nullptr, 0});
 }
 
-
 }  // namespace
 
 size_t mg_verify_plan(mg_verify *v, void *ws) {
@@ -607,12 +606,26 @@ size_t mg_verify_plan(mg_verify *v, void *ws) {
   return parts + masses + lasts;
 }
 
+// The grid of k_stats.
+struct Grid {
+  int64_t x, y, z;
+};
+static Grid stats_grid(const mg_drafts &d) {
+  const int64_t runs = (d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN;
+  return Grid{(runs + 3) / 4, d.max_new * (d.draft ? 2 : 1), d.batch};
+}
+int64_t mg_verify_groups(const mg_drafts &d) {
+  const Grid g = stats_grid(d);
+  const int64_t masses = d.draft ? (d.vocab + MG_DRAFTS_RUN - 1) / MG_DRAFTS_RUN * d.batch : 0;
+  return std::max(g.x * g.y * g.z, masses);
+}
+
 mg_status mg_verify_run(mg_ctx *ctx, const mg_verify &v) {
   const mg_drafts &d = v.d;
-  const unsigned runs = (unsigned)((v.nrun + 3) / 4);
   hipStream_t st = ctx->stream;
+  const Grid g = stats_grid(d);
   if (d.max_new > 0)
-    k_stats<<<dim3(runs, (unsigned)(d.max_new * (d.draft ? 2 : 1)), (unsigned)d.batch), dim3(256), 0, st>>>(v);
+    k_stats<<<dim3((unsigned)g.x, (unsigned)g.y, (unsigned)g.z), dim3(256), 0, st>>>(v);
   if (d.draft) {
     k_walk<true><<<dim3((unsigned)d.batch), dim3(1024), 0, st>>>(v);
     k_masses<<<dim3((unsigned)v.nrun, (unsigned)d.batch), dim3(256), 0, st>>>(v);

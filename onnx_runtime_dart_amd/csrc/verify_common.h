@@ -30,6 +30,8 @@ struct mg_verify {
   double *mass;
   mg_drafts_last *last;
 };
+// Workgroups of the largest launch of a call (of 256 threads; those of 1024 are one a sequence).
+int64_t mg_verify_groups(const mg_drafts &d);
 // The workspace of a problem (its pointers set from ws, where not null).
 size_t mg_verify_plan(mg_verify *v, void *ws);
 mg_status mg_verify_run(mg_ctx *ctx, const mg_verify &v);

@@ -44,6 +44,15 @@ def test_drafts_that_are_not_supported():
                   count=None) == 0
 
 
+def test_drafts_beyond_a_launch():
+    # 2^24 - 1 workgroups of 256 threads: four runs of 2048 logits each, of every row that a sequence may have.
+    assert verify(batch=16384, rows=2**24, max_new=1024, vocab=2048) == 2
+    assert verify(batch=16384, rows=2**24, max_new=1024, vocab=1) == 2
+    assert verify(batch=8192, rows=2**24, max_new=1024, vocab=8192, draft_ptr=P) == 2
+    assert verify(batch=8192, rows=2**24, max_new=1024, vocab=8193) == 2
+    assert verify(batch=65535, rows=2**24, max_new=257, vocab=100) == 2
+
+
 def copy(n=3, src=P, dst=P, cache=CACHE.ptr, ctx=CTX.ptr):
     return lib.mg_kv_cache_copy_pages_dev(ctx, cache, src, dst, n)
 
