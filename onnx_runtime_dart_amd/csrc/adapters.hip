@@ -603,15 +603,18 @@ int64_t mg_adapt_groups(const mg_adapters &h, int64_t rows) {
   return most_tiles(h, std::min(rows, MG_ADAPT_ROWS)) * ((most + kOuts - 1) / kOuts) * h.n;
 }
 
-size_t mg_adapt_ws(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
-  rows = std::min(rows, MG_ADAPT_ROWS);
+static size_t round_ws(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
   const size_t cols = (size_t)h.n * h.max_rank;
-  // (A last round of few rows needs no more than a whole one.)
   if (few_rows(h, rows)) return mg_align((size_t)rows * cols * 4);
   int parts;
   k_share(ctx, h, rows, &parts);
   return mg_align((size_t)rows * 4) + 256 + mg_align((size_t)most_tiles(h, rows) * sizeof(Tile)) +
          mg_align((size_t)parts * rows * cols * 4);
+}
+size_t mg_adapt_ws(const mg_ctx *ctx, const mg_adapters &h, int64_t rows) {
+  // (The last round's rows are fewer, the parts of their K more.)
+  const size_t last = round_ws(ctx, h, rows % MG_ADAPT_ROWS);
+  return rows < MG_ADAPT_ROWS ? last : std::max(last, round_ws(ctx, h, MG_ADAPT_ROWS));
 }
 
 mg_status mg_adapt_run(mg_ctx *ctx, const mg_adapt &p, void *ws) {

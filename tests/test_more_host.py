@@ -128,6 +128,23 @@ def test_adapters_out_of_bounds():
     assert apply(rows=0, x=None, slot=None, base=None, y=None) == 0
 
 
+@pytest.mark.parametrize("k, n, rank", [(16384, 1, 64), (16384, 3, 16), (2048, 2, 256), (300, 1, 5)])
+def test_adapters_workspace_holds_a_short_last_round(k, n, rank):
+    # Rows beyond 65536 go in rounds; a short one splits K into more parts, by the compute units there are.
+    need = lib["_Z11mg_adapt_wsPK6mg_ctxRK11mg_adaptersl"]
+    need.restype, need.argtypes = C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int64]
+    h = Handle(0, 0, n, rank, k, 0, k, 0, 4, 0, 0, 0, 8, 0)
+    for cus in (1, 32, 80, 256, 304, 1000):
+        ctx = Handle(*[0] * 22, cus)  # (compute units)
+        for rows in (1, 50, 513, 700, 1216, 1217, 4000, 20000, 65535):
+            assert need(ctx.ptr, h.ptr, 65536 + rows) >= need(ctx.ptr, h.ptr, rows)
+            assert need(ctx.ptr, h.ptr, 65536 + rows) >= need(ctx.ptr, h.ptr, 65536)
+    # (The field is the one that is meant.)
+    if k > 512:
+        few, many = (need(Handle(*[0] * 22, cus).ptr, h.ptr, 1216) for cus in (32, 256))
+        assert few < many
+
+
 def test_host_calls_check_their_arrays():
     x, u = np.zeros((3, 5), np.float32), np.zeros(3, np.float32)
     good = dict(target=x, tokens=[0, 1, 2], uniform=u, row_start=[0, 3], ctx=object())
