@@ -852,7 +852,9 @@ mg_status mg_kv_cache_fork_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_bat
  *   missing pages are taken from the free ones.
  * Free pages go by number, lowest first, to the sequences in order (a sequence's copy before
  * its new pages).  From the first one for which they do not suffice on, a sequence that needs any
- * gets none; neither does one that shares its page with such a sequence.  granted_dev[b]: whether
+ * gets none, and one that was to keep a page which others before it are to leave is not served
+ * either, whether these were or not: a later call finds it theirs or its own.  One that needs no
+ * page and begins in none that others hold is served always.  granted_dev[b]: whether
  * sequence b can be written now.  A sequence that breaks a bound, whose table has not all pages
  * of its past or is too short, is refused: left as it was, not granted.  Takes workspace. */
 mg_status mg_kv_cache_fit_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_batch *seqs,

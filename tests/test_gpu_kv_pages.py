@@ -360,6 +360,31 @@ def test_a_shared_page_waits_for_all_that_share_it(ops):
     np.testing.assert_array_equal(got[1], refs)
 
 
+@pytest.mark.parametrize("width", [101, 2800])  # (one workgroup, many)
+def test_the_last_to_share_a_page_waits_in_the_order(ops, width):
+    # A and C write into page 0; A gets its copy, so that C could keep page 0, but B between them asks for
+    # more than there is: nobody behind B is served who needs a page or keeps a shared one.  D needs
+    # and shares none.  The next call finds page 0 C's own.
+    c = Cache(ops, np.random.default_rng(30), 4, 16, heads=1)
+    table = np.full((4, width), -1, np.int32)
+    table[[0, 2, 3], 0] = [0, 0, 3]
+    refs, past = np.array([2, 0, 0, 1], np.int32), np.array([5, 0, 5, 7], np.int32)
+    new = np.array([1, 1600, 1, 1])
+    for granted, held in (([1, 0, 0, 1], [1, -1, 0, 3]), ([1, 0, 1, 1], [1, -1, 0, 3])):
+        want = P.fit(new, past, table, refs, 16)
+        table, refs, got = c.c.fit(row_start=np.r_[0, np.cumsum(new)], past=past, page_table=table, refs=refs)
+        np.testing.assert_array_equal(got, granted)
+        np.testing.assert_array_equal(table[:, 0], held)
+        np.testing.assert_array_equal(refs, [1, 1, 0, 1])
+        assert (table[:, 1:] == -1).all()
+        for g, w in zip((table, refs, got), want):
+            np.testing.assert_array_equal(g, w)
+    for x in c.now:
+        x[16:32] = x[:16]
+    c.check()
+    assert not c.c.refused()
+
+
 def test_captured_graph(ops):
     # A step that fits its sequences and moves rows: tables, lengths and refs change on the device.
     rng = np.random.default_rng(24)
