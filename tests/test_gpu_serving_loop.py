@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import drafts_reference as R
+import kv_reference as K
 from hip_graph import Captured
 
 pytestmark = pytest.mark.gpu
@@ -133,6 +134,79 @@ def test_speculative_decoding(ops, fmt, tree):
     assert (refs > 0).sum() == sum(-(-int(past[i]) // PAGE) for i in (0, 1))
     table, refs, granted = cache.fit(row_start=[0, 0, 0, 0], past=[0, 0, 0], page_table=table, refs=refs)
     assert (refs == 0).all() and (table == -1).all() and granted.all()
+
+
+def test_captured_steps_leave_out_whom_fit_does_not_serve(ops):
+    # A and B share their last page, C holds all others.  The step's calls get past -1 for those that are not
+    # granted: nothing of theirs is written, so the page they share stays as it is.
+    rng = np.random.default_rng(32)
+    with Captured(ops) as g:
+        cache = ops.KvCache(3, kv_heads=1, head_size=D, page_size=PAGE, fmt="int8", ctx=g.ctx)
+        whole = dict(row_start=PAGE * np.arange(4), past=np.zeros(3), page_table=np.arange(3)[:, None])
+        k, v = rng.standard_normal((2, 3 * PAGE, 1, D)).astype(np.float32)
+        cache.append(k, v, **whole)
+        held = [x.reshape(3, PAGE, 1, D) for x in cache.read(3 * PAGE, **whole)]
+        table = np.array([[0, -1], [0, -1], [1, 2]], np.int32)
+        refs, past = np.array([2, 1, 1], np.int32), np.array([5, 5, 20], np.int32)
+        start, kept, count = np.array([0, 2, 4, 6]), np.array([1, -1, 0, 1, 1, -1]), np.array([1, 2, 1])
+        d = {name: g.buffer(np.ascontiguousarray(a, np.int32)) for name, a in dict(
+            start=start, past=past, step=past, table=table, refs=refs, granted=np.zeros(3), kept=kept,
+            count=count).items()}
+        f = {name: g.buffer(np.zeros((6, 1, D), np.float32)) for name in ("k", "v", "q", "y")}
+
+        def batch(lengths):
+            return ops.SeqBatch(batch=3, rows=6, max_new=2, max_len=2 * PAGE, row_start_ptr=d["start"].ptr,
+                                past_ptr=d[lengths].ptr, page_table_ptr=d["table"].ptr, table_stride=2)
+
+        def fit():
+            cache.fit_dev(batch("past"), d["refs"].ptr, d["granted"].ptr)
+
+        def step():
+            cache.append_dev(batch("step"), f["k"].ptr, f["v"].ptr)
+            cache.attend_dev(batch("step"), f["q"].ptr, f["y"].ptr, 1)
+            cache.compact_dev(batch("step"), d["kept"].ptr, d["count"].ptr, past_out_ptr=d["step"].ptr)
+
+        fit()
+        g.put(d["step"], np.full(3, -1, np.int32))
+        step()  # (workspaces, nobody's rows)
+        assert cache.refused()
+        fit, step = g.capture(fit), g.capture(step)
+        for served in ([0, 0, 1], [0, 0, 1], [1, 1, 1], [1, 1, 1]):
+            rows = {name: rng.standard_normal((6, 1, D)).astype(np.float32) for name in ("k", "v", "q")}
+            for name, x in rows.items():
+                g.put(f[name], x)
+            g.put(f["y"], np.full((6, 1, D), 77, np.float32))
+            fit()
+            g.wait()
+            granted, table = (d[n].to_array(sh, np.int32) for n, sh in (("granted", (3,)), ("table", (3, 2))))
+            np.testing.assert_array_equal(granted, served)
+            g.put(d["step"], np.where(granted, past, -1).astype(np.int32))
+            step()
+            g.wait()
+            np.testing.assert_array_equal(d["step"].to_array((3,), np.int32), np.where(granted, past + count, -1))
+            y = f["y"].to_array((6, D), np.float32)
+            assert ((y == 77).all(1) == np.repeat(1 - granted, 2)).all()
+            if served[0] and past[0] == 5:  # A has a copy now
+                for x in held:
+                    x[table[0, 0]] = x[0]
+            now = [x.reshape(3, PAGE, 1, D) for x in cache.read(3 * PAGE, **whole)]
+            mine = np.zeros((3, PAGE), bool)  # places that may change
+            for b in np.nonzero(granted)[0]:
+                for p in range(past[b], past[b] + 2):
+                    mine[table[b, p // PAGE], p % PAGE] = True
+                for j, i in enumerate(kept[2 * b:2 * b + count[b]]):
+                    at = table[b, (past[b] + j) // PAGE], (past[b] + j) % PAGE
+                    for x, new in zip(now, (rows["k"], rows["v"])):
+                        np.testing.assert_array_equal(x[at], K.cached(new[2 * b + i][None], "int8")[0])
+            for x, was in zip(now, held):
+                np.testing.assert_array_equal(x[~mine], was[~mine])
+            held = now
+            assert cache.refused() == (not granted.all())
+            past = np.where(granted, past + count, past).astype(np.int32)
+            if served == [0, 0, 1] and past[2] == 22:
+                past[2] = 10  # C gives its second page back
+            g.put(d["past"], past)
+        cache.release()
 
 
 def test_contexts_at_once(ops):
