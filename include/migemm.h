@@ -913,7 +913,8 @@ typedef struct mg_drafts {
  * c.  At the end one more token is drawn by the weights left at c: the first whose running sum
  * exceeds uniform[row 0] of the whole.  A temperature that is not above 0: x stays if it is the
  * largest logit (the lowest of equal ones), which is also the last token.  Weights, sums and
- * comparisons are in 64 bits.  Where target row c has no distribution (NaN, +inf, only -inf),
+ * comparisons are in 64 bits; without draft, what rejected tokens leave of the 2048 logits around
+ * them is right to 2^-27 of itself.  Where target row c has no distribution (NaN, +inf, only -inf),
  * or nothing is left, the last token is -1; a token drafted from a draft row that has none is
  * rejected and leaves p_c.
  * out_tokens_dev / kept_dev [rows], from row_start[b] on: the count_dev[b] tokens emitted, and as

@@ -11,7 +11,8 @@
 // instructions, whose rate alone asks for 28, and the latency of the loads between them), up 253 to 284
 // (by bytes of base and y: 1.08 GB, 3.8 to 4.3 TB/s).  2494 rows of 5 prompts and 48 tokens, 2048 ->
 // 2048, 512, 512 by 16 in fp16: 5.5, 20 and 20 (latencies: 8 steps of 32 k a workgroup, 2 blocks of 128
-// outputs).  64 rows with adapters of their own, 2048 -> 2048 by 32 in fp32: 4.2 and 4.9 us, 35 MB.
+// outputs).  64 rows, 56 of them with one of 44 adapters, 2048 -> 2048 by 32 in fp32: 4.2 and 4.9 us, the
+// latencies of two launches (23 MB of weights, 2.5 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,8 +30,11 @@ constexpr int kTile = 64;   // rows of a tile
 constexpr int kCols = 64;   // values of A's rows that a workgroup takes
 constexpr int kOuts = 256;  // outputs that a workgroup takes at least
 // Few rows: up to 512, and 1.2 10^8 multiply-adds.  Measured where both take as long (all rows of one
-// slot / of 64 slots in turn): 2048 -> 2048 by 64, 450 and 384 rows (9 and 9 us at 32 against 25 and 26
-// sorted); 2048 -> 2 x 8192 by 64, 105 and 200; by 16, 300 and 350; 1024 -> 4096 by 8, beyond 512.
+// slot / of 64 slots in turn), fp32: 2048 -> 2048 by 64, 500 and 384 rows (9 and 11 us at 32 against 25
+// and 26 sorted); 2048 -> 2 x 8192 by 64, 115 and 185; by 16, 330 and 340; 1024 -> 4096 by 8, beyond 512.
+// In fp16: beyond; 120 and 360; 420 and beyond; beyond.  The numbers of rows, ranks and outputs
+// decide, so the rule is that of one slot; where rows are of many slots it sorts too early: 2 x 8192 by
+// 64 in 64 slots, 128 rows, 142 us sorted and 102 as few in fp32, 132 and 53 in fp16.
 inline bool few_rows(const mg_adapters &h, int64_t rows) {
   int64_t out = 0;
   for (int i = 0; i < h.n; i++) out += h.N[i];

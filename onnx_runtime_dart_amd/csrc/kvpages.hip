@@ -528,7 +528,10 @@ __global__ __launch_bounds__(256) void k_fit_give(const Fit a) {
 
 // All of it but the copies by one workgroup: what few sequences and pages need, without the waits
 // between launches, every table entry in a register of its own (64 sequences of 64 pages: 13
-// us, 21 in the kernels of their own and as many waits; 4 sequences: 9 and 17).  A chain: the entries, their
+// us, 21 in the kernels of their own and as many waits; 4 sequences: 9 and 17).  What it holds sets the
+// border: with the copies 64 sequences of 126 entries take 20 us here, of 128 entries 45 in the other
+// form, 512 of 128 67.  Many sequences of few pages are slower here, by the search for earlier ones
+// of the same page: 1024 of 6 entries 95, 1040 80 in the other form.  A chain: the entries, their
 // counts, what is let go, what is free, the entries written: 7 us of waits.
 constexpr int kOneBatch = 1024, kOnePages = 65536, kOneNeed = 8192, kOneEach = kOneNeed / 1024;
 // A count that other waves change in this launch.

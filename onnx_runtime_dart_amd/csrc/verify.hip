@@ -12,11 +12,12 @@
 //   k_masses  with them: the weights left in each run of the one row that it is drawn from
 //   k_pick    and the run, and the token in it, that the random number falls into
 //
-// k_stats is bound by bytes: 98 us for 64 sequences of 5 to 9 rows of 151936 logits of both kinds (two
-// at temperature 0 in ten need no draft rows), 5.2 TB/s; the series of 64 bits costs nothing there.  A
-// wave for 2048 logits, all loads at once, is the smallest part whose start is hidden.  The others are
-// chains of loads and steps of a workgroup: k_walk 5 to 7 us, 15 with the draw for trees of 25 tokens,
-// k_masses 16 (64 rows of both kinds, once more), k_pick 6.
+// k_stats is bound by bytes: 98 us for 64 sequences of 5 to 9 rows of 151936 logits of both kinds (12 of
+// them at temperature 0, whose draft rows are not read: 767 rows, 466 MB), 4.8 TB/s, the rate of a copy
+// (reads alone reach 6.1 to 6.4); the series of 64 bits costs nothing there.  A wave for 2048 logits,
+// all loads at once, is the smallest part whose start is hidden.  The others are chains of loads and
+// steps of a workgroup: k_walk 5 to 7 us, 15 to 16 with the draw for trees of 25 tokens, k_masses 16 (64
+// rows of both kinds, once more), k_pick 6.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
