@@ -853,11 +853,11 @@ mg_status mg_kv_cache_fork_dev(mg_ctx *ctx, mg_kv_cache *cache, const mg_seq_bat
  * Free pages go by number, lowest first, to the sequences in order (a sequence's copy before
  * its new pages).  From the first one for which they do not suffice on, a sequence that needs any
  * gets none, and one that was to keep a page which others before it are to leave is not served
- * either, whether these were or not: a later call finds it theirs or its own.  One that needs no
+ * either, whether these were or not: it waits for a later call.  One that needs no
  * page and begins in none that others hold is served always.  granted_dev[b]: whether
  * sequence b can be written now.  append and compact do not ask: in one that cannot they would write
  * into the page that it still shares.  They (and attention) leave it out where their batch's past[b]
- * is -1.  With ceil(rows of b / page_size) + 1 free pages for each b all are granted.  Pages are
+ * is -1.  With ceil(rows of b / page_size) + 1 free pages for each b none waits.  Pages are
  * copied in this cache alone: caches of other layers take the call too, with tables and refs of
  * their own.  A sequence that breaks a bound, whose table has not all pages
  * of its past or is too short, is refused: left as it was, not granted.  Takes workspace. */

@@ -350,9 +350,9 @@ struct Fit {
   mg_seq_batch s;
   int32_t *table, *refs, *granted;
   int64_t nrun;
-  // Workspace: a sequence's held pages (-1: refused), whether it takes a copy (1) or waits for
-  // those that share its page (2), its first page among those handed out, its copy's pages; the
-  // runs' free pages, then those before them.
+  // Workspace: a sequence's held pages (-1: refused), whether it takes a copy (1) or keeps a page that
+  // earlier ones are to leave (2: not granted where free pages end before it), its first page among
+  // those handed out, its copy's pages; the runs' free pages, then those before them.
   int32_t *held, *copy, *first, *need, *old, *own;
   int32_t *free;
 };
